@@ -85,6 +85,19 @@ SIGNATURES = [
     ("cuopx_asum", _int, [_i64, _fp, _i64, _fp, _vp, _sz, _vp]),
     ("cuopx_iamax", _int, [_i64, _fp, _i64, _vp, _vp, _sz, _vp]),
     ("cuopx_iamin", _int, [_i64, _fp, _i64, _vp, _vp, _sz, _vp]),
+    # Argument structs are passed as packed bytes (layers.py).
+    ("cuopx_linear_workspace_size", _sz, [_vp]),
+    ("cuopx_linear", _int, [_vp, _vp]),
+    ("cuopx_gated_linear_workspace_size", _sz, [_vp]),
+    ("cuopx_gated_linear", _int, [_vp, _vp]),
+    ("cuopx_linear_backward_workspace_size", _sz, [_vp]),
+    ("cuopx_linear_backward", _int, [_vp, _vp]),
+    ("cuopx_gated_linear_backward_workspace_size", _sz, [_vp]),
+    ("cuopx_gated_linear_backward", _int, [_vp, _vp]),
+    ("cuopx_layer_norm", _int, [_vp, _vp]),
+    ("cuopx_layer_norm_backward_workspace_size", _sz, [_vp]),
+    ("cuopx_layer_norm_backward", _int, [_vp, _vp]),
+    ("cuopx_dropout", _int, [_vp, _vp]),
 ]
 
 

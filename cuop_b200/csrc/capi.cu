@@ -12,14 +12,6 @@
 
 namespace cuopx {
 
-namespace {
-thread_local const char* t_last_kernel = "none";
-// Why the last CUOPX_CUDA_ERROR on this host thread happened (a CUDA error
-// name, or a short text for driver-API failures).
-thread_local const char* t_last_cuda_error = "none";
-std::atomic<int64_t> g_launches{0};
-std::atomic<int> g_sm_count[64] = {};
-
 bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes) {
   if (!a || !b || abytes == 0 || bbytes == 0) return false;
   const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
@@ -31,6 +23,14 @@ size_t span_bytes(int64_t rows, int64_t cols, int64_t ld, size_t es) {
   if (rows <= 0 || cols <= 0) return 0;
   return static_cast<size_t>((rows - 1) * ld + cols) * es;
 }
+
+namespace {
+thread_local const char* t_last_kernel = "none";
+// Why the last CUOPX_CUDA_ERROR on this host thread happened (a CUDA error
+// name, or a short text for driver-API failures).
+thread_local const char* t_last_cuda_error = "none";
+std::atomic<int64_t> g_launches{0};
+std::atomic<int> g_sm_count[64] = {};
 }  // namespace
 
 // Tracing, off unless asked for: CUOPX_NVTX=1 wraps every compute entry

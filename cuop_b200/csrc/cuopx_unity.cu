@@ -11,3 +11,6 @@
 #include "peer.cu"
 #include "gemm_tf32x3.cu"
 #include "vector_ops.cu"
+#include "layer_norm.cu"
+#include "dropout.cu"
+#include "linear.cu"

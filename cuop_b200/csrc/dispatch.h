@@ -24,6 +24,15 @@ int check_launch();
 // return CUOPX_CUDA_ERROR.
 int cuda_failure(cudaError_t e);
 int cuda_failure_text(const char* what);
+// Whether two byte ranges share a byte; bytes that a row-major matrix spans.
+bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes);
+size_t span_bytes(int64_t rows, int64_t cols, int64_t ld, size_t es);
+// Whether an output matrix may share memory with an input of the same shape:
+// not at all, or exactly (in place: same pointer and leading dimension).
+inline bool alias_ok(const void* out, int64_t ldo, const void* in, int64_t ldi, int64_t rows, int64_t cols, size_t es) {
+  if (out == in && ldo == ldi) return true;
+  return !overlaps(out, span_bytes(rows, cols, ldo, es), in, span_bytes(rows, cols, ldi, es));
+}
 // Process-wide fp32 arithmetic mode (cuopx_set_fp32_gemm_mode).
 int fp32_mode();
 
@@ -53,6 +62,10 @@ struct GemmProblem {
   const void* bias = nullptr;
   int epi = 0;
 };
+
+// A plain GEMM on the back-end that the variant table and the built-in
+// thresholds choose (capi.cu); arguments already validated.
+int gemm_route(const GemmProblem& p, cudaStream_t stream);
 
 // SIMT back-ends (gemm_simt.cu): generic any-dtype/any-layout kernel and
 // the register-blocked fp32 kernel.

@@ -288,6 +288,161 @@ int cuopx_iamax(int64_t n, const float* x, int64_t incx, int64_t* result, void* 
 int cuopx_iamin(int64_t n, const float* x, int64_t incx, int64_t* result, void* workspace,
                 size_t workspace_bytes, void* stream);
 
+/*
+ * Feed-forward layer operators (no counterpart in the reference beyond
+ * MatMulReluFused, see cuopx_gemm_ex).  Their arguments come in a struct:
+ * zero-fill it, set what the call uses, leave optional pointers NULL.  The
+ * pointers follow the rules above; sizes and leading dimensions are in
+ * elements, matrices are row-major.  An output may not overlap an input or
+ * another output, except where a comment allows it.
+ *
+ * Activations, with Phi the normal distribution function and s(z) =
+ * 1 / (1 + exp(-z)):
+ *   NONE z   RELU z > 0 ? z : +0   GELU z Phi(z)   SILU z s(z)   SIGMOID s(z)
+ *   GELU_TANH z s(2 sqrt(2/pi) (z + 0.044715 z^3))
+ */
+#define CUOPX_ACT_NONE 0
+#define CUOPX_ACT_RELU 1
+#define CUOPX_ACT_GELU 2
+#define CUOPX_ACT_GELU_TANH 3
+#define CUOPX_ACT_SILU 4
+#define CUOPX_ACT_SIGMOID 5
+
+typedef struct cuopx_linear_args {
+  int32_t dtype;      /* CUOPX_F16 or CUOPX_BF16, of every matrix and vector */
+  int32_t transW;     /* 0: W is stored [K][columns]; 1: [columns][K] */
+  int32_t activation; /* CUOPX_ACT_* */
+  int32_t reserved;   /* 0 */
+  int64_t M, N, K;
+  const void* X; /* [M][K] */
+  int64_t ldx;
+  const void* W; /* columns: N (linear), 2N (gated linear) */
+  int64_t ldw;
+  const void* bias;     /* [columns] or NULL */
+  const void* residual; /* [M][N] or NULL; may be Y itself (same ld).  NULL for gated linear */
+  int64_t ldr;
+  void* Y; /* [M][N] */
+  int64_t ldy;
+  void* preact; /* [M][columns] or NULL: receives Z */
+  int64_t ldz;
+  void* workspace; /* device, 256-byte aligned, not zeroed; see the size calls */
+  size_t workspace_bytes;
+} cuopx_linear_args;
+
+/*
+ * Linear layer: Z = X op(W) + bias, Y = act(Z) + residual.  fp32 accumulation
+ * and epilogue; Y is rounded once, from the unrounded Z; the stored Z is
+ * rounded once.  The workspace is wanted only when a matrix is not 16-byte
+ * aligned (base, or leading dimension in bytes); without it (or with less
+ * than cuopx_linear_workspace_size) a slower kernel takes such a call.
+ */
+size_t cuopx_linear_workspace_size(const cuopx_linear_args* args);
+int cuopx_linear(const cuopx_linear_args* args, void* stream);
+
+/*
+ * Gated linear layer: Z = [G | U] = X op(W) + bias with W's columns [0, N)
+ * the gate's and [N, 2N) the other projection's; Y = act(G) * U.  Rounding
+ * and workspace as above.
+ */
+size_t cuopx_gated_linear_workspace_size(const cuopx_linear_args* args);
+int cuopx_gated_linear(const cuopx_linear_args* args, void* stream);
+
+typedef struct cuopx_linear_backward_args {
+  int32_t dtype, transW, activation, reserved;
+  int64_t M, N, K;
+  const void* dY; /* [M][N] */
+  int64_t lddy;
+  const void* X; /* [M][K]; read for dW */
+  int64_t ldx;
+  const void* W; /* read for dX */
+  int64_t ldw;
+  const void* preact; /* Z as the forward pass stored it; not read by linear with CUOPX_ACT_NONE */
+  int64_t ldz;
+  void* dX; /* [M][K] or NULL */
+  int64_t lddx;
+  void* dW; /* W's layout, or NULL */
+  int64_t lddw;
+  void* dbias; /* [columns] or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} cuopx_linear_backward_args;
+
+/*
+ * Gradients of cuopx_linear: dZ = dY * act'(Z), dX = dZ op(W)^T, dW =
+ * X^T dZ (in W's layout), dbias = column sums of dZ (from the unrounded dZ).
+ * The residual's gradient is dY itself.  dZ is rounded to the 16-bit type
+ * between its computation and the two products, which take 16-bit operands.
+ * Of cuopx_gated_linear: dG = dY * U * act'(G), dU = dY * act(G), dZ =
+ * [dG | dU].  The workspace is required: CUOPX_RESOURCE_UNAVAILABLE when it
+ * is smaller than the size call says (which may be 0).
+ */
+size_t cuopx_linear_backward_workspace_size(const cuopx_linear_backward_args* args);
+int cuopx_linear_backward(const cuopx_linear_backward_args* args, void* stream);
+size_t cuopx_gated_linear_backward_workspace_size(const cuopx_linear_backward_args* args);
+int cuopx_gated_linear_backward(const cuopx_linear_backward_args* args, void* stream);
+
+typedef struct cuopx_layer_norm_args {
+  int32_t dtype;  /* of X, Y, dY, dX: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
+  int32_t wdtype; /* of weight, bias and their gradients: dtype or CUOPX_F32 */
+  int64_t rows, cols;
+  double eps; /* forward: finite, >= 0 */
+  const void* X;
+  int64_t ldx;
+  const void* weight; /* [cols] or NULL (ones) */
+  const void* bias;   /* [cols] or NULL (zeros); forward only */
+  void* Y;            /* forward; may be X itself (same ld) */
+  int64_t ldy;
+  float* mean; /* [rows]; forward: written when not NULL; backward: read */
+  float* rstd; /* [rows]; 1 / sqrt(var + eps), var divided by cols */
+  const void* dY;
+  int64_t lddy;
+  void* dX; /* may be dY itself (same ld); NULL: not computed */
+  int64_t lddx;
+  void* dweight; /* [cols] or NULL */
+  void* dbias;   /* [cols] or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} cuopx_layer_norm_args;
+
+/*
+ * Layer norm of each row: y = (x - mean) * rstd * weight + bias, and its
+ * gradients from the forward pass's mean and rstd: h = (x - mean) * rstd,
+ * t = dy * weight, dx = rstd * (t - avg(t) - h avg(t h)), dweight =
+ * sum over rows of dy h, dbias = sum over rows of dy.  Statistics and sums
+ * in fp32, results rounded once.  The backward workspace (needed for dweight
+ * and dbias) holds partial sums: CUOPX_RESOURCE_UNAVAILABLE when too small.
+ */
+int cuopx_layer_norm(const cuopx_layer_norm_args* args, void* stream);
+size_t cuopx_layer_norm_backward_workspace_size(const cuopx_layer_norm_args* args);
+int cuopx_layer_norm_backward(const cuopx_layer_norm_args* args, void* stream);
+
+typedef struct cuopx_dropout_args {
+  int32_t dtype; /* CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
+  int32_t reserved;
+  int64_t rows, cols;
+  double p;                   /* 0 <= p <= 1 */
+  uint64_t seed, offset;      /* key and first counter */
+  const uint64_t* offset_dev; /* device word added to `offset` when the kernel runs, or NULL */
+  const void* X;
+  int64_t ldx;
+  const void* residual; /* [rows][cols] or NULL; may be Y itself (same ld) */
+  int64_t ldr;
+  void* Y; /* may be X itself (same ld) */
+  int64_t ldy;
+} cuopx_dropout_args;
+
+/*
+ * Dropout: y = (keep ? x / (1 - p) : 0) + residual, a mask that is never
+ * stored: element i = row * cols + col takes word i % 4 of Philox4x32-10
+ * (Salmon, Moraes, Dror, Shaw, 2011) with key `seed` and 128-bit counter
+ * (offset + i / 4, 0), and is kept when that word is at least
+ * round(p * 2^32).  The gradient is the same call on dy, with the same p,
+ * seed and offset and no residual.  A call uses ceil(rows * cols / 4)
+ * counters; give the next call an offset past them.  offset_dev lets a
+ * captured graph draw a new mask at each replay.
+ */
+int cuopx_dropout(const cuopx_dropout_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
