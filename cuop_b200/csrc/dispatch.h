@@ -104,6 +104,35 @@ constexpr int kTf32x3SplitK2 = -2;
 // split over two pairs (a cluster of four); K-major A only.
 constexpr int kTf32x3PairSplitK2 = -3;
 
+// ---- layers (linear.cu): forward problem of a linear or gated linear layer ----
+struct LinearProblem {
+  int dtype;
+  bool transW;
+  int act;
+  bool gated;
+  int64_t M, N, K;
+  const void* X;
+  int64_t ldx;
+  const void* W;
+  int64_t ldw;
+  const void* bias;
+  const void* R;
+  int64_t ldr;
+  void* Y;
+  int64_t ldy;
+  void* Z;
+  int64_t ldz;
+  int64_t wide() const { return gated ? 2 * N : N; }  // columns of W and Z
+};
+
+// Base and rows on 16-byte boundaries (16-bit elements).
+inline bool row_aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && ld % 8 == 0; }
+
+// Layer forward pass on CTA pairs (gemm_tc2.cu); pbn: accumulator columns of
+// a tile, 256 or 128 (half as many outputs per row when gated).
+bool linear_tc2_supported(const LinearProblem& p);
+int linear_tc2(const LinearProblem& p, cudaStream_t stream, int pbn);
+
 // ---- variant selection (host/tuning.cpp) ----
 // GEMM variants a tuning table or an override may name.
 enum GemmVariant : int {

@@ -22,6 +22,12 @@
 //              slot 0 start as soon as slot 0 is free and its first MMAs
 //              into slot 1 wait only for the rest of the drain.
 //
+// MODE selects the epilogue: kPairGemm (alpha, beta, bias, ReLU, peers), or a
+// layer's (layer_epilogue.cuh).  In kPairGated a tile's accumulator holds the
+// same PBN / 2 output columns of two projections: the even CTA loads the
+// gate's columns of B and the odd one the other projection's, so one MMA
+// computes both and the epilogue finds them PBN / 2 accumulator columns apart.
+//
 //   warp 0      TMA producer (both CTAs): loads complete on the LEADER's
 //               `full` mbarrier (.cta_group::2); the leader posts the
 //               expected byte count for both halves.
@@ -42,6 +48,7 @@
 // the kernel so no CTA exits while its peer may still touch its shared memory.
 #include "common.cuh"
 #include "dispatch.h"
+#include "layer_epilogue.cuh"
 
 namespace cuopx {
 
@@ -70,9 +77,14 @@ struct PairCfg {
   static constexpr int STAGES = PBN == 128 ? 7 : (SPT == 1 ? 6 : 4);
 };
 
-template <int PBN>
+enum PairMode { kPairGemm = 0, kPairLinear = 1, kPairGated = 2 };
+
+// kPairGated stages three output tiles per chunk (both pre-activations and
+// the result) instead of two, which takes the room of one ring stage.
+template <int PBN, int MODE = kPairGemm>
 struct PairSmem {
-  static constexpr int STAGES = PairCfg<PBN>::STAGES;
+  static constexpr int STAGES = PairCfg<PBN>::STAGES - (MODE == kPairGated ? 1 : 0);
+  static constexpr int C_BUFS = MODE == kPairGated ? 3 : 2;
   static constexpr int A_STAGE = P_BM * P_BK * 2;               // 16 KB
   static constexpr int B_PIECE = (PairCfg<PBN>::SLOT / 2) * P_BK * 2;  // this CTA's half of one slot
   static constexpr int B_STAGE = PairCfg<PBN>::SPT * B_PIECE;
@@ -80,7 +92,7 @@ struct PairSmem {
   static constexpr int OFF_A = 0;
   static constexpr int OFF_B = STAGES * A_STAGE;
   static constexpr int OFF_C = OFF_B + STAGES * B_STAGE;
-  static constexpr int OFF_BAR = OFF_C + P_EPI_WARPS * 2 * C_STAGE;
+  static constexpr int OFF_BAR = OFF_C + P_EPI_WARPS * C_BUFS * C_STAGE;
   // full[S], empty[S], acc_full[SLOTS], acc_empty[SLOTS], drain
   static constexpr int NUM_BARS = 2 * STAGES + 2 * PairCfg<PBN>::SLOTS + 1;
   // Tile-scheduler ring: P_CLC_SLOTS 16-byte launch-control responses, then
@@ -108,6 +120,15 @@ struct PairParams {
   int epi;           // CUOPX_EPI_* flags
 };
 
+
+// What a layer's epilogue takes beyond PairParams; nothing for a plain GEMM.
+template <int MODE>
+struct PairLayer {
+  CUtensorMap tmZ, tmZ2;
+  LayerEpi epi;
+};
+template <>
+struct PairLayer<kPairGemm> {};
 
 // Next pair tile from a completed launch-control response (the cancelled
 // cluster's first CTA index / 2); false when none was left.
@@ -180,13 +201,15 @@ __device__ __forceinline__ uint32_t pack2_pair<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <typename T, bool A_MN, bool B_MN, int PBN>
+template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmC, const PairParams p) {
-  using L = PairSmem<PBN>;
+                    const __grid_constant__ CUtensorMap tmC, const PairParams p,
+                    const __grid_constant__ PairLayer<MODE> layer) {
+  using L = PairSmem<PBN, MODE>;
   constexpr int SPT = PairCfg<PBN>::SPT;
-  constexpr int P_STAGES = PairCfg<PBN>::STAGES;
+  static_assert(MODE == kPairGemm || SPT == 1, "layer epilogues overlap the next tile");
+  constexpr int P_STAGES = L::STAGES;
   constexpr int P_SLOT_COLS = PairCfg<PBN>::SLOT;
   constexpr int P_SLOTS = PairCfg<PBN>::SLOTS;
   constexpr int CHUNKS_PER_SLOT = P_SLOT_COLS / P_CHUNK;
@@ -278,7 +301,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         int b, mt, nt;
         pair_tile_coords(t, p, b, mt, nt);
         const int m0 = mt * 2 * P_BM + static_cast<int>(rank) * P_BM;
-        const int n0 = nt * PBN + static_cast<int>(rank) * (P_SLOT_COLS / 2);
+        // Gated: column n0 of this CTA's projection (rank 0 the gate's, rank 1 the other's).
+        const int n0 = MODE == kPairGated ? nt * (PBN / 2) + static_cast<int>(rank) * p.N
+                                          : nt * PBN + static_cast<int>(rank) * (P_SLOT_COLS / 2);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
             ok = false;
@@ -457,7 +482,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
     const int row_in_tile = 32 * q + lane;
-    unsigned char* const stage_base = smem + L::OFF_C + (warp - 2) * 2 * L::C_STAGE;  // two buffers
+    unsigned char* const stage_base = smem + L::OFF_C + (warp - 2) * L::C_BUFS * L::C_STAGE;
     int acc = 0;             // first TMEM slot of the tile (rotates when SPT == 1)
     uint32_t full_bits = 0;  // bit s: parity of slot s's next acc_full phase
     int sbuf = 0;
@@ -473,6 +498,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       tc_fence_after_sync();
       const uint32_t t_row =
           tmem_base + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(s0 * P_SLOT_COLS);
+      if constexpr (MODE != kPairGemm) {
+        constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
+        layer_epilogue_tile<T, MODE == kPairGated, COLS>(
+            t_row, nt * COLS, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ, &layer.tmZ2, stage_base, lane, sbuf,
+            [&] {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[s0], 0));
+            });
+      } else {
       const int64_t grow = static_cast<int64_t>(m0) + row_in_tile;
 #pragma unroll 1
       for (int ch = 0; ch < PBN / P_CHUNK; ++ch) {
@@ -550,6 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         }
         sbuf ^= 1;
       }
+      }
       full_bits ^= 1u << s0;
       if (SPT == 1) acc = acc + 1 == P_SLOTS ? 0 : acc + 1;
       const int cs = seq % P_CLC_SLOTS;
@@ -626,13 +662,73 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
   }
   // One cluster per pair tile; running clusters take over unlaunched ones.
   const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(P_THREADS), L::ALLOC,
-                                     stream, mA, mB, mC, prm);
+                                     stream, mA, mB, mC, prm, PairLayer<kPairGemm>{});
   if (lerr != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(lerr);
   }
   note_launch(name);
   return check_launch();
+}
+
+// A layer's forward pass: X [M][K] K-major, W [K][columns] (B_MN) or [columns][K].
+template <typename T, bool B_MN, int PBN, int MODE>
+int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* name) {
+  using L = PairSmem<PBN, MODE>;
+  constexpr int P_SLOT_COLS = PairCfg<PBN>::SLOT;
+  constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
+  const CUtensorMapDataType dt =
+      std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap mA, mB, mC;
+  PairLayer<MODE> layer = {};
+  bool ok = make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
+  if (B_MN) ok &= make_map(&mB, dt, p.W, p.wide(), p.K, 1, p.ldw, 0, 64, P_BK);
+  else ok &= make_map(&mB, dt, p.W, p.K, p.wide(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
+  ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
+  if (p.Z) {
+    ok &= make_map(&layer.tmZ, dt, p.Z, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
+    if (MODE == kPairGated) ok &= make_map(&layer.tmZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
+  }
+  if (!ok) return CUOPX_CUDA_ERROR;
+  layer.epi = layer_epi(p);
+  PairParams prm = {};
+  prm.M = static_cast<int>(p.M);
+  prm.N = static_cast<int>(p.N);
+  prm.K = static_cast<int>(p.K);
+  prm.batch = 1;
+  prm.tiles_m = static_cast<int>((p.M + 2 * P_BM - 1) / (2 * P_BM));
+  prm.tiles_n = static_cast<int>((p.N + COLS - 1) / COLS);
+  prm.num_tiles = prm.tiles_m * prm.tiles_n;
+  prm.k_blocks = static_cast<int>((p.K + P_BK - 1) / P_BK);
+  auto kern = gemm_tc2_kernel<T, false, B_MN, PBN, MODE>;
+  static std::atomic<bool> attr_set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
+  if (!attr_set[dev].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
+      return CUOPX_CUDA_ERROR;
+    attr_set[dev].store(true, std::memory_order_relaxed);
+  }
+  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(P_THREADS), L::ALLOC,
+                                      stream, mA, mB, mC, prm, layer);
+  if (lerr != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_failure(lerr);
+  }
+  note_launch(name);
+  return check_launch();
+}
+
+template <typename T, int PBN>
+int launch_tc2_layer_layout(const LinearProblem& p, cudaStream_t stream) {
+  if (p.gated) {
+    const char* name = PBN == 256 ? "gated_linear_tc2_256x128" : "gated_linear_tc2_256x64";
+    return p.transW ? launch_tc2_layer<T, false, PBN, kPairGated>(p, stream, name)
+                    : launch_tc2_layer<T, true, PBN, kPairGated>(p, stream, name);
+  }
+  const char* name = PBN == 256 ? "linear_tc2_256x256" : "linear_tc2_256x128";
+  return p.transW ? launch_tc2_layer<T, false, PBN, kPairLinear>(p, stream, name)
+                  : launch_tc2_layer<T, true, PBN, kPairLinear>(p, stream, name);
 }
 
 }  // namespace
@@ -702,6 +798,23 @@ int gemm_tc2_peers(const GemmProblem& p, void* const* peers, int npeers, cudaStr
   if (pbn == 128) return launch_tc2_layout<128>(p, peers, npeers, stream);
   return pbn == 512 ? launch_tc2_layout<512>(p, peers, npeers, stream)
                     : launch_tc2_layout<256>(p, peers, npeers, stream);
+}
+
+// TMA reads and writes whole 16-byte groups of aligned rows.
+bool linear_tc2_supported(const LinearProblem& p) {
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.N > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (!row_aligned16(p.X, p.ldx) || !row_aligned16(p.W, p.ldw) || !row_aligned16(p.Y, p.ldy)) return false;
+  if (p.Z && !row_aligned16(p.Z, p.ldz)) return false;
+  // The second projection's columns start N into W's rows and Z's.
+  if (p.gated && p.N % 8 && (!p.transW || p.Z)) return false;
+  return ((p.M + 255) / 256) * ((p.N + 63) / 64) < (int64_t(1) << 29);
+}
+
+int linear_tc2(const LinearProblem& p, cudaStream_t stream, int pbn) {
+  if (p.dtype == CUOPX_BF16)
+    return pbn == 256 ? launch_tc2_layer_layout<__nv_bfloat16, 256>(p, stream)
+                      : launch_tc2_layer_layout<__nv_bfloat16, 128>(p, stream);
+  return pbn == 256 ? launch_tc2_layer_layout<__half, 256>(p, stream) : launch_tc2_layer_layout<__half, 128>(p, stream);
 }
 
 }  // namespace cuopx

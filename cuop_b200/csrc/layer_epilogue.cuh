@@ -1,0 +1,191 @@
+// Epilogue of the tcgen05 layer kernels: bias, kept pre-activation,
+// activation, product of the two projections, residual, one rounding, TMA
+// stores.  A warp drains its 32 accumulator rows in 64-column chunks (the box
+// of a TMA store), each in two halves of 32 columns.
+#pragma once
+
+#include <cuda.h>
+
+#include "activation.cuh"
+#include "common.cuh"
+#include "dispatch.h"
+
+namespace cuopx {
+
+struct LayerEpi {
+  const void* bias;  // NULL: none.  Gated: the gate's N, then the other projection's N
+  const void* R;     // residual or NULL
+  int64_t ldr;
+  int act;
+  int has_z;     // store the pre-activation
+  int vec_bias;  // bias can be read in 16-byte groups
+  int vec_res;   // so can the residual's rows
+};
+
+inline LayerEpi layer_epi(const LinearProblem& p) {
+  LayerEpi e;
+  e.bias = p.bias;
+  e.R = p.R;
+  e.ldr = p.ldr;
+  e.act = p.act;
+  e.has_z = p.Z != nullptr;
+  e.vec_bias = p.N % 8 == 0 && row_aligned16(p.bias, 0);
+  e.vec_res = p.N % 8 == 0 && row_aligned16(p.R, p.ldr);
+  return e;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_layer(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2_layer(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    // bf16 is the upper half of a float.
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+  }
+}
+
+// 32 elements of a row from column `col` on, zeros past column N.
+template <typename T>
+__device__ __forceinline__ void load_row32(const T* row, int64_t col, int64_t N, bool vec, uint4 (&raw)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (vec) {  // N is a multiple of 8: a group is inside or outside
+      if (col + 8 * j < N) raw[j] = *reinterpret_cast<const uint4*>(row + col + 8 * j);
+    } else {
+      uint32_t* w = &raw[j].x;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + 8 * j + i < N)
+          w[i / 2] |= static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(row + col + 8 * j + i)) << (16 * (i & 1));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void add_row32(float (&v)[32], const uint4 (&raw)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2_layer<T>(w[i]);
+      v[8 * j + 2 * i] += f.x;
+      v[8 * j + 2 * i + 1] += f.y;
+    }
+  }
+}
+
+// Rounds 32 values into half `h` of this lane's 128-byte staging row
+// (128-byte swizzle: 16-byte group j of row r at j ^ (r & 7)).
+template <typename T>
+__device__ __forceinline__ void stage_row32(unsigned char* buf, int lane, int h, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 w;
+    w.x = pack2_layer<T>(v[8 * j + 0], v[8 * j + 1]);
+    w.y = pack2_layer<T>(v[8 * j + 2], v[8 * j + 3]);
+    w.z = pack2_layer<T>(v[8 * j + 4], v[8 * j + 5]);
+    w.w = pack2_layer<T>(v[8 * j + 6], v[8 * j + 7]);
+    *reinterpret_cast<uint4*>(buf + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)) = w;
+  }
+}
+
+// One warp's rows of one tile.  t_row: TMEM address of the tile's first
+// accumulator column in this warp's lane quarter; COLS output columns, those
+// of the second projection (GATED) COLS further on.  `stage`: 3 (GATED) or 2
+// staging buffers of 4 KB.  release() is called once the accumulator has been
+// read.  (n0, m0): output column and first row of this warp's box.
+template <typename T, bool GATED, int COLS, typename Release>
+__device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int m0, int M, int N, const LayerEpi& e,
+                                                    const CUtensorMap* tmY, const CUtensorMap* tmZ,
+                                                    const CUtensorMap* tmZ2, unsigned char* stage, int lane, int& ybuf,
+                                                    Release&& release) {
+  constexpr int BUF = 32 * 64 * 2;
+  constexpr int NBUF = GATED ? 3 : 2;
+  const int64_t grow = static_cast<int64_t>(m0) + lane;
+  const bool has_res = !GATED && e.R != nullptr && grow < M;
+  const T* rrow = static_cast<const T*>(e.R) + grow * e.ldr;
+  const T* bias = static_cast<const T*>(e.bias);
+  uint4 res[4];
+  if (has_res) load_row32<T>(rrow, n0, N, e.vec_res, res);
+#pragma unroll 1
+  for (int half = 0; half < COLS / 32; ++half) {
+    const int h = half & 1;
+    const int64_t col = static_cast<int64_t>(n0) + 32 * half;
+    uint32_t ra[32], rb[GATED ? 32 : 1];
+    tmem_ld_32x32b_x32(t_row + 32 * half, ra);
+    if constexpr (GATED) tmem_ld_32x32b_x32(t_row + COLS + 32 * half, rb);
+    tmem_wait_ld();
+    if (half == COLS / 32 - 1) release();
+    float a[32], b[GATED ? 32 : 1];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      a[i] = __uint_as_float(ra[i]);
+      if constexpr (GATED) b[i] = __uint_as_float(rb[i]);
+    }
+    if (bias) {
+      uint4 raw[4];
+      load_row32<T>(bias, col, N, e.vec_bias, raw);
+      add_row32<T>(a, raw);
+      if constexpr (GATED) {
+        load_row32<T>(bias + N, col, N, e.vec_bias, raw);
+        add_row32<T>(b, raw);
+      }
+    }
+    if (h == 0) {
+      // The buffers this chunk fills: with a kept pre-activation all of them,
+      // else one, the stores of the previous chunk having the other.
+      if (lane == 0) {
+        if (e.has_z) bulk_wait_group_read<0>();
+        else bulk_wait_group_read<1>();
+      }
+      __syncwarp();
+      if (e.has_z) ybuf = NBUF - 1;
+      else ybuf = ybuf == 0 ? 1 : 0;
+    }
+    if (e.has_z) {
+      stage_row32<T>(stage, lane, h, a);
+      if constexpr (GATED) stage_row32<T>(stage + BUF, lane, h, b);
+    }
+    with_activation(e.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a[i] = act_value<act.value>(a[i]);
+    });
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a[i] *= b[i];
+    }
+    if (has_res) {
+      add_row32<T>(a, res);
+      if (half + 1 < COLS / 32) load_row32<T>(rrow, col + 32, N, e.vec_res, res);
+    }
+    stage_row32<T>(stage + ybuf * BUF, lane, h, a);
+    if (h == 1) {
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        const int c = n0 + 32 * (half - 1);
+        if (e.has_z) {
+          tma_store_3d(tmZ, stage, c, m0, 0);
+          if constexpr (GATED) tma_store_3d(tmZ2, stage + BUF, c, m0, 0);
+        }
+        tma_store_3d(tmY, stage + ybuf * BUF, c, m0, 0);
+        bulk_commit_group();
+      }
+    }
+  }
+}
+
+}  // namespace cuopx

@@ -18,26 +18,6 @@ namespace cuopx {
 
 namespace {
 
-struct LinearProblem {
-  int dtype;
-  bool transW;
-  int act;
-  bool gated;
-  int64_t M, N, K;
-  const void* X;
-  int64_t ldx;
-  const void* W;
-  int64_t ldw;
-  const void* bias;
-  const void* R;
-  int64_t ldr;
-  void* Y;
-  int64_t ldy;
-  void* Z;
-  int64_t ldz;
-  int64_t wide() const { return gated ? 2 * N : N; }  // columns of W and Z
-};
-
 // ---------------------------------------------------------------- any size, stride and alignment
 // 64 x 64 outputs per CTA, 16-deep steps through shared memory, 4 x 4 outputs
 // per thread (of both projections when gated).
@@ -247,10 +227,6 @@ __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, in
   db[c] = from_acc<T>(s);
 }
 
-bool aligned16(const void* p, int64_t ld) {
-  return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && ld % 8 == 0;
-}
-
 // ---------------------------------------------------------------- backward plan
 struct BackwardPlan {
   bool need_dz;  // dZ differs from dY
@@ -267,8 +243,8 @@ BackwardPlan backward_plan(const cuopx_linear_backward_args& a, bool gated) {
   if (a.M <= 0 || a.N <= 0 || dtype_size(a.dtype) == 0) return q;
   q.need_dz = (gated || a.activation != CUOPX_ACT_NONE) && (a.dX || a.dW) && a.K > 0;
   q.lddz = (wide + 7) / 8 * 8;
-  const bool vec = a.N % 8 == 0 && aligned16(a.dY, a.lddy) &&
-                   ((!gated && a.activation == CUOPX_ACT_NONE) || aligned16(a.preact, a.ldz));
+  const bool vec = a.N % 8 == 0 && row_aligned16(a.dY, a.lddy) &&
+                   ((!gated && a.activation == CUOPX_ACT_NONE) || row_aligned16(a.preact, a.ldz));
   q.v = vec ? 8 : 1;
   const int64_t strips = (a.N + 32 * q.v - 1) / (32 * q.v);
   const int64_t want = (static_cast<int64_t>(device_sm_count()) * 4 + strips - 1) / strips;
@@ -332,6 +308,7 @@ int linear_forward(const cuopx_linear_args* a, bool gated, cudaStream_t stream) 
   if (const int v = validate_linear(*a, gated); v >= 0) return v;
   LinearProblem p{a->dtype, a->transW != 0, a->activation, gated, a->M,   a->N,   a->K,      a->X,   a->ldx, a->W,
                   a->ldw,   a->bias,        a->residual,   a->ldr, a->Y, a->ldy, a->preact, a->ldz};
+  if (linear_tc2_supported(p) && p.M >= 64) return linear_tc2(p, stream, 256);
   return linear_simt(p, stream);
 }
 
