@@ -13,4 +13,5 @@
 #include "vector_ops.cu"
 #include "layer_norm.cu"
 #include "dropout.cu"
+#include "linear_split.cu"
 #include "linear.cu"

@@ -132,6 +132,9 @@ inline bool row_aligned16(const void* p, int64_t ld) { return (reinterpret_cast<
 // a tile, 256 or 128 (half as many outputs per row when gated).
 bool linear_tc2_supported(const LinearProblem& p);
 int linear_tc2(const LinearProblem& p, cudaStream_t stream, int pbn);
+// Layer forward pass for few rows: swapped operands, K split over a cluster (linear_split.cu).
+bool linear_split_supported(const LinearProblem& p);
+int linear_split(const LinearProblem& p, cudaStream_t stream);
 
 // ---- variant selection (host/tuning.cpp) ----
 // GEMM variants a tuning table or an override may name.

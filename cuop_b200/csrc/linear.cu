@@ -308,6 +308,7 @@ int linear_forward(const cuopx_linear_args* a, bool gated, cudaStream_t stream) 
   if (const int v = validate_linear(*a, gated); v >= 0) return v;
   LinearProblem p{a->dtype, a->transW != 0, a->activation, gated, a->M,   a->N,   a->K,      a->X,   a->ldx, a->W,
                   a->ldw,   a->bias,        a->residual,   a->ldr, a->Y, a->ldy, a->preact, a->ldz};
+  if (p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
   if (linear_tc2_supported(p) && p.M >= 64) return linear_tc2(p, stream, 256);
   return linear_simt(p, stream);
 }
