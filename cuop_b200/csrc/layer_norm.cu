@@ -9,6 +9,14 @@
 // The variance is summed from (x - mean), not from x^2: no cancellation when
 // the mean is large.  All sums are fp32, in an order fixed by the launch
 // shape, without atomics, so results do not change from run to run.
+//
+// Bound by HBM: every element is read once and written once.  A row stays in
+// the registers of its threads (a warp, or a whole CTA) between the sums and
+// the result, and the loads of the next row are issued before the sums of the
+// current one are exchanged.  The backward kernel reads x and dy once for all
+// three gradients: a thread keeps the same columns for all rows of its CTA and
+// their two column sums in registers; one partial sum per CTA and column goes
+// to the workspace, and a second small kernel adds those in CTA order.
 #include "common.cuh"
 #include "dispatch.h"
 
@@ -23,6 +31,7 @@ struct NormParams {
   int64_t ldx;
   const void* w;
   const void* b;
+  bool vec_w, vec_b;  // weight, bias start on 16-byte boundaries
   void* y;
   int64_t ldy;
   float* mean;
@@ -51,6 +60,250 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   __syncthreads();
   const int warps = static_cast<int>(blockDim.x) >> 5;
   return warp_sum((threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : 0.f);
+}
+
+// ------------------------------------------------ rows in registers
+// A thread holds NV groups of V neighbouring columns: group g of thread t is
+// columns [V (t + G g), ...), G threads per row.  V elements are one 16-byte
+// load, or V = 1 where rows are not 16-byte aligned.
+template <typename T, int V>
+struct RowVec {
+  T e[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ RowVec<T, V> load_vec(const T* p) {
+  RowVec<T, V> r;
+  if constexpr (V == 1) {
+    r.e[0] = *p;
+  } else {
+    static_assert(sizeof(r) == 16, "16-byte groups");
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
+  }
+  return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const RowVec<T, V>& r) {
+  if constexpr (V == 1) *p = r.e[0];
+  else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
+}
+
+// V weights from column c on, in 16-byte loads where `vec` says that they start on such a boundary.
+template <typename W, int V>
+__device__ __forceinline__ void load_weights(const W* w, int64_t c, bool vec, float (&out)[V]) {
+  constexpr int E = 16 / static_cast<int>(sizeof(W));
+  if constexpr (V % E == 0) {
+    if (vec) {
+#pragma unroll
+      for (int j = 0; j < V / E; ++j) {
+        const RowVec<W, E> r = load_vec<W, E>(w + c + j * E);
+#pragma unroll
+        for (int i = 0; i < E; ++i) out[j * E + i] = to_acc<W>(r.e[i]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = to_acc<W>(w[c + i]);
+}
+
+// Sums of two values over the threads of a row: the warp, or the CTA through
+// one of two alternating buffers (one barrier: a thread writes a buffer again
+// only after every thread has arrived at the barrier after its last reads).
+template <bool WARP>
+__device__ __forceinline__ float2 row_sum(float a, float b, float2 (*buf)[32], int& parity) {
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if constexpr (!WARP) {
+    if ((threadIdx.x & 31) == 0) buf[parity][threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    const int warps = static_cast<int>(blockDim.x) >> 5;
+    const float2 v = (threadIdx.x & 31) < warps ? buf[parity][threadIdx.x & 31] : make_float2(0.f, 0.f);
+    a = warp_sum(v.x);
+    b = warp_sum(v.y);
+    parity ^= 1;
+  }
+  return make_float2(a, b);
+}
+
+template <typename T, typename W, int V, int NV, bool WARP, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) layer_norm_rows(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  int parity = 0;
+  const int G = WARP ? 32 : static_cast<int>(blockDim.x);
+  const int t = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
+  const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = WARP ? gridDim.x * static_cast<int64_t>(blockDim.x >> 5) : gridDim.x;
+  const float inv = 1.f / static_cast<float>(p.cols);
+  const T* x = static_cast<const T*>(p.x);
+  T* y = static_cast<T*>(p.y);
+  const W* w = static_cast<const W*>(p.w);
+  const W* b = static_cast<const W*>(p.b);
+  grid_dependency_wait();
+  RowVec<T, V> next[NV];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+      if (row < p.rows && c < p.cols) next[g] = load_vec<T, V>(x + row * p.ldx + c);
+    }
+  };
+  fetch(first);
+  for (int64_t row = first; row < p.rows; row += step) {
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const bool in = static_cast<int64_t>(V) * (t + G * g) < p.cols;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[g][i] = in ? to_acc<T>(next[g].e[i]) : 0.f;
+        s += v[g][i];
+      }
+    }
+    fetch(row + step);
+    const float mean = row_sum<WARP>(s, 0.f, buf, parity).x * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const bool in = static_cast<int64_t>(V) * (t + G * g) < p.cols;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[g][i] -= mean;
+        if (in) q = fmaf(v[g][i], v[g][i], q);
+      }
+    }
+    const float rstd = 1.f / sqrtf(fmaf(row_sum<WARP>(q, 0.f, buf, parity).x, inv, p.eps));
+    if (t == 0) {
+      if (p.mean) p.mean[row] = mean;
+      if (p.rstd) p.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+      if (c >= p.cols) continue;
+      float ww[V], bb[V];
+      if (w) load_weights<W, V>(w, c, p.vec_w, ww);
+      if (b) load_weights<W, V>(b, c, p.vec_b, bb);
+      RowVec<T, V> out;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        out.e[i] = from_acc<T>(fmaf(v[g][i] * rstd, w ? ww[i] : 1.f, b ? bb[i] : 0.f));
+      store_vec<T, V>(y + row * p.ldy + c, out);
+    }
+  }
+  grid_launch_dependents();
+}
+
+template <typename T, typename W, int V, int NV, bool WARP, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  extern __shared__ float warp_part[];  // WARP: [warps][2][32 V NV]
+  int parity = 0;
+  const int G = WARP ? 32 : static_cast<int>(blockDim.x);
+  const int t = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
+  const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = WARP ? gridDim.x * static_cast<int64_t>(blockDim.x >> 5) : gridDim.x;
+  const float inv = 1.f / static_cast<float>(p.cols);
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  T* dx = static_cast<T*>(p.dx);
+  const W* w = static_cast<const W*>(p.w);
+  float aw[NV][V] = {}, ab[NV][V] = {};
+  grid_dependency_wait();
+  RowVec<T, V> nx[NV], ng[NV];
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= p.rows) return;
+    nmean = p.mean[row];
+    nrstd = p.rstd[row];
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+      if (c < p.cols) {
+        nx[g] = load_vec<T, V>(x + row * p.ldx + c);
+        ng[g] = load_vec<T, V>(dy + row * p.lddy + c);
+      }
+    }
+  };
+  fetch(first);
+  for (int64_t row = first; row < p.rows; row += step) {
+    const float mean = nmean, rstd = nrstd;
+    float h[NV][V], d[NV][V];  // normalised x; dy, then dy w
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+      if (c < p.cols) {
+        float ww[V];
+        if (w) load_weights<W, V>(w, c, p.vec_w, ww);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          h[g][i] = (to_acc<T>(nx[g].e[i]) - mean) * rstd;
+          d[g][i] = to_acc<T>(ng[g].e[i]);
+          aw[g][i] = fmaf(d[g][i], h[g][i], aw[g][i]);
+          ab[g][i] += d[g][i];
+          if (w) d[g][i] *= ww[i];
+          s0 += d[g][i];
+          s1 = fmaf(d[g][i], h[g][i], s1);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[g][i] = d[g][i] = 0.f;
+      }
+    }
+    fetch(row + step);
+    if (dx) {
+      const float2 sum = row_sum<WARP>(s0, s1, buf, parity);
+      const float a0 = sum.x * inv, a1 = sum.y * inv;
+#pragma unroll
+      for (int g = 0; g < NV; ++g) {
+        const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+        if (c >= p.cols) continue;
+        RowVec<T, V> out;
+#pragma unroll
+        for (int i = 0; i < V; ++i) out.e[i] = from_acc<T>(rstd * (d[g][i] - a0 - h[g][i] * a1));
+        store_vec<T, V>(dx + row * p.lddx + c, out);
+      }
+    }
+  }
+  if (p.partial) {
+    float* out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
+    if constexpr (WARP) {
+      // Add the warps' sums in warp order.
+      constexpr int COLS = 32 * V * NV;
+      const int warps = static_cast<int>(blockDim.x >> 5);
+      float* mine = warp_part + static_cast<int>(threadIdx.x >> 5) * 2 * COLS;
+#pragma unroll
+      for (int g = 0; g < NV; ++g)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          mine[V * (t + 32 * g) + i] = aw[g][i];
+          mine[COLS + V * (t + 32 * g) + i] = ab[g][i];
+        }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 2 * COLS; e += static_cast<int>(blockDim.x)) {
+        const int c = e % COLS, which = e / COLS;
+        if (c >= p.cols) continue;
+        float s = 0.f;
+        for (int i = 0; i < warps; ++i) s += warp_part[i * 2 * COLS + e];
+        out[which * p.cols + c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NV; ++g) {
+        const int64_t c = static_cast<int64_t>(V) * (t + G * g);
+        if (c >= p.cols) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          out[c + i] = aw[g][i];
+          out[p.cols + c + i] = ab[g][i];
+        }
+      }
+    }
+  }
+  grid_launch_dependents();
 }
 
 // ------------------------------------------------ any size, stride and alignment
@@ -133,31 +386,109 @@ __global__ void __launch_bounds__(256) layer_norm_dw_any(const NormParams p) {
   }
 }
 
-// Adds the partial sums in ascending order and rounds once.
+// Adds the CTAs' partial sums: 32 columns of one of the two sums per CTA,
+// every eighth partial per warp, then the eight warps' sums in order; one
+// rounding.
 template <typename W>
 __global__ void __launch_bounds__(256) layer_norm_dw_finish(const NormParams p) {
-  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
-  if (c >= p.cols) return;
-  float aw = 0.f, ab = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float* in = p.partial + (static_cast<int64_t>(s) * 2) * p.cols;
-    aw += in[c];
-    ab += in[p.cols + c];
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t strips = (p.cols + 31) / 32;
+  const bool second = blockIdx.x >= strips;
+  const int64_t c = (blockIdx.x - (second ? strips : 0)) * 32 + lane;
+  void* out = second ? p.db : p.dw;
+  if (!out) return;
+  grid_dependency_wait();
+  float s = 0.f;
+  if (c < p.cols) {
+    const float* in = p.partial + (second ? p.cols : 0) + c;
+#pragma unroll 4
+    for (int i = warp; i < p.splits; i += 8) s += in[static_cast<int64_t>(i) * 2 * p.cols];
   }
-  if (p.dw) static_cast<W*>(p.dw)[c] = from_acc<W>(aw);
-  if (p.db) static_cast<W*>(p.db)[c] = from_acc<W>(ab);
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < p.cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][lane];
+    static_cast<W*>(out)[c] = from_acc<W>(s);
+  }
 }
 
-// Shares of the rows that the column sums are split into.
-int norm_splits(int64_t rows, int64_t cols) {
-  const int64_t strips = (cols + 31) / 32;
-  const int64_t want = (static_cast<int64_t>(device_sm_count()) * 8 + strips - 1) / strips;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (rows + 31) / 32, 256})));
+// How a call runs: rows in registers (a warp or a CTA per row, 16-byte groups
+// or single elements), or the kernels for any size.
+struct NormPlan {
+  bool rows, warp;
+  bool vec;
+  int nv;       // groups per thread
+  int threads;  // per CTA
+  int64_t ctas;
+  int partials;  // backward: partial sums per column
+};
+
+bool norm_aligned(const void* p, int64_t ld, size_t es) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && static_cast<size_t>(ld) * es % 16 == 0;
+}
+
+NormPlan norm_forward_plan(const cuopx_layer_norm_args& a) {
+  NormPlan q = {};
+  const size_t es = dtype_size(a.dtype);
+  const int v = static_cast<int>(16 / es);
+  const int64_t sms = device_sm_count();
+  q.vec = a.cols % v == 0 && norm_aligned(a.X, a.ldx, es) && norm_aligned(a.Y, a.ldy, es);
+  const int per = q.vec ? v : 1;
+  const int64_t warp_max = 32ll * (q.vec ? 4 * v : 16);
+  if (a.cols <= warp_max && a.rows > sms) {
+    q.rows = q.warp = true;
+    q.nv = q.vec ? 4 : 16;
+    q.threads = 256;
+    q.ctas = std::min<int64_t>((a.rows + 7) / 8, sms * 8);
+    return q;
+  }
+  // Few rows: as many threads per row as there are groups, for the shortest
+  // chain of loads; many rows: several groups per thread, several rows per SM.
+  const int small = q.vec ? 1 : 4, large = q.vec ? 4 : 16;
+  q.nv = a.rows <= 2 * sms && a.cols <= 1024ll * per * small ? small : large;
+  const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
+  q.threads = static_cast<int>((t + 31) / 32 * 32);
+  q.rows = q.threads <= (q.nv == large ? 512 : 1024);
+  q.ctas = std::min<int64_t>(a.rows, sms * std::max(1, 2048 / std::max(q.threads, 128)));
+  return q;
+}
+
+NormPlan norm_backward_plan(const cuopx_layer_norm_args& a) {
+  NormPlan q = {};
+  const size_t es = dtype_size(a.dtype);
+  const int v = static_cast<int>(16 / es);
+  const int64_t sms = device_sm_count();
+  q.vec = a.cols % v == 0 && norm_aligned(a.X, a.ldx, es) && norm_aligned(a.dY, a.lddy, es) &&
+          (!a.dX || norm_aligned(a.dX, a.lddx, es));
+  const int per = q.vec ? v : 1;
+  const int64_t warp_max = 32ll * (q.vec ? 4 * v : 16);
+  if (a.cols <= warp_max) {
+    q.rows = q.warp = true;
+    q.nv = q.vec ? 4 : 16;
+    q.threads = 256;
+    q.ctas = std::min<int64_t>((a.rows + 7) / 8, sms * 2);
+  } else {
+    q.nv = q.vec ? (es == 4 ? 4 : 2) : 16;
+    const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
+    q.threads = static_cast<int>((t + 31) / 32 * 32);
+    q.rows = t <= 1024;
+    q.ctas = std::min<int64_t>(a.rows, sms * std::max<int64_t>(1, 512 / std::max(q.threads, 64)));
+  }
+  if (!q.rows) {
+    // Shares of the rows for the column sums of the any-size kernel.
+    const int64_t strips = (a.cols + 31) / 32;
+    q.partials = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(sms * 8 + strips - 1) / strips, (a.rows + 31) / 32, 256})));
+  } else {
+    q.partials = static_cast<int>(q.ctas);
+  }
+  return q;
 }
 
 size_t norm_backward_workspace(const cuopx_layer_norm_args& a) {
-  if (a.rows <= 0 || a.cols <= 0 || (!a.dweight && !a.dbias)) return 0;
-  return static_cast<size_t>(norm_splits(a.rows, a.cols)) * 2 * static_cast<size_t>(a.cols) * sizeof(float);
+  if (a.rows <= 0 || a.cols <= 0 || (!a.dweight && !a.dbias) || dtype_size(a.dtype) == 0) return 0;
+  return static_cast<size_t>(norm_backward_plan(a).partials) * 2 * static_cast<size_t>(a.cols) * sizeof(float);
 }
 
 int norm_types_ok(const cuopx_layer_norm_args& a) {
@@ -184,6 +515,8 @@ NormParams norm_params(const cuopx_layer_norm_args& a) {
   p.ldx = a.ldx;
   p.w = a.weight;
   p.b = a.bias;
+  p.vec_w = reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
+  p.vec_b = reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
   p.y = a.Y;
   p.ldy = a.ldy;
   p.mean = a.mean;
@@ -220,6 +553,27 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
       if (overlaps(outs[i], outb[i], outs[j], outb[j])) return CUOPX_INVALID_ARGUMENT;
   }
   const NormParams p = norm_params(*a);
+  const NormPlan q = norm_forward_plan(*a);
+  if (q.rows) {
+    cudaError_t e = cudaSuccess;
+    with_norm_types(*a, [&](auto t, auto w) {
+      using T = decltype(t);
+      using W = decltype(w);
+      constexpr int V = 16 / static_cast<int>(sizeof(T));
+      auto go = [&](auto kern) {
+        e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), 0, stream, p);
+      };
+      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256>) : go(layer_norm_rows<T, W, 1, 16, true, 256>);
+      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024>) : go(layer_norm_rows<T, W, V, 4, false, 512>);
+      else q.nv == 4 ? go(layer_norm_rows<T, W, 1, 4, false, 1024>) : go(layer_norm_rows<T, W, 1, 16, false, 512>);
+    });
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_failure(e);
+    }
+    note_launch("layer_norm_rows");
+    return check_launch();
+  }
   with_norm_types(*a, [&](auto t, auto w) {
     layer_norm_any<decltype(t), decltype(w)><<<norm_row_ctas(p.rows), 256, 0, stream>>>(p);
   });
@@ -258,22 +612,47 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
     if (a->dbias && cudaMemsetAsync(a->dbias, 0, wb, stream) != cudaSuccess) return cuda_failure(cudaGetLastError());
     return CUOPX_SUCCESS;
   }
-  if (p.dw || p.db) {  // before dX, which may overwrite dY
-    p.partial = static_cast<float*>(a->workspace);
-    p.splits = norm_splits(p.rows, p.cols);
-    const dim3 grid(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(p.splits));
-    with_norm_types(*a, [&](auto t, auto w) {
-      layer_norm_dw_any<decltype(t)><<<grid, 256, 0, stream>>>(p);
-      note_launch("layer_norm_dw_any");
-      layer_norm_dw_finish<decltype(w)><<<static_cast<unsigned>((p.cols + 255) / 256), 256, 0, stream>>>(p);
+  const NormPlan q = norm_backward_plan(*a);
+  const bool sums = p.dw || p.db;
+  p.splits = q.partials;
+  if (sums) p.partial = static_cast<float*>(a->workspace);
+  cudaError_t e = cudaSuccess;
+  with_norm_types(*a, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    constexpr int NV = sizeof(T) == 4 ? 4 : 2;
+    if (q.rows) {
+      auto go = [&](auto kern, int cols) {
+        const size_t smem = q.warp ? static_cast<size_t>(q.threads / 32) * 2 * cols * sizeof(float) : 0;
+        if (smem > 48 * 1024)
+          e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e == cudaSuccess)
+          e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p);
+        note_launch("layer_norm_backward_rows");
+      };
+      if (q.warp) q.vec ? go(layer_norm_backward_rows<T, W, V, 4, true, 256>, 32 * V * 4) : go(layer_norm_backward_rows<T, W, 1, 16, true, 256>, 32 * 16);
+      else if (q.vec) q.threads <= 512 ? go(layer_norm_backward_rows<T, W, V, NV, false, 512>, 0) : go(layer_norm_backward_rows<T, W, V, NV, false, 1024>, 0);
+      else q.threads <= 512 ? go(layer_norm_backward_rows<T, W, 1, 16, false, 512>, 0) : go(layer_norm_backward_rows<T, W, 1, 16, false, 1024>, 0);
+    } else {
+      if (sums) {  // before dX, which may overwrite dY
+        layer_norm_dw_any<T><<<dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(q.partials)), 256, 0, stream>>>(p);
+        note_launch("layer_norm_dw_any");
+      }
+      if (p.dx) {
+        layer_norm_dx_any<T, W><<<norm_row_ctas(p.rows), 256, 0, stream>>>(p);
+        note_launch("layer_norm_dx_any");
+      }
+    }
+    if (e == cudaSuccess && sums) {
+      const unsigned strips = static_cast<unsigned>((p.cols + 31) / 32);
+      e = launch_pdl(layer_norm_dw_finish<W>, dim3(2 * strips), dim3(256), 0, stream, p);
       note_launch("layer_norm_dw_finish");
-    });
-  }
-  if (p.dx) {
-    with_norm_types(*a, [&](auto t, auto w) {
-      layer_norm_dx_any<decltype(t), decltype(w)><<<norm_row_ctas(p.rows), 256, 0, stream>>>(p);
-    });
-    note_launch("layer_norm_dx_any");
+    }
+  });
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_failure(e);
   }
   return check_launch();
 }
