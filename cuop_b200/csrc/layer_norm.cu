@@ -127,8 +127,12 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*buf)[32], i
   return make_float2(a, b);
 }
 
-template <typename T, typename W, int V, int NV, bool WARP, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) layer_norm_rows(const NormParams p) {
+// Forward.  The row stays packed (16 registers for NV = 4 groups of 16 bytes)
+// and is widened three times, for the mean, the squares and the result: few
+// registers, so that enough rows are in flight per SM to cover the latency of
+// HBM without prefetching.
+template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS>
+__global__ void __launch_bounds__(MAXT, CTAS) layer_norm_rows(const NormParams p) {
   __shared__ float2 buf[2][32];
   int parity = 0;
   const int G = WARP ? 32 : static_cast<int>(blockDim.x);
@@ -136,44 +140,31 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_rows(const NormParams p) {
   const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? gridDim.x * static_cast<int64_t>(blockDim.x >> 5) : gridDim.x;
   const float inv = 1.f / static_cast<float>(p.cols);
-  const T* x = static_cast<const T*>(p.x);
-  T* y = static_cast<T*>(p.y);
-  const W* w = static_cast<const W*>(p.w);
-  const W* b = static_cast<const W*>(p.b);
+  const int cols = static_cast<int>(p.cols);
   grid_dependency_wait();
-  RowVec<T, V> next[NV];
-  auto fetch = [&](int64_t row) {
-#pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-      if (row < p.rows && c < p.cols) next[g] = load_vec<T, V>(x + row * p.ldx + c);
-    }
-  };
-  fetch(first);
   for (int64_t row = first; row < p.rows; row += step) {
-    float v[NV][V];
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    T* y = static_cast<T*>(p.y) + row * p.ldy;
+    RowVec<T, V> v[NV];
+#pragma unroll
+    for (int g = 0; g < NV; ++g)
+      if (V * (t + G * g) < cols) v[g] = load_vec<T, V>(x + V * (t + G * g));
     float s = 0.f;
 #pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      const bool in = static_cast<int64_t>(V) * (t + G * g) < p.cols;
+    for (int g = 0; g < NV; ++g)
+      if (V * (t + G * g) < cols)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[g][i] = in ? to_acc<T>(next[g].e[i]) : 0.f;
-        s += v[g][i];
-      }
-    }
-    fetch(row + step);
+        for (int i = 0; i < V; ++i) s += to_acc<T>(v[g].e[i]);
     const float mean = row_sum<WARP>(s, 0.f, buf, parity).x * inv;
     float q = 0.f;
 #pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      const bool in = static_cast<int64_t>(V) * (t + G * g) < p.cols;
+    for (int g = 0; g < NV; ++g)
+      if (V * (t + G * g) < cols)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[g][i] -= mean;
-        if (in) q = fmaf(v[g][i], v[g][i], q);
-      }
-    }
+        for (int i = 0; i < V; ++i) {
+          const float d = to_acc<T>(v[g].e[i]) - mean;
+          q = fmaf(d, d, q);
+        }
     const float rstd = 1.f / sqrtf(fmaf(row_sum<WARP>(q, 0.f, buf, parity).x, inv, p.eps));
     if (t == 0) {
       if (p.mean) p.mean[row] = mean;
@@ -181,16 +172,21 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_rows(const NormParams p) {
     }
 #pragma unroll
     for (int g = 0; g < NV; ++g) {
-      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-      if (c >= p.cols) continue;
-      float ww[V], bb[V];
-      if (w) load_weights<W, V>(w, c, p.vec_w, ww);
-      if (b) load_weights<W, V>(b, c, p.vec_b, bb);
+      const int c = V * (t + G * g);
+      if (c >= cols) continue;
+      float f[V], u[V];
+      if (p.w) load_weights<W, V>(static_cast<const W*>(p.w), c, p.vec_w, f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = (to_acc<T>(v[g].e[i]) - mean) * rstd * (p.w ? f[i] : 1.f);
+      if (p.b) {
+        load_weights<W, V>(static_cast<const W*>(p.b), c, p.vec_b, u);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] += u[i];
+      }
       RowVec<T, V> out;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        out.e[i] = from_acc<T>(fmaf(v[g][i] * rstd, w ? ww[i] : 1.f, b ? bb[i] : 0.f));
-      store_vec<T, V>(y + row * p.ldy + c, out);
+      for (int i = 0; i < V; ++i) out.e[i] = from_acc<T>(f[i]);
+      store_vec<T, V>(y + c, out);
     }
   }
   grid_launch_dependents();
@@ -295,10 +291,15 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
       for (int g = 0; g < NV; ++g) {
         const int64_t c = static_cast<int64_t>(V) * (t + G * g);
         if (c >= p.cols) continue;
+        if constexpr (V % 4 == 0) {  // cols is a multiple of V: 16-byte boundaries
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          out[c + i] = aw[g][i];
-          out[p.cols + c + i] = ab[g][i];
+          for (int i = 0; i < V; i += 4) {
+            *reinterpret_cast<float4*>(out + c + i) = make_float4(aw[g][i], aw[g][i + 1], aw[g][i + 2], aw[g][i + 3]);
+            *reinterpret_cast<float4*>(out + p.cols + c + i) = make_float4(ab[g][i], ab[g][i + 1], ab[g][i + 2], ab[g][i + 3]);
+          }
+        } else {
+          out[c] = aw[g][0];
+          out[p.cols + c] = ab[g][0];
         }
       }
     }
@@ -441,7 +442,7 @@ NormPlan norm_forward_plan(const cuopx_layer_norm_args& a) {
     q.rows = q.warp = true;
     q.nv = q.vec ? 4 : 16;
     q.threads = 256;
-    q.ctas = std::min<int64_t>((a.rows + 7) / 8, sms * 8);
+    q.ctas = std::min<int64_t>((a.rows + 7) / 8, int64_t(1) << 30);
     return q;
   }
   // Few rows: as many threads per row as there are groups, for the shortest
@@ -451,7 +452,7 @@ NormPlan norm_forward_plan(const cuopx_layer_norm_args& a) {
   const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
   q.threads = static_cast<int>((t + 31) / 32 * 32);
   q.rows = q.threads <= (q.nv == large ? 512 : 1024);
-  q.ctas = std::min<int64_t>(a.rows, sms * std::max(1, 2048 / std::max(q.threads, 128)));
+  q.ctas = std::min<int64_t>(a.rows, int64_t(1) << 30);
   return q;
 }
 
@@ -563,9 +564,9 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
       auto go = [&](auto kern) {
         e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), 0, stream, p);
       };
-      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256>) : go(layer_norm_rows<T, W, 1, 16, true, 256>);
-      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024>) : go(layer_norm_rows<T, W, V, 4, false, 512>);
-      else q.nv == 4 ? go(layer_norm_rows<T, W, 1, 4, false, 1024>) : go(layer_norm_rows<T, W, 1, 16, false, 512>);
+      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256, 4>) : go(layer_norm_rows<T, W, 1, 16, true, 256, 4>);
+      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024, 1>) : go(layer_norm_rows<T, W, V, 4, false, 512, 2>);
+      else q.nv == 4 ? go(layer_norm_rows<T, W, 1, 4, false, 1024, 1>) : go(layer_norm_rows<T, W, 1, 16, false, 512, 2>);
     });
     if (e != cudaSuccess) {
       cudaGetLastError();
