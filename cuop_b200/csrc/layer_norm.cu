@@ -10,15 +10,17 @@
 // the mean is large.  All sums are fp32, in an order fixed by the launch
 // shape, without atomics, so results do not change from run to run.
 //
-// Bound by HBM: every element is read once and written once.  A row stays in
-// the registers of its threads (a warp, or a whole CTA) between the sums and
-// the result, and the loads of the next row are issued before the sums of the
-// current one are exchanged.  The backward kernel reads x and dy once for all
-// three gradients: a thread keeps the same columns for all rows of its CTA and
-// their two column sums in registers; one partial sum per CTA and column goes
-// to the workspace, and a second small kernel adds those in CTA order.
+// Bound by HBM: every element is read once and written once.  Persistent
+// groups of threads (a warp, or a CTA, per row) stream rows through a ring of
+// shared-memory stages filled by bulk copies, so that what is in flight does
+// not cost registers; a row stays packed in its threads' registers between
+// the sums and the result.  The backward kernel reads x and dy once for all
+// three gradients: a thread keeps the same columns for all rows of its group
+// and their two column sums in registers; one partial sum per CTA and column
+// goes to the workspace, and a second small kernel adds those in CTA order.
 #include "common.cuh"
 #include "dispatch.h"
+#include "layer_epilogue.cuh"
 
 namespace cuopx {
 
@@ -44,6 +46,60 @@ struct NormParams {
   void* db;
   float* partial;  // [splits][2][cols]: sums of dy h, then of dy
   int splits;
+};
+
+// ------------------------------------------------ ring of rows in shared memory
+// One bulk copy of `bytes` (a multiple of 16, both addresses on 16-byte
+// boundaries) from global to this CTA's shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The rows first, first + step, ... of up to two matrices, each stage one row
+// of every matrix.  A group's leader thread issues the copies; every thread
+// waits for a stage, and the stage is filled again once the whole group has
+// read it (which the caller orders).
+template <int NSRC>
+struct RowRing {
+  unsigned char* base;  // [stages][NSRC][bytes]
+  uint64_t* full;       // [stages]
+  int stages;
+  uint32_t bytes;
+  const unsigned char* src[NSRC];
+  int64_t pitch[NSRC];  // bytes from row to row
+  int64_t rows, step;
+  volatile int* abort;
+
+  __device__ __forceinline__ void fill(int stage, int64_t row) const {
+    mbar_arrive_expect_tx(&full[stage], NSRC * bytes);
+#pragma unroll
+    for (int i = 0; i < NSRC; ++i) bulk_load(base + (stage * NSRC + i) * bytes, src[i] + row * pitch[i], bytes, &full[stage]);
+  }
+  // Fills the first stages; the number filled.
+  __device__ __forceinline__ int64_t start(int64_t first) const {
+    int s = 0;
+    for (; s < stages && first + s * step < rows; ++s) fill(s, first + s * step);
+    return s;
+  }
+  // After a timeout (recorded): let the copies in flight land, with a limit of their own.
+  __device__ __forceinline__ void drain(int64_t filled) const {
+    for (int s = 0; s < stages && s < filled; ++s) {
+      const uint32_t parity = static_cast<uint32_t>((filled - s + stages - 1) / stages - 1) & 1u;
+      const unsigned long long t0 = global_timer_ns();
+      while (!mbar_try_wait(smem_u32(&full[s]), parity)) {
+        if (global_timer_ns() - t0 > kWaitLimitNs) {
+          record_device_error(kDevErrAbortDrain);
+          break;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ bool wait(int stage, uint32_t phase) const {
+    return mbar_wait_bounded(&full[stage], phase, kDevErrWaitTimeoutFull, abort);
+  }
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -89,6 +145,51 @@ __device__ __forceinline__ void store_vec(T* p, const RowVec<T, V>& r) {
   else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
+// Two fp32 operations per instruction (sm_100's packed f32x2 forms, each half
+// rounded like the scalar one): at 16 bits an element HBM leaves about 22
+// issue slots per element forward and 32 backward, and conversions take most.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Elements 2i and 2i + 1 of a group widened, and two results rounded into it.
+template <typename T, int V>
+__device__ __forceinline__ float2 widen2(const RowVec<T, V>& r, int i) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    return unpack2_layer<T>(reinterpret_cast<const uint32_t*>(&r)[i]);
+  } else {
+    return make_float2(to_acc<T>(r.e[2 * i]), to_acc<T>(r.e[2 * i + 1]));
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void round2(RowVec<T, V>& r, int i, float2 v) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    reinterpret_cast<uint32_t*>(&r)[i] = pack2_layer<T>(v.x, v.y);
+  } else {
+    r.e[2 * i] = from_acc<T>(v.x);
+    r.e[2 * i + 1] = from_acc<T>(v.y);
+  }
+}
+
 // V weights from column c on, in 16-byte loads where `vec` says that they start on such a boundary.
 template <typename W, int V>
 __device__ __forceinline__ void load_weights(const W* w, int64_t c, bool vec, float (&out)[V]) {
@@ -99,13 +200,26 @@ __device__ __forceinline__ void load_weights(const W* w, int64_t c, bool vec, fl
       for (int j = 0; j < V / E; ++j) {
         const RowVec<W, E> r = load_vec<W, E>(w + c + j * E);
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[j * E + i] = to_acc<W>(r.e[i]);
+        for (int i = 0; i < E / 2; ++i) {
+          const float2 f = widen2<W, E>(r, i);
+          out[j * E + 2 * i] = f.x;
+          out[j * E + 2 * i + 1] = f.y;
+        }
       }
       return;
     }
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) out[i] = to_acc<W>(w[c + i]);
+}
+
+// V weights from column c on, as pairs.
+template <typename W, int V>
+__device__ __forceinline__ void load_weights2(const W* w, int64_t c, bool vec, float2 (&out)[V / 2]) {
+  float f[V];
+  load_weights<W, V>(w, c, vec, f);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) out[i] = make_float2(f[2 * i], f[2 * i + 1]);
 }
 
 // Sums of two values over the threads of a row: the warp, or the CTA through
@@ -127,10 +241,114 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*buf)[32], i
   return make_float2(a, b);
 }
 
-// Forward.  The row stays packed (16 registers for NV = 4 groups of 16 bytes)
-// and is widened three times, for the mean, the squares and the result: few
-// registers, so that enough rows are in flight per SM to cover the latency of
-// HBM without prefetching.
+template <bool WARP>
+__device__ __forceinline__ float row_sum1(float a, float2 (*buf)[32], int& parity) {
+  a = warp_sum(a);
+  if constexpr (!WARP) {
+    if ((threadIdx.x & 31) == 0) buf[parity][threadIdx.x >> 5].x = a;
+    __syncthreads();
+    const int warps = static_cast<int>(blockDim.x) >> 5;
+    a = warp_sum((threadIdx.x & 31) < warps ? buf[parity][threadIdx.x & 31].x : 0.f);
+    parity ^= 1;
+  }
+  return a;
+}
+
+// Statistics and result of one row of 16-byte groups, widened once.
+template <typename T, typename W, int V, int NV, bool WARP>
+__device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, const RowVec<T, V> (&raw)[NV], int t, int G,
+                                             float2 (*buf)[32], int& parity) {
+  const int cols = static_cast<int>(p.cols);
+  const float inv = 1.f / static_cast<float>(cols);
+  T* y = static_cast<T*>(p.y) + row * p.ldy;
+  float2 v[NV][V / 2];
+  float2 s = both(0.f);
+#pragma unroll
+  for (int g = 0; g < NV; ++g)
+    if (V * (t + G * g) < cols)
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        v[g][i] = widen2<T, V>(raw[g], i);
+        s = add2(s, v[g][i]);
+      }
+  const float mean = row_sum1<WARP>(s.x + s.y, buf, parity) * inv;
+  float2 q = both(0.f);
+#pragma unroll
+  for (int g = 0; g < NV; ++g)
+    if (V * (t + G * g) < cols)
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        v[g][i] = add2(v[g][i], both(-mean));
+        q = fma2(v[g][i], v[g][i], q);
+      }
+  const float rstd = 1.f / sqrtf(fmaf(row_sum1<WARP>(q.x + q.y, buf, parity), inv, p.eps));
+  if (t == 0) {
+    if (p.mean) p.mean[row] = mean;
+    if (p.rstd) p.rstd[row] = rstd;
+  }
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+    const int c = V * (t + G * g);
+    if (c >= cols) continue;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) v[g][i] = mul2(v[g][i], both(rstd));
+    if (p.w) {
+      float2 w[V / 2], b[V / 2];
+      load_weights2<W, V>(static_cast<const W*>(p.w), c, p.vec_w, w);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) b[i] = both(0.f);
+      if (p.b) load_weights2<W, V>(static_cast<const W*>(p.b), c, p.vec_b, b);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) v[g][i] = fma2(v[g][i], w[i], b[i]);
+    } else if (p.b) {
+      float2 b[V / 2];
+      load_weights2<W, V>(static_cast<const W*>(p.b), c, p.vec_b, b);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) v[g][i] = add2(v[g][i], b[i]);
+    }
+    RowVec<T, V> out;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) round2<T, V>(out, i, v[g][i]);
+    store_vec<T, V>(y + c, out);
+  }
+}
+
+// The same for rows that are not 16-byte aligned: single elements.
+template <typename T, typename W, int NV, bool WARP>
+__device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, const RowVec<T, 1> (&raw)[NV], int t, int G,
+                                             float2 (*buf)[32], int& parity) {
+  const int cols = static_cast<int>(p.cols);
+  const float inv = 1.f / static_cast<float>(cols);
+  float v[NV], s = 0.f, q = 0.f;
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+    v[g] = t + G * g < cols ? to_acc<T>(raw[g].e[0]) : 0.f;
+    s += v[g];
+  }
+  const float mean = row_sum1<WARP>(s, buf, parity) * inv;
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+    v[g] -= mean;
+    if (t + G * g < cols) q = fmaf(v[g], v[g], q);
+  }
+  const float rstd = 1.f / sqrtf(fmaf(row_sum1<WARP>(q, buf, parity), inv, p.eps));
+  if (t == 0) {
+    if (p.mean) p.mean[row] = mean;
+    if (p.rstd) p.rstd[row] = rstd;
+  }
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+    const int c = t + G * g;
+    if (c >= cols) continue;
+    const float w = p.w ? to_acc<W>(static_cast<const W*>(p.w)[c]) : 1.f;
+    const float b = p.b ? to_acc<W>(static_cast<const W*>(p.b)[c]) : 0.f;
+    static_cast<T*>(p.y)[row * p.ldy + c] = from_acc<T>(fmaf(v[g] * rstd, w, b));
+  }
+}
+
+// Forward: rows loaded straight into registers.  A ring of rows in shared
+// memory, as the backward kernel has it, measured slower here (8192 x 8192
+// bf16: 80 against 68 us): with few registers enough rows are in flight.
 template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS>
 __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_rows(const NormParams p) {
   __shared__ float2 buf[2][32];
@@ -139,55 +357,15 @@ __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_rows(const NormParams p
   const int t = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
   const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? gridDim.x * static_cast<int64_t>(blockDim.x >> 5) : gridDim.x;
-  const float inv = 1.f / static_cast<float>(p.cols);
-  const int cols = static_cast<int>(p.cols);
   grid_dependency_wait();
   for (int64_t row = first; row < p.rows; row += step) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    T* y = static_cast<T*>(p.y) + row * p.ldy;
     RowVec<T, V> v[NV];
 #pragma unroll
     for (int g = 0; g < NV; ++g)
-      if (V * (t + G * g) < cols) v[g] = load_vec<T, V>(x + V * (t + G * g));
-    float s = 0.f;
-#pragma unroll
-    for (int g = 0; g < NV; ++g)
-      if (V * (t + G * g) < cols)
-#pragma unroll
-        for (int i = 0; i < V; ++i) s += to_acc<T>(v[g].e[i]);
-    const float mean = row_sum<WARP>(s, 0.f, buf, parity).x * inv;
-    float q = 0.f;
-#pragma unroll
-    for (int g = 0; g < NV; ++g)
-      if (V * (t + G * g) < cols)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = to_acc<T>(v[g].e[i]) - mean;
-          q = fmaf(d, d, q);
-        }
-    const float rstd = 1.f / sqrtf(fmaf(row_sum<WARP>(q, 0.f, buf, parity).x, inv, p.eps));
-    if (t == 0) {
-      if (p.mean) p.mean[row] = mean;
-      if (p.rstd) p.rstd[row] = rstd;
-    }
-#pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      const int c = V * (t + G * g);
-      if (c >= cols) continue;
-      float f[V], u[V];
-      if (p.w) load_weights<W, V>(static_cast<const W*>(p.w), c, p.vec_w, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = (to_acc<T>(v[g].e[i]) - mean) * rstd * (p.w ? f[i] : 1.f);
-      if (p.b) {
-        load_weights<W, V>(static_cast<const W*>(p.b), c, p.vec_b, u);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] += u[i];
-      }
-      RowVec<T, V> out;
-#pragma unroll
-      for (int i = 0; i < V; ++i) out.e[i] = from_acc<T>(f[i]);
-      store_vec<T, V>(y + c, out);
-    }
+      if (V * (t + G * g) < p.cols) v[g] = load_vec<T, V>(x + V * (t + G * g));
+    if constexpr (V == 1) norm_one_row<T, W, NV, WARP>(p, row, v, t, G, buf, parity);
+    else norm_one_row<T, W, V, NV, WARP>(p, row, v, t, G, buf, parity);
   }
   grid_launch_dependents();
 }
@@ -300,6 +478,149 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
         } else {
           out[c] = aw[g][0];
           out[p.cols + c] = ab[g][0];
+        }
+      }
+    }
+  }
+  grid_launch_dependents();
+}
+
+// The same for rows on 16-byte boundaries, through the ring.  WARP: eight
+// rings per CTA, one per warp.
+template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS>
+__global__ void __launch_bounds__(MAXT, CTAS) layer_norm_backward_ring(const NormParams p, int stages) {
+  extern __shared__ __align__(128) unsigned char ring_smem[];  // rings; WARP: afterwards [warps][2][32 V NV] sums
+  __shared__ float2 buf[2][32];
+  __shared__ uint64_t full[8 * 8];
+  __shared__ int abort_flag;
+  int parity = 0;
+  const int G = WARP ? 32 : static_cast<int>(blockDim.x);
+  const int t = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
+  const int group = WARP ? static_cast<int>(threadIdx.x >> 5) : 0;
+  const int groups = WARP ? static_cast<int>(blockDim.x >> 5) : 1;
+  const int64_t first = blockIdx.x * static_cast<int64_t>(groups) + group;
+  const int64_t step = gridDim.x * static_cast<int64_t>(groups);
+  const int cols = static_cast<int>(p.cols);
+  const float inv = 1.f / static_cast<float>(cols);
+  RowRing<2> ring;
+  ring.bytes = static_cast<uint32_t>(p.cols * static_cast<int64_t>(sizeof(T)));
+  ring.base = ring_smem + static_cast<size_t>(group) * stages * 2 * ring.bytes;
+  ring.full = full + group * stages;
+  ring.stages = stages;
+  ring.src[0] = static_cast<const unsigned char*>(p.x);
+  ring.src[1] = static_cast<const unsigned char*>(p.dy);
+  ring.pitch[0] = p.ldx * static_cast<int64_t>(sizeof(T));
+  ring.pitch[1] = p.lddy * static_cast<int64_t>(sizeof(T));
+  ring.rows = p.rows;
+  ring.step = step;
+  ring.abort = &abort_flag;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < groups * stages; ++s) mbar_init(&full[s], 1);
+    abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  int64_t filled = t == 0 ? ring.start(first) : 0;
+  float2 aw[NV][V / 2], ab[NV][V / 2], ww[NV][V / 2];
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) aw[g][i] = ab[g][i] = both(0.f), ww[g][i] = both(1.f);
+    if (p.w && V * (t + G * g) < cols) load_weights2<W, V>(static_cast<const W*>(p.w), V * (t + G * g), p.vec_w, ww[g]);
+  }
+  float nmean = 0.f, nrstd = 0.f;
+  if (first < p.rows) nmean = p.mean[first], nrstd = p.rstd[first];
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const float mean = nmean, rstd = nrstd;
+    if (row + step < p.rows) nmean = p.mean[row + step], nrstd = p.rstd[row + step];
+    ring.wait(stage, phase);  // after a timeout (recorded) the rest runs through on stale data
+    const T* sx = reinterpret_cast<const T*>(ring.base + stage * 2 * ring.bytes);
+    const T* sg = reinterpret_cast<const T*>(ring.base + (stage * 2 + 1) * ring.bytes);
+    // One group per thread keeps h and u = dy w widened between the sums and
+    // the result; several keep x and dy packed and widen them again.
+    RowVec<T, V> vx[NV], vg[NV];
+    float2 h[V / 2], u[V / 2];
+    float2 s0 = both(0.f), s1 = both(0.f);
+    auto widen = [&](int g, int i, float2& d) {
+      h[i] = mul2(add2(widen2<T, V>(vx[g], i), both(-mean)), both(rstd));
+      d = widen2<T, V>(vg[g], i);
+      u[i] = mul2(d, ww[g][i]);
+    };
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      const int c = V * (t + G * g);
+      if (c >= cols) continue;
+      vx[g] = load_vec<T, V>(sx + c);
+      vg[g] = load_vec<T, V>(sg + c);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        float2 d;
+        widen(g, i, d);
+        aw[g][i] = fma2(d, h[i], aw[g][i]);
+        ab[g][i] = add2(d, ab[g][i]);
+        s0 = add2(s0, u[i]);
+        s1 = fma2(u[i], h[i], s1);
+      }
+    }
+    const float2 sum = row_sum<WARP>(s0.x + s0.y, s1.x + s1.y, buf, parity);  // also: the whole group has read the stage
+    const int64_t ahead = row + stages * step;
+    if (t == 0 && ahead < p.rows && !*ring.abort) ring.fill(stage, ahead), ++filled;
+    if (p.dx) {
+      const float a0 = sum.x * inv, a1 = sum.y * inv;
+      T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+#pragma unroll
+      for (int g = 0; g < NV; ++g) {
+        const int c = V * (t + G * g);
+        if (c >= cols) continue;
+        RowVec<T, V> out;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          float2 d;
+          if constexpr (NV > 1) widen(g, i, d);
+          round2<T, V>(out, i, mul2(both(rstd), fma2(h[i], both(-a1), add2(u[i], both(-a0)))));
+        }
+        store_vec<T, V>(dx + c, out);
+      }
+    }
+    if (++stage == stages) stage = 0, phase ^= 1u;
+  }
+  if (t == 0 && *ring.abort) ring.drain(filled);
+  if (p.partial) {
+    float* out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
+    if constexpr (WARP) {
+      // Add the warps' sums in warp order; every copy has landed and been read.
+      __syncthreads();
+      constexpr int COLS = 32 * V * NV;
+      float* part = reinterpret_cast<float*>(ring_smem);
+      float* mine = part + group * 2 * COLS;
+#pragma unroll
+      for (int g = 0; g < NV; ++g)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          mine[V * (t + 32 * g) + i] = i % 2 ? aw[g][i / 2].y : aw[g][i / 2].x;
+          mine[COLS + V * (t + 32 * g) + i] = i % 2 ? ab[g][i / 2].y : ab[g][i / 2].x;
+        }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 2 * COLS; e += static_cast<int>(blockDim.x)) {
+        const int c = e % COLS, which = e / COLS;
+        if (c >= cols) continue;
+        float s = 0.f;
+        for (int i = 0; i < groups; ++i) s += part[i * 2 * COLS + e];
+        out[which * p.cols + c] = s;
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < NV; ++g) {
+        const int c = V * (t + G * g);
+        if (c >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {  // cols is a multiple of V: 16-byte boundaries
+          const float2 w0 = aw[g][i / 2], w1 = aw[g][i / 2 + 1], b0 = ab[g][i / 2], b1 = ab[g][i / 2 + 1];
+          *reinterpret_cast<float4*>(out + c + i) = make_float4(w0.x, w0.y, w1.x, w1.y);
+          *reinterpret_cast<float4*>(out + p.cols + c + i) = make_float4(b0.x, b0.y, b1.x, b1.y);
         }
       }
     }
@@ -420,6 +741,7 @@ __global__ void __launch_bounds__(256) layer_norm_dw_finish(const NormParams p) 
 struct NormPlan {
   bool rows, warp;
   bool vec;
+  int stages;   // of the ring; 0: no ring
   int nv;       // groups per thread
   int threads;  // per CTA
   int64_t ctas;
@@ -447,11 +769,11 @@ NormPlan norm_forward_plan(const cuopx_layer_norm_args& a) {
   }
   // Few rows: as many threads per row as there are groups, for the shortest
   // chain of loads; many rows: several groups per thread, several rows per SM.
-  const int small = q.vec ? 1 : 4, large = q.vec ? 4 : 16;
+  const int small = q.vec ? 1 : 4, large = q.vec ? 16 / v : 16;
   q.nv = a.rows <= 2 * sms && a.cols <= 1024ll * per * small ? small : large;
   const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
   q.threads = static_cast<int>((t + 31) / 32 * 32);
-  q.rows = q.threads <= (q.nv == large ? 512 : 1024);
+  q.rows = q.threads <= (q.nv == 16 ? 512 : 1024);
   q.ctas = std::min<int64_t>(a.rows, int64_t(1) << 30);
   return q;
 }
@@ -464,18 +786,26 @@ NormPlan norm_backward_plan(const cuopx_layer_norm_args& a) {
   q.vec = a.cols % v == 0 && norm_aligned(a.X, a.ldx, es) && norm_aligned(a.dY, a.lddy, es) &&
           (!a.dX || norm_aligned(a.dX, a.lddx, es));
   const int per = q.vec ? v : 1;
+  const int64_t row_bytes = 2 * a.cols * static_cast<int64_t>(es);  // of x and dy
   const int64_t warp_max = 32ll * (q.vec ? 4 * v : 16);
   if (a.cols <= warp_max) {
     q.rows = q.warp = true;
-    q.nv = q.vec ? 4 : 16;
+    q.nv = q.vec ? (a.cols <= 32 * v ? 1 : 4) : 16;
     q.threads = 256;
-    q.ctas = std::min<int64_t>((a.rows + 7) / 8, sms * 2);
+    const int per_sm = q.nv == 4 ? 1 : 2;
+    q.ctas = std::min<int64_t>((a.rows + 7) / 8, sms * per_sm);
+    if (q.vec) q.stages = static_cast<int>(std::min<int64_t>(8, 200 * 1024 / per_sm / (8 * row_bytes)));
   } else {
-    q.nv = q.vec ? (es == 4 ? 4 : 2) : 16;
+    q.nv = !q.vec ? 16 : a.cols <= 1024 * v ? 1 : 4;
     const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
-    q.threads = static_cast<int>((t + 31) / 32 * 32);
-    q.rows = t <= 1024;
-    q.ctas = std::min<int64_t>(a.rows, sms * std::max<int64_t>(1, 512 / std::max(q.threads, 64)));
+    q.threads = static_cast<int>(std::min<int64_t>(2048, (t + 31) / 32 * 32));
+    q.rows = q.threads <= (q.nv == 1 ? 1024 : 512);
+    const int per_sm = std::max(1, (q.nv == 1 ? 1024 : 512) / q.threads);
+    q.ctas = std::min<int64_t>(a.rows, sms * per_sm);
+    if (q.vec) {
+      q.stages = static_cast<int>(std::min<int64_t>(8, 200 * 1024 / per_sm / row_bytes));
+      if (q.stages < 2) q.rows = false;
+    }
   }
   if (!q.rows) {
     // Shares of the rows for the column sums of the any-size kernel.
@@ -564,8 +894,8 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
       auto go = [&](auto kern) {
         e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), 0, stream, p);
       };
-      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256, 4>) : go(layer_norm_rows<T, W, 1, 16, true, 256, 4>);
-      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024, 1>) : go(layer_norm_rows<T, W, V, 4, false, 512, 2>);
+      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256, 3>) : go(layer_norm_rows<T, W, 1, 16, true, 256, 3>);
+      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024, 1>) : go(layer_norm_rows<T, W, V, 16 / V, false, 1024, 1>);
       else q.nv == 4 ? go(layer_norm_rows<T, W, 1, 4, false, 1024, 1>) : go(layer_norm_rows<T, W, 1, 16, false, 512, 2>);
     });
     if (e != cudaSuccess) {
@@ -623,18 +953,22 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
     using W = decltype(w);
     constexpr int V = 16 / static_cast<int>(sizeof(T));
     constexpr int NV = sizeof(T) == 4 ? 4 : 2;
-    if (q.rows) {
+    if (q.rows && q.vec) {
       auto go = [&](auto kern, int cols) {
-        const size_t smem = q.warp ? static_cast<size_t>(q.threads / 32) * 2 * cols * sizeof(float) : 0;
-        if (smem > 48 * 1024)
-          e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        size_t smem = static_cast<size_t>(q.stages) * 2 * static_cast<size_t>(p.cols) * sizeof(T);
+        if (q.warp) smem = std::max(smem * 8, static_cast<size_t>(8 * 2 * cols) * sizeof(float));
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 211 * 1024);
         if (e == cudaSuccess)
-          e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p);
-        note_launch("layer_norm_backward_rows");
+          e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p, q.stages);
+        note_launch("layer_norm_backward_ring");
       };
-      if (q.warp) q.vec ? go(layer_norm_backward_rows<T, W, V, 4, true, 256>, 32 * V * 4) : go(layer_norm_backward_rows<T, W, 1, 16, true, 256>, 32 * 16);
-      else if (q.vec) q.threads <= 512 ? go(layer_norm_backward_rows<T, W, V, NV, false, 512>, 0) : go(layer_norm_backward_rows<T, W, V, NV, false, 1024>, 0);
-      else q.threads <= 512 ? go(layer_norm_backward_rows<T, W, 1, 16, false, 512>, 0) : go(layer_norm_backward_rows<T, W, 1, 16, false, 1024>, 0);
+      if (q.warp) q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, true, 256, 2>, 32 * V) : go(layer_norm_backward_ring<T, W, V, 4, true, 256, 1>, 32 * V * 4);
+      else q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, false, 1024, 1>, 0) : go(layer_norm_backward_ring<T, W, V, 4, false, 512, 1>, 0);
+    } else if (q.rows) {
+      const size_t smem = q.warp ? static_cast<size_t>(q.threads / 32) * 2 * 32 * 16 * sizeof(float) : 0;
+      e = launch_pdl(q.warp ? layer_norm_backward_rows<T, W, 1, 16, true, 256> : layer_norm_backward_rows<T, W, 1, 16, false, 512>,
+                     dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p);
+      note_launch("layer_norm_backward_rows");
     } else {
       if (sums) {  // before dX, which may overwrite dY
         layer_norm_dw_any<T><<<dim3(static_cast<unsigned>((p.cols + 31) / 32), static_cast<unsigned>(q.partials)), 256, 0, stream>>>(p);
