@@ -241,6 +241,37 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*buf)[32], i
   return make_float2(a, b);
 }
 
+// Four values at once: each exchange halves the number of values a lane still
+// sums, so the warp's four totals take 6 shuffles instead of 20.  After it,
+// lanes with (lane >> 3) == j hold the total of value j.
+__device__ __forceinline__ float warp_sum4(float4 v) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const bool hi = lane & 16, mid = lane & 8;
+  float a = hi ? v.z : v.x, b = hi ? v.w : v.y;  // kept
+  a += __shfl_xor_sync(0xffffffffu, hi ? v.x : v.z, 16);
+  b += __shfl_xor_sync(0xffffffffu, hi ? v.y : v.w, 16);
+  float c = mid ? b : a;
+  c += __shfl_xor_sync(0xffffffffu, mid ? a : b, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  return c;
+}
+
+template <bool WARP>
+__device__ __forceinline__ float4 row_sum4(float4 v, float4 (*buf)[32], int& parity) {
+  float c = warp_sum4(v);
+  if constexpr (!WARP) {
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    if ((lane & 7) == 0) reinterpret_cast<float*>(&buf[parity][threadIdx.x >> 5])[lane >> 3] = c;
+    __syncthreads();
+    const int warps = static_cast<int>(blockDim.x) >> 5;
+    c = warp_sum4(lane < warps ? buf[parity][lane] : make_float4(0.f, 0.f, 0.f, 0.f));
+    parity ^= 1;
+  }
+  return make_float4(__shfl_sync(0xffffffffu, c, 0), __shfl_sync(0xffffffffu, c, 8), __shfl_sync(0xffffffffu, c, 16),
+                     __shfl_sync(0xffffffffu, c, 24));
+}
+
 template <bool WARP>
 __device__ __forceinline__ float row_sum1(float a, float2 (*buf)[32], int& parity) {
   a = warp_sum(a);
@@ -254,23 +285,21 @@ __device__ __forceinline__ float row_sum1(float a, float2 (*buf)[32], int& parit
   return a;
 }
 
-// Statistics and result of one row of 16-byte groups, widened once.
+// Statistics and result of one row of 16-byte groups, kept packed and widened
+// for each of the three passes: keeping it widened costs the registers of a
+// third of the warps.
 template <typename T, typename W, int V, int NV, bool WARP>
 __device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, const RowVec<T, V> (&raw)[NV], int t, int G,
                                              float2 (*buf)[32], int& parity) {
   const int cols = static_cast<int>(p.cols);
   const float inv = 1.f / static_cast<float>(cols);
   T* y = static_cast<T*>(p.y) + row * p.ldy;
-  float2 v[NV][V / 2];
   float2 s = both(0.f);
 #pragma unroll
   for (int g = 0; g < NV; ++g)
     if (V * (t + G * g) < cols)
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        v[g][i] = widen2<T, V>(raw[g], i);
-        s = add2(s, v[g][i]);
-      }
+      for (int i = 0; i < V / 2; ++i) s = add2(s, widen2<T, V>(raw[g], i));
   const float mean = row_sum1<WARP>(s.x + s.y, buf, parity) * inv;
   float2 q = both(0.f);
 #pragma unroll
@@ -278,8 +307,8 @@ __device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, c
     if (V * (t + G * g) < cols)
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
-        v[g][i] = add2(v[g][i], both(-mean));
-        q = fma2(v[g][i], v[g][i], q);
+        const float2 d = add2(widen2<T, V>(raw[g], i), both(-mean));
+        q = fma2(d, d, q);
       }
   const float rstd = 1.f / sqrtf(fmaf(row_sum1<WARP>(q.x + q.y, buf, parity), inv, p.eps));
   if (t == 0) {
@@ -290,25 +319,15 @@ __device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, c
   for (int g = 0; g < NV; ++g) {
     const int c = V * (t + G * g);
     if (c >= cols) continue;
+    float2 w[V / 2], b[V / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) v[g][i] = mul2(v[g][i], both(rstd));
-    if (p.w) {
-      float2 w[V / 2], b[V / 2];
-      load_weights2<W, V>(static_cast<const W*>(p.w), c, p.vec_w, w);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) b[i] = both(0.f);
-      if (p.b) load_weights2<W, V>(static_cast<const W*>(p.b), c, p.vec_b, b);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) v[g][i] = fma2(v[g][i], w[i], b[i]);
-    } else if (p.b) {
-      float2 b[V / 2];
-      load_weights2<W, V>(static_cast<const W*>(p.b), c, p.vec_b, b);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) v[g][i] = add2(v[g][i], b[i]);
-    }
+    for (int i = 0; i < V / 2; ++i) w[i] = both(1.f), b[i] = both(0.f);
+    if (p.w) load_weights2<W, V>(static_cast<const W*>(p.w), c, p.vec_w, w);
+    if (p.b) load_weights2<W, V>(static_cast<const W*>(p.b), c, p.vec_b, b);
     RowVec<T, V> out;
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) round2<T, V>(out, i, v[g][i]);
+    for (int i = 0; i < V / 2; ++i)
+      round2<T, V>(out, i, fma2(mul2(add2(widen2<T, V>(raw[g], i), both(-mean)), both(rstd)), w[i], b[i]));
     store_vec<T, V>(y + c, out);
   }
 }
@@ -346,9 +365,10 @@ __device__ __forceinline__ void norm_one_row(const NormParams& p, int64_t row, c
   }
 }
 
-// Forward: rows loaded straight into registers.  A ring of rows in shared
-// memory, as the backward kernel has it, measured slower here (8192 x 8192
-// bf16: 80 against 68 us): with few registers enough rows are in flight.
+// Forward: rows loaded straight into registers.  The ring of the backward
+// kernel measured slower here (8192 x 8192 bf16: 80 us for a CTA per row, 216
+// for a warp per row): with 64 registers a thread, four CTAs of eight warps
+// per SM keep enough rows in flight and hide one another's barriers.
 template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS>
 __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_rows(const NormParams p) {
   __shared__ float2 buf[2][32];
@@ -487,10 +507,10 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
 
 // The same for rows on 16-byte boundaries, through the ring.  WARP: eight
 // rings per CTA, one per warp.
-template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS>
+template <typename T, typename W, int V, int NV, bool WARP, int MAXT, int CTAS, int ROWS>
 __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_backward_ring(const NormParams p, int stages) {
   extern __shared__ __align__(128) unsigned char ring_smem[];  // rings; WARP: afterwards [warps][2][32 V NV] sums
-  __shared__ float2 buf[2][32];
+  __shared__ float4 buf[2][32];
   __shared__ uint64_t full[8 * 8];
   __shared__ int abort_flag;
   int parity = 0;
@@ -529,63 +549,91 @@ __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_backward_ring(const Nor
     for (int i = 0; i < V / 2; ++i) aw[g][i] = ab[g][i] = both(0.f), ww[g][i] = both(1.f);
     if (p.w && V * (t + G * g) < cols) load_weights2<W, V>(static_cast<const W*>(p.w), V * (t + G * g), p.vec_w, ww[g]);
   }
-  float nmean = 0.f, nrstd = 0.f;
-  if (first < p.rows) nmean = p.mean[first], nrstd = p.rstd[first];
+  // ROWS (1 or 2) rows per step: one exchange of their sums.
+  float nmean[ROWS] = {}, nrstd[ROWS] = {};
+  auto statistics = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (row + r * step < p.rows) nmean[r] = p.mean[row + r * step], nrstd[r] = p.rstd[row + r * step];
+  };
+  statistics(first);
   int stage = 0;
   uint32_t phase = 0;
-  for (int64_t row = first; row < p.rows; row += step) {
-    const float mean = nmean, rstd = nrstd;
-    if (row + step < p.rows) nmean = p.mean[row + step], nrstd = p.rstd[row + step];
-    ring.wait(stage, phase);  // after a timeout (recorded) the rest runs through on stale data
-    const T* sx = reinterpret_cast<const T*>(ring.base + stage * 2 * ring.bytes);
-    const T* sg = reinterpret_cast<const T*>(ring.base + (stage * 2 + 1) * ring.bytes);
-    // One group per thread keeps h and u = dy w widened between the sums and
-    // the result; several keep x and dy packed and widen them again.
-    RowVec<T, V> vx[NV], vg[NV];
+  for (int64_t row = first; row < p.rows; row += ROWS * step) {
+    float mean[ROWS], rstd[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) mean[r] = nmean[r], rstd[r] = nrstd[r];
+    const bool two = ROWS == 2 && row + step < p.rows;
+    if (row + ROWS * step < p.rows) statistics(row + ROWS * step);
+    RowVec<T, V> vx[ROWS][NV], vg[ROWS][NV];
     float2 h[V / 2], u[V / 2];
-    float2 s0 = both(0.f), s1 = both(0.f);
-    auto widen = [&](int g, int i, float2& d) {
-      h[i] = mul2(add2(widen2<T, V>(vx[g], i), both(-mean)), both(rstd));
-      d = widen2<T, V>(vg[g], i);
+    float2 s[2][2] = {{both(0.f), both(0.f)}, {both(0.f), both(0.f)}};
+    // x and dy stay packed between the sums and the result and are widened twice.
+    auto widen = [&](int r, int g, int i, float2& d) {
+      h[i] = mul2(add2(widen2<T, V>(vx[r][g], i), both(-mean[r])), both(rstd[r]));
+      d = widen2<T, V>(vg[r][g], i);
       u[i] = mul2(d, ww[g][i]);
     };
+    int st[ROWS];
 #pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      const int c = V * (t + G * g);
-      if (c >= cols) continue;
-      vx[g] = load_vec<T, V>(sx + c);
-      vg[g] = load_vec<T, V>(sg + c);
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        float2 d;
-        widen(g, i, d);
-        aw[g][i] = fma2(d, h[i], aw[g][i]);
-        ab[g][i] = add2(d, ab[g][i]);
-        s0 = add2(s0, u[i]);
-        s1 = fma2(u[i], h[i], s1);
-      }
-    }
-    const float2 sum = row_sum<WARP>(s0.x + s0.y, s1.x + s1.y, buf, parity);  // also: the whole group has read the stage
-    const int64_t ahead = row + stages * step;
-    if (t == 0 && ahead < p.rows && !*ring.abort) ring.fill(stage, ahead), ++filled;
-    if (p.dx) {
-      const float a0 = sum.x * inv, a1 = sum.y * inv;
-      T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+    for (int r = 0; r < ROWS; ++r) {
+      st[r] = stage;
+      if (r == 1 && !two) break;
+      ring.wait(stage, phase);  // after a timeout (recorded) the rest runs through on stale data
+      const T* sx = reinterpret_cast<const T*>(ring.base + stage * 2 * ring.bytes);
+      const T* sg = reinterpret_cast<const T*>(ring.base + (stage * 2 + 1) * ring.bytes);
 #pragma unroll
       for (int g = 0; g < NV; ++g) {
         const int c = V * (t + G * g);
         if (c >= cols) continue;
-        RowVec<T, V> out;
+        vx[r][g] = load_vec<T, V>(sx + c);
+        vg[r][g] = load_vec<T, V>(sg + c);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
           float2 d;
-          if constexpr (NV > 1) widen(g, i, d);
-          round2<T, V>(out, i, mul2(both(rstd), fma2(h[i], both(-a1), add2(u[i], both(-a0)))));
+          widen(r, g, i, d);
+          aw[g][i] = fma2(d, h[i], aw[g][i]);
+          ab[g][i] = add2(d, ab[g][i]);
+          s[r][0] = add2(s[r][0], u[i]);
+          s[r][1] = fma2(u[i], h[i], s[r][1]);
         }
-        store_vec<T, V>(dx + c, out);
+      }
+      if (++stage == stages) stage = 0, phase ^= 1u;
+    }
+    float4 sum;
+    if constexpr (ROWS == 1) {
+      const float2 one = row_sum<WARP>(s[0][0].x + s[0][0].y, s[0][1].x + s[0][1].y, reinterpret_cast<float2(*)[32]>(buf), parity);
+      sum = make_float4(one.x, one.y, 0.f, 0.f);
+    } else sum = row_sum4<WARP>(make_float4(s[0][0].x + s[0][0].y, s[0][1].x + s[0][1].y, s[1][0].x + s[1][0].y,
+                                                  s[1][1].x + s[1][1].y), buf, parity);  // also: the group has read the stages
+    if (t == 0 && !*ring.abort) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const int64_t ahead = row + (stages + r) * step;
+        if (ahead < p.rows) ring.fill(st[r], ahead), ++filled;
       }
     }
-    if (++stage == stages) stage = 0, phase ^= 1u;
+    if (p.dx) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        if (r == 1 && !two) break;
+        const float a0 = (r ? sum.z : sum.x) * inv, a1 = (r ? sum.w : sum.y) * inv;
+        T* dx = static_cast<T*>(p.dx) + (row + r * step) * p.lddx;
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+          const int c = V * (t + G * g);
+          if (c >= cols) continue;
+          RowVec<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            float2 d;
+            widen(r, g, i, d);
+            round2<T, V>(out, i, mul2(both(rstd[r]), fma2(h[i], both(-a1), add2(u[i], both(-a0)))));
+          }
+          store_vec<T, V>(dx + c, out);
+        }
+      }
+    }
   }
   if (t == 0 && *ring.abort) ring.drain(filled);
   if (p.partial) {
@@ -769,7 +817,7 @@ NormPlan norm_forward_plan(const cuopx_layer_norm_args& a) {
   }
   // Few rows: as many threads per row as there are groups, for the shortest
   // chain of loads; many rows: several groups per thread, several rows per SM.
-  const int small = q.vec ? 1 : 4, large = q.vec ? 16 / v : 16;
+  const int small = q.vec ? 1 : 4, large = q.vec ? 4 : 16;
   q.nv = a.rows <= 2 * sms && a.cols <= 1024ll * per * small ? small : large;
   const int64_t t = (a.cols + static_cast<int64_t>(per) * q.nv - 1) / (static_cast<int64_t>(per) * q.nv);
   q.threads = static_cast<int>((t + 31) / 32 * 32);
@@ -894,8 +942,8 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
       auto go = [&](auto kern) {
         e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), 0, stream, p);
       };
-      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256, 3>) : go(layer_norm_rows<T, W, 1, 16, true, 256, 3>);
-      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024, 1>) : go(layer_norm_rows<T, W, V, 16 / V, false, 1024, 1>);
+      if (q.warp) q.vec ? go(layer_norm_rows<T, W, V, 4, true, 256, 4>) : go(layer_norm_rows<T, W, 1, 16, true, 256, 3>);
+      else if (q.vec) q.nv == 1 ? go(layer_norm_rows<T, W, V, 1, false, 1024, 1>) : go(layer_norm_rows<T, W, V, 4, false, 1024, 1>);
       else q.nv == 4 ? go(layer_norm_rows<T, W, 1, 4, false, 1024, 1>) : go(layer_norm_rows<T, W, 1, 16, false, 512, 2>);
     });
     if (e != cudaSuccess) {
@@ -962,8 +1010,9 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
           e = launch_pdl(kern, dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p, q.stages);
         note_launch("layer_norm_backward_ring");
       };
-      if (q.warp) q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, true, 256, 2>, 32 * V) : go(layer_norm_backward_ring<T, W, V, 4, true, 256, 1>, 32 * V * 4);
-      else q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, false, 1024, 1>, 0) : go(layer_norm_backward_ring<T, W, V, 4, false, 512, 1>, 0);
+      constexpr int ROWS = sizeof(T) == 2 ? 2 : 1;
+      if (q.warp) q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, true, 256, 2, 2>, 32 * V) : go(layer_norm_backward_ring<T, W, V, 4, true, 256, 1, 2>, 32 * V * 4);
+      else q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, false, 1024, 1, ROWS>, 0) : go(layer_norm_backward_ring<T, W, V, 4, false, 512, 1, 1>, 0);
     } else if (q.rows) {
       const size_t smem = q.warp ? static_cast<size_t>(q.threads / 32) * 2 * 32 * 16 * sizeof(float) : 0;
       e = launch_pdl(q.warp ? layer_norm_backward_rows<T, W, 1, 16, true, 256> : layer_norm_backward_rows<T, W, 1, 16, false, 512>,
