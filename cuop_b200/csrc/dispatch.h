@@ -122,7 +122,10 @@ struct LinearProblem {
   int64_t ldy;
   void* Z;
   int64_t ldz;
-  int64_t wide() const { return gated ? 2 * N : N; }  // columns of W and Z
+  int64_t w_up = 0;     // gated: first column (row when transW) of the second projection in W
+  bool transX = false;  // X is stored [K][M] (the weight gradient's products; CTA-pair kernel only)
+  int64_t wide() const { return gated ? 2 * N : N; }           // columns of W and Z
+  int64_t w_cols() const { return gated ? w_up + N : N; }      // columns that W spans
 };
 
 // Base and rows on 16-byte boundaries (16-bit elements).

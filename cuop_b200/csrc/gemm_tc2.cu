@@ -126,6 +126,7 @@ template <int MODE>
 struct PairLayer {
   CUtensorMap tmZ, tmZ2;
   LayerEpi epi;
+  int w_up;  // kPairGated: first column of the second projection in B
 };
 template <>
 struct PairLayer<kPairGemm> {};
@@ -255,7 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     fence_mbarrier_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
-    prefetch_tmap(&tmC);
+    if constexpr (MODE == kPairGemm) prefetch_tmap(&tmC);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -302,8 +303,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         pair_tile_coords(t, p, b, mt, nt);
         const int m0 = mt * 2 * P_BM + static_cast<int>(rank) * P_BM;
         // Gated: column n0 of this CTA's projection (rank 0 the gate's, rank 1 the other's).
-        const int n0 = MODE == kPairGated ? nt * (PBN / 2) + static_cast<int>(rank) * p.N
-                                          : nt * PBN + static_cast<int>(rank) * (P_SLOT_COLS / 2);
+        int n0;
+        if constexpr (MODE == kPairGated) n0 = nt * (PBN / 2) + static_cast<int>(rank) * layer.w_up;
+        else n0 = nt * PBN + static_cast<int>(rank) * (P_SLOT_COLS / 2);
         for (int kb = 0; kb < p.k_blocks; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
             ok = false;
@@ -671,26 +673,27 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
   return check_launch();
 }
 
-// A layer's forward pass: X [M][K] K-major, W [K][columns] (B_MN) or [columns][K].
-template <typename T, bool B_MN, int PBN, int MODE>
+// A layer's forward pass: X [M][K] (or, A_MN, [K][M]), W [K][columns] (B_MN) or [columns][K].
+template <typename T, bool A_MN, bool B_MN, int PBN, int MODE>
 int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* name) {
   using L = PairSmem<PBN, MODE>;
   constexpr int P_SLOT_COLS = PairCfg<PBN>::SLOT;
   constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap mA, mB, mC;
+  CUtensorMap mA, mB, mC = {};
   PairLayer<MODE> layer = {};
-  bool ok = make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
-  if (B_MN) ok &= make_map(&mB, dt, p.W, p.wide(), p.K, 1, p.ldw, 0, 64, P_BK);
-  else ok &= make_map(&mB, dt, p.W, p.K, p.wide(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
-  ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
-  if (p.Z) {
+  layer.epi = layer_epi(p);
+  layer.w_up = static_cast<int>(p.w_up);
+  bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, P_BK) : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
+  if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, P_BK);
+  else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
+  if (!layer.epi.Y) ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
+  if (p.Z && !layer.epi.Z) {
     ok &= make_map(&layer.tmZ, dt, p.Z, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
     if (MODE == kPairGated) ok &= make_map(&layer.tmZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
   }
   if (!ok) return CUOPX_CUDA_ERROR;
-  layer.epi = layer_epi(p);
   PairParams prm = {};
   prm.M = static_cast<int>(p.M);
   prm.N = static_cast<int>(p.N);
@@ -700,7 +703,7 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
   prm.tiles_n = static_cast<int>((p.N + COLS - 1) / COLS);
   prm.num_tiles = prm.tiles_m * prm.tiles_n;
   prm.k_blocks = static_cast<int>((p.K + P_BK - 1) / P_BK);
-  auto kern = gemm_tc2_kernel<T, false, B_MN, PBN, MODE>;
+  auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN, MODE>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -723,12 +726,13 @@ template <typename T, int PBN>
 int launch_tc2_layer_layout(const LinearProblem& p, cudaStream_t stream) {
   if (p.gated) {
     const char* name = PBN == 256 ? "gated_linear_tc2_256x128" : "gated_linear_tc2_256x64";
-    return p.transW ? launch_tc2_layer<T, false, PBN, kPairGated>(p, stream, name)
-                    : launch_tc2_layer<T, true, PBN, kPairGated>(p, stream, name);
+    return p.transW ? launch_tc2_layer<T, false, false, PBN, kPairGated>(p, stream, name)
+                    : launch_tc2_layer<T, false, true, PBN, kPairGated>(p, stream, name);
   }
   const char* name = PBN == 256 ? "linear_tc2_256x256" : "linear_tc2_256x128";
-  return p.transW ? launch_tc2_layer<T, false, PBN, kPairLinear>(p, stream, name)
-                  : launch_tc2_layer<T, true, PBN, kPairLinear>(p, stream, name);
+  if (p.transX) return launch_tc2_layer<T, true, true, PBN, kPairLinear>(p, stream, name);
+  return p.transW ? launch_tc2_layer<T, false, false, PBN, kPairLinear>(p, stream, name)
+                  : launch_tc2_layer<T, false, true, PBN, kPairLinear>(p, stream, name);
 }
 
 }  // namespace
@@ -800,13 +804,12 @@ int gemm_tc2_peers(const GemmProblem& p, void* const* peers, int npeers, cudaStr
                     : launch_tc2_layout<256>(p, peers, npeers, stream);
 }
 
-// TMA reads and writes whole 16-byte groups of aligned rows.
+// TMA reads X and W: rows on 16-byte boundaries.  Y, Z, residual and bias may have any alignment.
 bool linear_tc2_supported(const LinearProblem& p) {
-  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.N > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
-  if (!row_aligned16(p.X, p.ldx) || !row_aligned16(p.W, p.ldw) || !row_aligned16(p.Y, p.ldy)) return false;
-  if (p.Z && !row_aligned16(p.Z, p.ldz)) return false;
-  // The second projection's columns start N into W's rows and Z's.
-  if (p.gated && p.N % 8 && (!p.transW || p.Z)) return false;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.transX && (p.gated || p.transW)) return false;
+  if (!row_aligned16(p.X, p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
+  if (p.gated && !p.transW && p.w_up % 8) return false;  // an x coordinate of W's tiles
   return ((p.M + 255) / 256) * ((p.N + 63) / 64) < (int64_t(1) << 29);
 }
 

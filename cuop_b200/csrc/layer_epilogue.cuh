@@ -20,6 +20,13 @@ struct LayerEpi {
   int has_z;     // store the pre-activation
   int vec_bias;  // bias can be read in 16-byte groups
   int vec_res;   // so can the residual's rows
+  // Set where rows are not on 16-byte boundaries, which TMA cannot store: the
+  // staged tile then goes out in plain 2-byte stores, 64 columns of a row per
+  // two of a warp's.
+  void* Y;
+  int64_t ldy;
+  void* Z;
+  int64_t ldz;
 };
 
 inline LayerEpi layer_epi(const LinearProblem& p) {
@@ -31,6 +38,10 @@ inline LayerEpi layer_epi(const LinearProblem& p) {
   e.has_z = p.Z != nullptr;
   e.vec_bias = p.N % 8 == 0 && row_aligned16(p.bias, 0);
   e.vec_res = p.N % 8 == 0 && row_aligned16(p.R, p.ldr);
+  e.Y = row_aligned16(p.Y, p.ldy) ? nullptr : p.Y;
+  e.ldy = p.ldy;
+  e.Z = p.Z == nullptr || (row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0)) ? nullptr : p.Z;
+  e.ldz = p.ldz;
   return e;
 }
 
@@ -100,6 +111,22 @@ __device__ __forceinline__ void stage_row32(unsigned char* buf, int lane, int h,
     w.w = pack2_layer<T>(v[8 * j + 6], v[8 * j + 7]);
     *reinterpret_cast<uint4*>(buf + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)) = w;
   }
+}
+
+// The staged 32 x 64 chunk at `buf` (whole warp, after __syncwarp) to rows m0.. and columns c.. of an unaligned matrix.
+template <typename T>
+__device__ __forceinline__ void store_chunk_plain(const unsigned char* buf, T* out, int64_t ld, int64_t col0, int c, int m0,
+                                                  int M, int N, int lane) {
+  const int rows = min(32, M - m0);
+  const int col = c + 2 * lane;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    unsigned short* dst = reinterpret_cast<unsigned short*>(out + (static_cast<int64_t>(m0) + r) * ld + col0 + col);
+    if (col < N) dst[0] = static_cast<unsigned short>(w);
+    if (col + 1 < N) dst[1] = static_cast<unsigned short>(w >> 16);
+  }
+  __syncwarp();
 }
 
 // One warp's rows of one tile.  t_row: TMEM address of the tile's first
@@ -175,15 +202,20 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
     if (h == 1) {
       fence_proxy_async_shared();
       __syncwarp();
+      const int c = n0 + 32 * (half - 1);
       if (lane == 0) {
-        const int c = n0 + 32 * (half - 1);
-        if (e.has_z) {
+        if (e.has_z && !e.Z) {
           tma_store_3d(tmZ, stage, c, m0, 0);
           if constexpr (GATED) tma_store_3d(tmZ2, stage + BUF, c, m0, 0);
         }
-        tma_store_3d(tmY, stage + ybuf * BUF, c, m0, 0);
+        if (!e.Y) tma_store_3d(tmY, stage + ybuf * BUF, c, m0, 0);
         bulk_commit_group();
       }
+      if (e.Z) {
+        store_chunk_plain<T>(stage, static_cast<T*>(e.Z), e.ldz, 0, c, m0, M, N, lane);
+        if constexpr (GATED) store_chunk_plain<T>(stage + BUF, static_cast<T*>(e.Z), e.ldz, N, c, m0, M, N, lane);
+      }
+      if (e.Y) store_chunk_plain<T>(stage + ybuf * BUF, static_cast<T*>(e.Y), e.ldy, 0, c, m0, M, N, lane);
     }
   }
 }

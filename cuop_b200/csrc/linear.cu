@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinearProblem p)
           const int wk = p.transW ? e % LS_K : e / LS_T, wn = p.transW ? e / LS_K : e % LS_T;
           const int64_t kk = k0 + wk, n = n0 + wn;
           float v = 0.f;
-          if (kk < p.K && n < p.N) v = to_acc<T>(p.transW ? W[(h * p.N + n) * p.ldw + kk] : W[kk * p.ldw + h * p.N + n]);
+          if (kk < p.K && n < p.N) v = to_acc<T>(p.transW ? W[(h * p.w_up + n) * p.ldw + kk] : W[kk * p.ldw + h * p.w_up + n]);
           ws[h][wk][wn] = v;
         }
       }
@@ -105,6 +105,70 @@ int linear_simt(const LinearProblem& p, cudaStream_t stream) {
   note_launch(p.gated ? "gated_linear_simt" : "linear_simt");
   return check_launch();
 }
+
+// ---------------------------------------------------------------- copies on 16-byte boundaries
+// TMA reads rows that start on 16-byte boundaries.  An operand whose rows do
+// not is first copied to rows that do (one read and one write of it, which
+// buys the tensor cores for the product).  `halves`: the row's two
+// projections are copied apart, so that the second starts on a boundary too.
+struct RepackParams {
+  int64_t rows, cols;  // of one half
+  int halves;
+  const unsigned short* src;
+  int64_t ld, src_half;
+  unsigned short* dst;
+  int64_t ldd, dst_half;
+};
+
+__global__ void __launch_bounds__(256) linear_repack_kernel(const RepackParams p) {
+  const int64_t groups = (p.cols + 7) / 8, per_row = groups * p.halves;
+  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < p.rows * per_row; e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = e / per_row, g = e - row * per_row;
+    const int64_t half = g >= groups, c = (g - half * groups) * 8;
+    const unsigned short* s = p.src + row * p.ld + half * p.src_half + c;
+    uint32_t w[4];
+    if (c > 0 && c + 9 < p.cols) {
+      // Five aligned words around the eight elements, all inside the row.
+      const bool odd = reinterpret_cast<uintptr_t>(s) & 2;
+      const uint32_t* a = reinterpret_cast<const uint32_t*>(s - (odd ? 1 : 0));
+      uint32_t v[5];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) v[i] = a[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = odd ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = c + 2 * i < p.cols ? s[2 * i] : 0u, hi = c + 2 * i + 1 < p.cols ? s[2 * i + 1] : 0u;
+        w[i] = lo | hi << 16;
+      }
+    }
+    *reinterpret_cast<uint4*>(p.dst + row * p.ldd + half * p.dst_half + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// rows x cols of src to rows of round8(cols) at dst (halves: two such rows side by side).
+void linear_repack(const void* src, int64_t rows, int64_t cols, int64_t ld, int halves, int64_t src_half, void* dst,
+                   cudaStream_t stream) {
+  RepackParams r;
+  r.rows = rows;
+  r.cols = cols;
+  r.halves = halves;
+  r.src = static_cast<const unsigned short*>(src);
+  r.ld = ld;
+  r.src_half = src_half;
+  r.dst = static_cast<unsigned short*>(dst);
+  r.dst_half = round8(cols);
+  r.ldd = halves * r.dst_half;
+  const int64_t n = rows * halves * (r.dst_half / 8);
+  const unsigned ctas = static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, static_cast<int64_t>(device_sm_count()) * 32));
+  linear_repack_kernel<<<ctas, 256, 0, stream>>>(r);
+  note_launch("linear_repack");
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // ---------------------------------------------------------------- dZ and its column sums
 // One pass over dY (and Z): writes dZ and, per share of the rows, the fp32
@@ -227,39 +291,69 @@ __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, in
   db[c] = from_acc<T>(s);
 }
 
+// Below this many multiplications the SIMT kernel, which takes any alignment,
+// beats copying unaligned operands and running on the tensor cores: two more
+// launches cost about 4 us, in which it does some 2^24 products.
+constexpr double kRepackMinWork = 16777216.0;
+
+// The kernel for a problem whose operands are as aligned as they will be.
+int linear_route(const LinearProblem& p, cudaStream_t stream) {
+  if (p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
+  if (linear_tc2_supported(p)) return linear_tc2(p, stream, 256);
+  if (p.transX) return CUOPX_NOT_IMPLEMENTED;  // not reached: its operands are aligned copies
+  return linear_simt(p, stream);
+}
+
 // ---------------------------------------------------------------- backward plan
 struct BackwardPlan {
-  bool need_dz;  // dZ differs from dY
+  bool need_dz;          // dZ differs from dY, or dY's rows are not aligned
+  bool copy_x, copy_w;   // aligned copies for the products
+  bool tensor;           // products on the tensor cores whatever the alignment of dX and dW
   int64_t lddz;
   int v, splits;
-  size_t dz_off, partial_off, bytes;
+  size_t dz_off, partial_off, x_off, w_off, bytes;
 };
-
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 BackwardPlan backward_plan(const cuopx_linear_backward_args& a, bool gated) {
   BackwardPlan q = {};
   const int64_t wide = gated ? 2 * a.N : a.N;
-  if (a.M <= 0 || a.N <= 0 || dtype_size(a.dtype) == 0) return q;
-  q.need_dz = (gated || a.activation != CUOPX_ACT_NONE) && (a.dX || a.dW) && a.K > 0;
-  q.lddz = (wide + 7) / 8 * 8;
-  const bool vec = a.N % 8 == 0 && row_aligned16(a.dY, a.lddy) &&
-                   ((!gated && a.activation == CUOPX_ACT_NONE) || row_aligned16(a.preact, a.ldz));
+  if (a.M <= 0 || a.N <= 0 || dtype_size(a.dtype) != 2) return q;
+  const bool dx = a.dX && a.K > 0, dw = a.dW && a.K > 0;
+  const bool act = gated || a.activation != CUOPX_ACT_NONE;
+  q.tensor = static_cast<double>(a.M) * static_cast<double>(wide) * static_cast<double>(a.K) >= kRepackMinWork;
+  q.need_dz = (dx || dw) && (act || (q.tensor && !row_aligned16(a.dY, a.lddy)));
+  q.copy_x = dw && q.tensor && !row_aligned16(a.X, a.ldx);
+  q.copy_w = dx && q.tensor && !row_aligned16(a.W, a.ldw);
+  q.lddz = round8(wide);
+  const bool vec = a.N % 8 == 0 && row_aligned16(a.dY, a.lddy) && (!act || row_aligned16(a.preact, a.ldz));
   q.v = vec ? 8 : 1;
   const int64_t strips = (a.N + 32 * q.v - 1) / (32 * q.v);
   const int64_t want = (static_cast<int64_t>(device_sm_count()) * 4 + strips - 1) / strips;
   q.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (a.M + 15) / 16, 1024})));
   size_t off = 0;
-  if (q.need_dz) {
-    q.dz_off = off;
-    off += round256(static_cast<size_t>(a.M) * q.lddz * dtype_size(a.dtype));
-  }
-  if (a.dbias && q.splits > 1) {
-    q.partial_off = off;
-    off += round256(static_cast<size_t>(q.splits) * wide * sizeof(float));
-  }
+  auto take = [&](bool want_it, size_t bytes) {
+    const size_t at = off;
+    if (want_it) off += round256(bytes);
+    return at;
+  };
+  q.dz_off = take(q.need_dz, static_cast<size_t>(a.M) * q.lddz * 2);
+  q.partial_off = take(a.dbias && q.splits > 1, static_cast<size_t>(q.splits) * wide * sizeof(float));
+  q.x_off = take(q.copy_x, static_cast<size_t>(a.M) * round8(a.K) * 2);
+  const int64_t w_rows = a.transW ? wide : a.K, w_cols = a.transW ? a.K : wide;
+  q.w_off = take(q.copy_w, static_cast<size_t>(w_rows) * round8(w_cols) * 2);
   q.bytes = off;
   return q;
+}
+
+// C [M][N] = X op(W) for the backward pass: a plain product when C's rows are
+// aligned (the GEMM back-ends), else the layer kernels, which store any rows.
+int backward_product(const LinearProblem& p, bool tensor, cudaStream_t stream) {
+  if (!p.transX && p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
+  if (!tensor || row_aligned16(p.Y, p.ldy)) {
+    GemmProblem g{p.dtype, p.transX, p.transW, p.M, p.N, p.K, 1.0, 0.0, p.X, p.ldx, 0, p.W, p.ldw, 0, p.Y, p.ldy, 0, 1};
+    return gemm_route(g, stream);
+  }
+  return linear_route(p, stream);
 }
 
 template <typename T, bool GATED>
@@ -300,17 +394,63 @@ int validate_linear(const cuopx_linear_args& a, bool gated) {
       overlaps(a.preact, zb, a.residual, rb))
     return CUOPX_INVALID_ARGUMENT;
   if (a.residual && !alias_ok(a.Y, a.ldy, a.residual, a.ldr, a.M, a.N, es)) return CUOPX_INVALID_ARGUMENT;
+  if (overlaps(a.workspace, a.workspace_bytes, a.X, xb) || overlaps(a.workspace, a.workspace_bytes, a.W, wb) ||
+      overlaps(a.workspace, a.workspace_bytes, a.bias, bb) || overlaps(a.workspace, a.workspace_bytes, a.residual, rb) ||
+      overlaps(a.workspace, a.workspace_bytes, a.Y, yb) || overlaps(a.workspace, a.workspace_bytes, a.preact, zb))
+    return CUOPX_INVALID_ARGUMENT;
   return -1;
+}
+
+// Bytes of aligned copies of X and W, and the problem on them when `ws` is given.
+size_t repack_plan(LinearProblem& p, char* ws, cudaStream_t stream) {
+  size_t off = 0;
+  const bool x = !row_aligned16(p.X, p.M == 1 ? 0 : p.ldx);
+  const bool split = p.gated && !p.transW && p.w_up % 8;  // the second projection's columns
+  const bool w = split || !row_aligned16(p.W, p.ldw);
+  if (!x && !w) return 0;
+  if (static_cast<double>(p.M) * static_cast<double>(p.wide()) * static_cast<double>(p.K) < kRepackMinWork) return 0;
+  if (x) {
+    if (ws) {
+      linear_repack(p.X, p.M, p.K, p.ldx, 1, 0, ws + off, stream);
+      p.X = ws + off;
+      p.ldx = round8(p.K);
+    }
+    off += round256(static_cast<size_t>(p.M) * round8(p.K) * 2);
+  }
+  if (w) {
+    const int64_t rows = p.transW ? p.w_cols() : p.K, cols = p.transW ? p.K : split ? p.N : p.w_cols();
+    const int halves = split ? 2 : 1;
+    if (ws) {
+      linear_repack(p.W, rows, cols, p.ldw, halves, p.w_up, ws + off, stream);
+      p.W = ws + off;
+      p.ldw = halves * round8(cols);
+      if (split) p.w_up = round8(cols);
+    }
+    off += round256(static_cast<size_t>(rows) * halves * round8(cols) * 2);
+  }
+  return off;
+}
+
+LinearProblem linear_problem(const cuopx_linear_args& a, bool gated) {
+  LinearProblem p{a.dtype, a.transW != 0, a.activation, gated, a.M,   a.N,   a.K,      a.X,   a.ldx, a.W,
+                  a.ldw,   a.bias,        a.residual,   a.ldr, a.Y, a.ldy, a.preact, a.ldz};
+  p.w_up = a.N;
+  return p;
+}
+
+size_t linear_workspace(const cuopx_linear_args* a, bool gated) {
+  if (!a || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
+  LinearProblem p = linear_problem(*a, gated);
+  return repack_plan(p, nullptr, nullptr);
 }
 
 int linear_forward(const cuopx_linear_args* a, bool gated, cudaStream_t stream) {
   if (a == nullptr) return CUOPX_INVALID_ARGUMENT;
   if (const int v = validate_linear(*a, gated); v >= 0) return v;
-  LinearProblem p{a->dtype, a->transW != 0, a->activation, gated, a->M,   a->N,   a->K,      a->X,   a->ldx, a->W,
-                  a->ldw,   a->bias,        a->residual,   a->ldr, a->Y, a->ldy, a->preact, a->ldz};
-  if (p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
-  if (linear_tc2_supported(p) && p.M >= 64) return linear_tc2(p, stream, 256);
-  return linear_simt(p, stream);
+  LinearProblem p = linear_problem(*a, gated);
+  const size_t need = p.K > 0 ? repack_plan(p, nullptr, nullptr) : 0;
+  if (need > 0 && a->workspace && a->workspace_bytes >= need) repack_plan(p, static_cast<char*>(a->workspace), stream);
+  return linear_route(p, stream);
 }
 
 int validate_linear_backward(const cuopx_linear_backward_args& a, bool gated) {
@@ -379,18 +519,38 @@ int linear_backward(const cuopx_linear_backward_args* a, bool gated, cudaStream_
     if (const int rc = check_launch(); rc != CUOPX_SUCCESS) return rc;
   }
   if (a->dX && a->M > 0 && a->K > 0) {
-    // dX [M][K] = dZ [M][wide] W^T
-    GemmProblem g{a->dtype, false, a->transW == 0, a->M, a->K, wide, 1.0, 0.0, dz, lddz, 0, a->W, a->ldw, 0,
-                  a->dX, a->lddx, 0, 1};
-    if (const int rc = gemm_route(g, stream); rc != CUOPX_SUCCESS) return rc;
+    // dX [M][K] = dZ [M][wide] op(W)^T: W's columns are the products' depth.
+    LinearProblem p{};
+    p.dtype = a->dtype;
+    p.transW = a->transW == 0;
+    p.M = a->M, p.N = a->K, p.K = wide;
+    p.X = dz, p.ldx = lddz;
+    p.W = a->W, p.ldw = a->ldw;
+    p.Y = a->dX, p.ldy = a->lddx;
+    if (q.copy_w && wide > 0) {
+      const int64_t w_rows = a->transW ? wide : a->K, w_cols = a->transW ? a->K : wide;
+      linear_repack(a->W, w_rows, w_cols, a->ldw, 1, 0, ws + q.w_off, stream);
+      p.W = ws + q.w_off, p.ldw = round8(w_cols);
+    }
+    if (const int rc = backward_product(p, q.tensor, stream); rc != CUOPX_SUCCESS) return rc;
   }
   if (a->dW && a->N > 0 && a->K > 0) {
-    // dW [K][wide] = X^T dZ, or [wide][K] = dZ^T X
-    GemmProblem g = a->transW ? GemmProblem{a->dtype, true, false, wide, a->K, a->M, 1.0, 0.0, dz, lddz, 0, a->X, a->ldx,
-                                            0, a->dW, a->lddw, 0, 1}
-                              : GemmProblem{a->dtype, true, false, a->K, wide, a->M, 1.0, 0.0, a->X, a->ldx, 0, dz, lddz,
-                                            0, a->dW, a->lddw, 0, 1};
-    if (const int rc = gemm_route(g, stream); rc != CUOPX_SUCCESS) return rc;
+    // dW [K][wide] = X^T dZ, or [wide][K] = dZ^T X.
+    const void* x = a->X;
+    int64_t ldx = a->ldx;
+    if (q.copy_x) {
+      linear_repack(a->X, a->M, a->K, a->ldx, 1, 0, ws + q.x_off, stream);
+      x = ws + q.x_off, ldx = round8(a->K);
+    }
+    LinearProblem p{};
+    p.dtype = a->dtype;
+    p.transX = true;
+    p.K = a->M;
+    p.M = a->transW ? wide : a->K, p.N = a->transW ? a->K : wide;
+    p.X = a->transW ? dz : x, p.ldx = a->transW ? lddz : ldx;
+    p.W = a->transW ? x : dz, p.ldw = a->transW ? ldx : lddz;
+    p.Y = a->dW, p.ldy = a->lddw;
+    if (const int rc = backward_product(p, q.tensor, stream); rc != CUOPX_SUCCESS) return rc;
   }
   return CUOPX_SUCCESS;
 }
@@ -401,8 +561,8 @@ int linear_backward(const cuopx_linear_backward_args* a, bool gated, cudaStream_
 
 extern "C" {
 
-size_t cuopx_linear_workspace_size(const cuopx_linear_args*) { return 0; }
-size_t cuopx_gated_linear_workspace_size(const cuopx_linear_args*) { return 0; }
+size_t cuopx_linear_workspace_size(const cuopx_linear_args* args) { return cuopx::linear_workspace(args, false); }
+size_t cuopx_gated_linear_workspace_size(const cuopx_linear_args* args) { return cuopx::linear_workspace(args, true); }
 
 int cuopx_linear(const cuopx_linear_args* args, void* stream) {
   cuopx::ApiScope scope("cuopx_linear", args ? args->M : 0, args ? args->N : 0, args ? args->K : 0);

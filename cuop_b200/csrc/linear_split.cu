@@ -52,6 +52,7 @@ struct SplitParams {
   int M, N, K, k_blocks;
   int cs;       // CTAs per cluster
   int tiles_n;  // column tiles (N / 128, or N / 64 when gated)
+  int w_up;     // gated: first column of the second projection in W
   int act;
   int pairs;  // two columns per store: Y, Z, residual and bias can be read and written as 4-byte words
   const void* bias;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
     for (int kb = kb0; kb < min(kb1, kb0 + STAGES); ++kb) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int c = n0 + (GATED ? j * p.N : 64 * j);
+        const int c = n0 + (GATED ? j * p.w_up : 64 * j);
         if constexpr (W_MN) tma_prefetch_3d(&tmW, c, kb * LSP_BK, 0);
         else tma_prefetch_3d(&tmW, kb * LSP_BK, c, 0);
       }
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
         const int k0 = kb * LSP_BK;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {  // 64 columns of W each
-          const int c = n0 + (GATED ? j * p.N : 64 * j);
+          const int c = n0 + (GATED ? j * p.w_up : 64 * j);
           if constexpr (W_MN) tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], c, k0, 0);
           else tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], k0, c, 0);
         }
@@ -322,8 +323,8 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap mW, mX;
-  bool ok = W_MN ? make_map(&mW, dt, p.W, p.wide(), p.K, 1, p.ldw, 0, 64, LSP_BK)
-                 : make_map(&mW, dt, p.W, p.K, p.wide(), 1, p.ldw, 0, LSP_BK, 64);
+  bool ok = W_MN ? make_map(&mW, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, LSP_BK)
+                 : make_map(&mW, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LSP_BK, 64);
   // A single row has no stride: any multiple of 8 serves.
   ok &= make_map(&mX, dt, p.X, p.K, p.M, 1, p.M == 1 ? (p.K + 7) / 8 * 8 : p.ldx, 0, LSP_BK, TOK);
   if (!ok) return CUOPX_CUDA_ERROR;
@@ -334,6 +335,7 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   prm.K = static_cast<int>(p.K);
   prm.k_blocks = static_cast<int>((p.K + LSP_BK - 1) / LSP_BK);
   prm.tiles_n = static_cast<int>((p.N + TILE_N - 1) / TILE_N);
+  prm.w_up = static_cast<int>(p.w_up);
   prm.act = p.act;
   prm.pairs = p.N % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 4 == 0;
   prm.bias = p.bias;
@@ -387,9 +389,10 @@ int linear_split_rows(const LinearProblem& p, cudaStream_t stream) {
 
 // TMA reads X and W; Y, Z, residual and bias may have any alignment.
 bool linear_split_supported(const LinearProblem& p) {
-  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.N > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.transX) return false;
   if (!row_aligned16(p.X, p.M == 1 ? 0 : p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
-  if (p.gated && !p.transW && p.N % 8) return false;  // the second projection's first column in W's rows
+  if (p.gated && !p.transW && p.w_up % 8) return false;  // the second projection's first column in W's rows
   return ((p.N + 63) / 64) * ((p.M + 15) / 16) < (int64_t(1) << 27);
 }
 
