@@ -5,62 +5,124 @@
 
 namespace cuopx {
 
-// s(z) = 1 / (1 + exp(-z)).  exp(-z) = inf gives 0, the limit.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-
-// s'(z) = e / (1 + e)^2 with e = exp(-|z|): no cancellation in 1 - s(z), no overflow.
-__device__ __forceinline__ float sigmoid_slope_f(float z) {
-  const float e = __expf(-fabsf(z));
-  const float r = __fdividef(1.f, 1.f + e);
-  return e * r * r;
-}
-
-constexpr float kSqrtHalf = 0.70710678118654752f;
-constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluTanhTwoC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluTanhA = 0.044715f;
 
+// 2^x and 1 / x to about one unit in the last place (PTX approx forms; 2^x
+// overflows to infinity, and 1 / infinity is 0).
+__device__ __forceinline__ float2 exp2_2(float2 x) {
+  float2 r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(x.y));
+  return r;
+}
+__device__ __forceinline__ float2 rcp_2(float2 x) {
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(x.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(x.y));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Everything below works on pairs: the packed forms halve the instructions
+// that surround the two exponentials and divisions.
+
+// s(z) = 1 / (1 + exp(-z)); exp(-z) = inf gives 0, the limit.
+__device__ __forceinline__ float2 sigmoid_2(float2 z, float2& e) {
+  e = exp2_2(mul2(z, both(-kLog2e)));
+  return rcp_2(add2(e, both(1.f)));
+}
+
+// s'(z) = e s^2 with e = exp(-z) = (1 - s) / s: no cancellation in 1 - s.  e is
+// kept finite, so that s = 0 gives s' = 0.
+__device__ __forceinline__ float2 sigmoid_slope_2(float2 e, float2 s) {
+  return mul2(mul2(make_float2(fminf(e.x, 1e30f), fminf(e.y, 1e30f)), s), s);
+}
+
+// The normal density phi(z) and distribution function Phi(z): for x >= 0
+//   Phi(x) = 1 - phi(x) (b1 t + ... + b5 t^5) + eps(x),  t = 1 / (1 + p x),
+// |eps| < 7.5e-8 (Abramowitz and Stegun, 26.2.17, after Hastings 1955), and
+// Phi(-x) = 1 - Phi(x), here without the subtraction.  One exponential and one
+// division give both, a third of the instructions of erfcf and an exponential;
+// the error is that of rounding Phi itself to fp32.
+__device__ __forceinline__ float2 normal_2(float2 z, float2& density) {
+  const float2 t = rcp_2(fma2(both(0.2316419f), make_float2(fabsf(z.x), fabsf(z.y)), both(1.f)));
+  density = mul2(both(0.39894228040143268f), exp2_2(mul2(mul2(z, z), both(-0.5f * kLog2e))));
+  float2 q = fma2(both(1.330274429f), t, both(-1.821255978f));
+  q = fma2(q, t, both(1.781477937f));
+  q = fma2(q, t, both(-0.356563782f));
+  q = fma2(q, t, both(0.319381530f));
+  q = mul2(mul2(q, t), density);
+  return make_float2(z.x >= 0.f ? 1.f - q.x : q.x, z.y >= 0.f ? 1.f - q.y : q.y);
+}
+
+// 2 sqrt(2 / pi) (z + 0.044715 z^3)
+__device__ __forceinline__ float2 gelu_tanh_arg_2(float2 z) {
+  return mul2(z, fma2(both(kGeluTanhTwoC * kGeluTanhA), mul2(z, z), both(kGeluTanhTwoC)));
+}
+
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (ACT == CUOPX_ACT_RELU) return z > 0.f ? z : 0.f;
-  // Phi(z) = erfc(-z / sqrt 2) / 2 keeps its relative accuracy in the lower tail.
-  if constexpr (ACT == CUOPX_ACT_GELU) return z * (0.5f * erfcf(-kSqrtHalf * z));
-  if constexpr (ACT == CUOPX_ACT_GELU_TANH) return z * sigmoid_f(kGeluTanhTwoC * (z + kGeluTanhA * z * z * z));
-  if constexpr (ACT == CUOPX_ACT_SILU) return z * sigmoid_f(z);
-  if constexpr (ACT == CUOPX_ACT_SIGMOID) return sigmoid_f(z);
+__device__ __forceinline__ float2 act_value2(float2 z) {
+  float2 e;
+  if constexpr (ACT == CUOPX_ACT_RELU) return make_float2(z.x > 0.f ? z.x : 0.f, z.y > 0.f ? z.y : 0.f);
+  if constexpr (ACT == CUOPX_ACT_GELU) return mul2(z, normal_2(z, e));
+  if constexpr (ACT == CUOPX_ACT_GELU_TANH) return mul2(z, sigmoid_2(gelu_tanh_arg_2(z), e));
+  if constexpr (ACT == CUOPX_ACT_SILU) return mul2(z, sigmoid_2(z, e));
+  if constexpr (ACT == CUOPX_ACT_SIGMOID) return sigmoid_2(z, e);
   return z;
+}
+
+// a b + c where a's factor d of the product has not vanished, c where it has:
+// z may be infinite there, or its powers beyond the range, and z d -> 0.
+__device__ __forceinline__ float2 vanishing_fma2(float2 d, float2 a, float2 b, float2 c) {
+  const float2 v = fma2(a, b, c);
+  return make_float2(d.x > 0.f ? v.x : c.x, d.y > 0.f ? v.y : c.y);
 }
 
 // Value and derivative at z.
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z, float& value) {
+__device__ __forceinline__ float2 act_slope2(float2 z, float2& value) {
+  float2 e;
   if constexpr (ACT == CUOPX_ACT_RELU) {
-    value = z > 0.f ? z : 0.f;
-    return z > 0.f ? 1.f : 0.f;
+    value = act_value2<ACT>(z);
+    return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   }
   if constexpr (ACT == CUOPX_ACT_GELU) {
-    const float phi = 0.5f * erfcf(-kSqrtHalf * z);
-    value = z * phi;
-    const float d = kInvSqrt2Pi * __expf(-0.5f * z * z);
-    return d > 0.f ? fmaf(z, d, phi) : phi;  // z infinite or its square beyond the range: z d -> 0
+    const float2 phi = normal_2(z, e);
+    value = mul2(z, phi);
+    return vanishing_fma2(e, z, e, phi);
   }
   if constexpr (ACT == CUOPX_ACT_GELU_TANH) {
-    const float u = kGeluTanhTwoC * (z + kGeluTanhA * z * z * z);
-    const float s = sigmoid_f(u), d = sigmoid_slope_f(u);
-    value = z * s;
-    return d > 0.f ? fmaf(z * d, kGeluTanhTwoC * (1.f + 3.f * kGeluTanhA * z * z), s) : s;
+    const float2 s = sigmoid_2(gelu_tanh_arg_2(z), e);
+    const float2 d = sigmoid_slope_2(e, s);
+    value = mul2(z, s);
+    return vanishing_fma2(d, mul2(z, d), fma2(both(3.f * kGeluTanhTwoC * kGeluTanhA), mul2(z, z), both(kGeluTanhTwoC)), s);
   }
   if constexpr (ACT == CUOPX_ACT_SILU) {
-    const float s = sigmoid_f(z), d = sigmoid_slope_f(z);
-    value = z * s;
-    return d > 0.f ? fmaf(z, d, s) : s;
+    const float2 s = sigmoid_2(z, e);
+    const float2 d = sigmoid_slope_2(e, s);
+    value = mul2(z, s);
+    return vanishing_fma2(d, z, d, s);
   }
   if constexpr (ACT == CUOPX_ACT_SIGMOID) {
-    value = sigmoid_f(z);
-    return sigmoid_slope_f(z);
+    value = sigmoid_2(z, e);
+    return sigmoid_slope_2(e, value);
   }
   value = z;
-  return 1.f;
+  return both(1.f);
+}
+
+// The same for one element.
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  return act_value2<ACT>(both(z)).x;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z, float& value) {
+  float2 v;
+  const float2 d = act_slope2<ACT>(both(z), v);
+  value = v.x;
+  return d.x;
 }
 
 // Calls f with std::integral_constant<int, ACT>: one uniform branch around a

@@ -188,12 +188,12 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
     }
     with_activation(e.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) a[i] = act_value<act.value>(a[i]);
+      for (int i = 0; i < 32; i += 2) {
+        float2 y = act_value2<act.value>(make_float2(a[i], a[i + 1]));
+        if constexpr (GATED) y = mul2(y, make_float2(b[i], b[i + 1]));
+        a[i] = y.x, a[i + 1] = y.y;
+      }
     });
-    if constexpr (GATED) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) a[i] *= b[i];
-    }
     if (has_res) {
       add_row32<T>(a, res);
       if (half + 1 < COLS / 32) load_row32<T>(rrow, col + 32, N, e.vec_res, res);

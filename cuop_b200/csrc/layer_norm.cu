@@ -145,33 +145,9 @@ __device__ __forceinline__ void store_vec(T* p, const RowVec<T, V>& r) {
   else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
-// Two fp32 operations per instruction (sm_100's packed f32x2 forms, each half
-// rounded like the scalar one): at 16 bits an element HBM leaves about 22
-// issue slots per element forward and 32 backward, and conversions take most.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
 // Elements 2i and 2i + 1 of a group widened, and two results rounded into it.
+// Arithmetic is in packed pairs: at 16 bits an element HBM leaves about 22
+// issue slots per element forward and 32 backward.
 template <typename T, int V>
 __device__ __forceinline__ float2 widen2(const RowVec<T, V>& r, int i) {
   if constexpr (sizeof(T) == 2 && V % 2 == 0) {

@@ -13,6 +13,7 @@
 #include "activation.cuh"
 #include "common.cuh"
 #include "dispatch.h"
+#include "layer_epilogue.cuh"
 
 namespace cuopx {
 
@@ -196,9 +197,12 @@ __device__ __forceinline__ void load_acc(const T* src, float (&v)[V]) {
   } else {
     static_assert(V == 8, "16-byte groups");
     const uint4 raw = *reinterpret_cast<const uint4*>(src);
-    const T* e = reinterpret_cast<const T*>(&raw);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_acc<T>(e[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2_layer<T>(w[i]);
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
   }
 }
 
@@ -207,11 +211,8 @@ __device__ __forceinline__ void store_acc(T* dst, const float (&v)[V]) {
   if constexpr (V == 1) {
     *dst = from_acc<T>(v[0]);
   } else {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_acc<T>(v[i]);
-    *reinterpret_cast<uint4*>(dst) = raw;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2_layer<T>(v[0], v[1]), pack2_layer<T>(v[2], v[3]),
+                                                pack2_layer<T>(v[4], v[5]), pack2_layer<T>(v[6], v[7]));
   }
 }
 
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   const int64_t c = (blockIdx.x * 32ll + lane) * V;
   const int64_t r0 = p.M * blockIdx.y / p.splits, r1 = p.M * (blockIdx.y + 1) / p.splits;
   float sum[NB][V] = {};
+  grid_dependency_wait();
   if (c < p.N) {
     with_activation(p.act, [&](auto act) {
 #pragma unroll 2
@@ -233,20 +235,35 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
           float a[V], b[V];
           load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + c, a);
           load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + p.N + c, b);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
+          if constexpr (V == 1) {
             float value;
-            const float slope = act_slope<act.value>(a[i], value);
-            d[0][i] = g[i] * b[i] * slope;
-            d[NB - 1][i] = g[i] * value;
+            const float slope = act_slope<act.value>(a[0], value);
+            d[0][0] = g[0] * b[0] * slope;
+            d[NB - 1][0] = g[0] * value;
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+              float2 value;
+              const float2 slope = act_slope2<act.value>(make_float2(a[i], a[i + 1]), value);
+              const float2 gg = make_float2(g[i], g[i + 1]);
+              const float2 d0 = mul2(mul2(gg, make_float2(b[i], b[i + 1])), slope), d1 = mul2(gg, value);
+              d[0][i] = d0.x, d[0][i + 1] = d0.y;
+              d[NB - 1][i] = d1.x, d[NB - 1][i + 1] = d1.y;
+            }
           }
         } else if constexpr (act.value != CUOPX_ACT_NONE) {
           float z[V];
           load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + c, z);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
+          if constexpr (V == 1) {
             float value;
-            d[0][i] = g[i] * act_slope<act.value>(z[i], value);
+            d[0][0] = g[0] * act_slope<act.value>(z[0], value);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+              float2 value;
+              const float2 v = mul2(make_float2(g[i], g[i + 1]), act_slope2<act.value>(make_float2(z[i], z[i + 1]), value));
+              d[0][i] = v.x, d[0][i + 1] = v.y;
+            }
           }
         } else {
 #pragma unroll
@@ -281,20 +298,32 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   }
 }
 
-// Adds the shares' sums in ascending order and rounds once.
+// Adds the shares' sums: 32 columns per CTA, every eighth share per warp, then
+// the eight warps' sums in order; one rounding.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, int splits, int64_t wide, T* db) {
-  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
-  if (c >= wide) return;
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * 32ll + lane;
+  grid_dependency_wait();
   float s = 0.f;
-  for (int i = 0; i < splits; ++i) s += partial[i * wide + c];
-  db[c] = from_acc<T>(s);
+  if (c < wide) {
+#pragma unroll 4
+    for (int i = warp; i < splits; i += 8) s += partial[i * wide + c];
+  }
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < wide) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][lane];
+    db[c] = from_acc<T>(s);
+  }
 }
 
 // Below this many multiplications the SIMT kernel, which takes any alignment,
 // beats copying unaligned operands and running on the tensor cores: two more
-// launches cost about 4 us, in which it does some 2^24 products.
-constexpr double kRepackMinWork = 16777216.0;
+// launches cost about 4 us.
+constexpr double kRepackMinWork = 1048576.0;
 
 // The kernel for a problem whose operands are as aligned as they will be.
 int linear_route(const LinearProblem& p, cudaStream_t stream) {
@@ -328,7 +357,9 @@ BackwardPlan backward_plan(const cuopx_linear_backward_args& a, bool gated) {
   const bool vec = a.N % 8 == 0 && row_aligned16(a.dY, a.lddy) && (!act || row_aligned16(a.preact, a.ldz));
   q.v = vec ? 8 : 1;
   const int64_t strips = (a.N + 32 * q.v - 1) / (32 * q.v);
-  const int64_t want = (static_cast<int64_t>(device_sm_count()) * 4 + strips - 1) / strips;
+  // About 32 CTAs per SM, eight times what is resident, so that the last wave
+  // costs little (4096 x 28672: 6 shares 243 us, 43 shares see the table).
+  const int64_t want = (static_cast<int64_t>(device_sm_count()) * 32 + strips - 1) / strips;
   q.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (a.M + 15) / 16, 1024})));
   size_t off = 0;
   auto take = [&](bool want_it, size_t bytes) {
@@ -357,17 +388,21 @@ int backward_product(const LinearProblem& p, bool tensor, cudaStream_t stream) {
 }
 
 template <typename T, bool GATED>
-void launch_dz(const DzParams& d, int v, cudaStream_t stream) {
+int launch_dz(const DzParams& d, int v, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((d.N + 32 * v - 1) / (32 * v)), static_cast<unsigned>(d.splits));
-  if (v == 8) linear_dz_kernel<T, GATED, 8><<<grid, 256, 0, stream>>>(d);
-  else linear_dz_kernel<T, GATED, 1><<<grid, 256, 0, stream>>>(d);
+  cudaError_t e = launch_pdl(v == 8 ? linear_dz_kernel<T, GATED, 8> : linear_dz_kernel<T, GATED, 1>, grid, dim3(256), 0, stream, d);
   note_launch("linear_dz");
-  if (d.splits > 1 && d.db) {
+  if (e == cudaSuccess && d.splits > 1 && d.db) {
     const int64_t wide = GATED ? 2 * d.N : d.N;
-    linear_db_finish<T><<<static_cast<unsigned>((wide + 255) / 256), 256, 0, stream>>>(d.partial, d.splits, wide,
-                                                                                      static_cast<T*>(d.db));
+    e = launch_pdl(linear_db_finish<T>, dim3(static_cast<unsigned>((wide + 31) / 32)), dim3(256), 0, stream, d.partial,
+                   d.splits, wide, static_cast<T*>(d.db));
     note_launch("linear_db_finish");
   }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_failure(e);
+  }
+  return check_launch();
 }
 
 bool activation_ok(int act) { return act >= CUOPX_ACT_NONE && act <= CUOPX_ACT_SIGMOID; }
@@ -514,9 +549,10 @@ int linear_backward(const cuopx_linear_backward_args* a, bool gated, cudaStream_
     }
     d.db = a->dbias;
     if (a->dbias && q.splits > 1) d.partial = reinterpret_cast<float*>(ws + q.partial_off);
-    if (a->dtype == CUOPX_BF16) gated ? launch_dz<__nv_bfloat16, true>(d, q.v, stream) : launch_dz<__nv_bfloat16, false>(d, q.v, stream);
-    else gated ? launch_dz<__half, true>(d, q.v, stream) : launch_dz<__half, false>(d, q.v, stream);
-    if (const int rc = check_launch(); rc != CUOPX_SUCCESS) return rc;
+    int rc;
+    if (a->dtype == CUOPX_BF16) rc = gated ? launch_dz<__nv_bfloat16, true>(d, q.v, stream) : launch_dz<__nv_bfloat16, false>(d, q.v, stream);
+    else rc = gated ? launch_dz<__half, true>(d, q.v, stream) : launch_dz<__half, false>(d, q.v, stream);
+    if (rc != CUOPX_SUCCESS) return rc;
   }
   if (a->dX && a->M > 0 && a->K > 0) {
     // dX [M][K] = dZ [M][wide] op(W)^T: W's columns are the products' depth.

@@ -33,14 +33,18 @@ constexpr int LSP_BK = 64;
 
 template <int TOK>
 struct SplitSmem {
-  static constexpr int STAGES = TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : 4;
+  static constexpr int STAGES = TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : TOK <= 128 ? 6 : 4;
   static constexpr int CTAS = TOK <= 64 ? 2 : 1;  // resident per SM
+  // From 128 rows on the partial sums reuse the ring, once every CTA of the
+  // cluster has finished its products; below, they have room of their own.
+  static constexpr bool ALIAS = TOK >= 128;
   static constexpr int W_STAGE = LSP_COLS * LSP_BK * 2;
   static constexpr int X_STAGE = TOK * LSP_BK * 2;
   static constexpr int OFF_W = 0;
   static constexpr int OFF_X = OFF_W + STAGES * W_STAGE;
-  static constexpr int OFF_SUM = OFF_X + STAGES * X_STAGE;  // [cs][TOK][128 / cs] fp32
-  static constexpr int OFF_BAR = OFF_SUM + TOK * LSP_COLS * 4;
+  static constexpr int OFF_SUM = ALIAS ? 0 : OFF_X + STAGES * X_STAGE;  // [cs][TOK][128 / cs] fp32
+  static constexpr int OFF_BAR = OFF_X + STAGES * X_STAGE + (ALIAS ? 0 : TOK * LSP_COLS * 4);
+  static_assert(!ALIAS || TOK * LSP_COLS * 4 <= OFF_BAR, "the ring holds the partial sums");
   static constexpr int NUM_BARS = 2 * STAGES + 2;  // full, empty, acc_full, drain
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
@@ -136,8 +140,9 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  // Remote stores come only after every CTA of the cluster has started.
-  if (cs > 1) cluster_arrive_relaxed();
+  // Remote stores come only after every CTA of the cluster has started (or,
+  // into a ring, has read it: the epilogue warps arrive after their accumulator).
+  if (cs > 1 && !L::ALIAS) cluster_arrive_relaxed();
   const uint32_t tmem_base = *tmem_slot;
   grid_dependency_wait();
 
@@ -182,6 +187,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       }
     }
     __syncwarp();
+    if (cs > 1 && L::ALIAS) cluster_arrive();
     if (cs > 1) cluster_wait();
   } else if (warp == 1) {
     if (lane == 0) {
@@ -222,11 +228,13 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       }
     }
     __syncwarp();
+    if (cs > 1 && L::ALIAS) cluster_arrive();
     if (cs > 1) cluster_wait();
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full, 0, kDevErrWaitTimeoutAccFull, abort_flag));
     tc_fence_after_sync();
+    if (cs > 1 && L::ALIAS) cluster_arrive();
     if (cs > 1) cluster_wait();
     // Owner of this lane's column of W, and the column's place among its own.
     const int l = 32 * q + lane;
@@ -298,7 +306,8 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
           if (two) zp[1] = from_acc<T>(z[h][1]);
         }
       }
-      float y0 = act_value<act.value>(z[0][0]), y1 = act_value<act.value>(z[0][1]);
+      const float2 v = act_value2<act.value>(make_float2(z[0][0], z[0][1]));
+      float y0 = v.x, y1 = v.y;
       if constexpr (GATED) y0 *= z[1][0], y1 *= z[1][1];
       if (R) {
         const T* rp = R + row * p.ldr + col;
