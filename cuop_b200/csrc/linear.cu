@@ -174,11 +174,13 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // ---------------------------------------------------------------- dZ and its column sums
 // One pass over dY (and Z): writes dZ and, per share of the rows, the fp32
 // column sums of the unrounded dZ.  A thread owns V columns (V = 8: one
-// 16-byte load per matrix and row), a warp 32 V of them; the eight warps of a
-// CTA walk interleaved rows of its share.  Bound by HBM.
+// 16-byte load per matrix and row) of every row that it walks; `across` of a
+// CTA's eight warps lie side by side, so that a row is read in runs of up to 4
+// KB (512-byte runs of eight rows measured 3.3 TB/s), and the others take the
+// rows between.  Several rows are loaded before the first is used.  Bound by HBM.
 struct DzParams {
   int64_t M, N;
-  int act;
+  int act, across;
   const void* dY;
   int64_t lddy;
   const void* Z;
@@ -191,89 +193,87 @@ struct DzParams {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_acc(const T* src, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = to_acc<T>(*src);
+struct Packed {
+  uint32_t w[V == 8 ? 4 : 1];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Packed<T, V> load_packed(const T* src) {
+  Packed<T, V> r;
+  if constexpr (V == 8) {
+    const uint4 q = *reinterpret_cast<const uint4*>(src);
+    r.w[0] = q.x, r.w[1] = q.y, r.w[2] = q.z, r.w[3] = q.w;
   } else {
-    static_assert(V == 8, "16-byte groups");
-    const uint4 raw = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2_layer<T>(w[i]);
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
+    r.w[0] = *reinterpret_cast<const unsigned short*>(src);
   }
+  return r;
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void store_acc(T* dst, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    *dst = from_acc<T>(v[0]);
-  } else {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2_layer<T>(v[0], v[1]), pack2_layer<T>(v[2], v[3]),
-                                                pack2_layer<T>(v[4], v[5]), pack2_layer<T>(v[6], v[7]));
-  }
+__device__ __forceinline__ void store_packed(T* dst, const Packed<T, V>& r) {
+  if constexpr (V == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  else *reinterpret_cast<unsigned short*>(dst) = static_cast<unsigned short>(r.w[0]);
 }
 
 template <typename T, bool GATED, int V>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   constexpr int NB = GATED ? 2 : 1;
+  constexpr int PAIRS = V == 8 ? 4 : 1;   // a single column is the first half of a pair
+  constexpr int ROWS = GATED ? 2 : 4;     // loaded ahead
   __shared__ float sums[8][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (blockIdx.x * 32ll + lane) * V;
+  const int side = warp % p.across, phase = warp / p.across, phases = 8 / p.across;
+  const int64_t c = ((blockIdx.x * static_cast<int64_t>(p.across) + side) * 32 + lane) * V;
   const int64_t r0 = p.M * blockIdx.y / p.splits, r1 = p.M * (blockIdx.y + 1) / p.splits;
-  float sum[NB][V] = {};
+  const bool reads_z = GATED || p.act != CUOPX_ACT_NONE;
+  float2 sum[NB][PAIRS];
+#pragma unroll
+  for (int h = 0; h < NB; ++h)
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) sum[h][i] = both(0.f);
   grid_dependency_wait();
   if (c < p.N) {
     with_activation(p.act, [&](auto act) {
-#pragma unroll 2
-      for (int64_t r = r0 + warp; r < r1; r += 8) {
-        float g[V], d[NB][V];
-        load_acc<T, V>(static_cast<const T*>(p.dY) + r * p.lddy + c, g);
-        if constexpr (GATED) {
-          float a[V], b[V];
-          load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + c, a);
-          load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + p.N + c, b);
-          if constexpr (V == 1) {
-            float value;
-            const float slope = act_slope<act.value>(a[0], value);
-            d[0][0] = g[0] * b[0] * slope;
-            d[NB - 1][0] = g[0] * value;
-          } else {
+      for (int64_t rb = r0 + phase; rb < r1; rb += ROWS * phases) {
+        Packed<T, V> g[ROWS], z[ROWS][NB];
 #pragma unroll
-            for (int i = 0; i < V; i += 2) {
-              float2 value;
-              const float2 slope = act_slope2<act.value>(make_float2(a[i], a[i + 1]), value);
-              const float2 gg = make_float2(g[i], g[i + 1]);
-              const float2 d0 = mul2(mul2(gg, make_float2(b[i], b[i + 1])), slope), d1 = mul2(gg, value);
-              d[0][i] = d0.x, d[0][i + 1] = d0.y;
-              d[NB - 1][i] = d1.x, d[NB - 1][i + 1] = d1.y;
-            }
+        for (int j = 0; j < ROWS; ++j) {
+          const int64_t r = rb + j * phases;
+          if (r >= r1) break;
+          g[j] = load_packed<T, V>(static_cast<const T*>(p.dY) + r * p.lddy + c);
+          if (reads_z) {
+#pragma unroll
+            for (int h = 0; h < NB; ++h) z[j][h] = load_packed<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + h * p.N + c);
           }
-        } else if constexpr (act.value != CUOPX_ACT_NONE) {
-          float z[V];
-          load_acc<T, V>(static_cast<const T*>(p.Z) + r * p.ldz + c, z);
-          if constexpr (V == 1) {
-            float value;
-            d[0][0] = g[0] * act_slope<act.value>(z[0], value);
-          } else {
-#pragma unroll
-            for (int i = 0; i < V; i += 2) {
-              float2 value;
-              const float2 v = mul2(make_float2(g[i], g[i + 1]), act_slope2<act.value>(make_float2(z[i], z[i + 1]), value));
-              d[0][i] = v.x, d[0][i + 1] = v.y;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) d[0][i] = g[i];
         }
 #pragma unroll
-        for (int h = 0; h < NB; ++h) {
-          if (p.dZ) store_acc<T, V>(static_cast<T*>(p.dZ) + r * p.lddz + h * p.N + c, d[h]);
+        for (int j = 0; j < ROWS; ++j) {
+          const int64_t r = rb + j * phases;
+          if (r >= r1) break;
+          Packed<T, V> out[NB];
 #pragma unroll
-          for (int i = 0; i < V; ++i) sum[h][i] += d[h][i];
+          for (int i = 0; i < PAIRS; ++i) {
+            const float2 gg = unpack2_layer<T>(g[j].w[i]);
+            float2 d[NB], value;
+            if constexpr (GATED) {
+              const float2 slope = act_slope2<act.value>(unpack2_layer<T>(z[j][0].w[i]), value);
+              d[0] = mul2(mul2(gg, unpack2_layer<T>(z[j][NB - 1].w[i])), slope);
+              d[NB - 1] = mul2(gg, value);
+            } else if constexpr (act.value != CUOPX_ACT_NONE) {
+              d[0] = mul2(gg, act_slope2<act.value>(unpack2_layer<T>(z[j][0].w[i]), value));
+            } else {
+              d[0] = gg;
+            }
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+              sum[h][i] = add2(sum[h][i], d[h]);
+              out[h].w[i] = pack2_layer<T>(d[h].x, d[h].y);
+            }
+          }
+          if (p.dZ) {
+#pragma unroll
+            for (int h = 0; h < NB; ++h) store_packed<T, V>(static_cast<T*>(p.dZ) + r * p.lddz + h * p.N + c, out[h]);
+          }
         }
       }
     });
@@ -283,14 +283,14 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   for (int h = 0; h < NB; ++h) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[warp][i * 32 + lane] = sum[h][i];
+    for (int i = 0; i < V; ++i) sums[warp][i * 32 + lane] = i % 2 ? sum[h][i / 2].y : sum[h][i / 2].x;
     __syncthreads();
-    // Thread t adds the eight warps' sums of V / 8 (at least one) column of the CTA.
-    for (int e = threadIdx.x; e < 32 * V; e += 256) {
+    // Adds the row phases' sums of every column of the CTA, in phase order.
+    for (int e = threadIdx.x; e < p.across * 32 * V; e += 256) {
+      const int w = e / (32 * V), k = e % (32 * V);
       float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) s += sums[w][e];
-      const int64_t col = (blockIdx.x * 32ll + (e & 31)) * V + (e >> 5);
+      for (int q = 0; q < phases; ++q) s += sums[q * p.across + w][k];
+      const int64_t col = ((blockIdx.x * static_cast<int64_t>(p.across) + w) * 32 + (k & 31)) * V + (k >> 5);
       if (col >= p.N) continue;
       if (p.splits > 1) p.partial[blockIdx.y * (NB * p.N) + h * p.N + col] = s;
       else static_cast<T*>(p.db)[h * p.N + col] = from_acc<T>(s);
@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   }
 }
 
-// Adds the shares' sums: 32 columns per CTA, every eighth share per warp, then
-// the eight warps' sums in order; one rounding.
+// Adds the shares' sums: 32 columns per CTA, every eighth share per warp (eight
+// loads in flight), then the warps' sums in order; one rounding.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, int splits, int64_t wide, T* db) {
   __shared__ float part[8][32];
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, in
   grid_dependency_wait();
   float s = 0.f;
   if (c < wide) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < splits; i += 8) s += partial[i * wide + c];
   }
   part[warp][lane] = s;
@@ -339,7 +339,7 @@ struct BackwardPlan {
   bool copy_x, copy_w;   // aligned copies for the products
   bool tensor;           // products on the tensor cores whatever the alignment of dX and dW
   int64_t lddz;
-  int v, splits;
+  int v, across, splits;
   size_t dz_off, partial_off, x_off, w_off, bytes;
 };
 
@@ -356,11 +356,13 @@ BackwardPlan backward_plan(const cuopx_linear_backward_args& a, bool gated) {
   q.lddz = round8(wide);
   const bool vec = a.N % 8 == 0 && row_aligned16(a.dY, a.lddy) && (!act || row_aligned16(a.preact, a.ldz));
   q.v = vec ? 8 : 1;
-  const int64_t strips = (a.N + 32 * q.v - 1) / (32 * q.v);
-  // About 32 CTAs per SM, eight times what is resident, so that the last wave
-  // costs little (4096 x 28672: 6 shares 243 us, 43 shares see the table).
-  const int64_t want = (static_cast<int64_t>(device_sm_count()) * 32 + strips - 1) / strips;
-  q.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (a.M + 15) / 16, 1024})));
+  q.across = a.N > 128 * q.v ? 8 : a.N > 64 * q.v ? 4 : a.N > 32 * q.v ? 2 : 1;
+  const int64_t strips = (a.N + 32 * q.v * q.across - 1) / (32 * q.v * q.across);
+  // About 16 CTAs per SM, several times what is resident, so that the last
+  // wave costs little; at least 8 rows (two batches of loads) for every row phase.
+  const int64_t want = (static_cast<int64_t>(device_sm_count()) * 16 + strips - 1) / strips;
+  const int64_t least = 8 * (8 / q.across);
+  q.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (a.M + least - 1) / least, 1024})));
   size_t off = 0;
   auto take = [&](bool want_it, size_t bytes) {
     const size_t at = off;
@@ -389,7 +391,8 @@ int backward_product(const LinearProblem& p, bool tensor, cudaStream_t stream) {
 
 template <typename T, bool GATED>
 int launch_dz(const DzParams& d, int v, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((d.N + 32 * v - 1) / (32 * v)), static_cast<unsigned>(d.splits));
+  const int64_t strip = 32ll * v * d.across;
+  const dim3 grid(static_cast<unsigned>((d.N + strip - 1) / strip), static_cast<unsigned>(d.splits));
   cudaError_t e = launch_pdl(v == 8 ? linear_dz_kernel<T, GATED, 8> : linear_dz_kernel<T, GATED, 1>, grid, dim3(256), 0, stream, d);
   note_launch("linear_dz");
   if (e == cudaSuccess && d.splits > 1 && d.db) {
@@ -541,6 +544,7 @@ int linear_backward(const cuopx_linear_backward_args* a, bool gated, cudaStream_
     d.Z = a->preact;
     d.ldz = a->ldz;
     d.splits = q.splits;
+    d.across = q.across;
     if (q.need_dz) {
       d.dZ = ws + q.dz_off;
       d.lddz = q.lddz;
