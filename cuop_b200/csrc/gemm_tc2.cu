@@ -56,17 +56,12 @@ namespace {
 
 constexpr int P_BM = 128;  // rows per CTA (pair: 256)
 constexpr int P_BK = 64;
-constexpr int P_THREADS = 192;
-constexpr int P_EPI_WARPS = 4;
 constexpr int P_CHUNK = 64;
 constexpr uint32_t P_TMEM_COLS = 512;
 constexpr int P_MAX_SLOTS = 4;    // TMEM slots at the narrowest tile (128 columns each)
 constexpr int P_GROUP_M = 8;      // pair-row tiles per raster group
 // Scheduler ring depth (> the producers' lead over the epilogue, in tiles).
 constexpr int P_CLC_SLOTS = 16;
-// Arrivals on the leader's clc_empty per slot: leader producer, MMA issuer and
-// epilogue warps, plus the partner's producer and epilogue warps (remote).
-constexpr int P_CLC_READERS = (2 + P_EPI_WARPS) + (1 + P_EPI_WARPS);
 
 template <int PBN>
 struct PairCfg {
@@ -79,11 +74,23 @@ struct PairCfg {
 
 enum PairMode { kPairGemm = 0, kPairLinear = 1, kPairGated = 2 };
 
-// kPairGated stages three output tiles per chunk (both pre-activations and
-// the result) instead of two, which takes the room of one ring stage.
+// kPairLinear drains a tile with eight warps, two per TMEM lane quarter and
+// half of the columns each: its activation and residual make the drain of the
+// last tile, which nothing overlaps, several microseconds long.  kPairGated
+// stages three output tiles per chunk (both pre-activations and the result)
+// instead of two.  Either takes the room of a ring stage, both would take two.
+template <int MODE>
+struct PairWarps {
+  static constexpr int EPI = MODE == kPairLinear ? 8 : 4;
+  static constexpr int THREADS = 32 * (2 + EPI);
+  // Arrivals on the leader's clc_empty per slot: leader producer, MMA issuer and
+  // epilogue warps, plus the partner's producer and epilogue warps (remote).
+  static constexpr int CLC_READERS = (2 + EPI) + (1 + EPI);
+};
+
 template <int PBN, int MODE = kPairGemm>
 struct PairSmem {
-  static constexpr int STAGES = PairCfg<PBN>::STAGES - (MODE == kPairGated ? 1 : 0);
+  static constexpr int STAGES = PairCfg<PBN>::STAGES - (MODE == kPairGemm ? 0 : PBN == 128 && MODE == kPairLinear ? 2 : 1);
   static constexpr int C_BUFS = MODE == kPairGated ? 3 : 2;
   static constexpr int A_STAGE = P_BM * P_BK * 2;               // 16 KB
   static constexpr int B_PIECE = (PairCfg<PBN>::SLOT / 2) * P_BK * 2;  // this CTA's half of one slot
@@ -92,7 +99,7 @@ struct PairSmem {
   static constexpr int OFF_A = 0;
   static constexpr int OFF_B = STAGES * A_STAGE;
   static constexpr int OFF_C = OFF_B + STAGES * B_STAGE;
-  static constexpr int OFF_BAR = OFF_C + P_EPI_WARPS * C_BUFS * C_STAGE;
+  static constexpr int OFF_BAR = OFF_C + PairWarps<MODE>::EPI * C_BUFS * C_STAGE;
   // full[S], empty[S], acc_full[SLOTS], acc_empty[SLOTS], drain
   static constexpr int NUM_BARS = 2 * STAGES + 2 * PairCfg<PBN>::SLOTS + 1;
   // Tile-scheduler ring: P_CLC_SLOTS 16-byte launch-control responses, then
@@ -203,7 +210,7 @@ __device__ __forceinline__ uint32_t pack2_pair<__half>(float lo, float hi) {
 }
 
 template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THREADS, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const PairParams p,
                     const __grid_constant__ PairLayer<MODE> layer) {
@@ -245,11 +252,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     }
     for (int a = 0; a < P_SLOTS; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 2 * P_EPI_WARPS);  // leader's copy: 4 local + 4 remote arrivals
+      mbar_init(&acc_empty[a], 2 * PairWarps<MODE>::EPI);  // leader's copy: local + remote arrivals
     }
     for (int c = 0; c < P_CLC_SLOTS; ++c) {
       mbar_init(&clc_full[c], 1);  // leader: its expect_tx; partner: the leader's forward
-      mbar_init(&clc_empty[c], P_CLC_READERS);  // used on the leader only
+      mbar_init(&clc_empty[c], PairWarps<MODE>::CLC_READERS);  // used on the leader only
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -502,8 +509,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
           tmem_base + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(s0 * P_SLOT_COLS);
       if constexpr (MODE != kPairGemm) {
         constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
-        layer_epilogue_tile<T, MODE == kPairGated, COLS>(
-            t_row, nt * COLS, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ, &layer.tmZ2, stage_base, lane, sbuf,
+        constexpr int PART = COLS * 4 / PairWarps<MODE>::EPI;  // this warp's columns of the tile
+        const int c0 = (warp - 2) / 4 * PART;
+        layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
+            t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ, &layer.tmZ2, stage_base, lane, sbuf,
             [&] {
               tc_fence_before_sync();
               __syncwarp();
@@ -663,7 +672,7 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
   // One cluster per pair tile; running clusters take over unlaunched ones.
-  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(P_THREADS), L::ALLOC,
+  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(PairWarps<kPairGemm>::THREADS), L::ALLOC,
                                      stream, mA, mB, mC, prm, PairLayer<kPairGemm>{});
   if (lerr != cudaSuccess) {
     cudaGetLastError();
@@ -712,7 +721,7 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
       return CUOPX_CUDA_ERROR;
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
-  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(P_THREADS), L::ALLOC,
+  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(PairWarps<MODE>::THREADS), L::ALLOC,
                                       stream, mA, mB, mC, prm, layer);
   if (lerr != cudaSuccess) {
     cudaGetLastError();

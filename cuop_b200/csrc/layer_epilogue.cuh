@@ -129,12 +129,12 @@ __device__ __forceinline__ void store_chunk_plain(const unsigned char* buf, T* o
   __syncwarp();
 }
 
-// One warp's rows of one tile.  t_row: TMEM address of the tile's first
-// accumulator column in this warp's lane quarter; COLS output columns, those
-// of the second projection (GATED) COLS further on.  `stage`: 3 (GATED) or 2
+// One warp's rows of PART columns of one tile.  t_row: TMEM address of the
+// first of them in this warp's lane quarter; the second projection's (GATED)
+// are COLS further on.  `stage`: 3 (GATED) or 2
 // staging buffers of 4 KB.  release() is called once the accumulator has been
 // read.  (n0, m0): output column and first row of this warp's box.
-template <typename T, bool GATED, int COLS, typename Release>
+template <typename T, bool GATED, int COLS, int PART, typename Release>
 __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int m0, int M, int N, const LayerEpi& e,
                                                     const CUtensorMap* tmY, const CUtensorMap* tmZ,
                                                     const CUtensorMap* tmZ2, unsigned char* stage, int lane, int& ybuf,
@@ -148,14 +148,14 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
   uint4 res[4];
   if (has_res) load_row32<T>(rrow, n0, N, e.vec_res, res);
 #pragma unroll 1
-  for (int half = 0; half < COLS / 32; ++half) {
+  for (int half = 0; half < PART / 32; ++half) {
     const int h = half & 1;
     const int64_t col = static_cast<int64_t>(n0) + 32 * half;
     uint32_t ra[32], rb[GATED ? 32 : 1];
     tmem_ld_32x32b_x32(t_row + 32 * half, ra);
     if constexpr (GATED) tmem_ld_32x32b_x32(t_row + COLS + 32 * half, rb);
     tmem_wait_ld();
-    if (half == COLS / 32 - 1) release();
+    if (half == PART / 32 - 1) release();
     float a[32], b[GATED ? 32 : 1];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
@@ -196,7 +196,7 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
     });
     if (has_res) {
       add_row32<T>(a, res);
-      if (half + 1 < COLS / 32) load_row32<T>(rrow, col + 32, N, e.vec_res, res);
+      if (half + 1 < PART / 32) load_row32<T>(rrow, col + 32, N, e.vec_res, res);
     }
     stage_row32<T>(stage + ybuf * BUF, lane, h, a);
     if (h == 1) {
