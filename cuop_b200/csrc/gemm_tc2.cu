@@ -503,22 +503,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
       const int m0 = mt * 2 * P_BM + static_cast<int>(rank) * P_BM;
       const int n0 = nt * PBN;
       const int s0 = SPT == 1 ? acc : 0;
-      if (!mbar_wait_bounded(&acc_full[s0], (full_bits >> s0) & 1u, kDevErrWaitTimeoutAccFull, abort_flag)) break;
-      tc_fence_after_sync();
+      auto products = [&] {
+        const bool done = mbar_wait_bounded(&acc_full[s0], (full_bits >> s0) & 1u, kDevErrWaitTimeoutAccFull, abort_flag);
+        tc_fence_after_sync();
+        return done;
+      };
       const uint32_t t_row =
           tmem_base + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(s0 * P_SLOT_COLS);
       if constexpr (MODE != kPairGemm) {
         constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
         constexpr int PART = COLS * 4 / PairWarps<MODE>::EPI;  // this warp's columns of the tile
         const int c0 = (warp - 2) / 4 * PART;
-        layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
+        const bool done = layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
             t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ, &layer.tmZ2, stage_base, lane, sbuf,
+            [&] { return __all_sync(0xffffffffu, products()); },
             [&] {
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[s0], 0));
             });
+        if (!done) break;
       } else {
+      if (!products()) break;
       const int64_t grow = static_cast<int64_t>(m0) + row_in_tile;
 #pragma unroll 1
       for (int ch = 0; ch < PBN / P_CHUNK; ++ch) {

@@ -134,19 +134,31 @@ __device__ __forceinline__ void store_chunk_plain(const unsigned char* buf, T* o
 // are COLS further on.  `stage`: 3 (GATED) or 2
 // staging buffers of 4 KB.  release() is called once the accumulator has been
 // read.  (n0, m0): output column and first row of this warp's box.
-template <typename T, bool GATED, int COLS, int PART, typename Release>
-__device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int m0, int M, int N, const LayerEpi& e,
+template <typename T, bool GATED, int COLS, int PART, typename Wait, typename Release>
+__device__ __forceinline__ bool layer_epilogue_tile(uint32_t t_row, int n0, int m0, int M, int N, const LayerEpi& e,
                                                     const CUtensorMap* tmY, const CUtensorMap* tmZ,
                                                     const CUtensorMap* tmZ2, unsigned char* stage, int lane, int& ybuf,
-                                                    Release&& release) {
+                                                    Wait&& wait, Release&& release) {
   constexpr int BUF = 32 * 64 * 2;
   constexpr int NBUF = GATED ? 3 : 2;
   const int64_t grow = static_cast<int64_t>(m0) + lane;
   const bool has_res = !GATED && e.R != nullptr && grow < M;
   const T* rrow = static_cast<const T*>(e.R) + grow * e.ldr;
   const T* bias = static_cast<const T*>(e.bias);
-  uint4 res[4];
-  if (has_res) load_row32<T>(rrow, n0, N, e.vec_res, res);
+  // Bias and residual of the first half are on their way before the products
+  // are done, those of every other one while the one before it is worked on.
+  uint4 nbias[GATED ? 2 : 1][4], nres[GATED ? 1 : 4];
+  auto fetch = [&](int64_t col) {
+    if (bias) {
+      load_row32<T>(bias, col, N, e.vec_bias, nbias[0]);
+      if constexpr (GATED) load_row32<T>(bias + N, col, N, e.vec_bias, nbias[1]);
+    }
+    if constexpr (!GATED) {
+      if (has_res) load_row32<T>(rrow, col, N, e.vec_res, nres);
+    }
+  };
+  fetch(n0);
+  if (!wait()) return false;
 #pragma unroll 1
   for (int half = 0; half < PART / 32; ++half) {
     const int h = half & 1;
@@ -163,14 +175,15 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
       if constexpr (GATED) b[i] = __uint_as_float(rb[i]);
     }
     if (bias) {
-      uint4 raw[4];
-      load_row32<T>(bias, col, N, e.vec_bias, raw);
-      add_row32<T>(a, raw);
-      if constexpr (GATED) {
-        load_row32<T>(bias + N, col, N, e.vec_bias, raw);
-        add_row32<T>(b, raw);
-      }
+      add_row32<T>(a, nbias[0]);
+      if constexpr (GATED) add_row32<T>(b, nbias[1]);
     }
+    uint4 res[GATED ? 1 : 4];
+    if constexpr (!GATED) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) res[i] = nres[i];
+    }
+    if (half + 1 < PART / 32) fetch(col + 32);
     if (h == 0) {
       // The buffers this chunk fills: with a kept pre-activation all of them,
       // else one, the stores of the previous chunk having the other.
@@ -194,9 +207,8 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
         a[i] = y.x, a[i + 1] = y.y;
       }
     });
-    if (has_res) {
-      add_row32<T>(a, res);
-      if (half + 1 < PART / 32) load_row32<T>(rrow, col + 32, N, e.vec_res, res);
+    if constexpr (!GATED) {
+      if (has_res) add_row32<T>(a, res);
     }
     stage_row32<T>(stage + ybuf * BUF, lane, h, a);
     if (h == 1) {
@@ -217,7 +229,7 @@ __device__ __forceinline__ void layer_epilogue_tile(uint32_t t_row, int n0, int 
       }
       if (e.Y) store_chunk_plain<T>(stage + ybuf * BUF, static_cast<T*>(e.Y), e.ldy, 0, c, m0, M, N, lane);
     }
-  }
+  }  return true;
 }
 
 }  // namespace cuopx
