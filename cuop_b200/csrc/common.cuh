@@ -209,6 +209,30 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(Params...), dim3 grid, dim3
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Host: clusters of `cluster_x` CTAs of `kernel` that run at once on the
+// current device (the part's SMs come in groups that a cluster cannot span,
+// so this is less than SMs / cluster_x); 0 when it cannot be found out.
+template <typename... Params>
+inline int cluster_capacity(void (*kernel)(Params...), unsigned threads, size_t smem, unsigned cluster_x) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster_x);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster_x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
 // ---------------------------------------------------------------------------
 // Cluster launch control (sm_100): a running CTA asks the hardware to cancel
 // a CTA of the same grid that has not been launched yet and takes over its

@@ -13,5 +13,6 @@
 #include "vector_ops.cu"
 #include "layer_norm.cu"
 #include "dropout.cu"
+#include "linear_pair.cu"
 #include "linear_split.cu"
 #include "linear.cu"

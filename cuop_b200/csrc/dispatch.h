@@ -131,10 +131,13 @@ struct LinearProblem {
 // Base and rows on 16-byte boundaries (16-bit elements).
 inline bool row_aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && ld % 8 == 0; }
 
-// Layer forward pass on CTA pairs (gemm_tc2.cu); pbn: accumulator columns of
-// a tile, 256 or 128 (half as many outputs per row when gated).
+// Layer forward pass on CTA pairs (gemm_tc2.cu): 256 x 256 accumulator tiles
+// (256 x 128 outputs when gated).
 bool linear_tc2_supported(const LinearProblem& p);
-int linear_tc2(const LinearProblem& p, cudaStream_t stream, int pbn);
+int linear_tc2(const LinearProblem& p, cudaStream_t stream);
+// The same tiles with K split over the ks (2; linear also 4) pairs of a cluster (linear_pair.cu).
+int linear_pair(const LinearProblem& p, int ks, cudaStream_t stream);
+int linear_pair_capacity(int ks);  // tiles that run at once
 // Layer forward pass for few rows: swapped operands, K split over a cluster (linear_split.cu).
 bool linear_split_supported(const LinearProblem& p);
 int linear_split(const LinearProblem& p, cudaStream_t stream);

@@ -90,7 +90,7 @@ struct PairWarps {
 
 template <int PBN, int MODE = kPairGemm>
 struct PairSmem {
-  static constexpr int STAGES = PairCfg<PBN>::STAGES - (MODE == kPairGemm ? 0 : PBN == 128 && MODE == kPairLinear ? 2 : 1);
+  static constexpr int STAGES = PairCfg<PBN>::STAGES - (MODE == kPairGemm ? 0 : 1);
   static constexpr int C_BUFS = MODE == kPairGated ? 3 : 2;
   static constexpr int A_STAGE = P_BM * P_BK * 2;               // 16 KB
   static constexpr int B_PIECE = (PairCfg<PBN>::SLOT / 2) * P_BK * 2;  // this CTA's half of one slot
@@ -740,11 +740,11 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
 template <typename T, int PBN>
 int launch_tc2_layer_layout(const LinearProblem& p, cudaStream_t stream) {
   if (p.gated) {
-    const char* name = PBN == 256 ? "gated_linear_tc2_256x128" : "gated_linear_tc2_256x64";
+    const char* name = "gated_linear_tc2_256x128";
     return p.transW ? launch_tc2_layer<T, false, false, PBN, kPairGated>(p, stream, name)
                     : launch_tc2_layer<T, false, true, PBN, kPairGated>(p, stream, name);
   }
-  const char* name = PBN == 256 ? "linear_tc2_256x256" : "linear_tc2_256x128";
+  const char* name = "linear_tc2_256x256";
   if (p.transX) return launch_tc2_layer<T, true, true, PBN, kPairLinear>(p, stream, name);
   return p.transW ? launch_tc2_layer<T, false, false, PBN, kPairLinear>(p, stream, name)
                   : launch_tc2_layer<T, false, true, PBN, kPairLinear>(p, stream, name);
@@ -828,11 +828,9 @@ bool linear_tc2_supported(const LinearProblem& p) {
   return ((p.M + 255) / 256) * ((p.N + 63) / 64) < (int64_t(1) << 29);
 }
 
-int linear_tc2(const LinearProblem& p, cudaStream_t stream, int pbn) {
-  if (p.dtype == CUOPX_BF16)
-    return pbn == 256 ? launch_tc2_layer_layout<__nv_bfloat16, 256>(p, stream)
-                      : launch_tc2_layer_layout<__nv_bfloat16, 128>(p, stream);
-  return pbn == 256 ? launch_tc2_layer_layout<__half, 256>(p, stream) : launch_tc2_layer_layout<__half, 128>(p, stream);
+int linear_tc2(const LinearProblem& p, cudaStream_t stream) {
+  return p.dtype == CUOPX_BF16 ? launch_tc2_layer_layout<__nv_bfloat16, 256>(p, stream)
+                               : launch_tc2_layer_layout<__half, 256>(p, stream);
 }
 
 }  // namespace cuopx

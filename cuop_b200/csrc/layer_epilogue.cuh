@@ -132,13 +132,19 @@ __device__ __forceinline__ void store_chunk_plain(const unsigned char* buf, T* o
 // One warp's rows of PART columns of one tile.  t_row: TMEM address of the
 // first of them in this warp's lane quarter; the second projection's (GATED)
 // are COLS further on.  `stage`: 3 (GATED) or 2
-// staging buffers of 4 KB.  release() is called once the accumulator has been
-// read.  (n0, m0): output column and first row of this warp's box.
-template <typename T, bool GATED, int COLS, int PART, typename Wait, typename Release>
+// staging buffers of 4 KB.  wait() returns once the accumulator is complete (false: give up),
+// release() is called once it has been read, partial() adds what other CTAs
+// have summed.  (n0, m0): output column and first row of this warp's box.
+struct NoPartialSums {
+  template <typename... A>
+  __device__ __forceinline__ void operator()(A&&...) const {}
+};
+
+template <typename T, bool GATED, int COLS, int PART, typename Wait, typename Release, typename Partial = NoPartialSums>
 __device__ __forceinline__ bool layer_epilogue_tile(uint32_t t_row, int n0, int m0, int M, int N, const LayerEpi& e,
                                                     const CUtensorMap* tmY, const CUtensorMap* tmZ,
                                                     const CUtensorMap* tmZ2, unsigned char* stage, int lane, int& ybuf,
-                                                    Wait&& wait, Release&& release) {
+                                                    Wait&& wait, Release&& release, Partial&& partial = Partial{}) {
   constexpr int BUF = 32 * 64 * 2;
   constexpr int NBUF = GATED ? 3 : 2;
   const int64_t grow = static_cast<int64_t>(m0) + lane;
@@ -174,6 +180,7 @@ __device__ __forceinline__ bool layer_epilogue_tile(uint32_t t_row, int n0, int 
       a[i] = __uint_as_float(ra[i]);
       if constexpr (GATED) b[i] = __uint_as_float(rb[i]);
     }
+    partial(half, a, b);
     if (bias) {
       add_row32<T>(a, nbias[0]);
       if constexpr (GATED) add_row32<T>(b, nbias[1]);

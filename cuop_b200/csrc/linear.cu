@@ -325,10 +325,39 @@ __global__ void __launch_bounds__(256) linear_db_finish(const float* partial, in
 // launches cost about 4 us.
 constexpr double kRepackMinWork = 1048576.0;
 
+// How many pairs share a 256 x 256 tile's K loop.  Measured on B200 (bf16, us
+// for 1, 2 and 4 pairs): 256 x 2048 x 8192: 43.1, 26.4, 21.8; 512 x 4096 x
+// 4096: 25.3, 19.3, 48.0 (32 tiles: two waves of clusters of eight); 256 x
+// 1024 x 1024: 10.5, 9.7, 11.4; 1024 x 4096 x 4096 (64 tiles): 27.6, 37.6,
+// 81.1.  So: split while one wave holds all tiles, in four only for deep K.
+int pair_split(const LinearProblem& p) {
+  const int64_t cols = p.gated ? 128 : 256;
+  const int64_t tiles = ((p.M + 255) / 256) * ((p.N + cols - 1) / cols), k_blocks = (p.K + 63) / 64;
+  if (!p.gated && k_blocks >= 96 && tiles <= linear_pair_capacity(4)) return 4;
+  return k_blocks >= 12 && tiles <= linear_pair_capacity(2) ? 2 : 1;
+}
+
+// Whether few rows are better served by the split kernel than by pair tiles.
+// Up to 64 rows W's bytes bound it and two CTAs share an SM.  Above, a CTA's
+// 128 x 128 tile costs as many L2 bytes per K block as a pair's 256 x 256 one,
+// and it wins only while the pairs do not fill the part (128 rows, bf16, us,
+// split / pairs: 1024 x 1024 7.2 / 9.8; 4096 x 4096 14.2 / 17.5; N 16384, K
+// 4096 36.8 / 30.1; N 2048, K 8192 26.7 / 21.6).
+bool few_rows(const LinearProblem& p) {
+  if (p.M <= 64) return true;
+  if (p.M > 128) return false;
+  const int64_t tiles = (p.wide() + 255) / 256;
+  return tiles <= 32 && (p.K < 6144 || tiles > linear_pair_capacity(4));
+}
+
 // The kernel for a problem whose operands are as aligned as they will be.
 int linear_route(const LinearProblem& p, cudaStream_t stream) {
-  if (p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
-  if (linear_tc2_supported(p)) return linear_tc2(p, stream, 256);
+  const bool pair = linear_tc2_supported(p);
+  if (linear_split_supported(p) && few_rows(p)) return linear_split(p, stream);
+  if (pair) {
+    const int ks = pair_split(p);
+    return ks > 1 ? linear_pair(p, ks, stream) : linear_tc2(p, stream);
+  }
   if (p.transX) return CUOPX_NOT_IMPLEMENTED;  // not reached: its operands are aligned copies
   return linear_simt(p, stream);
 }
@@ -378,15 +407,17 @@ BackwardPlan backward_plan(const cuopx_linear_backward_args& a, bool gated) {
   return q;
 }
 
-// C [M][N] = X op(W) for the backward pass: a plain product when C's rows are
-// aligned (the GEMM back-ends), else the layer kernels, which store any rows.
+// C [M][N] = X op(W) for the backward pass, without an epilogue: the GEMM
+// back-ends when C's rows are aligned and there are tiles enough for them,
+// else the layer kernels, which store any rows and split K.
 int backward_product(const LinearProblem& p, bool tensor, cudaStream_t stream) {
-  if (!p.transX && p.M <= 128 && linear_split_supported(p)) return linear_split(p, stream);
-  if (!tensor || row_aligned16(p.Y, p.ldy)) {
-    GemmProblem g{p.dtype, p.transX, p.transW, p.M, p.N, p.K, 1.0, 0.0, p.X, p.ldx, 0, p.W, p.ldw, 0, p.Y, p.ldy, 0, 1};
-    return gemm_route(g, stream);
+  if (tensor && p.K > 0) {
+    const bool few = !p.transX && p.M <= 128 && linear_split_supported(p);
+    const bool pair = linear_tc2_supported(p);
+    if (few || (pair && (!row_aligned16(p.Y, p.ldy) || pair_split(p) > 1))) return linear_route(p, stream);
   }
-  return linear_route(p, stream);
+  GemmProblem g{p.dtype, p.transX, p.transW, p.M, p.N, p.K, 1.0, 0.0, p.X, p.ldx, 0, p.W, p.ldw, 0, p.Y, p.ldy, 0, 1};
+  return gemm_route(g, stream);
 }
 
 template <typename T, bool GATED>

@@ -355,20 +355,24 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   prm.Z = p.Z;
   prm.ldz = p.ldz;
   const int64_t tiles = static_cast<int64_t>(prm.tiles_n) * ((p.M + TOK - 1) / TOK);
-  // Split K while the clusters still run in one wave and every CTA keeps two K blocks.
-  const int64_t slots = static_cast<int64_t>(device_sm_count()) * L::CTAS;
-  int cs = 1;
-  while (cs < 8 && tiles * cs * 2 <= slots && prm.k_blocks >= cs * 4) cs *= 2;
-  prm.cs = cs;
   auto kern = linear_split_kernel<T, W_MN, GATED, TOK>;
   static std::atomic<bool> attr_set[64] = {};
+  static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
-  if (!attr_set[dev].load(std::memory_order_relaxed)) {
+  if (!attr_set[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
       return CUOPX_CUDA_ERROR;
-    attr_set[dev].store(true, std::memory_order_relaxed);
+    for (int i = 0; i < 4; ++i) capacity[dev][i].store(cluster_capacity(kern, LSP_THREADS, L::ALLOC, 1u << i), std::memory_order_relaxed);
+    attr_set[dev].store(true, std::memory_order_release);
   }
+  // Split K while the clusters still run in one wave and every CTA keeps two
+  // K blocks (a second wave of clusters of eight: 128 x 2048 x 8192 took 26.7
+  // us, clusters of four 18).
+  int cs = 1;
+  for (int i = 1; i < 4; ++i)
+    if (tiles <= capacity[dev][i].load(std::memory_order_relaxed) && prm.k_blocks >= (2 << i)) cs = 1 << i;
+  prm.cs = cs;
   const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), L::ALLOC,
                                              stream, static_cast<unsigned>(cs), mW, mX, prm);
   if (err != cudaSuccess) {

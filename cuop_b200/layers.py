@@ -117,7 +117,7 @@ def _linear(fn, gated: bool, x, w, bias, residual, activation, trans_w, out, pre
     ldx = _matrix(x, m, k, dtype, device, "x")
     ldw = _matrix(w, wide, k, dtype, device, "w") if trans_w else _matrix(w, k, wide, dtype, device, "w")
     if out is None:
-        out = _empty((m, n), dtype=dtype, device=x.device)
+        out = x.new_empty((m, n))
         ldy = n
     else:
         ldy = _matrix(out, m, n, dtype, device, "out")
@@ -256,7 +256,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     wp = 0 if weight is None else _vector(weight, cols, wdtype, device, "weight")
     bp = 0 if bias is None else _vector(bias, cols, wdtype, device, "bias")
     if out is None:
-        out = _empty((rows, cols), dtype=dtype, device=x.device)
+        out = x.new_empty((rows, cols))
         ldy = cols
     else:
         ldy = _matrix(out, rows, cols, dtype, device, "out")
