@@ -33,6 +33,11 @@ inline bool alias_ok(const void* out, int64_t ldo, const void* in, int64_t ldi, 
   if (out == in && ldo == ldi) return true;
   return !overlaps(out, span_bytes(rows, cols, ldo, es), in, span_bytes(rows, cols, ldi, es));
 }
+// Whether every pointer starts on a multiple of `bytes` (NULL does).
+template <typename... P>
+inline bool starts_on(size_t bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) % bytes) == 0;
+}
 // Process-wide fp32 arithmetic mode (cuopx_set_fp32_gemm_mode).
 int fp32_mode();
 

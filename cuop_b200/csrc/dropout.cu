@@ -167,6 +167,7 @@ int dropout_impl(const cuopx_dropout_args* a, cudaStream_t stream) {
   if (!a->X || !a->Y || a->ldx < a->cols || a->ldy < a->cols || (a->residual && a->ldr < a->cols))
     return CUOPX_INVALID_ARGUMENT;
   const size_t es = dtype_size(a->dtype);
+  if (!starts_on(es, a->X, a->residual, a->Y) || !starts_on(8, a->offset_dev)) return CUOPX_INVALID_ARGUMENT;
   if (!alias_ok(a->Y, a->ldy, a->X, a->ldx, a->rows, a->cols, es)) return CUOPX_INVALID_ARGUMENT;
   if (a->residual && !alias_ok(a->Y, a->ldy, a->residual, a->ldr, a->rows, a->cols, es)) return CUOPX_INVALID_ARGUMENT;
   if (a->offset_dev && overlaps(a->Y, span_bytes(a->rows, a->cols, a->ldy, es), a->offset_dev, 8))

@@ -450,6 +450,7 @@ int validate_linear(const cuopx_linear_args& a, bool gated) {
   if (a.M == 0 || a.N == 0) return CUOPX_SUCCESS;
   const int64_t wide = gated ? 2 * a.N : a.N;
   const int64_t w_rows = a.transW ? wide : a.K, w_cols = a.transW ? a.K : wide;
+  if (!starts_on(2, a.X, a.W, a.bias, a.residual, a.Y, a.preact) || !starts_on(256, a.workspace)) return CUOPX_INVALID_ARGUMENT;
   if (!a.Y || a.ldy < a.N || (a.preact && a.ldz < wide) || (a.residual && a.ldr < a.N)) return CUOPX_INVALID_ARGUMENT;
   if (a.K > 0 && (!a.X || !a.W || a.ldx < a.K || a.ldw < w_cols)) return CUOPX_INVALID_ARGUMENT;
   const size_t es = 2;
@@ -531,6 +532,7 @@ int validate_linear_backward(const cuopx_linear_backward_args& a, bool gated) {
   const bool reads_z = gated || a.activation != CUOPX_ACT_NONE;
   const bool dx = a.dX && a.K > 0 && a.M > 0, dw = a.dW && a.K > 0 && a.N > 0, db = a.dbias && a.N > 0;
   if (!dx && !dw && !db) return CUOPX_SUCCESS;
+  if (!starts_on(2, a.dY, a.X, a.W, a.preact, a.dX, a.dW, a.dbias) || !starts_on(256, a.workspace)) return CUOPX_INVALID_ARGUMENT;
   if (a.M > 0 && a.N > 0) {
     if (!a.dY || a.lddy < a.N || (reads_z && (!a.preact || a.ldz < wide))) return CUOPX_INVALID_ARGUMENT;
     if (dx && (!a.W || a.ldw < w_cols)) return CUOPX_INVALID_ARGUMENT;

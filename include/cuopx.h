@@ -292,8 +292,8 @@ int cuopx_iamin(int64_t n, const float* x, int64_t incx, int64_t* result, void* 
  * Feed-forward layer operators (no counterpart in the reference beyond
  * MatMulReluFused, see cuopx_gemm_ex).  Their arguments come in a struct:
  * zero-fill it, set what the call uses, leave optional pointers NULL.  The
- * pointers follow the rules above; sizes and leading dimensions are in
- * elements, matrices are row-major.  An output may not overlap an input or
+ * pointers follow the rules above and start on a multiple of their element's
+ * size; sizes and leading dimensions are in elements, matrices are row-major.  An output may not overlap an input or
  * another output, except where a comment allows it.
  *
  * Activations, with Phi the normal distribution function and s(z) =

@@ -57,6 +57,37 @@ def check_linear(x, w, b, r, act, trans_w, gated, preact=True, **kw):
     return y, z
 
 
+# name, rows, outputs, depth: each reaches the kernel of that name (also through aligned copies).
+KERNELS = [("linear_simt", 3, 8, 5), ("linear_split", 1, 264, 512), ("linear_split", 16, 136, 2000), ("linear_split", 30, 520, 320),
+           ("linear_split", 64, 1000, 700), ("linear_split", 100, 300, 264), ("linear_split", 5, 7, 40000),
+           ("linear_pair_k2", 129, 257, 801), ("linear_pair_k2", 700, 264, 1000), ("linear_pair_k2", 300, 1000, 1536),
+           ("linear_pair_k4", 140, 264, 6208), ("linear_pair_k4", 512, 257, 8001), ("linear_tc2_256x256", 300, 520, 264),
+           ("linear_tc2_256x256", 2600, 2056, 136)]
+GATED_KERNELS = [("gated_linear_simt", 3, 8, 5), ("gated_linear_split", 2, 72, 640), ("gated_linear_split", 50, 200, 1032),
+                 ("gated_linear_pair_k2", 129, 130, 801), ("gated_linear_pair_k2", 600, 264, 1000),
+                 ("gated_linear_tc2_256x128", 300, 264, 264), ("gated_linear_tc2_256x128", 1500, 1032, 200)]
+
+
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("name,m,n,k", KERNELS + GATED_KERNELS)
+def test_every_forward_kernel(name, m, n, k, trans_w):
+    g = gen(m + n)
+    gated = name.startswith("gated")
+    for dt, pad, shift in ((BF, 0, 0), (HF, 8, 8), (BF, 1, 1)):
+        x, w, b, r = operands(g, m, n, k, dt, trans_w, gated, True, not gated)
+        if pad:
+            x, w = strided(x, pad, shift)[0], strided(w, pad, shift)[0]
+        check_linear(x, w, b, r, "gelu_tanh", trans_w, gated)
+        # below 2^20 multiplications unaligned operands are not copied but take the SIMT kernel
+        small = shift == 1 and m * n * (2 if gated else 1) * k < 1 << 20
+        assert cx.last_kernel() == (("gated_linear_simt" if gated else "linear_simt") if small else name)
+        y = (cx.gated_linear(x, w) if gated else cx.linear(x, w)) if not trans_w else None
+        if y is not None and k < 3000:
+            act = "silu" if gated else "none"
+            ref, _, bound, _ = R.linear(x, w, None, None, act, False, gated)
+            R.assert_within(y, ref, bound, "no bias")
+
+
 SIZES = [(1, 1, 1), (1, 8, 8), (1, 64, 128), (1, 1000, 72), (2, 7, 31), (3, 40, 200), (5, 128, 64), (8, 264, 136),
          (16, 256, 512), (17, 129, 65), (24, 1024, 328), (33, 64, 1024), (64, 136, 96), (65, 512, 264), (129, 128, 64),
          (130, 72, 1000), (200, 333, 77), (257, 264, 256), (300, 1000, 200), (512, 512, 448), (700, 392, 512)]
@@ -146,7 +177,7 @@ def test_forward_special_values():
 def test_forward_is_deterministic_and_row_independent():
     """The same bits twice; a row's result does not depend on the other rows of the batch."""
     g = gen(9)
-    for m, n, k in ((4, 1024, 2048), (48, 512, 1024), (256, 512, 512)):
+    for m, n, k in ((4, 1024, 2048), (48, 512, 1024), (256, 512, 512), (256, 512, 2048), (300, 520, 6400)):
         x, w, b, r = operands(g, m, n, k, BF, False, False, True, True)
         y = cx.linear(x, w, b, r, activation="gelu")
         assert torch.equal(y, cx.linear(x, w, b, r, activation="gelu"))
@@ -158,7 +189,8 @@ def test_forward_is_deterministic_and_row_independent():
 @pytest.mark.parametrize("trans_w", [False, True])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 64, 128), (3, 7, 31), (16, 264, 136), (65, 129, 77), (130, 72, 200),
-                                   (257, 264, 256), (300, 1000, 200), (520, 512, 640)])
+                                   (257, 264, 256), (300, 1000, 200), (520, 512, 640), (1100, 136, 200),
+                                   (300, 1001, 333), (6300, 40, 72)])
 def test_backward_sizes(m, n, k, gated, trans_w):
     g = gen(m + n + k)
     for dt, act in ((BF, "silu"), (HF, "gelu"), (BF, "none")):
@@ -291,7 +323,8 @@ def test_layer_norm_sizes(rows, cols, dt, wt):
                 R.assert_within(t, ref, bound, name)
 
 
-@pytest.mark.parametrize("rows,cols", [(5, 40), (700, 512), (1500, 1024)])
+@pytest.mark.parametrize("rows,cols", [(5, 40), (700, 512), (1500, 1024), (2003, 96), (1201, 4096), (700, 8192), (301, 16384),
+                                       (1500, 333)])
 def test_layer_norm_without_weight_or_bias_and_many_rows(rows, cols):
     g = gen(4)
     x, dy = rnd(g, rows, cols), rnd(g, rows, cols)
