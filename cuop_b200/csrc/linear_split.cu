@@ -357,7 +357,7 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   const int64_t tiles = static_cast<int64_t>(prm.tiles_n) * ((p.M + TOK - 1) / TOK);
   auto kern = linear_split_kernel<T, W_MN, GATED, TOK>;
   static std::atomic<bool> attr_set[64] = {};
-  static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once
+  static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once, one CTA per SM
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
   if (!attr_set[dev].load(std::memory_order_acquire)) {
@@ -367,11 +367,17 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
     attr_set[dev].store(true, std::memory_order_release);
   }
   // Split K while the clusters still run in one wave and every CTA keeps two
-  // K blocks (a second wave of clusters of eight: 128 x 2048 x 8192 took 26.7
-  // us, clusters of four 18).
+  // K blocks.  The query counts one CTA per SM.  Where two fit, a few clusters
+  // more than a wave cost less than a shallower split: the others have the
+  // bandwidth meanwhile (us for clusters of 1, 2, 4, 8: 1 x 4096 x 4096, 32
+  // tiles, 30 at once: 21.5, 12.7, 9.6, 8.8; 24 x 8192 x 8192, 64 tiles: 44.7,
+  // 29.2, 23.6, 27.8; 128 x 2048 x 4096, one CTA per SM, 16 tiles, 15 at once:
+  // 33.3, 19.6, 12.7, 18.7).
   int cs = 1;
-  for (int i = 1; i < 4; ++i)
-    if (tiles <= capacity[dev][i].load(std::memory_order_relaxed) && prm.k_blocks >= (2 << i)) cs = 1 << i;
+  for (int i = 1; i < 4; ++i) {
+    const int64_t once = capacity[dev][i].load(std::memory_order_relaxed);
+    if (tiles <= (L::CTAS == 2 ? once * 20 / 9 : once) && prm.k_blocks >= (2 << i)) cs = 1 << i;
+  }
   prm.cs = cs;
   const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), L::ALLOC,
                                              stream, static_cast<unsigned>(cs), mW, mX, prm);
