@@ -94,6 +94,14 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutParams p)
   grid_dependency_wait();
   const uint64_t offset = p.offset + (p.offset_dev ? *p.offset_dev : 0);
   const int64_t per_row = (p.cols + V - 1) / V, groups = p.rows * per_row;
+  // Kept out of the constant bank, from which each round loads them anew:
+  // 44.4 -> 42.4 us for 8192 x 4096 bf16 with a residual (fp32 8192 x 8192: 137
+  // -> 128), but 33.5 -> 37.1 without one.
+  PhiloxKeys keys = p.keys;
+  if constexpr (RES) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) asm volatile("" : "+r"(keys.k0[r]), "+r"(keys.k1[r]));
+  }
   for (int64_t g = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; g < groups; g += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = p.rows == 1 ? 0 : g / per_row;
     const int64_t col = (g - row * per_row) * V;
@@ -119,7 +127,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutParams p)
     T* y = reinterpret_cast<T*>(&yr);
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
-      const Philox4 rnd = philox4x32_10(p.keys, offset + static_cast<uint64_t>(g * (V / 4) + q));
+      const Philox4 rnd = philox4x32_10(keys, offset + static_cast<uint64_t>(g * (V / 4) + q));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = 4 * q + j;

@@ -3,12 +3,15 @@
 several tiles, both weight layouts, strided and unaligned operands, single
 tokens, in-place operands, streams, captured graphs, and a whole block run
 forward and backward."""
+import threading
+
 import pytest
 import torch
 
 import cuop_b200 as cx
 import layer_refs as R
 from cuop_b200 import _native as N
+from cuop_b200 import layers as L
 
 pytestmark = pytest.mark.gpu
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -518,6 +521,103 @@ def test_two_captured_graphs():
     first = [t.clone() for t in graphs[0][1]]
     graphs[0][0].replay()
     assert not torch.equal(first[1], graphs[0][1][1])  # the counter moved on
+
+
+def test_several_host_threads():
+    """Four threads with a stream each give what one gives alone."""
+    g = gen(43)
+    x, w, b, _ = operands(g, 256, 512, 2048, BF, False, False, True, False)
+    dy = rnd(g, 256, 512)
+
+    def calls():
+        return (cx.linear(x, w, b, activation="gelu"), cx.linear(x[:3], w, b), cx.layer_norm(x)) + cx.linear_backward(dy, x, w)
+
+    ref, bad = calls(), []
+    torch.cuda.synchronize()
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                got = calls()
+            s.synchronize()
+        bad.extend(i for i, (a, c) in enumerate(zip(got, ref)) if not torch.equal(a, c))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.parametrize("m", [64, 700])
+def test_chains_of_dependent_launches(m):
+    """Every launch reads what the one before it wrote; launches may start early, their reads may not."""
+    g = gen(44)
+    x, ws = rnd(g, m, 1024), [rnd(g, 1024, 1024, scale=1 / 32) for _ in range(8)]
+
+    def chain():
+        t = x
+        for i, w in enumerate(ws):
+            t = cx.dropout(cx.layer_norm(cx.linear(t, w, residual=t, activation="silu")), 0.1, i)
+        return t
+
+    ref = chain()
+    torch.cuda.synchronize()
+    t = x
+    for i, w in enumerate(ws):  # step by step, each finished before the next
+        y = cx.linear(t, w, residual=t, activation="silu")
+        torch.cuda.synchronize()
+        h = cx.layer_norm(y)
+        torch.cuda.synchronize()
+        t = cx.dropout(h, 0.1, i)
+        torch.cuda.synchronize()
+    assert torch.equal(ref, t)
+    for _ in range(20):
+        assert torch.equal(chain(), ref)
+
+
+# ------------------------------------------------------------------ workspaces, through the C ABI
+def test_workspaces_are_large_enough():
+    """Calls with exactly the bytes that the size calls ask for write nothing behind them."""
+    lib, g = N.lib(), gen(45)
+    stream = torch.cuda.current_stream().cuda_stream
+    for m, n, k in ((5, 301, 999), (200, 133, 701), (333, 520, 64)):
+        for gated in (0, 1):
+            wide = 2 * n if gated else n
+            x, w, dy, z = rnd(g, m, k), rnd(g, k, wide, scale=k ** -0.5), rnd(g, m, n), rnd(g, m, wide)
+            y, dx, dw, db = (torch.empty_like(t) for t in (dy, x, w, w[0]))
+            head = (N.BF16, 0, 4, 0, m, n, k)
+            fwd = head + (x.data_ptr(), k, w.data_ptr(), wide, 0, 0, 0, y.data_ptr(), n, 0, 0)
+            bwd = head + (dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), wide, z.data_ptr(), wide, dx.data_ptr(), k,
+                          dw.data_ptr(), wide, db.data_ptr())
+            for name, fmt, args in (("linear", L._LINEAR, fwd), ("linear_backward", L._LINEAR_BACKWARD, bwd)):
+                name = ("gated_" if gated else "") + name
+                need = getattr(lib, f"cuopx_{name}_workspace_size")(fmt.pack(*args, 0, 0))
+                ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+                assert getattr(lib, "cuopx_" + name)(fmt.pack(*args, ws.data_ptr() if need else 0, need), stream) == N.SUCCESS
+                assert (ws[need:] == 0x5A).all()
+            yr, _, ey, _ = R.linear(x, w, None, None, "silu", False, bool(gated))
+            R.assert_within(y, yr, ey)
+            for t, (ref, bound) in zip((dx, dw, db), R.linear_backward(dy, x, w, z, "silu", False, bool(gated))):
+                R.assert_within(t, ref, bound)
+            # without a workspace a kernel for any alignment takes the forward call
+            y.zero_()
+            assert getattr(lib, "cuopx_gated_linear" if gated else "cuopx_linear")(L._LINEAR.pack(*fwd, 0, 0), stream) == 0
+            R.assert_within(y, yr, ey)
+    for rows, cols in ((7, 96), (900, 1000), (300, 9000), (40, 333)):
+        x, dy, w = rnd(g, rows, cols), rnd(g, rows, cols), rnd(g, cols)
+        mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+        dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(w)
+        args = (N.BF16, N.BF16, rows, cols, 0.0, x.data_ptr(), cols, w.data_ptr(), 0, 0, 0, mean.data_ptr(), rstd.data_ptr(),
+                dy.data_ptr(), cols, dx.data_ptr(), cols, dw.data_ptr(), db.data_ptr())
+        need = lib.cuopx_layer_norm_backward_workspace_size(L._NORM.pack(*args, 0, 0))
+        ws = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+        assert lib.cuopx_layer_norm_backward(L._NORM.pack(*args, ws.data_ptr(), need), stream) == N.SUCCESS
+        assert (ws[need:] == 0x5A).all()
+        for t, (ref, bound) in zip((dx, dw, db), R.layer_norm_backward(dy, x, mean, rstd, w)):
+            R.assert_within(t, ref, bound)
 
 
 # ------------------------------------------------------------------ offsets past 32 bits
