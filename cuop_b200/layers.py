@@ -196,9 +196,9 @@ def _linear_backward(fn, gated: bool, dy, x, w, preact, activation, trans_w, nee
     elif gated or act:
         _error(N.INVALID_ARGUMENT, f"{what}: the forward pass's preact is needed")
     dev = dy.device
-    dx = _empty((m, k), dtype=dtype, device=dev) if need_dx else None
-    dw = _empty(w_shape, dtype=dtype, device=dev) if need_dw else None
-    db = _empty(wide, dtype=dtype, device=dev) if need_db else None
+    dx = dy.new_empty((m, k)) if need_dx else None
+    dw = dy.new_empty(w_shape) if need_dw else None
+    db = dy.new_empty(wide) if need_db else None
     head = (code, 1 if trans_w else 0, act, 0, m, n, k, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, zp,
             ldz, dx.data_ptr() if need_dx else 0, k, dw.data_ptr() if need_dw else 0, w_shape[1],
             db.data_ptr() if need_db else 0)
@@ -296,7 +296,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     mp = _vector(mean, rows, torch.float32, device, "mean")
     rp = _vector(rstd, rows, torch.float32, device, "rstd")
     dev = x.device
-    dx = _empty((rows, cols), dtype=dtype, device=dev) if need_dx else None
+    dx = x.new_empty((rows, cols)) if need_dx else None
     dw = _empty(cols, dtype=wdtype, device=dev) if need_dw else None
     db = _empty(cols, dtype=wdtype, device=dev) if need_db else None
     head = (code, _DT[wdtype], rows, cols, 0.0, x.data_ptr(), ldx, wp, 0, 0, 0, mp, rp, dy.data_ptr(), lddy,
