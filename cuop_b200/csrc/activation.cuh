@@ -112,17 +112,10 @@ __device__ __forceinline__ float2 act_slope2(float2 z, float2& value) {
   return both(1.f);
 }
 
-// The same for one element.
+// The value at one element.
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   return act_value2<ACT>(both(z)).x;
-}
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z, float& value) {
-  float2 v;
-  const float2 d = act_slope2<ACT>(both(z), v);
-  value = v.x;
-  return d.x;
 }
 
 // Calls f with std::integral_constant<int, ACT>: one uniform branch around a

@@ -366,23 +366,25 @@ __global__ void __launch_bounds__(MAXT, CTAS) layer_norm_rows(const NormParams p
   grid_launch_dependents();
 }
 
-template <typename T, typename W, int V, int NV, bool WARP, int MAXT>
+// Backward for rows that are not 16-byte aligned: single elements, NV columns
+// per thread, the next row's on their way while a row is worked on.
+template <typename T, typename W, int NV, bool WARP, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormParams p) {
   __shared__ float2 buf[2][32];
-  extern __shared__ float warp_part[];  // WARP: [warps][2][32 V NV]
+  extern __shared__ float warp_part[];  // WARP: [warps][2][32 NV]
   int parity = 0;
   const int G = WARP ? 32 : static_cast<int>(blockDim.x);
   const int t = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
   const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = WARP ? gridDim.x * static_cast<int64_t>(blockDim.x >> 5) : gridDim.x;
-  const float inv = 1.f / static_cast<float>(p.cols);
+  const int cols = static_cast<int>(p.cols);
+  const float inv = 1.f / static_cast<float>(cols);
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
   T* dx = static_cast<T*>(p.dx);
-  const W* w = static_cast<const W*>(p.w);
-  float aw[NV][V] = {}, ab[NV][V] = {};
+  float aw[NV] = {}, ab[NV] = {};
   grid_dependency_wait();
-  RowVec<T, V> nx[NV], ng[NV];
+  T nx[NV], ng[NV];
   float nmean = 0.f, nrstd = 0.f;
   auto fetch = [&](int64_t row) {
     if (row >= p.rows) return;
@@ -390,38 +392,27 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
     nrstd = p.rstd[row];
 #pragma unroll
     for (int g = 0; g < NV; ++g) {
-      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-      if (c < p.cols) {
-        nx[g] = load_vec<T, V>(x + row * p.ldx + c);
-        ng[g] = load_vec<T, V>(dy + row * p.lddy + c);
-      }
+      const int c = t + G * g;
+      if (c < cols) nx[g] = x[row * p.ldx + c], ng[g] = dy[row * p.lddy + c];
     }
   };
   fetch(first);
   for (int64_t row = first; row < p.rows; row += step) {
     const float mean = nmean, rstd = nrstd;
-    float h[NV][V], d[NV][V];  // normalised x; dy, then dy w
+    float h[NV], d[NV];  // normalised x; dy w
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int g = 0; g < NV; ++g) {
-      const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-      if (c < p.cols) {
-        float ww[V];
-        if (w) load_weights<W, V>(w, c, p.vec_w, ww);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          h[g][i] = (to_acc<T>(nx[g].e[i]) - mean) * rstd;
-          d[g][i] = to_acc<T>(ng[g].e[i]);
-          aw[g][i] = fmaf(d[g][i], h[g][i], aw[g][i]);
-          ab[g][i] += d[g][i];
-          if (w) d[g][i] *= ww[i];
-          s0 += d[g][i];
-          s1 = fmaf(d[g][i], h[g][i], s1);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[g][i] = d[g][i] = 0.f;
-      }
+      const int c = t + G * g;
+      h[g] = d[g] = 0.f;
+      if (c >= cols) continue;
+      h[g] = (to_acc<T>(nx[g]) - mean) * rstd;
+      d[g] = to_acc<T>(ng[g]);
+      aw[g] = fmaf(d[g], h[g], aw[g]);
+      ab[g] += d[g];
+      if (p.w) d[g] *= to_acc<W>(static_cast<const W*>(p.w)[c]);
+      s0 += d[g];
+      s1 = fmaf(d[g], h[g], s1);
     }
     fetch(row + step);
     if (dx) {
@@ -429,12 +420,8 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
       const float a0 = sum.x * inv, a1 = sum.y * inv;
 #pragma unroll
       for (int g = 0; g < NV; ++g) {
-        const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-        if (c >= p.cols) continue;
-        RowVec<T, V> out;
-#pragma unroll
-        for (int i = 0; i < V; ++i) out.e[i] = from_acc<T>(rstd * (d[g][i] - a0 - h[g][i] * a1));
-        store_vec<T, V>(dx + row * p.lddx + c, out);
+        const int c = t + G * g;
+        if (c < cols) dx[row * p.lddx + c] = from_acc<T>(rstd * (d[g] - a0 - h[g] * a1));
       }
     }
   }
@@ -442,20 +429,15 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
     float* out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
     if constexpr (WARP) {
       // Add the warps' sums in warp order.
-      constexpr int COLS = 32 * V * NV;
+      constexpr int COLS = 32 * NV;
       const int warps = static_cast<int>(blockDim.x >> 5);
       float* mine = warp_part + static_cast<int>(threadIdx.x >> 5) * 2 * COLS;
 #pragma unroll
-      for (int g = 0; g < NV; ++g)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          mine[V * (t + 32 * g) + i] = aw[g][i];
-          mine[COLS + V * (t + 32 * g) + i] = ab[g][i];
-        }
+      for (int g = 0; g < NV; ++g) mine[t + 32 * g] = aw[g], mine[COLS + t + 32 * g] = ab[g];
       __syncthreads();
       for (int e = threadIdx.x; e < 2 * COLS; e += static_cast<int>(blockDim.x)) {
         const int c = e % COLS, which = e / COLS;
-        if (c >= p.cols) continue;
+        if (c >= cols) continue;
         float s = 0.f;
         for (int i = 0; i < warps; ++i) s += warp_part[i * 2 * COLS + e];
         out[which * p.cols + c] = s;
@@ -463,18 +445,8 @@ __global__ void __launch_bounds__(MAXT, 1) layer_norm_backward_rows(const NormPa
     } else {
 #pragma unroll
       for (int g = 0; g < NV; ++g) {
-        const int64_t c = static_cast<int64_t>(V) * (t + G * g);
-        if (c >= p.cols) continue;
-        if constexpr (V % 4 == 0) {  // cols is a multiple of V: 16-byte boundaries
-#pragma unroll
-          for (int i = 0; i < V; i += 4) {
-            *reinterpret_cast<float4*>(out + c + i) = make_float4(aw[g][i], aw[g][i + 1], aw[g][i + 2], aw[g][i + 3]);
-            *reinterpret_cast<float4*>(out + p.cols + c + i) = make_float4(ab[g][i], ab[g][i + 1], ab[g][i + 2], ab[g][i + 3]);
-          }
-        } else {
-          out[c] = aw[g][0];
-          out[p.cols + c] = ab[g][0];
-        }
+        const int c = t + G * g;
+        if (c < cols) out[c] = aw[g], out[p.cols + c] = ab[g];
       }
     }
   }
@@ -996,7 +968,7 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
       else q.nv == 1 ? go(layer_norm_backward_ring<T, W, V, 1, false, 1024, 1, ROWS>, 0) : go(layer_norm_backward_ring<T, W, V, 4, false, 512, 1, 1>, 0);
     } else if (q.rows) {
       const size_t smem = q.warp ? static_cast<size_t>(q.threads / 32) * 2 * 32 * 16 * sizeof(float) : 0;
-      e = launch_pdl(q.warp ? layer_norm_backward_rows<T, W, 1, 16, true, 256> : layer_norm_backward_rows<T, W, 1, 16, false, 512>,
+      e = launch_pdl(q.warp ? layer_norm_backward_rows<T, W, 16, true, 256> : layer_norm_backward_rows<T, W, 16, false, 512>,
                      dim3(static_cast<unsigned>(q.ctas)), dim3(static_cast<unsigned>(q.threads)), smem, stream, p);
       note_launch("layer_norm_backward_rows");
     } else {
