@@ -170,6 +170,13 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 
+// Barrier over the cluster that publishes nothing (rings are free, partners
+// have got this far, mbarriers published by fence.mbarrier_init).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  cluster_arrive_relaxed();
+  cluster_wait();
+}
+
 // Bulk copy of `bytes` (a multiple of 16; both addresses 16-byte aligned)
 // from this CTA's shared memory to `dst` in another CTA of the cluster (a
 // shared::cluster address from map_to_rank); the copy completes `bytes` of

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
   }
   tc_fence_before_sync();
   __syncthreads();
-  cluster_sync_all();  // barriers and TMEM of the whole cluster are ready
+  cluster_sync_relaxed();  // barriers and TMEM of the whole cluster are ready
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   grid_dependency_wait();
@@ -166,9 +166,8 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       }
     }
     __syncwarp();
-    cluster_arrive();
-    cluster_wait();  // every ring of the cluster is free
-    cluster_arrive();
+    cluster_sync_relaxed();  // every ring of the cluster is free
+    cluster_arrive_relaxed();
     cluster_wait();  // partial sums have arrived
   } else if (warp == 1) {
     if (side == 0 && lane == 0) {
@@ -210,17 +209,15 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       }
     }
     __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    cluster_arrive();
+    cluster_sync_relaxed();
+    cluster_arrive_relaxed();
     cluster_wait();
   } else {
     const int q = warp & 3, group = (warp - 2) / 4;  // two warps per TMEM lane quarter
     const int row = 32 * q + lane;
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full, 0, kDevErrWaitTimeoutAccFull, abort_flag));
     tc_fence_after_sync();
-    cluster_arrive();
-    cluster_wait();
+    cluster_sync_relaxed();
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(32 * q) << 16);
     // Receive area of a CTA: [source, own pair left out][column][128 rows] fp32.  Columns of both
     // projections when gated: OWN of the gate's, then OWN of the other's.
@@ -284,7 +281,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
 
   tc_fence_before_sync();
   __syncthreads();
-  cluster_sync_all();  // the pair partner is done with this CTA's TMEM
+  cluster_sync_relaxed();  // the pair partner is done with this CTA's TMEM
   if (warp == 1) {
     tc_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(LP_TMEM_COLS) : "memory");

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       }
     }
     __syncwarp();
-    if (cs > 1 && L::ALIAS) cluster_arrive();
+    if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
     if (cs > 1) cluster_wait();
   } else if (warp == 1) {
     if (lane == 0) {
@@ -228,13 +228,13 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       }
     }
     __syncwarp();
-    if (cs > 1 && L::ALIAS) cluster_arrive();
+    if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
     if (cs > 1) cluster_wait();
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full, 0, kDevErrWaitTimeoutAccFull, abort_flag));
     tc_fence_after_sync();
-    if (cs > 1 && L::ALIAS) cluster_arrive();
+    if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
     if (cs > 1) cluster_wait();
     // Owner of this lane's column of W, and the column's place among its own.
     const int l = 32 * q + lane;
