@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(256) layer_norm_dw_finish(const NormParams p) 
   float s = 0.f;
   if (c < p.cols) {
     const float* in = p.partial + (second ? p.cols : 0) + c;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < p.splits; i += 8) s += in[static_cast<int64_t>(i) * 2 * p.cols];
   }
   part[warp][lane] = s;
