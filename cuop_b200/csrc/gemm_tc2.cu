@@ -516,7 +516,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
         constexpr int PART = COLS * 4 / PairWarps<MODE>::EPI;  // this warp's columns of the tile
         const int c0 = (warp - 2) / 4 * PART;
         const bool done = layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
-            t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ, &layer.tmZ2, stage_base, lane, sbuf,
+            t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ,
+            &layer.tmZ2, stage_base, lane, sbuf,
             [&] { return __all_sync(0xffffffffu, products()); },
             [&] {
               // The accumulator is in registers and nothing else is handed
@@ -686,8 +687,8 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
   // One cluster per pair tile; running clusters take over unlaunched ones.
-  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(PairWarps<kPairGemm>::THREADS), L::ALLOC,
-                                     stream, mA, mB, mC, prm, PairLayer<kPairGemm>{});
+  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)),
+                                     dim3(PairWarps<kPairGemm>::THREADS), L::ALLOC, stream, mA, mB, mC, prm, PairLayer<kPairGemm>{});
   if (lerr != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(lerr);
@@ -708,13 +709,15 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
   PairLayer<MODE> layer = {};
   layer.epi = layer_epi(p);
   layer.w_up = static_cast<int>(p.w_up);
-  bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, P_BK) : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
+  bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, P_BK)
+                 : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, P_BK);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
   if (!layer.epi.Y) ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
   if (p.Z && !layer.epi.Z) {
     ok &= make_map(&layer.tmZ, dt, p.Z, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
-    if (MODE == kPairGated) ok &= make_map(&layer.tmZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
+    if (MODE == kPairGated)
+      ok &= make_map(&layer.tmZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
   }
   if (!ok) return CUOPX_CUDA_ERROR;
   PairParams prm = {};
@@ -735,8 +738,8 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
       return CUOPX_CUDA_ERROR;
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
-  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)), dim3(PairWarps<MODE>::THREADS), L::ALLOC,
-                                      stream, mA, mB, mC, prm, layer);
+  const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)),
+                                      dim3(PairWarps<MODE>::THREADS), L::ALLOC, stream, mA, mB, mC, prm, layer);
   if (lerr != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(lerr);
@@ -829,7 +832,8 @@ int gemm_tc2_peers(const GemmProblem& p, void* const* peers, int npeers, cudaStr
 
 // TMA reads X and W: rows on 16-byte boundaries.  Y, Z, residual and bias may have any alignment.
 bool linear_tc2_supported(const LinearProblem& p) {
-  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0) return false;
+  if (p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX && (p.gated || p.transW)) return false;
   if (!row_aligned16(p.X, p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
   if (p.gated && !p.transW && p.w_up % 8) return false;  // an x coordinate of W's tiles

@@ -219,7 +219,7 @@ template <typename T, bool GATED, int V>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   constexpr int NB = GATED ? 2 : 1;
   constexpr int PAIRS = V == 8 ? 4 : 1;   // a single column is the first half of a pair
-  constexpr int ROWS = GATED ? 2 : 4;     // loaded ahead
+  constexpr int ROWS = V == 1 ? 8 : GATED ? 2 : 4;  // loaded ahead
   __shared__ float sums[8][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int side = warp % p.across, phase = warp / p.across, phases = 8 / p.across;
@@ -590,8 +590,10 @@ int linear_backward(const cuopx_linear_backward_args* a, bool gated, cudaStream_
     d.db = a->dbias;
     if (a->dbias && q.splits > 1) d.partial = reinterpret_cast<float*>(ws + q.partial_off);
     int rc;
-    if (a->dtype == CUOPX_BF16) rc = gated ? launch_dz<__nv_bfloat16, true>(d, q.v, stream) : launch_dz<__nv_bfloat16, false>(d, q.v, stream);
-    else rc = gated ? launch_dz<__half, true>(d, q.v, stream) : launch_dz<__half, false>(d, q.v, stream);
+    if (a->dtype == CUOPX_BF16)
+      rc = gated ? launch_dz<__nv_bfloat16, true>(d, q.v, stream) : launch_dz<__nv_bfloat16, false>(d, q.v, stream);
+    else
+      rc = gated ? launch_dz<__half, true>(d, q.v, stream) : launch_dz<__half, false>(d, q.v, stream);
     if (rc != CUOPX_SUCCESS) return rc;
   }
   if (a->dX && a->M > 0 && a->K > 0) {

@@ -310,7 +310,8 @@ int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
   CUtensorMap mA, mB, mY = {}, mZ = {}, mZ2 = {};
   LpParams prm = {};
   prm.epi = layer_epi(p);
-  bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, LP_BK) : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, LP_BK, LP_BM);
+  bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, LP_BK)
+                 : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, LP_BK, LP_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, LP_BK);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LP_BK, LP_BN / 2);
   if (!prm.epi.Y) ok &= make_map(&mY, dt, p.Y, p.N, p.M, 1, p.ldy, 0, 64, 32);
@@ -340,10 +341,16 @@ int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
 template <typename T>
 int linear_pair_typed(const LinearProblem& p, int ks, cudaStream_t stream) {
   if (p.gated)
-    return p.transW ? launch_linear_pair<T, false, false, true, 2>(p, stream) : launch_linear_pair<T, false, true, true, 2>(p, stream);
-  if (p.transX) return ks == 2 ? launch_linear_pair<T, true, true, false, 2>(p, stream) : launch_linear_pair<T, true, true, false, 4>(p, stream);
-  if (p.transW) return ks == 2 ? launch_linear_pair<T, false, false, false, 2>(p, stream) : launch_linear_pair<T, false, false, false, 4>(p, stream);
-  return ks == 2 ? launch_linear_pair<T, false, true, false, 2>(p, stream) : launch_linear_pair<T, false, true, false, 4>(p, stream);
+    return p.transW ? launch_linear_pair<T, false, false, true, 2>(p, stream)
+                    : launch_linear_pair<T, false, true, true, 2>(p, stream);
+  if (p.transX)
+    return ks == 2 ? launch_linear_pair<T, true, true, false, 2>(p, stream)
+                   : launch_linear_pair<T, true, true, false, 4>(p, stream);
+  if (p.transW)
+    return ks == 2 ? launch_linear_pair<T, false, false, false, 2>(p, stream)
+                   : launch_linear_pair<T, false, false, false, 4>(p, stream);
+  return ks == 2 ? launch_linear_pair<T, false, true, false, 2>(p, stream)
+                 : launch_linear_pair<T, false, true, false, 4>(p, stream);
 }
 
 }  // namespace

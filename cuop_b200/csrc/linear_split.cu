@@ -363,7 +363,8 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
       return CUOPX_CUDA_ERROR;
-    for (int i = 0; i < 4; ++i) capacity[dev][i].store(cluster_capacity(kern, LSP_THREADS, L::ALLOC, 1u << i), std::memory_order_relaxed);
+    for (int i = 0; i < 4; ++i)
+      capacity[dev][i].store(cluster_capacity(kern, LSP_THREADS, L::ALLOC, 1u << i), std::memory_order_relaxed);
     attr_set[dev].store(true, std::memory_order_release);
   }
   // Split K while the clusters still run in one wave and every CTA keeps two
@@ -408,7 +409,8 @@ int linear_split_rows(const LinearProblem& p, cudaStream_t stream) {
 
 // TMA reads X and W; Y, Z, residual and bias may have any alignment.
 bool linear_split_supported(const LinearProblem& p) {
-  if (p.M <= 0 || p.N <= 0 || p.K <= 0 || p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.M <= 0 || p.N <= 0 || p.K <= 0) return false;
+  if (p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX) return false;
   if (!row_aligned16(p.X, p.M == 1 ? 0 : p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
   if (p.gated && !p.transW && p.w_up % 8) return false;  // the second projection's first column in W's rows
