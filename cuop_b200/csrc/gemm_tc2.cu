@@ -27,6 +27,8 @@
 // same PBN / 2 output columns of two projections: the even CTA loads the
 // gate's columns of B and the odd one the other projection's, so one MMA
 // computes both and the epilogue finds them PBN / 2 accumulator columns apart.
+// Measured: gated 8192 x (2 x 10240) x 4096 bf16 with both pre-activations kept
+// 899 us (1529 TFLOP/s, alone; the power cap makes it 1.05-1.1 ms in a loop).
 //
 //   warp 0      TMA producer (both CTAs): loads complete on the LEADER's
 //               `full` mbarrier (.cta_group::2); the leader posts the
