@@ -33,6 +33,9 @@ inline bool alias_ok(const void* out, int64_t ldo, const void* in, int64_t ldi, 
   if (out == in && ldo == ldi) return true;
   return !overlaps(out, span_bytes(rows, cols, ldo, es), in, span_bytes(rows, cols, ldi, es));
 }
+// Whether a matrix of `rows` rows `ld` elements apart can exist: its span in
+// bytes must be countable.
+inline bool extent_ok(int64_t rows, int64_t ld) { return rows <= 1 || ld <= (int64_t(1) << 58) / rows; }
 // Whether every pointer starts on a multiple of `bytes` (NULL does).
 template <typename... P>
 inline bool starts_on(size_t bytes, const P*... p) {

@@ -175,6 +175,8 @@ int dropout_impl(const cuopx_dropout_args* a, cudaStream_t stream) {
   if (a->rows == 0 || a->cols == 0) return CUOPX_SUCCESS;
   if (!a->X || !a->Y || a->ldx < a->cols || a->ldy < a->cols || (a->residual && a->ldr < a->cols))
     return CUOPX_INVALID_ARGUMENT;
+  if (!extent_ok(a->rows, a->ldx) || !extent_ok(a->rows, a->ldy) || (a->residual && !extent_ok(a->rows, a->ldr)))
+    return CUOPX_INVALID_ARGUMENT;
   const size_t es = dtype_size(a->dtype);
   if (!starts_on(es, a->X, a->residual, a->Y) || !starts_on(8, a->offset_dev)) return CUOPX_INVALID_ARGUMENT;
   if (!alias_ok(a->Y, a->ldy, a->X, a->ldx, a->rows, a->cols, es)) return CUOPX_INVALID_ARGUMENT;

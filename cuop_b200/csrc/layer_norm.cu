@@ -878,6 +878,7 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
   if (a->rows == 0 || a->cols == 0) return CUOPX_SUCCESS;
   if (!a->X || !a->Y || a->ldx < a->cols || a->ldy < a->cols) return CUOPX_INVALID_ARGUMENT;
   const size_t es = dtype_size(a->dtype), ws = dtype_size(a->wdtype);
+  if (!extent_ok(a->rows, a->ldx) || !extent_ok(a->rows, a->ldy)) return CUOPX_INVALID_ARGUMENT;
   if (!starts_on(es, a->X, a->Y) || !starts_on(ws, a->weight, a->bias) || !starts_on(4, a->mean, a->rstd))
     return CUOPX_INVALID_ARGUMENT;
   const size_t yb = span_bytes(a->rows, a->cols, a->ldy, es), xb = span_bytes(a->rows, a->cols, a->ldx, es);
@@ -931,6 +932,8 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
   if (a->rows > 0) {
     if (!a->X || !a->dY || !a->mean || !a->rstd || a->ldx < a->cols || a->lddy < a->cols) return CUOPX_INVALID_ARGUMENT;
     if (a->dX && a->lddx < a->cols) return CUOPX_INVALID_ARGUMENT;
+    if (!extent_ok(a->rows, a->ldx) || !extent_ok(a->rows, a->lddy) || (a->dX && !extent_ok(a->rows, a->lddx)))
+      return CUOPX_INVALID_ARGUMENT;
   }
   if (!starts_on(es, a->X, a->dY, a->dX) || !starts_on(ws, a->weight, a->dweight, a->dbias) ||
       !starts_on(4, a->mean, a->rstd) || !starts_on(256, a->workspace))

@@ -456,6 +456,9 @@ int validate_linear(const cuopx_linear_args& a, bool gated) {
   const int64_t wide = gated ? 2 * a.N : a.N;
   const int64_t w_rows = a.transW ? wide : a.K, w_cols = a.transW ? a.K : wide;
   if (!starts_on(2, a.X, a.W, a.bias, a.residual, a.Y, a.preact) || !starts_on(256, a.workspace)) return CUOPX_INVALID_ARGUMENT;
+  if (!extent_ok(a.M, a.ldy) || (a.K > 0 && (!extent_ok(a.M, a.ldx) || !extent_ok(w_rows, a.ldw))) ||
+      (a.preact && !extent_ok(a.M, a.ldz)) || (a.residual && !extent_ok(a.M, a.ldr)))
+    return CUOPX_INVALID_ARGUMENT;
   if (!a.Y || a.ldy < a.N || (a.preact && a.ldz < wide) || (a.residual && a.ldr < a.N)) return CUOPX_INVALID_ARGUMENT;
   if (a.K > 0 && (!a.X || !a.W || a.ldx < a.K || a.ldw < w_cols)) return CUOPX_INVALID_ARGUMENT;
   const size_t es = 2;
@@ -544,6 +547,10 @@ int validate_linear_backward(const cuopx_linear_backward_args& a, bool gated) {
     if (dw && (!a.X || a.ldx < a.K)) return CUOPX_INVALID_ARGUMENT;
   }
   if ((dx && a.lddx < a.K) || (dw && a.lddw < w_cols)) return CUOPX_INVALID_ARGUMENT;
+  if (!extent_ok(a.M, a.lddy) || !extent_ok(a.M, wide) || !extent_ok(a.M, a.K) || (reads_z && !extent_ok(a.M, a.ldz)) ||
+      (dx && (!extent_ok(a.M, a.lddx) || !extent_ok(w_rows, a.ldw))) ||
+      (dw && (!extent_ok(a.M, a.ldx) || !extent_ok(w_rows, a.lddw))))
+    return CUOPX_INVALID_ARGUMENT;
   const size_t need = backward_plan(a, gated).bytes;
   if (need > 0 && (!a.workspace || a.workspace_bytes < need)) return CUOPX_RESOURCE_UNAVAILABLE;
   const size_t es = 2;

@@ -53,7 +53,7 @@ BAD, TYPE, OK, ROOM = N.INVALID_ARGUMENT, N.UNSUPPORTED_TYPE, N.SUCCESS, N.RESOU
     (dict(Z=3 * A + 16, ldz=8), BAD), (dict(Z=A, ldz=8), BAD), (dict(R=3 * A + 2, ldr=8), BAD),
     (dict(R=3 * A, ldr=9), BAD), (dict(X=A + 1), BAD), (dict(W=2 * A + 1), BAD), (dict(Y=3 * A + 1), BAD),
     (dict(bias=4 * A + 1), BAD), (dict(R=4 * A + 1, ldr=8), BAD), (dict(Z=4 * A + 1, ldz=8), BAD), (dict(ws=4 * A + 128, wsb=8), BAD),
-    (dict(ws=A, wsb=1 << 20), BAD), (dict(M=0), OK), (dict(N=0), OK)])
+    (dict(ws=A, wsb=1 << 20), BAD), (dict(M=1 << 40, ldx=1 << 40), BAD), (dict(ldw=1 << 60), BAD), (dict(M=0), OK), (dict(N=0), OK)])
 def test_linear_refusals(change, status):
     assert N.lib().cuopx_linear(lin(**change), None) == status
 
@@ -71,7 +71,7 @@ def test_gated_linear_refusals(change, status):
     (dict(dX=A), BAD), (dict(dW=4 * A), BAD), (dict(db=5 * A), BAD), (dict(dX=3 * A), BAD),
     (dict(act=2, Z=8 * A, ldz=8, wsb=0), ROOM), (dict(act=2, Z=8 * A, ldz=8, ws=8 * A), BAD),
     (dict(dY=A + 1), BAD), (dict(X=2 * A + 1), BAD), (dict(W=3 * A + 1), BAD), (dict(act=2, Z=8 * A + 1, ldz=8), BAD),
-    (dict(dX=4 * A + 1), BAD), (dict(dW=5 * A + 1), BAD), (dict(db=6 * A + 1), BAD), (dict(act=2, Z=8 * A, ldz=8, ws=7 * A + 16), BAD),
+    (dict(M=1 << 56), BAD), (dict(lddw=1 << 60), BAD), (dict(dX=4 * A + 1), BAD), (dict(dW=5 * A + 1), BAD), (dict(db=6 * A + 1), BAD), (dict(act=2, Z=8 * A, ldz=8, ws=7 * A + 16), BAD),
     (dict(dX=0, dW=0, db=0), OK)])
 def test_linear_backward_refusals(change, status):
     assert N.lib().cuopx_linear_backward(lin_bwd(**change), None) == status
@@ -87,7 +87,7 @@ def test_gated_backward_needs_the_pre_activation():
     (dict(eps=float("nan")), BAD), (dict(eps=float("inf")), BAD), (dict(X=0), BAD), (dict(Y=0), BAD), (dict(ldx=7), BAD),
     (dict(ldy=7), BAD), (dict(Y=A + 16), BAD), (dict(Y=2 * A), BAD), (dict(mean=A), BAD), (dict(rstd=5 * A + 4), BAD),
     (dict(X=A + 1), BAD), (dict(Y=4 * A + 1), BAD), (dict(w=2 * A + 2), BAD), (dict(b=3 * A + 2), BAD), (dict(mean=5 * A + 2), BAD),
-    (dict(rstd=6 * A + 1), BAD), (dict(rows=0), OK), (dict(cols=0), OK)])
+    (dict(rstd=6 * A + 1), BAD), (dict(rows=1 << 40, ldx=1 << 40), BAD), (dict(rows=0), OK), (dict(cols=0), OK)])
 def test_layer_norm_refusals(change, status):
     assert N.lib().cuopx_layer_norm(norm(**change), None) == status
 
@@ -106,7 +106,7 @@ def test_layer_norm_backward_refusals(change, status):
     (dict(dtype=N.F64), TYPE), (dict(rows=-1), BAD), (dict(p=-0.1), BAD), (dict(p=1.1), BAD), (dict(p=float("nan")), BAD),
     (dict(X=0), BAD), (dict(Y=0), BAD), (dict(ldx=7), BAD), (dict(ldy=7), BAD), (dict(R=3 * A, ldr=7), BAD),
     (dict(Y=A + 4), BAD), (dict(Y=A, ldy=9), BAD), (dict(R=2 * A + 4, ldr=8), BAD), (dict(dev=2 * A + 8), BAD),
-    (dict(dev=4 * A + 4), BAD), (dict(X=A + 2), BAD), (dict(Y=2 * A + 2), BAD), (dict(R=3 * A + 2, ldr=8), BAD),
+    (dict(ldx=1 << 60), BAD), (dict(dev=4 * A + 4), BAD), (dict(X=A + 2), BAD), (dict(Y=2 * A + 2), BAD), (dict(R=3 * A + 2, ldr=8), BAD),
     (dict(rows=1 << 40, cols=1 << 40, ldx=1 << 40, ldy=1 << 40), BAD), (dict(rows=0), OK)])
 def test_dropout_refusals(change, status):
     assert N.lib().cuopx_dropout(drop(**change), None) == status
