@@ -79,7 +79,8 @@ __device__ __forceinline__ float2 vanishing_fma2(float2 d, float2 a, float2 b, f
   return make_float2(d.x > 0.f ? v.x : c.x, d.y > 0.f ? v.y : c.y);
 }
 
-// Value and derivative at z.
+// Value and derivative at z.  The derivative of an infinite z is its limit; the
+// value needs a finite z (-inf * 0 is NaN).
 template <int ACT>
 __device__ __forceinline__ float2 act_slope2(float2 z, float2& value) {
   float2 e;

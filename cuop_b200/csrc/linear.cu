@@ -217,6 +217,19 @@ __device__ __forceinline__ void store_packed(T* dst, const Packed<T, V>& r) {
   else *reinterpret_cast<unsigned short*>(dst) = static_cast<unsigned short>(r.w[0]);
 }
 
+// A kept pre-activation is infinite where the number itself left the range of
+// the 16-bit type (in fp16 from 65520 on), while the forward pass went on with
+// the number.  It counts as 3e38, with its sign: a factor that has vanished
+// (dY, act', act) makes 0 of it, as it did of the number, and act' (1.13 at
+// most) does not take it out of fp32's range before dY multiplies it.  NaN
+// stays NaN.  One minimum of magnitudes an element.
+__device__ __forceinline__ float2 kept2(float2 z) {
+  float2 r;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r.x) : "f"(z.x), "f"(3.0e38f));
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r.y) : "f"(z.y), "f"(3.0e38f));
+  return r;
+}
+
 template <typename T, bool GATED, int V>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
   constexpr int NB = GATED ? 2 : 1;
@@ -258,8 +271,9 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
             const float2 gg = unpack2_layer<T>(g[j].w[i]);
             float2 d[NB], value;
             if constexpr (GATED) {
-              const float2 slope = act_slope2<act.value>(unpack2_layer<T>(z[j][0].w[i]), value);
-              d[0] = mul2(mul2(gg, unpack2_layer<T>(z[j][NB - 1].w[i])), slope);
+              const float2 slope = act_slope2<act.value>(kept2(unpack2_layer<T>(z[j][0].w[i])), value);
+              // act'(G) first: where it has vanished, dY * U may be beyond fp32's range.
+              d[0] = mul2(mul2(kept2(unpack2_layer<T>(z[j][NB - 1].w[i])), slope), gg);
               d[NB - 1] = mul2(gg, value);
             } else if constexpr (act.value != CUOPX_ACT_NONE) {
               d[0] = mul2(gg, act_slope2<act.value>(unpack2_layer<T>(z[j][0].w[i]), value));

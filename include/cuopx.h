@@ -373,7 +373,9 @@ typedef struct cuopx_linear_backward_args {
  * The residual's gradient is dY itself.  dZ is rounded to the 16-bit type
  * between its computation and the two products, which take 16-bit operands.
  * Of cuopx_gated_linear: dG = dY * U * act'(G), dU = dY * act(G), dZ =
- * [dG | dU].  The workspace is required: CUOPX_RESOURCE_UNAVAILABLE when it
+ * [dG | dU].  Where the stored Z is infinite (fp16: the number was beyond
+ * 65504), act' has its limit, and the gated form counts it as 3e38 with its
+ * sign, so that a factor of 0 makes 0 of it.  The workspace is required: CUOPX_RESOURCE_UNAVAILABLE when it
  * is smaller than the size call says (which may be 0).
  */
 size_t cuopx_linear_backward_workspace_size(const cuopx_linear_backward_args* args);

@@ -1,0 +1,72 @@
+"""Layer operators at values and in layouts where formulas and checks can go wrong: infinite and vanishing
+pre-activations, the activations' tails, results beside their inputs in one buffer, single rows through the tensor
+cores, in-place gradients.  Tolerances are those of layer_refs.py unless a test derives its own."""
+import pytest
+import torch
+
+import cuop_b200 as cx
+import layer_refs as R
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+INF = float("inf")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rnd(g, *shape, scale=1.0, dtype=BF):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# ------------------------------------------------------------------ infinite and very large kept pre-activations
+@pytest.mark.parametrize("act", R.ACTS)
+@pytest.mark.parametrize("dt,big", [(HF, 65504.0), (BF, 1e30)])
+@pytest.mark.parametrize("vec", [True, False])
+def test_backward_of_infinite_and_very_large_pre_activations(act, dt, big, vec):
+    """One row, so that db is dZ.  A kept infinity counts as 3e38: act and act' have their limits there, and a factor
+    that has vanished (dY, act', act) makes 0 of it."""
+    zs = [-INF, -big, -300.0, -20.0, 0.0, 1.5, 20.0, 300.0, big, INF]
+    us = [-INF, -big, -1.5, 0.0, 2.0, big, INF]
+    gs = [0.0, 0.5, -0.25, 1024.0]
+    rows = [(g, z, u) for g in gs for z in zs for u in us]
+    while len(rows) % 8 != (0 if vec else 3):
+        rows.append((1.0, 1.0, 1.0))
+    n = len(rows)
+    dy, z, up = (torch.tensor([[r[i] for r in rows]], device="cuda").to(dt) for i in range(3))
+    g, a, b = (t.double().clamp(-3e38, 3e38)[0] for t in (dy, z, up))
+    value, slope = R.value(a, act), R.slope(a, act)
+    x, kept = torch.ones(1, 8, dtype=dt, device="cuda"), torch.cat((z, up), 1)
+    db = cx.gated_linear_backward(dy, x, torch.ones(8, 2 * n, dtype=dt, device="cuda"), kept, activation=act,
+                                  need_dx=False, need_dw=False)[2]
+    one = cx.linear_backward(dy, x, torch.ones(8, n, dtype=dt, device="cuda"), z, activation=act, need_dx=False, need_dw=False)[2]
+    # act_error grows with z without limit, act and act' are at their limits beyond 300
+    near = a.clamp(-300, 300)
+    rel, floor = 3 * R.act_error(near, act) + 2.0 ** -21, R.act_floor(near, act)
+    for what, got, ref, factor in (("dg", db[:n], g * (b * slope), (g * b).abs()), ("du", db[n:], g * value, g.abs()),
+                                   ("linear", one, g * slope, g.abs())):
+        assert not torch.isnan(got).any(), (what, [rows[i] for i in torch.isnan(got).nonzero()[:3, 0].tolist()])
+        ok = (got == ref.to(dt)) | ((got.double() - ref).abs() <= (R.u(dt) + rel) * ref.abs() + floor * factor + 4 * R.TINY[dt])
+        assert ok.all(), (what, [(rows[i], got[i].item(), ref[i].item()) for i in (~ok).nonzero()[:5, 0].tolist()])
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 24), (70, 136, 264), (300, 264, 136)])
+def test_gated_backward_stays_finite_where_the_forward_pass_does(act, m, n, k):
+    """fp16 gates below -65504 are kept as -inf; the forward result there is finite, and so are all three gradients."""
+    g = gen(7)
+    x, dy = rnd(g, m, k, dtype=HF), rnd(g, m, n, dtype=HF)
+    w = rnd(g, k, 2 * n, scale=k ** -0.5, dtype=HF)
+    z = rnd(g, m, 2 * n, dtype=HF)
+    z[1, :n] = -INF
+    z[m - 1, 3] = -INF
+    got = cx.gated_linear_backward(dy, x, w, z, activation=act)
+    # the definition at -65504: every activation and derivative is 0 there, to 64 bits
+    ref = R.linear_backward(dy, x, w, z.clamp_min(-65504.0), act, False, True)
+    # act_error grows without limit there while act stays 0: the bounds are those of z = 0 in the same places, whose
+    # terms are larger than the zeros', and the last rounding of this sum
+    calm = R.linear_backward(dy, x, w, torch.where(z < -1e4, torch.zeros_like(z), z), act, False, True)
+    for name, t, (r, _), (_, bound) in zip(("dx", "dw", "db"), got, ref, calm):
+        assert torch.isfinite(t).all(), name
+        R.assert_within(t, r, bound + R.u(HF) * r.abs(), name)
