@@ -33,10 +33,12 @@ __device__ __forceinline__ float2 sigmoid_2(float2 z, float2& e) {
   return rcp_2(add2(e, both(1.f)));
 }
 
-// s'(z) = e s^2 with e = exp(-z) = (1 - s) / s: no cancellation in 1 - s.  e is
-// kept finite, so that s = 0 gives s' = 0.
+// s'(z) = s (1 - s) with 1 - s = e s, e = exp(-z): no cancellation.  e s is
+// taken to be 1 at most, and where e = inf and s = 0 (the minimum of NaN and 1
+// is 1), so that s = 0 gives s' = 0; s = NaN gives NaN.
 __device__ __forceinline__ float2 sigmoid_slope_2(float2 e, float2 s) {
-  return mul2(mul2(make_float2(fminf(e.x, 1e30f), fminf(e.y, 1e30f)), s), s);
+  const float2 r = mul2(e, s);
+  return mul2(make_float2(fminf(r.x, 1.f), fminf(r.y, 1.f)), s);
 }
 
 // The normal density phi(z) and distribution function Phi(z): for x >= 0

@@ -1,6 +1,8 @@
 """Layer operators at values and in layouts where formulas and checks can go wrong: infinite and vanishing
 pre-activations, the activations' tails, results beside their inputs in one buffer, single rows through the tensor
 cores, in-place gradients.  Tolerances are those of layer_refs.py unless a test derives its own."""
+import math
+
 import pytest
 import torch
 
@@ -70,3 +72,29 @@ def test_gated_backward_stays_finite_where_the_forward_pass_does(act, m, n, k):
     for name, t, (r, _), (_, bound) in zip(("dx", "dw", "db"), got, ref, calm):
         assert torch.isfinite(t).all(), name
         R.assert_within(t, r, bound + R.u(HF) * r.abs(), name)
+
+
+# ------------------------------------------------------------------ sigmoids in the tails
+def spread(lo, hi, dt, count=4096):
+    return torch.linspace(lo, hi, count, device="cuda", dtype=torch.float64).to(dt).unique()
+
+
+@pytest.mark.parametrize("act,dt,far", [("sigmoid", BF, 86.0), ("sigmoid", HF, 17.0), ("silu", BF, 86.0), ("silu", HF, 17.0),
+                                        ("gelu_tanh", BF, 9.9), ("gelu_tanh", HF, 5.0)])
+def test_sigmoid_slopes_keep_their_relative_accuracy(act, dt, far):
+    """s' = s (1 - s) and the slopes made of it, to act_error relative (of their terms), as far as the exponential stays
+    a normal fp32 number (its argument below 87)."""
+    z = spread(-far, far, dt)[None]
+    n = z.shape[1]
+    one = torch.ones(1, n, dtype=dt, device="cuda")
+    got = cx.linear_backward(one, one[:, :8], torch.ones(8, n, dtype=dt, device="cuda"), z, activation=act, need_dx=False,
+                             need_dw=False)[2]
+    zz = z.double()[0]
+    if act == "gelu_tanh":
+        c = 2 * math.sqrt(2 / math.pi)
+        arg, inner = c * (zz + 0.044715 * zz ** 3), c * (1 + 0.134145 * zz ** 2)
+    else:
+        arg, inner = zz, torch.ones_like(zz)
+    s, d = torch.sigmoid(arg), torch.sigmoid(arg) * torch.sigmoid(-arg) * inner
+    ref, size = (d, d) if act == "sigmoid" else (s + zz * d, s + (zz * d).abs())
+    R.assert_within(got, ref, R.u(dt) * ref.abs() + 1.01 * (2 * R.act_error(zz, act) + 2.0 ** -22) * size + R.TINY[dt])
