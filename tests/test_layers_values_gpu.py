@@ -98,3 +98,30 @@ def test_sigmoid_slopes_keep_their_relative_accuracy(act, dt, far):
     s, d = torch.sigmoid(arg), torch.sigmoid(arg) * torch.sigmoid(-arg) * inner
     ref, size = (d, d) if act == "sigmoid" else (s + zz * d, s + (zz * d).abs())
     R.assert_within(got, ref, R.u(dt) * ref.abs() + 1.01 * (2 * R.act_error(zz, act) + 2.0 ** -22) * size + R.TINY[dt])
+
+
+# ------------------------------------------------------------------ gelu in the tails
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("rows", [16, 1024])
+def test_gelu_keeps_its_relative_accuracy_in_the_tails(dt, rows):
+    """z Phi(z) and its derivative to act_error relative (of the derivative's two terms), with no absolute part, as far as
+    the normal density stays a normal fp32 number (|z| < 13.2)."""
+    zs = spread(-13.1, 13.1, dt, 8192)
+    zs = torch.cat((zs, zs[:-zs.numel() % rows])) if zs.numel() % rows else zs
+    w = torch.zeros(8, 8, dtype=dt, device="cuda")
+    w[0] = 1.0
+    got = []
+    for part in zs.view(-1, rows):
+        x = torch.zeros(rows, 8, dtype=dt, device="cuda")
+        x[:, 0] = part  # one product with 1: the kernel's z is exact
+        got.append(cx.linear(x, w, activation="gelu")[:, 5])
+    z = zs.double()
+    ref = R.value(z, "gelu")
+    R.assert_within(torch.cat(got), ref, R.u(dt) * ref.abs() + 1.01 * R.act_error(z, "gelu") * ref.abs() + R.TINY[dt], "value")
+    n = zs.numel()
+    one = torch.ones(1, n, dtype=dt, device="cuda")
+    db = cx.linear_backward(one, one[:, :8], torch.ones(8, n, dtype=dt, device="cuda"), zs[None], activation="gelu",
+                            need_dx=False, need_dw=False)[2]
+    ref = R.slope(z, "gelu")
+    size = 0.5 * torch.special.erfc(-z / math.sqrt(2)) + z.abs() * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    R.assert_within(db, ref, R.u(dt) * ref.abs() + 1.01 * (R.act_error(z, "gelu") + 2.0 ** -22) * size + R.TINY[dt], "slope")
