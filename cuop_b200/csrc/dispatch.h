@@ -27,11 +27,30 @@ int cuda_failure_text(const char* what);
 // Whether two byte ranges share a byte; bytes that a row-major matrix spans.
 bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes);
 size_t span_bytes(int64_t rows, int64_t cols, int64_t ld, size_t es);
+// A row-major matrix in memory (a vector is one row).
+struct Extent {
+  const void* p;
+  int64_t rows, cols, ld;
+  size_t es;
+};
+inline Extent vector_extent(const void* p, size_t bytes) { return {p, 1, static_cast<int64_t>(bytes), 0, 1}; }
+// Whether two matrices share a byte.  Exact for matrices of the same row pitch,
+// such as column slices of one buffer: their columns, counted from the same
+// row start, must not meet.  Otherwise the bytes from the first to the last
+// element must not.
+inline bool overlaps(const Extent& a, const Extent& b) {
+  if (!overlaps(a.p, span_bytes(a.rows, a.cols, a.ld, a.es), b.p, span_bytes(b.rows, b.cols, b.ld, b.es))) return false;
+  if (a.rows <= 1 || b.rows <= 1 || a.ld != b.ld || a.es != b.es) return true;
+  const int64_t es = static_cast<int64_t>(a.es);
+  const int64_t bytes = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+  if (bytes % es != 0) return true;
+  const int64_t first = ((bytes / es) % a.ld + a.ld) % a.ld;  // b's first column, a's being 0
+  return first < a.cols || first + b.cols > a.ld;
+}
 // Whether an output matrix may share memory with an input of the same shape:
 // not at all, or exactly (in place: same pointer and leading dimension).
 inline bool alias_ok(const void* out, int64_t ldo, const void* in, int64_t ldi, int64_t rows, int64_t cols, size_t es) {
-  if (out == in && ldo == ldi) return true;
-  return !overlaps(out, span_bytes(rows, cols, ldo, es), in, span_bytes(rows, cols, ldi, es));
+  return (out == in && ldo == ldi) || !overlaps({out, rows, cols, ldo, es}, {in, rows, cols, ldi, es});
 }
 // Whether a matrix of `rows` rows `ld` elements apart can exist: its span in
 // bytes must be countable.

@@ -881,16 +881,16 @@ int layer_norm_impl(const cuopx_layer_norm_args* a, cudaStream_t stream) {
   if (!extent_ok(a->rows, a->ldx) || !extent_ok(a->rows, a->ldy)) return CUOPX_INVALID_ARGUMENT;
   if (!starts_on(es, a->X, a->Y) || !starts_on(ws, a->weight, a->bias) || !starts_on(4, a->mean, a->rstd))
     return CUOPX_INVALID_ARGUMENT;
-  const size_t yb = span_bytes(a->rows, a->cols, a->ldy, es), xb = span_bytes(a->rows, a->cols, a->ldx, es);
   const size_t wb = static_cast<size_t>(a->cols) * ws, sb = static_cast<size_t>(a->rows) * sizeof(float);
   if (!alias_ok(a->Y, a->ldy, a->X, a->ldx, a->rows, a->cols, es)) return CUOPX_INVALID_ARGUMENT;
-  const void* outs[3] = {a->Y, a->mean, a->rstd};
-  const size_t outb[3] = {yb, sb, sb};
+  const Extent x{a->X, a->rows, a->cols, a->ldx, es};
+  const Extent weight = vector_extent(a->weight, wb), bias = vector_extent(a->bias, wb);
+  const Extent outs[3] = {{a->Y, a->rows, a->cols, a->ldy, es}, vector_extent(a->mean, sb), vector_extent(a->rstd, sb)};
   for (int i = 0; i < 3; ++i) {
-    if (overlaps(outs[i], outb[i], a->weight, wb) || overlaps(outs[i], outb[i], a->bias, wb)) return CUOPX_INVALID_ARGUMENT;
-    if (i > 0 && overlaps(outs[i], outb[i], a->X, xb)) return CUOPX_INVALID_ARGUMENT;
+    if (overlaps(outs[i], weight) || overlaps(outs[i], bias)) return CUOPX_INVALID_ARGUMENT;
+    if (i > 0 && overlaps(outs[i], x)) return CUOPX_INVALID_ARGUMENT;
     for (int j = 0; j < i; ++j)
-      if (overlaps(outs[i], outb[i], outs[j], outb[j])) return CUOPX_INVALID_ARGUMENT;
+      if (overlaps(outs[i], outs[j])) return CUOPX_INVALID_ARGUMENT;
   }
   const NormParams p = norm_params(*a);
   const NormPlan q = norm_forward_plan(*a);
@@ -940,18 +940,18 @@ int layer_norm_backward_impl(const cuopx_layer_norm_args* a, cudaStream_t stream
     return CUOPX_INVALID_ARGUMENT;
   const size_t need = norm_backward_workspace(*a);
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return CUOPX_RESOURCE_UNAVAILABLE;
-  const size_t xb = span_bytes(a->rows, a->cols, a->ldx, es), gb = span_bytes(a->rows, a->cols, a->lddy, es);
-  const void* outs[4] = {a->dX, a->dweight, a->dbias, need ? a->workspace : nullptr};
-  const size_t outb[4] = {span_bytes(a->rows, a->cols, a->lddx, es), wb, wb, need};
+  const Extent ins[4] = {{a->X, a->rows, a->cols, a->ldx, es}, vector_extent(a->weight, wb), vector_extent(a->mean, sb),
+                         vector_extent(a->rstd, sb)};
+  const Extent grad{a->dY, a->rows, a->cols, a->lddy, es};
+  const Extent outs[4] = {{a->dX, a->rows, a->cols, a->lddx, es}, vector_extent(a->dweight, wb), vector_extent(a->dbias, wb),
+                          vector_extent(need ? a->workspace : nullptr, need)};
   for (int i = 0; i < 4; ++i) {
-    if (overlaps(outs[i], outb[i], a->X, xb) || overlaps(outs[i], outb[i], a->weight, wb) ||
-        overlaps(outs[i], outb[i], a->mean, sb) || overlaps(outs[i], outb[i], a->rstd, sb))
-      return CUOPX_INVALID_ARGUMENT;
-    if (i == 0 ? a->dX && !alias_ok(a->dX, a->lddx, a->dY, a->lddy, a->rows, a->cols, es)
-               : overlaps(outs[i], outb[i], a->dY, gb))
+    for (const Extent& in : ins)
+      if (overlaps(outs[i], in)) return CUOPX_INVALID_ARGUMENT;
+    if (i == 0 ? a->dX && !alias_ok(a->dX, a->lddx, a->dY, a->lddy, a->rows, a->cols, es) : overlaps(outs[i], grad))
       return CUOPX_INVALID_ARGUMENT;
     for (int j = 0; j < i; ++j)
-      if (overlaps(outs[i], outb[i], outs[j], outb[j])) return CUOPX_INVALID_ARGUMENT;
+      if (overlaps(outs[i], outs[j])) return CUOPX_INVALID_ARGUMENT;
   }
   NormParams p = norm_params(*a);
   if (a->rows == 0) {  // sums over no rows

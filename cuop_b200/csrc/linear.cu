@@ -476,20 +476,15 @@ int validate_linear(const cuopx_linear_args& a, bool gated) {
   if (!a.Y || a.ldy < a.N || (a.preact && a.ldz < wide) || (a.residual && a.ldr < a.N)) return CUOPX_INVALID_ARGUMENT;
   if (a.K > 0 && (!a.X || !a.W || a.ldx < a.K || a.ldw < w_cols)) return CUOPX_INVALID_ARGUMENT;
   const size_t es = 2;
-  const size_t yb = span_bytes(a.M, a.N, a.ldy, es), zb = a.preact ? span_bytes(a.M, wide, a.ldz, es) : 0;
-  const size_t xb = span_bytes(a.M, a.K, a.ldx, es), wb = span_bytes(w_rows, w_cols, a.ldw, es);
-  const size_t bb = static_cast<size_t>(wide) * es, rb = a.residual ? span_bytes(a.M, a.N, a.ldr, es) : 0;
-  if (overlaps(a.Y, yb, a.X, xb) || overlaps(a.Y, yb, a.W, wb) || overlaps(a.Y, yb, a.bias, bb) ||
-      overlaps(a.Y, yb, a.preact, zb))
-    return CUOPX_INVALID_ARGUMENT;
-  if (overlaps(a.preact, zb, a.X, xb) || overlaps(a.preact, zb, a.W, wb) || overlaps(a.preact, zb, a.bias, bb) ||
-      overlaps(a.preact, zb, a.residual, rb))
-    return CUOPX_INVALID_ARGUMENT;
+  const Extent x{a.X, a.M, a.K, a.ldx, es}, w{a.W, w_rows, w_cols, a.ldw, es}, r{a.residual, a.M, a.N, a.ldr, es};
+  const Extent y{a.Y, a.M, a.N, a.ldy, es}, z{a.preact, a.M, wide, a.ldz, es};
+  const Extent bias = vector_extent(a.bias, static_cast<size_t>(wide) * es);
+  const Extent scratch = vector_extent(a.workspace, a.workspace_bytes);
+  if (overlaps(y, x) || overlaps(y, w) || overlaps(y, bias) || overlaps(y, z)) return CUOPX_INVALID_ARGUMENT;
+  if (overlaps(z, x) || overlaps(z, w) || overlaps(z, bias) || overlaps(z, r)) return CUOPX_INVALID_ARGUMENT;
   if (a.residual && !alias_ok(a.Y, a.ldy, a.residual, a.ldr, a.M, a.N, es)) return CUOPX_INVALID_ARGUMENT;
-  if (overlaps(a.workspace, a.workspace_bytes, a.X, xb) || overlaps(a.workspace, a.workspace_bytes, a.W, wb) ||
-      overlaps(a.workspace, a.workspace_bytes, a.bias, bb) || overlaps(a.workspace, a.workspace_bytes, a.residual, rb) ||
-      overlaps(a.workspace, a.workspace_bytes, a.Y, yb) || overlaps(a.workspace, a.workspace_bytes, a.preact, zb))
-    return CUOPX_INVALID_ARGUMENT;
+  for (const Extent& e : {x, w, bias, r, y, z})
+    if (overlaps(scratch, e)) return CUOPX_INVALID_ARGUMENT;
   return -1;
 }
 
@@ -568,17 +563,19 @@ int validate_linear_backward(const cuopx_linear_backward_args& a, bool gated) {
   const size_t need = backward_plan(a, gated).bytes;
   if (need > 0 && (!a.workspace || a.workspace_bytes < need)) return CUOPX_RESOURCE_UNAVAILABLE;
   const size_t es = 2;
-  const void* in[4] = {a.dY, dw ? a.X : nullptr, dx ? a.W : nullptr, reads_z ? a.preact : nullptr};
-  const size_t inb[4] = {span_bytes(a.M, a.N, a.lddy, es), span_bytes(a.M, a.K, a.ldx, es),
-                         span_bytes(w_rows, w_cols, a.ldw, es), span_bytes(a.M, wide, a.ldz, es)};
-  const void* out[4] = {dx ? a.dX : nullptr, dw ? a.dW : nullptr, db ? a.dbias : nullptr, need ? a.workspace : nullptr};
-  const size_t outb[4] = {span_bytes(a.M, a.K, a.lddx, es), span_bytes(w_rows, w_cols, a.lddw, es),
-                          static_cast<size_t>(wide) * es, need};
+  const Extent in[4] = {{a.dY, a.M, a.N, a.lddy, es},
+                        {dw ? a.X : nullptr, a.M, a.K, a.ldx, es},
+                        {dx ? a.W : nullptr, w_rows, w_cols, a.ldw, es},
+                        {reads_z ? a.preact : nullptr, a.M, wide, a.ldz, es}};
+  const Extent out[4] = {{dx ? a.dX : nullptr, a.M, a.K, a.lddx, es},
+                         {dw ? a.dW : nullptr, w_rows, w_cols, a.lddw, es},
+                         vector_extent(db ? a.dbias : nullptr, static_cast<size_t>(wide) * es),
+                         vector_extent(need ? a.workspace : nullptr, need)};
   for (int i = 0; i < 4; ++i) {
     for (int j = 0; j < 4; ++j)
-      if (overlaps(out[i], outb[i], in[j], inb[j])) return CUOPX_INVALID_ARGUMENT;
+      if (overlaps(out[i], in[j])) return CUOPX_INVALID_ARGUMENT;
     for (int j = 0; j < i; ++j)
-      if (overlaps(out[i], outb[i], out[j], outb[j])) return CUOPX_INVALID_ARGUMENT;
+      if (overlaps(out[i], out[j])) return CUOPX_INVALID_ARGUMENT;
   }
   return -1;
 }

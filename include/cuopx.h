@@ -293,8 +293,11 @@ int cuopx_iamin(int64_t n, const float* x, int64_t incx, int64_t* result, void* 
  * MatMulReluFused, see cuopx_gemm_ex).  Their arguments come in a struct:
  * zero-fill it, set what the call uses, leave optional pointers NULL.  The
  * pointers follow the rules above and start on a multiple of their element's
- * size; sizes and leading dimensions are in elements, matrices are row-major.  An output may not overlap an input or
- * another output, except where a comment allows it.
+ * size; sizes and leading dimensions are in elements, matrices are row-major.
+ * An output may not overlap an input or another output, except where a comment
+ * allows it.  Matrices with the same leading dimension overlap when they share
+ * an element (column slices of one buffer do not); others when the bytes from
+ * their first to their last element meet.
  *
  * Activations, with Phi the normal distribution function and s(z) =
  * 1 / (1 + exp(-z)):
@@ -375,8 +378,9 @@ typedef struct cuopx_linear_backward_args {
  * Of cuopx_gated_linear: dG = dY * U * act'(G), dU = dY * act(G), dZ =
  * [dG | dU].  Where the stored Z is infinite (fp16: the number was beyond
  * 65504), act' has its limit, and the gated form counts it as 3e38 with its
- * sign, so that a factor of 0 makes 0 of it.  The workspace is required: CUOPX_RESOURCE_UNAVAILABLE when it
- * is smaller than the size call says (which may be 0).
+ * sign, so that a factor of 0 makes 0 of it.  The workspace is required:
+ * CUOPX_RESOURCE_UNAVAILABLE when it is smaller than the size call says (which
+ * may be 0).
  */
 size_t cuopx_linear_backward_workspace_size(const cuopx_linear_backward_args* args);
 int cuopx_linear_backward(const cuopx_linear_backward_args* args, void* stream);

@@ -8,9 +8,11 @@ import torch
 
 import cuop_b200 as cx
 import layer_refs as R
+from cuop_b200 import _native as N
+from cuop_b200 import layers as L
 
 pytestmark = pytest.mark.gpu
-BF, HF = torch.bfloat16, torch.float16
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 INF = float("inf")
 
 
@@ -125,3 +127,93 @@ def test_gelu_keeps_its_relative_accuracy_in_the_tails(dt, rows):
     ref = R.slope(z, "gelu")
     size = 0.5 * torch.special.erfc(-z / math.sqrt(2)) + z.abs() * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     R.assert_within(db, ref, R.u(dt) * ref.abs() + 1.01 * (R.act_error(z, "gelu") + 2.0 ** -22) * size + R.TINY[dt], "slope")
+
+
+# ------------------------------------------------------------------ matrices side by side in one buffer
+def beside(*parts, gap=0):
+    """The same matrices as column slices of one buffer (NaN between them)."""
+    rows = parts[0].shape[0]
+    buf = torch.full((rows, sum(t.shape[1] + gap for t in parts)), float("nan"), dtype=parts[0].dtype, device="cuda")
+    out, at = [], 0
+    for t in parts:
+        v = buf[:, at:at + t.shape[1]]
+        v.copy_(t)
+        out.append(v)
+        at += t.shape[1] + gap
+    return buf, out
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 8, 8), (40, 136, 264), (300, 264, 136), (140, 264, 6208), (1500, 520, 72), (70, 33, 45)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_forward_between_columns_of_one_buffer(m, n, k, gated):
+    g = gen(m)
+    wide = 2 * n if gated else n
+    x, r, w = rnd(g, m, k), rnd(g, m, n), rnd(g, k, wide, scale=k ** -0.5)
+    y, z = torch.zeros_like(r), torch.zeros(m, wide, dtype=BF, device="cuda")
+    for gap in (0, 8, 3):
+        buf, (xs, ys, rs, zs) = beside(x, y, r, z, gap=gap)
+        holes = torch.isnan(buf)
+        if gated:
+            cx.gated_linear(xs, w, activation="silu", out=ys, preact=zs)
+        else:
+            cx.linear(xs, w, None, rs, activation="silu", out=ys, preact=zs)
+        yr, zr, ey, ez = R.linear(x, w, None, None if gated else r, "silu", False, gated)
+        R.assert_within(ys, yr, ey, "y")
+        R.assert_within(zs, zr, ez, "z")
+        assert torch.equal(torch.isnan(buf), holes) and torch.equal(xs, x) and torch.equal(rs, r)
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 8), (300, 256), (40, 1001), (9, 4096), (3, 20000)])
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_norm_and_dropout_between_columns_of_one_buffer(rows, cols, dt):
+    g = gen(rows)
+    x, w = rnd(g, rows, cols, dtype=dt), rnd(g, cols, dtype=dt)
+    for gap in (0, 8):
+        buf, (xs, ys) = beside(x, torch.zeros_like(x), gap=gap)
+        holes = torch.isnan(buf)
+        cx.layer_norm(xs, w, out=ys)
+        ref, _, _, bound, _, _ = R.layer_norm(x, w, None, 1e-5)
+        R.assert_within(ys, ref, bound)
+        cx.dropout(xs, 0.3, 5, 9, out=ys)
+        assert torch.equal(ys, cx.dropout(x, 0.3, 5, 9))
+        assert torch.equal(torch.isnan(buf), holes) and torch.equal(xs, x)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_backward_between_columns_of_one_buffer(gated):
+    """Through the C ABI, which lets a caller place dX: beside dY, X and Z; dW beside W."""
+    lib, g = N.lib(), gen(3)
+    stream = torch.cuda.current_stream().cuda_stream
+    m, n, k = 140, 136, 264
+    wide = 2 * n if gated else n
+    x, dy, z, w = rnd(g, m, k), rnd(g, m, n), rnd(g, m, wide), rnd(g, k, wide, scale=k ** -0.5)
+    buf, (dys, xs, zs, dxs) = beside(dy, x, z, torch.zeros_like(x))
+    wbuf, (ws, dws) = beside(w, torch.zeros_like(w))
+    db = torch.empty(wide, dtype=BF, device="cuda")
+    ld, ldw = buf.stride(0), wbuf.stride(0)
+    name = "cuopx_gated_linear_backward" if gated else "cuopx_linear_backward"
+    args = (N.BF16, 0, 4, 0, m, n, k, dys.data_ptr(), ld, xs.data_ptr(), ld, ws.data_ptr(), ldw, zs.data_ptr(), ld,
+            dxs.data_ptr(), ld, dws.data_ptr(), ldw, db.data_ptr())
+    need = getattr(lib, name + "_workspace_size")(L._LINEAR_BACKWARD.pack(*args, 0, 0))
+    scratch = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    assert getattr(lib, name)(L._LINEAR_BACKWARD.pack(*args, scratch.data_ptr() if need else 0, need), stream) == N.SUCCESS
+    for what, t, (ref, bound) in zip(("dx", "dw", "db"), (dxs, dws, db), R.linear_backward(dy, x, w, z, "silu", False, gated)):
+        R.assert_within(t, ref, bound, what)
+    assert torch.equal(dys, dy) and torch.equal(xs, x) and torch.equal(zs, z) and torch.equal(ws, w)
+
+
+def test_columns_that_do_overlap_are_refused():
+    """One shared column, or a slice that runs on into the next row's columns of the other."""
+    buf = torch.zeros(40, 64, dtype=BF, device="cuda")
+    w = torch.zeros(16, 16, dtype=BF, device="cuda")
+    x = buf[:, :16]
+    flat = buf.view(-1)
+    wrapped = flat[56:56 + 38 * 64].as_strided((38, 16), (64, 1), 56)  # columns 56..63 and 0..7 of the next row
+    for call in (lambda: cx.linear(x, w, out=buf[:, 15:31]), lambda: cx.linear(x, w, out=x),
+                 lambda: cx.linear(x, w, out=buf[:, 16:32], preact=buf[:, 31:47]),
+                 lambda: cx.linear(x, w, residual=buf[:, 16:32], out=buf[:, 17:33]),
+                 lambda: cx.linear(x[:38], w, out=wrapped), lambda: cx.linear(x[:20], w, out=buf.view(80, 32)[:20, 16:]),
+                 lambda: cx.layer_norm(x, out=buf[:, 15:31]), lambda: cx.layer_norm(x[:38], out=wrapped),
+                 lambda: cx.dropout(x, 0.5, 1, out=buf[:, 8:24]), lambda: cx.dropout(x[:38], 0.5, 1, out=wrapped)):
+        with pytest.raises(cx.CuopError):
+            call()
