@@ -303,6 +303,9 @@ int cuopx_iamin(int64_t n, const float* x, int64_t incx, int64_t* result, void* 
  * 1 / (1 + exp(-z)):
  *   NONE z   RELU z > 0 ? z : +0   GELU z Phi(z)   SILU z s(z)   SIGMOID s(z)
  *   GELU_TANH z s(2 sqrt(2/pi) (z + 0.044715 z^3))
+ * RELU makes +0 of NaN; the others keep it.  Evaluated in fp32: s counts as 0
+ * where it is below 2^-126 (its argument below -87.3), and Phi where the normal
+ * density is (z < -13.2).
  */
 #define CUOPX_ACT_NONE 0
 #define CUOPX_ACT_RELU 1
@@ -374,7 +377,9 @@ typedef struct cuopx_linear_backward_args {
  * Gradients of cuopx_linear: dZ = dY * act'(Z), dX = dZ op(W)^T, dW =
  * X^T dZ (in W's layout), dbias = column sums of dZ (from the unrounded dZ).
  * The residual's gradient is dY itself.  dZ is rounded to the 16-bit type
- * between its computation and the two products, which take 16-bit operands.
+ * between its computation and the two products, which take 16-bit operands: in
+ * fp16 a dZ beyond 65504 makes infinities (or NaN) of dX and dW, as any fp16
+ * gradient of that size does; bf16 has fp32's range.
  * Of cuopx_gated_linear: dG = dY * U * act'(G), dU = dY * act(G), dZ =
  * [dG | dU].  Where the stored Z is infinite (fp16: the number was beyond
  * 65504), act' has its limit, and the gated form counts it as 3e38 with its

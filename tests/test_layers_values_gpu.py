@@ -217,3 +217,43 @@ def test_columns_that_do_overlap_are_refused():
                  lambda: cx.dropout(x, 0.5, 1, out=buf[:, 8:24]), lambda: cx.dropout(x[:38], 0.5, 1, out=wrapped)):
         with pytest.raises(cx.CuopError):
             call()
+
+
+# ------------------------------------------------------------------ documented values
+def test_relu_of_special_values():
+    """z > 0 ? z : +0, so NaN gives 0, with a derivative of 0."""
+    x = torch.zeros(4, 8, dtype=BF, device="cuda")
+    x[:, 0] = torch.tensor([INF, -INF, float("nan"), -3.0])
+    w = torch.zeros(8, 8, dtype=BF, device="cuda")
+    w[0] = 1.0
+    y = cx.linear(x, w, activation="relu")
+    assert (y[0] == INF).all() and (y[1:] == 0).all() and not torch.signbit(y[1:]).any()
+    one = torch.ones(1, 4, dtype=BF, device="cuda")
+    z = x[:, 0].contiguous()[None]
+    db = cx.linear_backward(one, one, torch.ones(4, 4, dtype=BF, device="cuda"), z, activation="relu",
+                            need_dx=False, need_dw=False)[2]
+    assert db.tolist() == [1.0, 0.0, 0.0, 0.0]
+
+
+def test_activations_below_the_normal_range_are_zero():
+    """s(z) and the normal density count as 0 where they leave fp32's normal range (z < -87.3, |z| > 13.2)."""
+    x = torch.zeros(2, 8, dtype=BF, device="cuda")
+    w = torch.zeros(8, 8, dtype=BF, device="cuda")
+    w[0] = 1.0
+    for act, inside, beyond in (("silu", -86.0, -95.0), ("sigmoid", -86.0, -95.0), ("gelu", -13.0, -14.0)):
+        x[0, 0], x[1, 0] = inside, beyond
+        y = cx.linear(x, w, activation=act)
+        assert (y[0] != 0).all() and (y[1] == 0).all(), act
+
+
+def test_fp16_dz_beyond_its_range():
+    """dZ is rounded to the operands' type for the two products: in fp16 it is infinite beyond 65504 while db, summed from
+    the unrounded dZ, is not; in bf16 the same numbers are in range."""
+    for dt in (HF, BF):
+        dy = torch.full((2, 8), 300.0, dtype=dt, device="cuda")
+        z = torch.full((2, 16), 20.0, dtype=dt, device="cuda")
+        z[0, 8:], z[1, 8:] = 300.0, -299.0
+        x, w = torch.ones(2, 8, dtype=dt, device="cuda"), torch.full((8, 16), 1.0 / 512, dtype=dt, device="cuda")
+        dx, dw, db = cx.gated_linear_backward(dy, x, w, z, activation="silu")
+        assert torch.isfinite(db).all()
+        assert torch.isfinite(dx).all() == (dt == BF)
