@@ -257,3 +257,54 @@ def test_fp16_dz_beyond_its_range():
         dx, dw, db = cx.gated_linear_backward(dy, x, w, z, activation="silu")
         assert torch.isfinite(db).all()
         assert torch.isfinite(dx).all() == (dt == BF)
+
+
+# ------------------------------------------------------------------ single rows, in-place gradients, repeated calls
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("trans_w", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 1200), (1, 2731, 520), (1, 520, 2047), (2, 1032, 1032), (3, 4096, 264)])
+def test_single_rows_backward_through_the_tensor_cores(m, n, k, trans_w, gated):
+    """2^20 multiplications and more: aligned operands, or copies of unaligned ones; dW has a depth of one to three."""
+    g = gen(n)
+    wide = 2 * n if gated else n
+    for dt, act in ((BF, "silu"), (HF, "gelu")):
+        x, dy, z = rnd(g, m, k, dtype=dt), rnd(g, m, n, dtype=dt), rnd(g, m, wide, dtype=dt)
+        w = rnd(g, *((wide, k) if trans_w else (k, wide)), scale=k ** -0.5, dtype=dt)
+        fn = cx.gated_linear_backward if gated else cx.linear_backward
+        got = fn(dy, x, w, z, activation=act, trans_w=trans_w)
+        for name, t, (ref, bound) in zip(("dx", "dw", "db"), got, R.linear_backward(dy, x, w, z, act, trans_w, gated)):
+            R.assert_within(t, ref, bound, name)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (50, 96), (700, 512), (900, 333), (300, 1001), (400, 4096), (160, 8192),
+                                       (40, 16384), (5, 20001), (160, 65536)])
+def test_norm_gradient_in_place_of_dy(rows, cols, dt):
+    """dX may be dY: the same bits as apart from it."""
+    lib, g = N.lib(), gen(cols)
+    stream = torch.cuda.current_stream().cuda_stream
+    x, dy, w = rnd(g, rows, cols, dtype=dt), rnd(g, rows, cols, dtype=dt), rnd(g, cols, dtype=dt)
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    cx.layer_norm(x, w, mean=mean, rstd=rstd)
+    ref = cx.layer_norm_backward(dy, x, mean, rstd, w)
+    grad, dw, db = dy.clone(), torch.empty_like(w), torch.empty_like(w)
+    code = N.F32 if dt == F32 else N.BF16
+    args = (code, code, rows, cols, 0.0, x.data_ptr(), cols, w.data_ptr(), 0, 0, 0, mean.data_ptr(), rstd.data_ptr(),
+            grad.data_ptr(), cols, grad.data_ptr(), cols, dw.data_ptr(), db.data_ptr())
+    need = lib.cuopx_layer_norm_backward_workspace_size(L._NORM.pack(*args, 0, 0))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert lib.cuopx_layer_norm_backward(L._NORM.pack(*args, ws.data_ptr(), need), stream) == N.SUCCESS
+    for a, b in zip((grad, dw, db), ref):
+        assert torch.equal(a, b)
+
+
+def test_repeated_calls_give_the_same_bits():
+    g = gen(17)
+    for m, n, k in ((4, 1024, 1024), (200, 520, 1024), (999, 683, 512), (1500, 1032, 512)):
+        x, dy, z = rnd(g, m, k, dtype=HF), rnd(g, m, n, dtype=HF), rnd(g, m, 2 * n, dtype=HF)
+        w = rnd(g, k, 2 * n, scale=k ** -0.5, dtype=HF)
+        first = (cx.gated_linear(x, w, activation="silu"),) + cx.gated_linear_backward(dy, x, w, z, activation="gelu")
+        for _ in range(3):
+            again = (cx.gated_linear(x, w, activation="silu"),) + cx.gated_linear_backward(dy, x, w, z, activation="gelu")
+            for a, b in zip(first, again):
+                assert torch.equal(a, b)
