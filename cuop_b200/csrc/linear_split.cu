@@ -35,11 +35,12 @@ constexpr int LSP_BK = 64;
 
 template <int TOK>
 struct SplitSmem {
-  static constexpr int STAGES = TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : TOK <= 128 ? 6 : 4;
+  static constexpr int STAGES = TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : 6;
   static constexpr int CTAS = TOK <= 64 ? 2 : 1;  // resident per SM
-  // From 128 rows on the partial sums reuse the ring, once every CTA of the
+  // With 128 rows the partial sums reuse the ring, once every CTA of the
   // cluster has finished its products; below, they have room of their own.
-  static constexpr bool ALIAS = TOK >= 128;
+  static constexpr bool ALIAS = TOK == 128;
+  static_assert(TOK <= 128, "one tile holds all rows");
   static constexpr int W_STAGE = LSP_COLS * LSP_BK * 2;
   static constexpr int X_STAGE = TOK * LSP_BK * 2;
   static constexpr int OFF_W = 0;
@@ -55,12 +56,11 @@ struct SplitSmem {
 };
 
 struct SplitParams {
-  int M, N, K, k_blocks;
+  int M, N, k_blocks;
   int cs;       // CTAs per cluster
-  int tiles_n;  // column tiles (N / 128, or N / 64 when gated)
   int w_up;     // gated: first column of the second projection in W
   int act;
-  int pairs;  // two columns per store: Y, Z, residual and bias can be read and written as 4-byte words
+  int pairs;  // Y's stores take two columns: N is even, Y's rows start on 4-byte boundaries
   const void* bias;
   const void* R;
   int64_t ldr;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   const int cs = p.cs;
   const int rank = static_cast<int>(cluster_ctarank());
   const int tile = static_cast<int>(blockIdx.x) / cs;
-  const int n0 = (tile % p.tiles_n) * TILE_N, m0 = (tile / p.tiles_n) * TOK;
+  const int n0 = tile * TILE_N;
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / cs);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / cs);
 
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
           if constexpr (W_MN) tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], c, k0, 0);
           else tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], k0, c, 0);
         }
-        tma_load_3d(smem + L::OFF_X + stage * L::X_STAGE, &tmX, &full[stage], k0, m0, 0);
+        tma_load_3d(smem + L::OFF_X + stage * L::X_STAGE, &tmX, &full[stage], k0, 0, 0);
         issued_mask |= 1u << stage;
         phase_mask = (phase_mask & ~(1u << stage)) | (phase << stage);
         if (++stage == STAGES) stage = 0, phase ^= 1u;
@@ -278,17 +278,17 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
 
   // Two neighbouring output columns of one row per step.
   const int own = LSP_COLS / cs, outs = TILE_N / cs;
-  const int rows = min(TOK, p.M - m0), col0 = n0 + rank * outs;
+  const int col0 = n0 + rank * outs;
   const T* bias = static_cast<const T*>(p.bias);
   const T* R = static_cast<const T*>(p.R);
   T* Y = static_cast<T*>(p.Y);
   T* Z = static_cast<T*>(p.Z);
   with_activation(p.act, [&](auto act) {
-    for (int e = threadIdx.x; e < rows * (outs / 2); e += LSP_THREADS) {
+    for (int e = threadIdx.x; e < p.M * (outs / 2); e += LSP_THREADS) {
       const int t = e / (outs / 2), f = 2 * (e % (outs / 2));
       const int col = col0 + f;
       if (col >= p.N) continue;
-      const int64_t row = static_cast<int64_t>(m0) + t;
+      const int64_t row = t;
       const bool two = col + 1 < p.N;
       float z[2][2] = {};  // [projection][column]
 #pragma unroll
@@ -343,9 +343,7 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   SplitParams prm;
   prm.M = static_cast<int>(p.M);
   prm.N = static_cast<int>(p.N);
-  prm.K = static_cast<int>(p.K);
   prm.k_blocks = static_cast<int>((p.K + LSP_BK - 1) / LSP_BK);
-  prm.tiles_n = static_cast<int>((p.N + TILE_N - 1) / TILE_N);
   prm.w_up = static_cast<int>(p.w_up);
   prm.act = p.act;
   prm.pairs = p.N % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 4 == 0;
@@ -356,7 +354,7 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   prm.ldy = p.ldy;
   prm.Z = p.Z;
   prm.ldz = p.ldz;
-  const int64_t tiles = static_cast<int64_t>(prm.tiles_n) * ((p.M + TOK - 1) / TOK);
+  const int64_t tiles = (p.N + TILE_N - 1) / TILE_N;
   auto kern = linear_split_kernel<T, W_MN, GATED, TOK>;
   static std::atomic<bool> attr_set[64] = {};
   static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once, one CTA per SM
@@ -409,14 +407,13 @@ int linear_split_rows(const LinearProblem& p, cudaStream_t stream) {
 
 }  // namespace
 
-// TMA reads X and W; Y, Z, residual and bias may have any alignment.
+// Up to 128 rows.  TMA reads X and W; Y, Z, residual and bias may have any alignment.
 bool linear_split_supported(const LinearProblem& p) {
-  if (p.M <= 0 || p.N <= 0 || p.K <= 0) return false;
-  if (p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
+  if (p.M <= 0 || p.M > 128 || p.N <= 0 || p.K <= 0) return false;
+  if (p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX) return false;
   if (!row_aligned16(p.X, p.M == 1 ? 0 : p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
-  if (p.gated && !p.transW && p.w_up % 8) return false;  // the second projection's first column in W's rows
-  return ((p.N + 63) / 64) * ((p.M + 15) / 16) < (int64_t(1) << 27);
+  return !p.gated || p.transW || p.w_up % 8 == 0;  // the second projection's first column in W's rows
 }
 
 int linear_split(const LinearProblem& p, cudaStream_t stream) {
