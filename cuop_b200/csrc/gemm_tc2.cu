@@ -531,84 +531,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
             });
         if (!done) break;
       } else {
-      if (!products()) break;
-      const int64_t grow = static_cast<int64_t>(m0) + row_in_tile;
+        if (!products()) break;
+        const int64_t grow = static_cast<int64_t>(m0) + row_in_tile;
 #pragma unroll 1
-      for (int ch = 0; ch < PBN / P_CHUNK; ++ch) {
-        // Chunk ch is TMEM columns [64ch, 64ch+64) of the tile's slots.
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32b_x32(t_row + ch * P_CHUNK, r0);
-        tmem_ld_32x32b_x32(t_row + ch * P_CHUNK + 32, r1);
-        tmem_wait_ld();
-        if (ch % CHUNKS_PER_SLOT == CHUNKS_PER_SLOT - 1) {
-          // Last read of this slot: the MMA issuer may overwrite it.
-          tc_fence_before_sync();
+        for (int ch = 0; ch < PBN / P_CHUNK; ++ch) {
+          // Chunk ch is TMEM columns [64ch, 64ch+64) of the tile's slots.
+          uint32_t r0[32], r1[32];
+          tmem_ld_32x32b_x32(t_row + ch * P_CHUNK, r0);
+          tmem_ld_32x32b_x32(t_row + ch * P_CHUNK + 32, r1);
+          tmem_wait_ld();
+          if (ch % CHUNKS_PER_SLOT == CHUNKS_PER_SLOT - 1) {
+            // Last read of this slot: the MMA issuer may overwrite it.
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[s0 + ch / CHUNKS_PER_SLOT], 0));
+          }
+          float v[64];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] = __uint_as_float(r0[i]);
+            v[32 + i] = __uint_as_float(r1[i]);
+          }
+          if (p.beta != 0.f && grow < p.M) {
+            const int64_t gcol0 = static_cast<int64_t>(n0) + ch * P_CHUNK;
+            const T* crow = Cin + static_cast<int64_t>(b) * p.strideC + grow * p.ldc;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              v[i] = gcol0 + i < p.N ? epi_axpby(p.alpha, v[i], p.beta, to_acc<T>(crow[gcol0 + i]))
+                                     : epi_scale(p.alpha, v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = epi_scale(p.alpha, v[i]);
+          }
+          if (p.epi) {
+            const int64_t gcol0 = static_cast<int64_t>(n0) + ch * P_CHUNK;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (gcol0 + i < p.N) v[i] = apply_epilogue<T>(v[i], p.bias, gcol0 + i, p.epi);
+          }
+          if (lane == 0) bulk_wait_group_read<1>();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[s0 + ch / CHUNKS_PER_SLOT], 0));
-        }
-        float v[64];
+          unsigned char* sbase = stage_base + sbuf * L::C_STAGE;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          v[i] = __uint_as_float(r0[i]);
-          v[32 + i] = __uint_as_float(r1[i]);
-        }
-        if (p.beta != 0.f && grow < p.M) {
-          const int64_t gcol0 = static_cast<int64_t>(n0) + ch * P_CHUNK;
-          const T* crow = Cin + static_cast<int64_t>(b) * p.strideC + grow * p.ldc;
+          for (int j = 0; j < 8; ++j) {
+            uint4 w;
+            w.x = pack2_pair<T>(v[8 * j + 0], v[8 * j + 1]);
+            w.y = pack2_pair<T>(v[8 * j + 2], v[8 * j + 3]);
+            w.z = pack2_pair<T>(v[8 * j + 4], v[8 * j + 5]);
+            w.w = pack2_pair<T>(v[8 * j + 6], v[8 * j + 7]);
+            *reinterpret_cast<uint4*>(sbase + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
+          }
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&tmC, sbase, n0 + ch * P_CHUNK, m0 + 32 * q, b);
+            bulk_commit_group();
+          }
+          if (p.npeers > 0) {
+            // Same 32 x 64 chunk to every peer's output: lanes 8r..8r+7 write
+            // the 128 contiguous bytes of one row, so each warp store is four
+            // full 128-byte lines over NVLink.  Rows past M and 16-byte
+            // column groups past N are skipped (N is a multiple of 8).
+            const int c16 = lane & 7;
+            const int64_t gcol = static_cast<int64_t>(n0) + ch * P_CHUNK + 8 * c16;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            v[i] = gcol0 + i < p.N ? epi_axpby(p.alpha, v[i], p.beta, to_acc<T>(crow[gcol0 + i]))
-                                   : epi_scale(p.alpha, v[i]);
-        } else {
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              const int64_t grow_r = static_cast<int64_t>(m0) + 32 * q + r;
+              const uint4 w = *reinterpret_cast<const uint4*>(sbase + r * 128 + ((c16 ^ (r & 7)) << 4));
+              if (grow_r < p.M && gcol < p.N) {
+                const int64_t off = grow_r * p.ldc + gcol;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = epi_scale(p.alpha, v[i]);
-        }
-        if (p.epi) {
-          const int64_t gcol0 = static_cast<int64_t>(n0) + ch * P_CHUNK;
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (gcol0 + i < p.N) v[i] = apply_epilogue<T>(v[i], p.bias, gcol0 + i, p.epi);
-        }
-        if (lane == 0) bulk_wait_group_read<1>();
-        __syncwarp();
-        unsigned char* sbase = stage_base + sbuf * L::C_STAGE;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint4 w;
-          w.x = pack2_pair<T>(v[8 * j + 0], v[8 * j + 1]);
-          w.y = pack2_pair<T>(v[8 * j + 2], v[8 * j + 3]);
-          w.z = pack2_pair<T>(v[8 * j + 4], v[8 * j + 5]);
-          w.w = pack2_pair<T>(v[8 * j + 6], v[8 * j + 7]);
-          *reinterpret_cast<uint4*>(sbase + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(&tmC, sbase, n0 + ch * P_CHUNK, m0 + 32 * q, b);
-          bulk_commit_group();
-        }
-        if (p.npeers > 0) {
-          // Same 32 x 64 chunk to every peer's output: lanes 8r..8r+7 write
-          // the 128 contiguous bytes of one row, so each warp store is four
-          // full 128-byte lines over NVLink.  Rows past M and 16-byte
-          // column groups past N are skipped (N is a multiple of 8).
-          const int c16 = lane & 7;
-          const int64_t gcol = static_cast<int64_t>(n0) + ch * P_CHUNK + 8 * c16;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3);
-            const int64_t grow_r = static_cast<int64_t>(m0) + 32 * q + r;
-            const uint4 w = *reinterpret_cast<const uint4*>(sbase + r * 128 + ((c16 ^ (r & 7)) << 4));
-            if (grow_r < p.M && gcol < p.N) {
-              const int64_t off = grow_r * p.ldc + gcol;
-#pragma unroll
-              for (int d = 0; d < P_MAX_PEERS; ++d)  // constant indices keep peer_C in the param bank
-                if (d < p.npeers) *reinterpret_cast<uint4*>(static_cast<T*>(p.peer_C[d]) + off) = w;
+                for (int d = 0; d < P_MAX_PEERS; ++d)  // constant indices keep peer_C in the param bank
+                  if (d < p.npeers) *reinterpret_cast<uint4*>(static_cast<T*>(p.peer_C[d]) + off) = w;
+              }
             }
           }
+          sbuf ^= 1;
         }
-        sbuf ^= 1;
-      }
       }
       full_bits ^= 1u << s0;
       if (SPT == 1) acc = acc + 1 == P_SLOTS ? 0 : acc + 1;

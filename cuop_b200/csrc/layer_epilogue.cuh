@@ -236,7 +236,8 @@ __device__ __forceinline__ bool layer_epilogue_tile(uint32_t t_row, int n0, int 
       }
       if (e.Y) store_chunk_plain<T>(stage + ybuf * BUF, static_cast<T*>(e.Y), e.ldy, 0, c, m0, M, N, lane);
     }
-  }  return true;
+  }
+  return true;
 }
 
 }  // namespace cuopx
