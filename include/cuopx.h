@@ -303,9 +303,9 @@ int cuopx_iamin(int64_t n, const float* x, int64_t incx, int64_t* result, void* 
  * 1 / (1 + exp(-z)):
  *   NONE z   RELU z > 0 ? z : +0   GELU z Phi(z)   SILU z s(z)   SIGMOID s(z)
  *   GELU_TANH z s(2 sqrt(2/pi) (z + 0.044715 z^3))
- * RELU makes +0 of NaN; the others keep it.  Evaluated in fp32: s counts as 0
- * where it is below 2^-126 (its argument below -87.3), and Phi where the normal
- * density is (z < -13.2).
+ * RELU makes +0 of NaN; the others keep it, and GELU, GELU_TANH and SILU make it
+ * of -inf (-inf * 0).  Evaluated in fp32: s counts as 0 where it is below 2^-126
+ * (its argument below -87.3), and Phi where the normal density is (z < -13.2).
  */
 #define CUOPX_ACT_NONE 0
 #define CUOPX_ACT_RELU 1
