@@ -406,6 +406,41 @@ __device__ __forceinline__ void tma_store_3d(const void* tmap, const void* smem_
       : "memory");
 }
 
+// A TMA store fills whole 16-byte groups: where a row ends inside one, it also
+// overwrites what lies behind the row up to the group's end (measured: rows of 3
+// 16-bit elements, columns 3 to 7).  So only these chunks may go out by TMA:
+// all of them when rows end with a group, else those that end inside the row.
+template <int ES>
+__device__ __forceinline__ bool tma_store_exact(int64_t chunk_end, int64_t N) {
+  return N * ES % 16 == 0 || chunk_end <= N;
+}
+
+// The others go out here: rows m0.. of a 32 x 128-byte chunk, staged with the
+// 128-byte swizzle (16-byte group j of row r at j ^ (r & 7)), to columns c.. of
+// `out`, in elements of ES (2 or 4) bytes, those inside M x N only.  The whole
+// warp, after __syncwarp.
+template <int ES>
+__device__ __forceinline__ void store_staged_chunk(const unsigned char* buf, void* out, int64_t ld, int64_t c, int m0, int M,
+                                                   int N, int lane) {
+  if (c >= N) return;
+  const int rows = min(32, M - m0);
+  const int64_t col = c + (ES == 2 ? 2 * lane : lane);
+  const bool one = col < N, two = ES == 2 && col + 1 < N;
+  const unsigned char* src = buf + (lane & 3) * 4;
+  unsigned char* dst = static_cast<unsigned char*>(out) + (m0 * ld + col) * ES;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r, dst += ld * ES) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(src + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+    if constexpr (ES == 2) {
+      if (one) reinterpret_cast<unsigned short*>(dst)[0] = static_cast<unsigned short>(w);
+      if (two) reinterpret_cast<unsigned short*>(dst)[1] = static_cast<unsigned short>(w >> 16);
+    } else {
+      if (one) *reinterpret_cast<uint32_t*>(dst) = w;
+    }
+  }
+  __syncwarp();
+}
+
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Wait until at most N committed bulk groups still read shared memory.

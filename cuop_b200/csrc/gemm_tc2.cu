@@ -715,8 +715,8 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
                  : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, P_BK);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
-  if (!layer.epi.Y) ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
-  if (p.Z && !layer.epi.Z) {
+  if (layer.epi.tma_y) ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
+  if (layer.epi.tma_z) {
     ok &= make_map(&layer.tmZ, dt, p.Z, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);
     if (MODE == kPairGated)
       ok &= make_map(&layer.tmZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, P_CHUNK, 32);

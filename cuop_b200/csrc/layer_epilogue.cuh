@@ -20,13 +20,14 @@ struct LayerEpi {
   int has_z;     // store the pre-activation
   int vec_bias;  // bias can be read in 16-byte groups
   int vec_res;   // so can the residual's rows
-  // Set where rows are not on 16-byte boundaries, which TMA cannot store: the
-  // staged tile then goes out in plain 2-byte stores, 64 columns of a row per
-  // two of a warp's.
   void* Y;
   int64_t ldy;
   void* Z;
   int64_t ldz;
+  // 64-column chunks that end at or before this column go out by TMA, the
+  // others in plain 2-byte stores, 64 columns of a row per two of a warp's: 0
+  // where rows do not start on 16-byte boundaries, N where they do not end on one.
+  int tma_y, tma_z;
 };
 
 inline LayerEpi layer_epi(const LinearProblem& p) {
@@ -38,10 +39,13 @@ inline LayerEpi layer_epi(const LinearProblem& p) {
   e.has_z = p.Z != nullptr;
   e.vec_bias = p.N % 8 == 0 && row_aligned16(p.bias, 0);
   e.vec_res = p.N % 8 == 0 && row_aligned16(p.R, p.ldr);
-  e.Y = row_aligned16(p.Y, p.ldy) ? nullptr : p.Y;
+  e.Y = p.Y;
   e.ldy = p.ldy;
-  e.Z = p.Z == nullptr || (row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0)) ? nullptr : p.Z;
+  e.Z = p.Z;
   e.ldz = p.ldz;
+  const int inside = p.N % 8 == 0 ? INT32_MAX : static_cast<int>(p.N);
+  e.tma_y = row_aligned16(p.Y, p.ldy) ? inside : 0;
+  e.tma_z = p.Z && row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0) ? inside : 0;  // gated: U starts at column N
   return e;
 }
 
@@ -111,22 +115,6 @@ __device__ __forceinline__ void stage_row32(unsigned char* buf, int lane, int h,
     w.w = pack2_layer<T>(v[8 * j + 6], v[8 * j + 7]);
     *reinterpret_cast<uint4*>(buf + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)) = w;
   }
-}
-
-// The staged 32 x 64 chunk at `buf` (whole warp, after __syncwarp) to rows m0.. and columns c.. of an unaligned matrix.
-template <typename T>
-__device__ __forceinline__ void store_chunk_plain(const unsigned char* buf, T* out, int64_t ld, int64_t col0, int c, int m0,
-                                                  int M, int N, int lane) {
-  const int rows = min(32, M - m0);
-  const int col = c + 2 * lane;
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-    unsigned short* dst = reinterpret_cast<unsigned short*>(out + (static_cast<int64_t>(m0) + r) * ld + col0 + col);
-    if (col < N) dst[0] = static_cast<unsigned short>(w);
-    if (col + 1 < N) dst[1] = static_cast<unsigned short>(w >> 16);
-  }
-  __syncwarp();
 }
 
 // One warp's rows of PART columns of one tile.  t_row: TMEM address of the
@@ -223,18 +211,18 @@ __device__ __forceinline__ bool layer_epilogue_tile(uint32_t t_row, int n0, int 
       __syncwarp();
       const int c = n0 + 32 * (half - 1);
       if (lane == 0) {
-        if (e.has_z && !e.Z) {
+        if (e.has_z && c + 64 <= e.tma_z) {
           tma_store_3d(tmZ, stage, c, m0, 0);
           if constexpr (GATED) tma_store_3d(tmZ2, stage + BUF, c, m0, 0);
         }
-        if (!e.Y) tma_store_3d(tmY, stage + ybuf * BUF, c, m0, 0);
+        if (c + 64 <= e.tma_y) tma_store_3d(tmY, stage + ybuf * BUF, c, m0, 0);
         bulk_commit_group();
       }
-      if (e.Z) {
-        store_chunk_plain<T>(stage, static_cast<T*>(e.Z), e.ldz, 0, c, m0, M, N, lane);
-        if constexpr (GATED) store_chunk_plain<T>(stage + BUF, static_cast<T*>(e.Z), e.ldz, N, c, m0, M, N, lane);
+      if (e.has_z && c + 64 > e.tma_z) {
+        store_staged_chunk<2>(stage, e.Z, e.ldz, c, m0, M, N, lane);
+        if constexpr (GATED) store_staged_chunk<2>(stage + BUF, static_cast<T*>(e.Z) + N, e.ldz, c, m0, M, N, lane);
       }
-      if (e.Y) store_chunk_plain<T>(stage + ybuf * BUF, static_cast<T*>(e.Y), e.ldy, 0, c, m0, M, N, lane);
+      if (c + 64 > e.tma_y) store_staged_chunk<2>(stage + ybuf * BUF, e.Y, e.ldy, c, m0, M, N, lane);
     }
   }
   return true;

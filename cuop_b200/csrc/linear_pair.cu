@@ -316,8 +316,8 @@ int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
                  : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, LP_BK, LP_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, LP_BK);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LP_BK, LP_BN / 2);
-  if (!prm.epi.Y) ok &= make_map(&mY, dt, p.Y, p.N, p.M, 1, p.ldy, 0, 64, 32);
-  if (p.Z && !prm.epi.Z) {
+  if (prm.epi.tma_y) ok &= make_map(&mY, dt, p.Y, p.N, p.M, 1, p.ldy, 0, 64, 32);
+  if (prm.epi.tma_z) {
     ok &= make_map(&mZ, dt, p.Z, p.N, p.M, 1, p.ldz, 0, 64, 32);
     if (GATED) ok &= make_map(&mZ2, dt, static_cast<const T*>(p.Z) + p.N, p.N, p.M, 1, p.ldz, 0, 64, 32);
   }

@@ -219,6 +219,39 @@ def test_columns_that_do_overlap_are_refused():
             call()
 
 
+# ------------------------------------------------------------------ rows that end inside a 16-byte group
+def guarded(rows, cols, dt, at=0):
+    """A rows x cols matrix whose rows start on 16-byte boundaries and end anywhere, NaN all around it, also right behind
+    its last element."""
+    ld = (cols + at + 7) // 8 * 8 + 8
+    buf = torch.full((8 + rows * ld + 8,), float("nan"), dtype=dt, device="cuda")
+    return buf[8:8 + rows * ld].view(rows, ld)[:, at:at + cols], buf
+
+
+def only_inside(view, buf):
+    """Whether every NaN around the matrix is still there and none is left in it."""
+    return not torch.isnan(view).any() and int((~torch.isnan(buf)).sum()) == view.numel()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(20, 3, 64), (300, 3, 128), (300, 61, 72), (200, 377, 1024), (140, 70, 6208), (513, 257, 136),
+                                   (2600, 1027, 136)])
+def test_forward_writes_end_where_rows_end(m, n, k, gated):
+    g = gen(n)
+    for dt in (BF, HF):
+        wide = 2 * n if gated else n
+        x, w = rnd(g, m, k, dtype=dt), rnd(g, k, wide, scale=k ** -0.5, dtype=dt)
+        (y, ybuf), (z, zbuf) = guarded(m, n, dt), guarded(m, wide, dt)
+        if gated:
+            cx.gated_linear(x, w, activation="silu", out=y, preact=z)
+        else:
+            cx.linear(x, w, activation="silu", out=y, preact=z)
+        yr, zr, ey, ez = R.linear(x, w, None, None, "silu", False, gated)
+        R.assert_within(y, yr, ey, "y")
+        R.assert_within(z, zr, ez, "z")
+        assert only_inside(y, ybuf) and only_inside(z, zbuf), cx.last_kernel()
+
+
 # ------------------------------------------------------------------ documented values
 def test_relu_of_special_values():
     """z > 0 ? z : +0, so NaN gives 0, with a derivative of 0."""
