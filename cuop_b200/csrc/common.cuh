@@ -408,11 +408,12 @@ __device__ __forceinline__ void tma_store_3d(const void* tmap, const void* smem_
 
 // A TMA store fills whole 16-byte groups: where a row ends inside one, it also
 // overwrites what lies behind the row up to the group's end (measured: rows of 3
-// 16-bit elements, columns 3 to 7).  So only these chunks may go out by TMA:
-// all of them when rows end with a group, else those that end inside the row.
+// 16-bit elements, columns 3 to 7).  So only chunks that end at or before this
+// column may go out by TMA: all of them when rows of N end with a group, else
+// those that end inside the row.
 template <int ES>
-__device__ __forceinline__ bool tma_store_exact(int64_t chunk_end, int64_t N) {
-  return N * ES % 16 == 0 || chunk_end <= N;
+inline int tma_store_cols(int64_t N) {
+  return N * ES % 16 == 0 ? INT32_MAX : static_cast<int>(N);
 }
 
 // The others go out here: rows m0.. of a 32 x 128-byte chunk, staged with the

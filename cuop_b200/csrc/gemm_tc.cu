@@ -54,11 +54,17 @@ constexpr int CLC_SLOTS = 16;
 // Arrivals that free a scheduler slot: producer, MMA issuer, epilogue warps.
 constexpr int CLC_READERS = 2 + EPI_WARPS;
 
+// How output chunks leave: by TMA; also to peers; or, kTcRagged, the last one of
+// a row in plain stores, which N other than a multiple of 8 needs
+// (tma_store_cols).  An instantiation of its own: the branch alone cost the
+// others 0.4 % (4096 x 128 x 128 x 64 bf16).
+enum TcStore { kTcTma = 0, kTcPeers = 1, kTcRagged = 2 };
+
 struct TcParams {
   int M, N, K, batch;
   int tiles_m, tiles_n, num_tiles, k_blocks;
   float alpha, beta;
-  const void* C_in;  // read only when beta != 0
+  void* C;  // read when beta != 0, written where TMA would write past a row's end
   int64_t ldc, strideC;
   const void* bias;  // CUOPX_EPI_BIAS: N elements of the output type
   int epi;           // CUOPX_EPI_* flags
@@ -137,7 +143,7 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <typename T, int BN, int STAGES, bool A_MN, bool B_MN, bool PEERS = false, int CPS = 1>
+template <typename T, int BN, int STAGES, bool A_MN, bool B_MN, int STORE = kTcTma, int CPS = 1>
 __global__ void __launch_bounds__(NUM_THREADS, CPS)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, const TcParams p) {
@@ -393,7 +399,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CPS)
     int acc = 0;
     uint32_t acc_phase = 0;
     int sbuf = 0;
-    const T* Cin = static_cast<const T*>(p.C_in);
+    const T* Cin = static_cast<const T*>(p.C);
     int t = blockIdx.x;
     for (int seq = 0;; ++seq) {
       int b, mt, nt;
@@ -453,11 +459,16 @@ __global__ void __launch_bounds__(NUM_THREADS, CPS)
         }
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(&tmC, sbase, n0 + ch * STAGE_CHUNK_COLS, m0 + 32 * q, b);
+        const int c0 = n0 + ch * STAGE_CHUNK_COLS;
+        if (STORE == kTcRagged && c0 + STAGE_CHUNK_COLS > p.N) {
+          store_staged_chunk<2>(sbase, static_cast<T*>(p.C) + static_cast<int64_t>(b) * p.strideC, p.ldc, c0, m0 + 32 * q,
+                                p.M, p.N, lane);
+          if (lane == 0) bulk_commit_group();
+        } else if (lane == 0) {
+          tma_store_3d(&tmC, sbase, c0, m0 + 32 * q, b);
           bulk_commit_group();
         }
-        if (PEERS && p.npeers > 0) {
+        if (STORE == kTcPeers && p.npeers > 0) {
           // Same 32 x 64 chunk to every peer's output: lanes 8r..8r+7 write
           // the 128 contiguous bytes of one row (four full 128-byte lines per
           // warp store).  Rows past M and 16-byte groups past N are skipped.
@@ -497,13 +508,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CPS)
     // With peer outputs, the local stores are also waited for completely
     // before this thread's system-scope fence.
     if (lane == 0) {
-      if (PEERS) bulk_wait_group<0>();
+      if (STORE == kTcPeers) bulk_wait_group<0>();
       else bulk_wait_group_read<0>();
     }
     __syncwarp();
     // Peer stores of this thread are ordered before anything the stream runs
     // after the kernel (the peer barrier's release).
-    if (PEERS && p.npeers > 0) __threadfence_system();
+    if (STORE == kTcPeers && p.npeers > 0) __threadfence_system();
   }
 
   tc_fence_before_sync();
@@ -559,7 +570,7 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int64_
   return make_map_es(map, dt, 2, base, inner, rows, batch, ld, bstride, box_inner, box_rows);
 }
 
-template <typename T, int BN, int STAGES, bool A_MN, bool B_MN, bool PEERS = false, int CPS = 1>
+template <typename T, int BN, int STAGES, bool A_MN, bool B_MN, int STORE = kTcTma, int CPS = 1>
 int launch_tc(const GemmProblem& p, cudaStream_t stream, const char* name, void* const* peers = nullptr,
               int npeers = 0) {
   using L = SmemLayout<BN, STAGES, CPS>;
@@ -591,7 +602,7 @@ int launch_tc(const GemmProblem& p, cudaStream_t stream, const char* name, void*
   prm.k_blocks = static_cast<int>((p.K + BK - 1) / BK);
   prm.alpha = static_cast<float>(p.alpha);
   prm.beta = static_cast<float>(p.beta);
-  prm.C_in = p.C;
+  prm.C = p.C;
   prm.ldc = p.ldc;
   prm.strideC = p.strideC;
   prm.bias = p.bias;
@@ -610,7 +621,7 @@ int launch_tc(const GemmProblem& p, cudaStream_t stream, const char* name, void*
     prm.prefetch_tiles = static_cast<int>(std::max<int64_t>(1, std::min(reach, cap)));
   }
 
-  auto kern = gemm_tc_kernel<T, BN, STAGES, A_MN, B_MN, PEERS, CPS>;
+  auto kern = gemm_tc_kernel<T, BN, STAGES, A_MN, B_MN, STORE, CPS>;
   static std::atomic<bool> attr_set[64] = {};  // per instantiation and device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -632,13 +643,19 @@ int launch_tc(const GemmProblem& p, cudaStream_t stream, const char* name, void*
   return check_launch();
 }
 
+template <typename T, int BN, int STAGES, int CPS, int STORE>
+int launch_tc_store(const GemmProblem& p, cudaStream_t stream, const char* name) {
+  const bool a_mn = p.transA, b_mn = !p.transB;
+  if (!a_mn && b_mn) return launch_tc<T, BN, STAGES, false, true, STORE, CPS>(p, stream, name);
+  if (!a_mn && !b_mn) return launch_tc<T, BN, STAGES, false, false, STORE, CPS>(p, stream, name);
+  if (a_mn && b_mn) return launch_tc<T, BN, STAGES, true, true, STORE, CPS>(p, stream, name);
+  return launch_tc<T, BN, STAGES, true, false, STORE, CPS>(p, stream, name);
+}
+
 template <typename T, int BN, int STAGES, int CPS = 1>
 int launch_tc_layout(const GemmProblem& p, cudaStream_t stream, const char* name) {
-  const bool a_mn = p.transA, b_mn = !p.transB;
-  if (!a_mn && b_mn) return launch_tc<T, BN, STAGES, false, true, false, CPS>(p, stream, name);
-  if (!a_mn && !b_mn) return launch_tc<T, BN, STAGES, false, false, false, CPS>(p, stream, name);
-  if (a_mn && b_mn) return launch_tc<T, BN, STAGES, true, true, false, CPS>(p, stream, name);
-  return launch_tc<T, BN, STAGES, true, false, false, CPS>(p, stream, name);
+  return p.N % 8 == 0 ? launch_tc_store<T, BN, STAGES, CPS, kTcTma>(p, stream, name)
+                      : launch_tc_store<T, BN, STAGES, CPS, kTcRagged>(p, stream, name);
 }
 
 }  // namespace
@@ -696,11 +713,11 @@ int gemm_tc_peers(const GemmProblem& p, void* const* peers, int npeers, cudaStre
   const bool wide = bn == 256;
   const char* name = wide ? "gemm_tc_128x256_peer" : "gemm_tc_128x128_peer";
   if (p.dtype == CUOPX_BF16) {
-    return wide ? launch_tc<__nv_bfloat16, 256, 4, false, true, true>(p, stream, name, peers, npeers)
-                : launch_tc<__nv_bfloat16, 128, 6, false, true, true>(p, stream, name, peers, npeers);
+    return wide ? launch_tc<__nv_bfloat16, 256, 4, false, true, kTcPeers>(p, stream, name, peers, npeers)
+                : launch_tc<__nv_bfloat16, 128, 6, false, true, kTcPeers>(p, stream, name, peers, npeers);
   }
-  return wide ? launch_tc<__half, 256, 4, false, true, true>(p, stream, name, peers, npeers)
-              : launch_tc<__half, 128, 6, false, true, true>(p, stream, name, peers, npeers);
+  return wide ? launch_tc<__half, 256, 4, false, true, kTcPeers>(p, stream, name, peers, npeers)
+              : launch_tc<__half, 128, 6, false, true, kTcPeers>(p, stream, name, peers, npeers);
 }
 
 }  // namespace cuopx

@@ -75,6 +75,9 @@ struct PairCfg {
 };
 
 enum PairMode { kPairGemm = 0, kPairLinear = 1, kPairGated = 2 };
+// RAGGED (kPairGemm): a row's last output chunk leaves in plain stores, which N
+// other than a multiple of 8 needs (tma_store_cols).  The layers' epilogue does
+// so by itself.
 
 // kPairLinear drains a tile with eight warps, two per TMEM lane quarter and
 // half of the columns each: its activation and residual make the drain of the
@@ -119,7 +122,7 @@ struct PairParams {
   int M, N, K, batch;
   int tiles_m, tiles_n, num_tiles, k_blocks;  // tiles are 256 x PBN pair tiles
   float alpha, beta;
-  const void* C_in;
+  void* C;  // read when beta != 0, written where TMA would write past a row's end
   int64_t ldc, strideC;
   // Peer-store all-gather: each staged output chunk is also written to
   // peer_C[i] (same row stride ldc, same column offset) for i < npeers.
@@ -211,7 +214,7 @@ __device__ __forceinline__ uint32_t pack2_pair<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm>
+template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm, bool RAGGED = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THREADS, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const PairParams p,
@@ -498,7 +501,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
     int acc = 0;             // first TMEM slot of the tile (rotates when SPT == 1)
     uint32_t full_bits = 0;  // bit s: parity of slot s's next acc_full phase
     int sbuf = 0;
-    const T* Cin = static_cast<const T*>(p.C_in);
+    const T* Cin = static_cast<const T*>(p.C);
     int t = pair;
     for (int seq = 0;; ++seq) {
       int b, mt, nt;
@@ -583,8 +586,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
           }
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) {
-            tma_store_3d(&tmC, sbase, n0 + ch * P_CHUNK, m0 + 32 * q, b);
+          const int c0 = n0 + ch * P_CHUNK;
+          if (RAGGED && c0 + P_CHUNK > p.N) {
+            store_staged_chunk<2>(sbase, static_cast<T*>(p.C) + static_cast<int64_t>(b) * p.strideC, p.ldc, c0, m0 + 32 * q,
+                                  p.M, p.N, lane);
+            if (lane == 0) bulk_commit_group();
+          } else if (lane == 0) {
+            tma_store_3d(&tmC, sbase, c0, m0 + 32 * q, b);
             bulk_commit_group();
           }
           if (p.npeers > 0) {
@@ -645,7 +653,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
   }
 }
 
-template <typename T, bool A_MN, bool B_MN, int PBN>
+template <typename T, bool A_MN, bool B_MN, int PBN, bool RAGGED>
 int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void* const* peers = nullptr,
                int npeers = 0) {
   using L = PairSmem<PBN>;
@@ -671,7 +679,7 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
   prm.k_blocks = static_cast<int>((p.K + P_BK - 1) / P_BK);
   prm.alpha = static_cast<float>(p.alpha);
   prm.beta = static_cast<float>(p.beta);
-  prm.C_in = p.C;
+  prm.C = p.C;
   prm.ldc = p.ldc;
   prm.strideC = p.strideC;
   prm.bias = p.bias;
@@ -679,7 +687,7 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
   if (npeers < 0 || npeers > P_MAX_PEERS) return CUOPX_INVALID_ARGUMENT;
   prm.npeers = npeers;
   for (int i = 0; i < P_MAX_PEERS; ++i) prm.peer_C[i] = i < npeers ? peers[i] : nullptr;
-  auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN>;
+  auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN, kPairGemm, RAGGED>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -786,22 +794,22 @@ int gemm_tc2(const GemmProblem& p, cudaStream_t stream, int pbn) { return gemm_t
 
 namespace {
 
-template <int PBN>
+template <int PBN, bool RAGGED = false>
 int launch_tc2_layout(const GemmProblem& p, void* const* peers, int npeers, cudaStream_t stream) {
   const bool a_mn = p.transA, b_mn = !p.transB;
   const char* name = PBN == 512   ? (npeers > 0 ? "gemm_tc2_256x512_peer" : "gemm_tc2_256x512")
                      : PBN == 256 ? (npeers > 0 ? "gemm_tc2_256x256_peer" : "gemm_tc2_256x256")
                                   : (npeers > 0 ? "gemm_tc2_256x128_peer" : "gemm_tc2_256x128");
   if (p.dtype == CUOPX_BF16) {
-    if (!a_mn && b_mn) return launch_tc2<__nv_bfloat16, false, true, PBN>(p, stream, name, peers, npeers);
-    if (!a_mn && !b_mn) return launch_tc2<__nv_bfloat16, false, false, PBN>(p, stream, name, peers, npeers);
-    if (a_mn && b_mn) return launch_tc2<__nv_bfloat16, true, true, PBN>(p, stream, name, peers, npeers);
-    return launch_tc2<__nv_bfloat16, true, false, PBN>(p, stream, name, peers, npeers);
+    if (!a_mn && b_mn) return launch_tc2<__nv_bfloat16, false, true, PBN, RAGGED>(p, stream, name, peers, npeers);
+    if (!a_mn && !b_mn) return launch_tc2<__nv_bfloat16, false, false, PBN, RAGGED>(p, stream, name, peers, npeers);
+    if (a_mn && b_mn) return launch_tc2<__nv_bfloat16, true, true, PBN, RAGGED>(p, stream, name, peers, npeers);
+    return launch_tc2<__nv_bfloat16, true, false, PBN, RAGGED>(p, stream, name, peers, npeers);
   }
-  if (!a_mn && b_mn) return launch_tc2<__half, false, true, PBN>(p, stream, name, peers, npeers);
-  if (!a_mn && !b_mn) return launch_tc2<__half, false, false, PBN>(p, stream, name, peers, npeers);
-  if (a_mn && b_mn) return launch_tc2<__half, true, true, PBN>(p, stream, name, peers, npeers);
-  return launch_tc2<__half, true, false, PBN>(p, stream, name, peers, npeers);
+  if (!a_mn && b_mn) return launch_tc2<__half, false, true, PBN, RAGGED>(p, stream, name, peers, npeers);
+  if (!a_mn && !b_mn) return launch_tc2<__half, false, false, PBN, RAGGED>(p, stream, name, peers, npeers);
+  if (a_mn && b_mn) return launch_tc2<__half, true, true, PBN, RAGGED>(p, stream, name, peers, npeers);
+  return launch_tc2<__half, true, false, PBN, RAGGED>(p, stream, name, peers, npeers);
 }
 
 }  // namespace
@@ -826,6 +834,7 @@ int gemm_tc2_pick_width(const GemmProblem& p, bool peers) {
 }
 
 int gemm_tc2_peers(const GemmProblem& p, void* const* peers, int npeers, cudaStream_t stream, int pbn) {
+  if (p.N % 8 != 0) return launch_tc2_layout<256, true>(p, peers, npeers, stream);
   if (pbn == 0) pbn = gemm_tc2_pick_width(p, npeers > 0);
   if (pbn == 128) return launch_tc2_layout<128>(p, peers, npeers, stream);
   return pbn == 512 ? launch_tc2_layout<512>(p, peers, npeers, stream)

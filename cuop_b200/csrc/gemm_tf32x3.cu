@@ -55,7 +55,7 @@ struct X3Params {
   int tiles_m, tiles_n, num_tiles, k_blocks;
   float alpha, beta;
   const float* C_in;
-  float* C_out;  // the same matrix as C_in (written by plain stores in the pair kernel)
+  float* C_out;  // the same matrix as C_in (for plain stores: the pair kernel's, and ragged right edges)
   int64_t ldc, strideC;
   const void* bias;  // CUOPX_EPI_BIAS: N elements of the output type
   int epi;           // CUOPX_EPI_* flags
@@ -139,7 +139,9 @@ __device__ __forceinline__ void split_tf32_lo(const unsigned char* x, unsigned c
         make_float4(tf32_residual(v[i].x), tf32_residual(v[i].y), tf32_residual(v[i].z), tf32_residual(v[i].w));
 }
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, int CG, int KSPLIT>
+// RAGGED: a row's last output chunk leaves in plain stores, which N other than
+// a multiple of 4 needs (tma_store_cols).
+template <int BN, int STAGES, bool A_MN, bool B_MN, int CG, int KSPLIT, bool RAGGED>
 __global__ void __launch_bounds__(x3_threads(CG), 1)
     gemm_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmC, const X3Params p) {
@@ -438,8 +440,12 @@ __global__ void __launch_bounds__(x3_threads(CG), 1)
             make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       fence_proxy_async_shared();
       __syncwarp();
-      if (lane == 0) {
-        tma_store_3d(&tmC, sbase, n0 + ch * X3_CHUNK, m0 + 32 * q, b);
+      const int c0 = n0 + ch * X3_CHUNK;
+      if (RAGGED && c0 + X3_CHUNK > p.N) {
+        store_staged_chunk<4>(sbase, p.C_out + static_cast<int64_t>(b) * p.strideC, p.ldc, c0, m0 + 32 * q, p.M, p.N, lane);
+        if (lane == 0) bulk_commit_group();
+      } else if (lane == 0) {
+        tma_store_3d(&tmC, sbase, c0, m0 + 32 * q, b);
         bulk_commit_group();
       }
       sbuf ^= 1;
@@ -570,7 +576,7 @@ __global__ void __launch_bounds__(x3_threads(CG), 1)
   }
 }
 
-template <int BN, int STAGES, bool A_MN, bool B_MN, int CG, int KSPLIT>
+template <int BN, int STAGES, bool A_MN, bool B_MN, int CG, int KSPLIT, bool RAGGED>
 int launch_x3(const GemmProblem& p, cudaStream_t stream, const char* name) {
   using L = X3Smem<BN, STAGES, A_MN, KSPLIT>;
   const auto dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
@@ -600,7 +606,7 @@ int launch_x3(const GemmProblem& p, cudaStream_t stream, const char* name) {
   prm.strideC = p.strideC;
   prm.bias = p.bias;
   prm.epi = p.epi;
-  auto kern = gemm_tf32x3_kernel<BN, STAGES, A_MN, B_MN, CG, KSPLIT>;
+  auto kern = gemm_tf32x3_kernel<BN, STAGES, A_MN, B_MN, CG, KSPLIT, RAGGED>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -627,13 +633,16 @@ int launch_x3(const GemmProblem& p, cudaStream_t stream, const char* name) {
 
 // Stage counts: K-major A (A split in TMEM, smaller stages) runs deeper
 // rings — 6 x 64 or 4 x 64 TMEM columns of A next to the accumulators.
-template <int BN, int STAGES_TMEM_A, int STAGES_SMEM_A, int CG = 2, int KSPLIT = 1>
+template <int BN, int STAGES_TMEM_A, int STAGES_SMEM_A, int CG = 2, int KSPLIT = 1, bool RAGGED = false>
 int launch_x3_layout(const GemmProblem& p, cudaStream_t stream, const char* name) {
   const bool a_mn = p.transA, b_mn = !p.transB;
-  if (!a_mn && b_mn) return launch_x3<BN, STAGES_TMEM_A, false, true, CG, KSPLIT>(p, stream, name);
-  if (!a_mn && !b_mn) return launch_x3<BN, STAGES_TMEM_A, false, false, CG, KSPLIT>(p, stream, name);
-  if (a_mn && b_mn) return launch_x3<BN, STAGES_SMEM_A, true, true, CG, KSPLIT>(p, stream, name);
-  return launch_x3<BN, STAGES_SMEM_A, true, false, CG, KSPLIT>(p, stream, name);
+  if constexpr (!RAGGED) {
+    if (p.N % 4 != 0) return launch_x3_layout<BN, STAGES_TMEM_A, STAGES_SMEM_A, CG, KSPLIT, true>(p, stream, name);
+  }
+  if (!a_mn && b_mn) return launch_x3<BN, STAGES_TMEM_A, false, true, CG, KSPLIT, RAGGED>(p, stream, name);
+  if (!a_mn && !b_mn) return launch_x3<BN, STAGES_TMEM_A, false, false, CG, KSPLIT, RAGGED>(p, stream, name);
+  if (a_mn && b_mn) return launch_x3<BN, STAGES_SMEM_A, true, true, CG, KSPLIT, RAGGED>(p, stream, name);
+  return launch_x3<BN, STAGES_SMEM_A, true, false, CG, KSPLIT, RAGGED>(p, stream, name);
 }
 
 // ---------------------------------------------------------------------------

@@ -43,7 +43,7 @@ inline LayerEpi layer_epi(const LinearProblem& p) {
   e.ldy = p.ldy;
   e.Z = p.Z;
   e.ldz = p.ldz;
-  const int inside = p.N % 8 == 0 ? INT32_MAX : static_cast<int>(p.N);
+  const int inside = tma_store_cols<2>(p.N);
   e.tma_y = row_aligned16(p.Y, p.ldy) ? inside : 0;
   e.tma_z = p.Z && row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0) ? inside : 0;  // gated: U starts at column N
   return e;

@@ -252,6 +252,27 @@ def test_forward_writes_end_where_rows_end(m, n, k, gated):
         assert only_inside(y, ybuf) and only_inside(z, zbuf), cx.last_kernel()
 
 
+# ------------------------------------------------------------------ gradients whose rows end inside one
+@pytest.mark.parametrize("trans_w", [0, 1])
+@pytest.mark.parametrize("m,n,k", [(20, 133, 77), (300, 61, 135), (1100, 261, 523), (300, 1027, 37)])
+def test_backward_writes_end_where_rows_end(m, n, k, trans_w):
+    """Through the C ABI, which lets a caller place dX and dW."""
+    lib, g = N.lib(), gen(k)
+    stream = torch.cuda.current_stream().cuda_stream
+    x, dy, z = rnd(g, m, k), rnd(g, m, n), rnd(g, m, n)
+    w = rnd(g, *((n, k) if trans_w else (k, n)), scale=k ** -0.5)
+    (dx, dxb), (dw, dwb) = guarded(m, k, BF), guarded(*w.shape, BF)
+    db = torch.empty(n, dtype=BF, device="cuda")
+    args = (N.BF16, trans_w, 4, 0, m, n, k, dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), w.shape[1], z.data_ptr(), n,
+            dx.data_ptr(), dx.stride(0), dw.data_ptr(), dw.stride(0), db.data_ptr())
+    need = lib.cuopx_linear_backward_workspace_size(L._LINEAR_BACKWARD.pack(*args, 0, 0))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    assert lib.cuopx_linear_backward(L._LINEAR_BACKWARD.pack(*args, ws.data_ptr() if need else 0, need), stream) == N.SUCCESS
+    for what, t, (ref, bound) in zip(("dx", "dw", "db"), (dx, dw, db), R.linear_backward(dy, x, w, z, "silu", bool(trans_w), False)):
+        R.assert_within(t, ref, bound, what)
+    assert only_inside(dx, dxb) and only_inside(dw, dwb)
+
+
 # ------------------------------------------------------------------ documented values
 def test_relu_of_special_values():
     """z > 0 ? z : +0, so NaN gives 0, with a derivative of 0."""
