@@ -85,10 +85,12 @@ __global__ void __launch_bounds__(256) dropout_kernel(const DropoutParams p) {
 }
 
 // 16-byte groups (V elements, V / 4 counters) of rows that start on 16-byte
-// boundaries.  Bound by HBM (one read or two, one write): per element
-// the ten rounds cost 5 wide multiplies and 5 three-way xors, which bound the
-// 16-bit types: 8192 x 4096 bf16 33.8 us, with a residual 42.5 us (4.7 TB/s);
-// fp32 8192 x 8192 94 and 128 us (5.7 and 6.3 TB/s).
+// boundaries.  In fp32 bound by HBM (one read or two, one write): 8192 x 8192 94
+// us, with a residual 128 us (5.7 and 6.3 TB/s).  At 16 bits a group has two
+// counters, whose ten rounds cost 5 wide multiplies and 5 three-way xors an
+// element: 8192 x 4096 bf16 33.8 us, bound by those (ALU pipe 58 %, dispatch
+// stalls); with a residual 42.5 us (4.7 TB/s), bound by latency (issue 59 %
+// active, loads the longest stall): a thread has one group in flight.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutParams p) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));

@@ -10,17 +10,22 @@
 // the mean is large.  All sums are fp32, in an order fixed by the launch
 // shape, without atomics, so results do not change from run to run.
 //
-// Bound by HBM: every element is read once and written once.  Persistent
-// groups of threads (a warp, or a CTA, per row) stream rows through a ring of
-// shared-memory stages filled by bulk copies, so that what is in flight does
-// not cost registers; a row stays packed in its threads' registers between
-// the sums and the result.  The backward kernel reads x and dy once for all
-// three gradients: a thread keeps the same columns for all rows of its group
-// and their two column sums in registers; one partial sum per CTA and column
-// goes to the workspace, and a second small kernel adds those in CTA order.
+// Bound by HBM: every element is read once and written once.  A warp or a CTA
+// has a row, which stays packed in its threads' registers between the sums and
+// the result.  Forward (layer_norm_rows), rows are loaded straight into
+// registers, with a CTA, or a warp, for every row.  Backward, one kernel reads x
+// and dy once for all three gradients: persistent groups of threads, each with
+// the same columns of all its rows, whose two column sums stay in registers; one
+// partial sum per CTA and column goes to the workspace, and a second small
+// kernel adds those in CTA order.  Rows on 16-byte boundaries come through a
+// ring of shared-memory stages filled by bulk copies (layer_norm_backward_ring),
+// so that what is in flight costs no registers; others as single elements
+// (layer_norm_backward_rows).  The *_any kernels take what neither does.
 // Measured: fp32 16384 x 4096 forward 93 us (5.7 TB/s), backward 132 us (6.1);
-// bf16 8192 x 8192 63 us (4.3) and 92 us (4.4), where the instructions around
-// each element, conversions first, cost more than its bytes.
+// bf16 8192 x 8192 63 us (4.3 TB/s), bound by the instructions around each
+// element, conversions first (issue 72 % active), and 92 us (4.4), bound by
+// latency (issue 54 %): one CTA of 1024 threads per SM, whose warps meet at a
+// barrier every two rows.
 #include "common.cuh"
 #include "dispatch.h"
 #include "layer_epilogue.cuh"

@@ -178,8 +178,9 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // CTA's eight warps lie side by side, so that a row is read in runs of up to 4
 // KB (512-byte runs of eight rows measured 3.3 TB/s), and the others take the
 // rows between.  Several rows are loaded before the first is used.  Bound by
-// HBM (4096 x 28672 bf16, GELU: 137 us, 5.1 TB/s), in single elements by the
-// number of loads (999 x 2731 f16, gated: 17 us).
+// HBM (4096 x 28672 bf16, GELU: 127 us for the sums alone, 152 with dZ stored,
+// 4.6 TB/s), in single elements by the number of loads (999 x 2731 f16, gated: 18
+// us).
 struct DzParams {
   int64_t M, N;
   int act, across;
