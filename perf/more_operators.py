@@ -186,7 +186,8 @@ def _quantize(x):
     magnitude counts as 2^-100 at least."""
     x = x.float()
     top = x.abs().amax(1).clamp_min(2.0 ** -100)
-    return torch.round(x * (127.0 / top)[:, None]), top / 127.0
+    most = torch.full_like(top, 127.0)  # a tensor: torch divides by and into Python numbers with another rounding
+    return torch.round(x * (most / top)[:, None]), top / most
 
 
 def _newton_schulz(x):
@@ -295,7 +296,7 @@ def exact(case, seed):
         if not case["given"]:
             x32 = s["x"].float()
             top = torch.linalg.vector_norm(x32, float("inf"), dim=1, keepdim=True).clamp(min=2.0 ** -100)
-            x = torch.round(torch.mul(x32, torch.div(127.0, top))).double() * (top.double() / 127)
+            x = torch.round(torch.mul(x32, torch.div(torch.tensor(127.0, device="cuda"), top))).double() * (top.double() / 127)
         else:
             x = x * d["xs"][:, None]
         z = torch.mm(x, (d["wq"] * d["ws"][:, None]).mT) + d.get("bias", 0)
