@@ -4,6 +4,7 @@ The compute lives in libcuopx.so (hand-written CUDA for sm_100a behind the C
 ABI in include/cuopx.h); this package is the Python host side over that ABI.
 """
 from ._native import CuopError, lib, lib_path  # noqa: F401
+from .int8 import int8_gated_linear, int8_linear, quantize_int8  # noqa: F401
 from .layers import (  # noqa: F401
     dropout, dropout_backward, gated_linear, gated_linear_backward, layer_norm, layer_norm_backward, linear,
     linear_backward,

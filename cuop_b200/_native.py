@@ -98,6 +98,12 @@ SIGNATURES = [
     ("cuopx_layer_norm_backward_workspace_size", _sz, [_vp]),
     ("cuopx_layer_norm_backward", _int, [_vp, _vp]),
     ("cuopx_dropout", _int, [_vp, _vp]),
+    ("cuopx_quantize_workspace_size", _sz, [_vp]),
+    ("cuopx_quantize", _int, [_vp, _vp]),
+    ("cuopx_int8_linear_workspace_size", _sz, [_vp]),
+    ("cuopx_int8_linear", _int, [_vp, _vp]),
+    ("cuopx_int8_gated_linear_workspace_size", _sz, [_vp]),
+    ("cuopx_int8_gated_linear", _int, [_vp, _vp]),
 ]
 
 

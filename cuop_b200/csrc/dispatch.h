@@ -151,12 +151,23 @@ struct LinearProblem {
   int64_t ldz;
   int64_t w_up = 0;     // gated: first column (row when transW) of the second projection in W
   bool transX = false;  // X is stored [K][M] (the weight gradient's products; CTA-pair kernel only)
+  // X and W (stored [columns][K]) are int8, with a scale for each row of X and
+  // each column of the product; dtype is that of bias, R and Y.
+  bool int8 = false;
+  const float* xs = nullptr;
+  const float* ws = nullptr;
   int64_t wide() const { return gated ? 2 * N : N; }           // columns of W and Z
   int64_t w_cols() const { return gated ? w_up + N : N; }      // columns that W spans
+  int64_t k_blocks() const { return int8 ? (K + 127) / 128 : (K + 63) / 64; }  // 128 bytes of a row each
 };
 
 // Base and rows on 16-byte boundaries (16-bit elements).
 inline bool row_aligned16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && ld % 8 == 0; }
+
+// The same for an operand of a layer's product.
+inline bool operand_aligned16(const LinearProblem& p, const void* base, int64_t ld) {
+  return row_aligned16(base, p.int8 ? ld / 2 : ld) && (!p.int8 || ld % 2 == 0);
+}
 
 // Layer forward pass on CTA pairs (gemm_tc2.cu): 256 x 256 accumulator tiles
 // (256 x 128 outputs when gated).

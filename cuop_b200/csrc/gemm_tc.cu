@@ -570,6 +570,11 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int64_
   return make_map_es(map, dt, 2, base, inner, rows, batch, ld, bstride, box_inner, box_rows);
 }
 
+// A K-major int8 operand: boxes of 128 bytes by box_rows rows.
+bool make_map_i8(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, int box_rows) {
+  return make_map_es(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, inner, rows, 1, ld, 0, 128, box_rows);
+}
+
 template <typename T, int BN, int STAGES, bool A_MN, bool B_MN, int STORE = kTcTma, int CPS = 1>
 int launch_tc(const GemmProblem& p, cudaStream_t stream, const char* name, void* const* peers = nullptr,
               int npeers = 0) {

@@ -178,6 +178,16 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive on `bar` (same offset) in both CTAs of the pair when all prior
 // tcgen05 ops of this thread complete.
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
@@ -214,7 +224,10 @@ __device__ __forceinline__ uint32_t pack2_pair<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm, bool RAGGED = false>
+// Op: the operands' type, T (fp16 or bf16, then the output's too) or int8, K-major,
+// with int32 accumulators that the layer epilogue scales.  A K block is 128 bytes of
+// a row either way, so ring, boxes and descriptors are the same.
+template <typename T, bool A_MN, bool B_MN, int PBN, int MODE = kPairGemm, bool RAGGED = false, typename Op = T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THREADS, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const PairParams p,
@@ -227,8 +240,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
   constexpr int P_SLOTS = PairCfg<PBN>::SLOTS;
   constexpr int CHUNKS_PER_SLOT = P_SLOT_COLS / P_CHUNK;
   constexpr uint32_t PAIR_TX = 2u * static_cast<uint32_t>(L::A_STAGE + L::B_STAGE);
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
+  static_assert(!I8 || (MODE != kPairGemm && !A_MN && !B_MN), "int8: the layers, K-major operands");
+  constexpr int BK = I8 ? 2 * P_BK : P_BK;  // elements of a K block
   constexpr uint32_t AB_FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr uint32_t IDESC = make_idesc(AB_FMT, A_MN, B_MN, 2 * P_BM, P_SLOT_COLS);
+  constexpr uint32_t IDESC =
+      I8 ? make_idesc_i8(2 * P_BM, P_SLOT_COLS) : make_idesc(AB_FMT, A_MN, B_MN, 2 * P_BM, P_SLOT_COLS);
 
   extern __shared__ __align__(1024) unsigned char pair_smem_raw[];
   unsigned char* smem = align_smem_1024(pair_smem_raw);
@@ -328,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
           const uint32_t mbar = map_to_rank(&full[stage], 0);
           unsigned char* sa = smem + L::OFF_A + stage * L::A_STAGE;
           unsigned char* sb = smem + L::OFF_B + stage * L::B_STAGE;
-          const int k0 = kb * P_BK;
+          const int k0 = kb * BK;
           if constexpr (A_MN) {
 #pragma unroll
             for (int j = 0; j < P_BM / 64; ++j) tma_load_3d_pair(sa + j * (64 * P_BK * 2), &tmA, mbar, m0 + 64 * j, k0, b);
@@ -459,7 +476,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
                                        : make_smem_desc_sw128(sa + kk * 32, 16, 1024);
               const uint64_t bd = B_MN ? make_smem_desc_sw128(sbh + kk * 2048, 64 * P_BK * 2, 1024)
                                        : make_smem_desc_sw128(sbh + kk * 32, 16, 1024);
-              umma_f16_pair(d_tmem, ad, bd, IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
+              if constexpr (I8) umma_i8_pair(d_tmem, ad, bd, IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
+              else umma_f16_pair(d_tmem, ad, bd, IDESC, (kb > 0 || kk > 0) ? 1u : 0u);
             }
             issued = true;
           }
@@ -520,6 +538,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
         constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
         constexpr int PART = COLS * 4 / PairWarps<MODE>::EPI;  // this warp's columns of the tile
         const int c0 = (warp - 2) / 4 * PART;
+        auto sums = [&](int half, float (&a)[32], float (&b)[MODE == kPairGated ? 32 : 1]) {
+          if constexpr (I8) {
+            const int64_t col = nt * COLS + c0 + 32 * half;
+            const float xs = m0 + row_in_tile < p.M ? __ldg(layer.epi.xs + m0 + row_in_tile) : 0.f;
+            scale_row32(a, xs, layer.epi.ws, col, p.N, layer.epi.vec_ws);
+            if constexpr (MODE == kPairGated) scale_row32(b, xs, layer.epi.ws + p.N, col, p.N, layer.epi.vec_ws);
+          }
+        };
         const bool done = layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
             t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ,
             &layer.tmZ2, stage_base, lane, sbuf,
@@ -531,7 +557,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive_remote(map_to_rank(&acc_empty[s0], 0));
-            });
+            },
+            sums);
         if (!done) break;
       } else {
         if (!products()) break;
@@ -708,11 +735,12 @@ int launch_tc2(const GemmProblem& p, cudaStream_t stream, const char* name, void
 }
 
 // A layer's forward pass: X [M][K] (or, A_MN, [K][M]), W [K][columns] (B_MN) or [columns][K].
-template <typename T, bool A_MN, bool B_MN, int PBN, int MODE>
+template <typename T, bool A_MN, bool B_MN, int PBN, int MODE, typename Op = T>
 int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* name) {
   using L = PairSmem<PBN, MODE>;
   constexpr int P_SLOT_COLS = PairCfg<PBN>::SLOT;
   constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap mA, mB, mC = {};
@@ -720,8 +748,10 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
   layer.epi = layer_epi(p);
   layer.w_up = static_cast<int>(p.w_up);
   bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, P_BK)
+            : I8 ? make_map_i8(&mA, p.X, p.K, p.M, p.ldx, P_BM)
                  : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, P_BK, P_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, P_BK);
+  else if (I8) ok &= make_map_i8(&mB, p.W, p.K, p.w_cols(), p.ldw, P_SLOT_COLS / 2);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, P_BK, P_SLOT_COLS / 2);
   if (layer.epi.tma_y) ok &= make_map(&mC, dt, p.Y, p.N, p.M, 1, p.ldy, 0, P_CHUNK, 32);
   if (layer.epi.tma_z) {
@@ -738,8 +768,8 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
   prm.tiles_m = static_cast<int>((p.M + 2 * P_BM - 1) / (2 * P_BM));
   prm.tiles_n = static_cast<int>((p.N + COLS - 1) / COLS);
   prm.num_tiles = prm.tiles_m * prm.tiles_n;
-  prm.k_blocks = static_cast<int>((p.K + P_BK - 1) / P_BK);
-  auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN, MODE>;
+  prm.k_blocks = static_cast<int>(p.k_blocks());
+  auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN, MODE, false, Op>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -760,6 +790,9 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
 
 template <typename T, int PBN>
 int launch_tc2_layer_layout(const LinearProblem& p, cudaStream_t stream) {
+  if (p.int8)
+    return p.gated ? launch_tc2_layer<T, false, false, PBN, kPairGated, int8_t>(p, stream, "int8_gated_linear_tc2_256x128")
+                   : launch_tc2_layer<T, false, false, PBN, kPairLinear, int8_t>(p, stream, "int8_linear_tc2_256x256");
   if (p.gated) {
     const char* name = "gated_linear_tc2_256x128";
     return p.transW ? launch_tc2_layer<T, false, false, PBN, kPairGated>(p, stream, name)
@@ -846,7 +879,7 @@ bool linear_tc2_supported(const LinearProblem& p) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return false;
   if (p.M > INT32_MAX / 2 || p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX && (p.gated || p.transW)) return false;
-  if (!row_aligned16(p.X, p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
+  if (!operand_aligned16(p, p.X, p.ldx) || !operand_aligned16(p, p.W, p.ldw)) return false;
   if (p.gated && !p.transW && p.w_up % 8) return false;  // an x coordinate of W's tiles
   return ((p.M + 255) / 256) * ((p.N + 63) / 64) < (int64_t(1) << 29);
 }

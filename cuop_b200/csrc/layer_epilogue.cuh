@@ -28,6 +28,11 @@ struct LayerEpi {
   // others in plain 2-byte stores, 64 columns of a row per two of a warp's: 0
   // where rows do not start on 16-byte boundaries, N where they do not end on one.
   int tma_y, tma_z;
+  // int8 operands: factors of the product's rows and columns (gated: the
+  // gate's N, then the other projection's N).
+  const float* xs;
+  const float* ws;
+  int vec_ws;  // ws can be read in 16-byte groups
 };
 
 inline LayerEpi layer_epi(const LinearProblem& p) {
@@ -46,6 +51,9 @@ inline LayerEpi layer_epi(const LinearProblem& p) {
   const int inside = tma_store_cols<2>(p.N);
   e.tma_y = row_aligned16(p.Y, p.ldy) ? inside : 0;
   e.tma_z = p.Z && row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0) ? inside : 0;  // gated: U starts at column N
+  e.xs = p.xs;
+  e.ws = p.ws;
+  e.vec_ws = p.N % 4 == 0 && row_aligned16(p.ws, 0);
   return e;
 }
 
@@ -114,6 +122,30 @@ __device__ __forceinline__ void stage_row32(unsigned char* buf, int lane, int h,
     w.z = pack2_layer<T>(v[8 * j + 4], v[8 * j + 5]);
     w.w = pack2_layer<T>(v[8 * j + 6], v[8 * j + 7]);
     *reinterpret_cast<uint4*>(buf + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)) = w;
+  }
+}
+
+// Integer sums (their bits in v) of columns `col`.. times the row's factor and
+// theirs: one rounding of the sum to 24 bits, one for each product.  The
+// factors are the same for all lanes.
+__device__ __forceinline__ void scale_row32(float (&v)[32], float xs, const float* ws, int64_t col, int64_t N, bool vec) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int64_t c = col + 4 * j;
+    if (vec) {
+      if (c < N) f = __ldg(reinterpret_cast<const float4*>(ws + c));
+    } else {
+      if (c < N) f.x = __ldg(ws + c);
+      if (c + 1 < N) f.y = __ldg(ws + c + 1);
+      if (c + 2 < N) f.z = __ldg(ws + c + 2);
+      if (c + 3 < N) f.w = __ldg(ws + c + 3);
+    }
+    float2 lo = make_float2(__int2float_rn(__float_as_int(v[4 * j])), __int2float_rn(__float_as_int(v[4 * j + 1])));
+    float2 hi = make_float2(__int2float_rn(__float_as_int(v[4 * j + 2])), __int2float_rn(__float_as_int(v[4 * j + 3])));
+    lo = mul2(mul2(lo, both(xs)), make_float2(f.x, f.y));
+    hi = mul2(mul2(hi, both(xs)), make_float2(f.z, f.w));
+    v[4 * j] = lo.x, v[4 * j + 1] = lo.y, v[4 * j + 2] = hi.x, v[4 * j + 3] = hi.y;
   }
 }
 

@@ -349,7 +349,7 @@ constexpr double kRepackMinWork = 1048576.0;
 // 81.1.  So: split while one wave holds all tiles, in four only for deep K.
 int pair_split(const LinearProblem& p) {
   const int64_t cols = p.gated ? 128 : 256;
-  const int64_t tiles = ((p.M + 255) / 256) * ((p.N + cols - 1) / cols), k_blocks = (p.K + 63) / 64;
+  const int64_t tiles = ((p.M + 255) / 256) * ((p.N + cols - 1) / cols), k_blocks = p.k_blocks();
   if (!p.gated && k_blocks >= 96 && tiles <= linear_pair_capacity(4)) return 4;
   return k_blocks >= 12 && tiles <= linear_pair_capacity(2) ? 2 : 1;
 }
@@ -364,7 +364,7 @@ bool few_rows(const LinearProblem& p) {
   if (p.M <= 64) return true;
   if (p.M > 128) return false;
   const int64_t tiles = (p.wide() + 255) / 256;
-  return tiles <= 32 && (p.K < 6144 || tiles > linear_pair_capacity(4));
+  return tiles <= 32 && (p.K < (p.int8 ? 2 : 1) * 6144 || tiles > linear_pair_capacity(4));
 }
 
 // The kernel for a problem whose operands are as aligned as they will be.

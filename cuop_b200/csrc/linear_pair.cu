@@ -53,7 +53,8 @@ struct LpParams {
   LayerEpi epi;
 };
 
-template <typename T, bool A_MN, bool B_MN, bool GATED, int KS>
+// Op: T, or int8 (K-major; the exchanged sums are int32, exact in any order).
+template <typename T, bool A_MN, bool B_MN, bool GATED, int KS, typename Op = T>
 __global__ void __launch_bounds__(LP_THREADS, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmZ,
@@ -66,7 +67,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
   static_assert(PART % 64 == 0, "whole TMA store boxes");
   constexpr uint32_t PAIR_TX = 2u * static_cast<uint32_t>(L::A_STAGE + L::B_STAGE);
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr uint32_t IDESC = make_idesc(FMT, A_MN, B_MN, 2 * LP_BM, LP_BN);
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
+  static_assert(!I8 || (!A_MN && !B_MN), "int8: K-major operands");
+  constexpr int BK = I8 ? 2 * LP_BK : LP_BK;  // elements of a K block
+  constexpr uint32_t IDESC = I8 ? make_idesc_i8(2 * LP_BM, LP_BN) : make_idesc(FMT, A_MN, B_MN, 2 * LP_BM, LP_BN);
 
   extern __shared__ __align__(1024) unsigned char lp_smem_raw[];
   unsigned char* smem = align_smem_1024(lp_smem_raw);
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
         const uint32_t mbar = map_to_rank(&full[stage], even);
         unsigned char* sa = smem + L::OFF_A + stage * L::A_STAGE;
         unsigned char* sb = smem + L::OFF_B + stage * L::B_STAGE;
-        const int k0 = kb * LP_BK;
+        const int k0 = kb * BK;
         if constexpr (A_MN) {
 #pragma unroll
           for (int j = 0; j < LP_BM / 64; ++j) tma_load_3d_pair(sa + j * (64 * LP_BK * 2), &tmA, mbar, m0 + 64 * j, k0, 0);
@@ -190,7 +194,8 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
                                    : make_smem_desc_sw128(sa + kk * 32, 16, 1024);
           const uint64_t bd = B_MN ? make_smem_desc_sw128(sb + kk * 2048, 64 * LP_BK * 2, 1024)
                                    : make_smem_desc_sw128(sb + kk * 32, 16, 1024);
-          umma_f16_pair(tmem_base, ad, bd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
+          if constexpr (I8) umma_i8_pair(tmem_base, ad, bd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
+          else umma_f16_pair(tmem_base, ad, bd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
         }
         issued = true;
         umma_commit_pair_mask(&empty[stage], pair_mask);
@@ -258,6 +263,26 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
           [&](int half, float (&a)[32], float (&b)[GATED ? 32 : 1]) {
             // The sums of all pairs in pair order; this pair's own are in a and b.
             const float* col = recv + (c0 + 32 * half) * LP_BM + row;
+            if constexpr (I8) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                int sa = __float_as_int(a[i]), sb = 0;
+                if constexpr (GATED) sb = __float_as_int(b[i]);
+#pragma unroll
+                for (int s = 0; s < KS - 1; ++s) {
+                  const float* src = col + (s * OWN_ACC + i) * LP_BM;
+                  sa += __float_as_int(*src);
+                  if constexpr (GATED) sb += __float_as_int(src[OWN * LP_BM]);
+                }
+                a[i] = __int_as_float(sa);
+                if constexpr (GATED) b[i] = __int_as_float(sb);
+              }
+              const int64_t first = n0 + kp * OWN + c0 + 32 * half;
+              const float xs = m0 + row < p.M ? __ldg(p.epi.xs + m0 + row) : 0.f;
+              scale_row32(a, xs, p.epi.ws, first, p.N, p.epi.vec_ws);
+              if constexpr (GATED) scale_row32(b, xs, p.epi.ws + p.N, first, p.N, p.epi.vec_ws);
+              return;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               float sa = 0.f, sb = 0.f;
@@ -290,22 +315,23 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
   }
 }
 
-template <typename T, bool A_MN, bool B_MN, bool GATED, int KS>
+template <typename T, bool A_MN, bool B_MN, bool GATED, int KS, typename Op = T>
 int prepare_linear_pair() {
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
   if (!attr_set[dev].load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(linear_pair_kernel<T, A_MN, B_MN, GATED, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             LpSmem::ALLOC) != cudaSuccess)
+    if (cudaFuncSetAttribute(linear_pair_kernel<T, A_MN, B_MN, GATED, KS, Op>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, LpSmem::ALLOC) != cudaSuccess)
       return CUOPX_CUDA_ERROR;
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
   return CUOPX_SUCCESS;
 }
 
-template <typename T, bool A_MN, bool B_MN, bool GATED, int KS>
+template <typename T, bool A_MN, bool B_MN, bool GATED, int KS, typename Op = T>
 int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
   constexpr int COLS = GATED ? LP_BN / 2 : LP_BN;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -313,8 +339,10 @@ int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
   LpParams prm = {};
   prm.epi = layer_epi(p);
   bool ok = A_MN ? make_map(&mA, dt, p.X, p.M, p.K, 1, p.ldx, 0, 64, LP_BK)
+            : I8 ? make_map_i8(&mA, p.X, p.K, p.M, p.ldx, LP_BM)
                  : make_map(&mA, dt, p.X, p.K, p.M, 1, p.ldx, 0, LP_BK, LP_BM);
   if (B_MN) ok &= make_map(&mB, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, LP_BK);
+  else if (I8) ok &= make_map_i8(&mB, p.W, p.K, p.w_cols(), p.ldw, LP_BN / 2);
   else ok &= make_map(&mB, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LP_BK, LP_BN / 2);
   if (prm.epi.tma_y) ok &= make_map(&mY, dt, p.Y, p.N, p.M, 1, p.ldy, 0, 64, 32);
   if (prm.epi.tma_z) {
@@ -325,23 +353,29 @@ int launch_linear_pair(const LinearProblem& p, cudaStream_t stream) {
   prm.M = static_cast<int>(p.M);
   prm.N = static_cast<int>(p.N);
   prm.tiles_m = static_cast<int>((p.M + 2 * LP_BM - 1) / (2 * LP_BM));
-  prm.k_blocks = static_cast<int>((p.K + LP_BK - 1) / LP_BK);
+  prm.k_blocks = static_cast<int>(p.k_blocks());
   prm.w_up = static_cast<int>(p.w_up);
   const int64_t tiles = static_cast<int64_t>(prm.tiles_m) * ((p.N + COLS - 1) / COLS);
-  auto kern = linear_pair_kernel<T, A_MN, B_MN, GATED, KS>;
-  if (const int rc = prepare_linear_pair<T, A_MN, B_MN, GATED, KS>(); rc != CUOPX_SUCCESS) return rc;
+  auto kern = linear_pair_kernel<T, A_MN, B_MN, GATED, KS, Op>;
+  if (const int rc = prepare_linear_pair<T, A_MN, B_MN, GATED, KS, Op>(); rc != CUOPX_SUCCESS) return rc;
   const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * 2 * KS)), dim3(LP_THREADS), LpSmem::ALLOC,
                                              stream, 2 * KS, mA, mB, mY, mZ, mZ2, prm);
   if (err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
-  note_launch(GATED ? "gated_linear_pair_k2" : KS == 2 ? "linear_pair_k2" : "linear_pair_k4");
+  if (I8) note_launch(GATED ? "int8_gated_linear_pair_k2" : KS == 2 ? "int8_linear_pair_k2" : "int8_linear_pair_k4");
+  else note_launch(GATED ? "gated_linear_pair_k2" : KS == 2 ? "linear_pair_k2" : "linear_pair_k4");
   return check_launch();
 }
 
 template <typename T>
 int linear_pair_typed(const LinearProblem& p, int ks, cudaStream_t stream) {
+  if (p.int8) {
+    if (p.gated) return launch_linear_pair<T, false, false, true, 2, int8_t>(p, stream);
+    return ks == 2 ? launch_linear_pair<T, false, false, false, 2, int8_t>(p, stream)
+                   : launch_linear_pair<T, false, false, false, 4, int8_t>(p, stream);
+  }
   if (p.gated)
     return p.transW ? launch_linear_pair<T, false, false, true, 2>(p, stream)
                     : launch_linear_pair<T, false, true, true, 2>(p, stream);

@@ -68,6 +68,8 @@ struct SplitParams {
   int64_t ldy;
   void* Z;
   int64_t ldz;
+  const float* xs;  // int8: factors of X's rows and of the product's columns
+  const float* ws;
 };
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
@@ -84,7 +86,8 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
-template <typename T, bool W_MN, bool GATED, int TOK>
+// Op: T, or int8 (K-major; the partial sums are int32).
+template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T>
 __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                         const SplitParams p) {
@@ -92,7 +95,10 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t STAGE_TX = static_cast<uint32_t>(L::W_STAGE + L::X_STAGE);
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr uint32_t IDESC = make_idesc(FMT, W_MN, false, LSP_COLS, TOK);
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
+  static_assert(!I8 || !W_MN, "int8: K-major operands");
+  constexpr int BK = I8 ? 2 * LSP_BK : LSP_BK;  // elements of a K block
+  constexpr uint32_t IDESC = I8 ? make_idesc_i8(LSP_COLS, TOK) : make_idesc(FMT, W_MN, false, LSP_COLS, TOK);
   constexpr int TILE_N = GATED ? LSP_COLS / 2 : LSP_COLS;  // output columns per cluster
 
   extern __shared__ __align__(1024) unsigned char split_smem_raw[];
@@ -130,8 +136,8 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int c = n0 + (GATED ? j * p.w_up : 64 * j);
-        if constexpr (W_MN) tma_prefetch_3d(&tmW, c, kb * LSP_BK, 0);
-        else tma_prefetch_3d(&tmW, kb * LSP_BK, c, 0);
+        if constexpr (W_MN) tma_prefetch_3d(&tmW, c, kb * BK, 0);
+        else tma_prefetch_3d(&tmW, kb * BK, c, 0);
       }
     }
   }
@@ -160,7 +166,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
         }
         mbar_arrive_expect_tx(&full[stage], STAGE_TX);
         unsigned char* sw = smem + L::OFF_W + stage * L::W_STAGE;
-        const int k0 = kb * LSP_BK;
+        const int k0 = kb * BK;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {  // 64 columns of W each
           const int c = n0 + (GATED ? j * p.w_up : 64 * j);
@@ -209,7 +215,8 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
           const uint64_t wd = W_MN ? make_smem_desc_sw128(sw + kk * 2048, 64 * LSP_BK * 2, 1024)
                                    : make_smem_desc_sw128(sw + kk * 32, 16, 1024);
           const uint64_t xd = make_smem_desc_sw128(sx + kk * 32, 16, 1024);
-          umma_f16(tmem_base, wd, xd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
+          if constexpr (I8) umma_i8(tmem_base, wd, xd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
+          else umma_f16(tmem_base, wd, xd, IDESC, (kb > kb0 || kk > 0) ? 1u : 0u);
         }
         issued = true;
         umma_commit(&empty[stage]);
@@ -293,10 +300,23 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       float z[2][2] = {};  // [projection][column]
 #pragma unroll
       for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-        for (int s = 0; s < cs; ++s) {
-          const float2 v = *reinterpret_cast<const float2*>(sums + (s * TOK + t) * own + h * outs + f);
-          z[h][0] += v.x;
-          z[h][1] += v.y;
+        if constexpr (I8) {
+          int i0 = 0, i1 = 0;
+          for (int s = 0; s < cs; ++s) {
+            const int2 v = *reinterpret_cast<const int2*>(sums + (s * TOK + t) * own + h * outs + f);
+            i0 += v.x;
+            i1 += v.y;
+          }
+          const float xs = p.xs[t];
+          const float* ws = p.ws + static_cast<int64_t>(h) * p.N + col;
+          z[h][0] = __int2float_rn(i0) * xs * ws[0];
+          if (two) z[h][1] = __int2float_rn(i1) * xs * ws[1];
+        } else {
+          for (int s = 0; s < cs; ++s) {
+            const float2 v = *reinterpret_cast<const float2*>(sums + (s * TOK + t) * own + h * outs + f);
+            z[h][0] += v.x;
+            z[h][1] += v.y;
+          }
         }
         if (bias) {
           z[h][0] += to_acc<T>(bias[static_cast<int64_t>(h) * p.N + col]);
@@ -328,22 +348,25 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   });
 }
 
-template <typename T, bool W_MN, bool GATED, int TOK>
+template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T>
 int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   using L = SplitSmem<TOK>;
+  constexpr bool I8 = std::is_same<Op, int8_t>::value;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap mW, mX;
   bool ok = W_MN ? make_map(&mW, dt, p.W, p.w_cols(), p.K, 1, p.ldw, 0, 64, LSP_BK)
+            : I8 ? make_map_i8(&mW, p.W, p.K, p.w_cols(), p.ldw, 64)
                  : make_map(&mW, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LSP_BK, 64);
-  // A single row has no stride: any multiple of 8 serves.
-  ok &= make_map(&mX, dt, p.X, p.K, p.M, 1, p.M == 1 ? (p.K + 7) / 8 * 8 : p.ldx, 0, LSP_BK, TOK);
+  // A single row has no stride: any multiple of 16 bytes serves.
+  const int64_t ldx = p.M > 1 ? p.ldx : I8 ? (p.K + 15) / 16 * 16 : (p.K + 7) / 8 * 8;
+  ok &= I8 ? make_map_i8(&mX, p.X, p.K, p.M, ldx, TOK) : make_map(&mX, dt, p.X, p.K, p.M, 1, ldx, 0, LSP_BK, TOK);
   if (!ok) return CUOPX_CUDA_ERROR;
   constexpr int TILE_N = GATED ? LSP_COLS / 2 : LSP_COLS;
   SplitParams prm;
   prm.M = static_cast<int>(p.M);
   prm.N = static_cast<int>(p.N);
-  prm.k_blocks = static_cast<int>((p.K + LSP_BK - 1) / LSP_BK);
+  prm.k_blocks = static_cast<int>(p.k_blocks());
   prm.w_up = static_cast<int>(p.w_up);
   prm.act = p.act;
   prm.pairs = p.N % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.Y) % 4 == 0;
@@ -354,8 +377,10 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   prm.ldy = p.ldy;
   prm.Z = p.Z;
   prm.ldz = p.ldz;
+  prm.xs = p.xs;
+  prm.ws = p.ws;
   const int64_t tiles = (p.N + TILE_N - 1) / TILE_N;
-  auto kern = linear_split_kernel<T, W_MN, GATED, TOK>;
+  auto kern = linear_split_kernel<T, W_MN, GATED, TOK, Op>;
   static std::atomic<bool> attr_set[64] = {};
   static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once, one CTA per SM
   int dev = 0;
@@ -386,12 +411,16 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
     cudaGetLastError();
     return cuda_failure(err);
   }
-  note_launch(GATED ? "gated_linear_split" : "linear_split");
+  if (I8) note_launch(GATED ? "int8_gated_linear_split" : "int8_linear_split");
+  else note_launch(GATED ? "gated_linear_split" : "linear_split");
   return check_launch();
 }
 
 template <typename T, int TOK>
 int linear_split_layout(const LinearProblem& p, cudaStream_t stream) {
+  if (p.int8)
+    return p.gated ? launch_linear_split<T, false, true, TOK, int8_t>(p, stream)
+                   : launch_linear_split<T, false, false, TOK, int8_t>(p, stream);
   if (p.gated)
     return p.transW ? launch_linear_split<T, false, true, TOK>(p, stream) : launch_linear_split<T, true, true, TOK>(p, stream);
   return p.transW ? launch_linear_split<T, false, false, TOK>(p, stream) : launch_linear_split<T, true, false, TOK>(p, stream);
@@ -412,7 +441,7 @@ bool linear_split_supported(const LinearProblem& p) {
   if (p.M <= 0 || p.M > 128 || p.N <= 0 || p.K <= 0) return false;
   if (p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX) return false;
-  if (!row_aligned16(p.X, p.M == 1 ? 0 : p.ldx) || !row_aligned16(p.W, p.ldw)) return false;
+  if (!operand_aligned16(p, p.X, p.M == 1 ? 0 : p.ldx) || !operand_aligned16(p, p.W, p.ldw)) return false;
   return !p.gated || p.transW || p.w_up % 8 == 0;  // the second projection's first column in W's rows
 }
 

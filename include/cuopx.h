@@ -454,6 +454,70 @@ typedef struct cuopx_dropout_args {
  */
 int cuopx_dropout(const cuopx_dropout_args* args, void* stream);
 
+/*
+ * 8-bit integer layers: a linear layer's weights and activations as int8 with
+ * one scale for each of W's columns and each of X's rows, for serving (no
+ * gradients).
+ */
+typedef struct cuopx_quantize_args {
+  int32_t dtype; /* of X: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
+  int32_t trans; /* 0: Q is [rows][cols], a scale for each row; 1: Q is [cols][rows], a scale for each column of X */
+  int64_t rows, cols;
+  const void* X; /* [rows][cols] */
+  int64_t ldx;
+  int8_t* Q;
+  int64_t ldq;
+  float* scale;    /* [rows], or with trans [cols] */
+  void* workspace; /* 256-byte aligned, not zeroed */
+  size_t workspace_bytes;
+} cuopx_quantize_args;
+
+/*
+ * Symmetric quantisation: with a the largest magnitude of a row of X (of a
+ * column with trans), at least 2^-100,
+ *   scale = a / 127,   Q = rint(X * (127 / a)),
+ * each operation rounded in fp32, ties to even; so |Q| <= 127.  A row with an
+ * infinity or a NaN gets that as its scale, and zeros.  The layout with trans is the one in
+ * which cuopx_int8_linear takes weights stored [K][columns].
+ * CUOPX_RESOURCE_UNAVAILABLE when the workspace is smaller than the size call
+ * says (0 without trans).
+ */
+size_t cuopx_quantize_workspace_size(const cuopx_quantize_args* args);
+int cuopx_quantize(const cuopx_quantize_args* args, void* stream);
+
+typedef struct cuopx_int8_linear_args {
+  int32_t dtype;      /* CUOPX_F16 or CUOPX_BF16: of Y, bias, residual, and of X unless x_scale is set */
+  int32_t activation; /* CUOPX_ACT_* */
+  int64_t M, N, K;    /* K <= 131071, so that no sum leaves int32 */
+  const void* X;      /* [M][K]: int8 with x_scale, else of dtype and quantised by the call */
+  int64_t ldx;
+  const float* x_scale; /* [M] or NULL */
+  const int8_t* W;      /* [columns][K]; columns: N (linear), 2N (gated linear) */
+  int64_t ldw;
+  const float* w_scale; /* [columns] */
+  const void* bias;     /* [columns] or NULL */
+  const void* residual; /* [M][N] or NULL; may be Y itself (same ld).  NULL for gated linear */
+  int64_t ldr;
+  void* Y; /* [M][N] */
+  int64_t ldy;
+  void* workspace; /* 256-byte aligned, not zeroed */
+  size_t workspace_bytes;
+} cuopx_int8_linear_args;
+
+/*
+ * int8 linear layer: Z[i][j] = x_scale[i] * w_scale[j] * sum_k X[i][k] W[j][k]
+ * + bias[j], Y = act(Z) + residual; gated: Z = [G | U], Y = act(G) * U.  The
+ * sum is exact (int32); it is rounded to fp32, multiplied by the two scales
+ * and goes on in fp32; Y is rounded once.  An X of dtype is quantised row by
+ * row first, as cuopx_quantize does.  CUOPX_RESOURCE_UNAVAILABLE when the
+ * workspace is smaller than the size call says: the quantised X, and copies of
+ * int8 operands whose rows do not start on 16-byte boundaries.
+ */
+size_t cuopx_int8_linear_workspace_size(const cuopx_int8_linear_args* args);
+int cuopx_int8_linear(const cuopx_int8_linear_args* args, void* stream);
+size_t cuopx_int8_gated_linear_workspace_size(const cuopx_int8_linear_args* args);
+int cuopx_int8_gated_linear(const cuopx_int8_linear_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
