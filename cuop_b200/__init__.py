@@ -9,6 +9,7 @@ from .layers import (  # noqa: F401
     dropout, dropout_backward, gated_linear, gated_linear_backward, layer_norm, layer_norm_backward, linear,
     linear_backward,
 )
+from .muon import muon_step, orthogonalize  # noqa: F401
 from .ops import (  # noqa: F401
     asum, axpy, batched_gemm, batched_gemm_host, clear_device_error, copy, device_error, dot, gather_column_blocks,
     gemm, gemv, iamax, iamin, last_kernel, launch_count, nrm2, rot, scal, swap,

@@ -518,6 +518,69 @@ int cuopx_int8_linear(const cuopx_int8_linear_args* args, void* stream);
 size_t cuopx_int8_gated_linear_workspace_size(const cuopx_int8_linear_args* args);
 int cuopx_int8_gated_linear(const cuopx_int8_linear_args* args, void* stream);
 
+/*
+ * Orthogonalised updates.  Newton-Schulz products take the singular values of
+ * a matrix towards 1 and leave its singular vectors:
+ *   X = G / (||G|| + eps),  then `steps` times  X = a X + (b A + c A A) X,  A = X X^T
+ * (||G|| the Frobenius norm).  Matrices are row-major; stacks of them have a
+ * stride between matrices, which may lie side by side in wider rows (column
+ * slices of one buffer).
+ */
+typedef struct cuopx_orthogonalize_args {
+  int32_t dtype;     /* of G: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
+  int32_t out_dtype; /* of out, likewise */
+  int32_t steps;     /* 0 to 32 */
+  int32_t reserved;  /* 0 */
+  int64_t batch, rows, cols;
+  double eps;                 /* finite, >= 0 */
+  const double* coefficients; /* host, steps x (a, b, c) */
+  const void* G;
+  int64_t ldg, strideG;
+  void* out; /* may be G itself (same type and strides) */
+  int64_t ldo, strideO;
+  void* workspace; /* 256-byte aligned, not zeroed */
+  size_t workspace_bytes;
+} cuopx_orthogonalize_args;
+
+/*
+ * out = the iteration's X.  The norm is summed in 64 bits; products take fp16
+ * operands (scaled by powers of two to fit) and sum in fp32; X is kept in 22
+ * bits between them.  Against the iteration in 64 bits the result is off by 2e-4 to 2e-3 of its
+ * norm, whatever the types.  Coefficients that let a singular value in [0, 1]
+ * grow beyond 1024 are refused.  CUOPX_RESOURCE_UNAVAILABLE when the workspace
+ * is smaller than the size call says (about 6 bytes an element of G and 4 an
+ * element of A).
+ */
+size_t cuopx_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols);
+int cuopx_orthogonalize(const cuopx_orthogonalize_args* args, void* stream);
+
+typedef struct cuopx_muon_args {
+  int32_t wdtype, gdtype, mdtype; /* of W, G and momentum: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
+  int32_t steps;                  /* as above */
+  int32_t nesterov;               /* 0 or 1 */
+  int32_t reserved;               /* 0 */
+  int64_t batch, rows, cols;
+  double eps;
+  const double* coefficients;
+  double lr, mu, decay, scale;
+  const float* lr_dev; /* device word that multiplies lr when the kernel runs, or NULL */
+  void* W;             /* updated */
+  int64_t ldw, strideW;
+  void* momentum; /* updated */
+  int64_t ldm, strideM;
+  const void* G;
+  int64_t ldg, strideG;
+  void* workspace; /* cuopx_orthogonalize_workspace_size */
+  size_t workspace_bytes;
+} cuopx_muon_args;
+
+/*
+ * One step of Muon (K. Jordan, 2024): momentum = mu momentum + G,
+ * U = G + mu momentum with nesterov, else momentum (as stored), O = U
+ * orthogonalised, W = (1 - lr decay) W - lr scale O; each matrix rounded once.
+ */
+int cuopx_muon_step(const cuopx_muon_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
