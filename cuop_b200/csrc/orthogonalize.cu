@@ -618,7 +618,10 @@ __global__ void __launch_bounds__(256) ortho_scale_kernel(const OrthoIo p) {
     if (threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
     __syncthreads();
   }
-  const float f = static_cast<float>(p.x_scale / (sqrt(part[0]) + p.eps));
+  // Small gradients: the factor leaves fp32's range below a norm of 1e-34, and is split.
+  const double factor = p.x_scale / (sqrt(part[0]) + p.eps);
+  const float pre = factor > 0x1p100 ? 0x1p100f : 1.f;
+  const float f = static_cast<float>(factor > 0x1p100 ? factor * 0x1p-100 : factor);
   for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t row = e / p.groups, c = (e - row * p.groups) * 8;
     float g[8];
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(256) ortho_scale_kernel(const OrthoIo p) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 v = make_float2(g[2 * i] * f, g[2 * i + 1] * f);
+      const float2 v = make_float2(g[2 * i] * pre * f, g[2 * i + 1] * pre * f);
       h[i] = pack2_layer<__half>(v.x, v.y);
       const float2 r = unpack2_layer<__half>(h[i]);
       l[i] = pack2_layer<__half>(v.x - r.x, v.y - r.y);

@@ -42,7 +42,7 @@ def _schedule(coefficients, steps: int, what: str):
     if steps < 0:
         _error(N.INVALID_ARGUMENT, f"{what}: {steps} steps")
     try:
-        if isinstance(coefficients[0], (int, float)):
+        if len(coefficients) and isinstance(coefficients[0], (int, float)):
             triples = (tuple(coefficients),) * steps
         else:
             triples = tuple(tuple(t) for t in coefficients)
