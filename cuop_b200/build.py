@@ -104,8 +104,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if src.suffix == ".cpp":  # host-only C++: nvcc hands it to the host compiler
             cmd = [nvcc, *COMMON, "-c", str(src), "-o", str(obj)]
         else:
-            # One translation unit, compiled on all cores.
-            cmd = [nvcc, *ARCH, *COMMON, "-split-compile=0", "-Xptxas", "-v", "-c", str(src), "-o", str(obj)]
+            cmd = [nvcc, *ARCH, *COMMON, "-Xptxas", "-v", "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -156,6 +156,10 @@ struct LinearProblem {
   bool int8 = false;
   const float* xs = nullptr;
   const float* ws = nullptr;
+  // The launch before is the call's own, which writes only X and its scales and lets
+  // the next kernel start no sooner than all kernels before it have completed.
+  bool early_w = false;
+  bool quant_x = false;  // X is of dtype, and the split kernel quantises it (split_quantises)
   int64_t wide() const { return gated ? 2 * N : N; }           // columns of W and Z
   int64_t w_cols() const { return gated ? w_up + N : N; }      // columns that W spans
   int64_t k_blocks() const { return int8 ? (K + 127) / 128 : (K + 63) / 64; }  // 128 bytes of a row each
@@ -178,6 +182,7 @@ int linear_pair(const LinearProblem& p, int ks, cudaStream_t stream);
 int linear_pair_capacity(int ks);  // tiles that run at once
 // Layer forward pass for few rows: swapped operands, K split over a cluster (linear_split.cu).
 bool linear_split_supported(const LinearProblem& p);
+bool split_quantises(int64_t M, int64_t N, int64_t K, bool gated);
 int linear_split(const LinearProblem& p, cudaStream_t stream);
 
 // ---- variant selection (host/tuning.cpp) ----

@@ -159,6 +159,7 @@ LinearProblem int8_problem(const cuopx_int8_linear_args& a, bool gated) {
 // What the workspace holds: the quantised X with its scales, or X's aligned
 // copy, and W's.
 struct Int8Plan {
+  bool fused;  // the product's kernel quantises X
   bool quantise, copy_x, copy_w;
   size_t x_off, scale_off, w_off, bytes;
 };
@@ -171,8 +172,12 @@ Int8Plan int8_plan(const cuopx_int8_linear_args& a, bool gated) {
   q.quantise = a.x_scale == nullptr;
   // Unaligned int8 operands are copied where the tensor cores pay for it (kRepackMinWork).
   const bool tensor = static_cast<double>(a.M) * static_cast<double>(wide) * static_cast<double>(a.K) >= kRepackMinWork;
-  q.copy_x = !q.quantise && tensor && !operand_aligned16(p, a.X, a.M == 1 ? 0 : a.ldx);
+  q.copy_x = a.x_scale && tensor && !operand_aligned16(p, a.X, a.M == 1 ? 0 : a.ldx);
   q.copy_w = tensor && !operand_aligned16(p, a.W, a.ldw);
+  if (q.quantise && split_quantises(a.M, a.N, a.K, gated) && (q.copy_w || operand_aligned16(p, a.W, a.ldw))) {
+    q.fused = true;
+    q.quantise = false;
+  }
   size_t off = 0;
   q.x_off = off;
   if (q.quantise || q.copy_x) off += round256(static_cast<size_t>(a.M) * round16(a.K));
@@ -227,6 +232,7 @@ int int8_forward(const cuopx_int8_linear_args* a, bool gated, cudaStream_t strea
                             reinterpret_cast<float*>(ws + q.scale_off)};
     if (const int rc = quantize_rows(a->dtype, quant, stream); rc != CUOPX_SUCCESS) return rc;
     p.xs = quant.scale;
+    p.early_w = !q.copy_w;
   } else if (q.copy_x) {
     if (const int rc = int8_repack(a->X, a->M, a->K, a->ldx, ws + q.x_off, stream); rc != CUOPX_SUCCESS) return rc;
   }
@@ -239,6 +245,7 @@ int int8_forward(const cuopx_int8_linear_args* a, bool gated, cudaStream_t strea
     p.W = ws + q.w_off;
     p.ldw = round16(a->K);
   }
+  p.quant_x = q.fused;
   if (linear_split_supported(p) && few_rows(p)) return linear_split(p, stream);
   if (linear_tc2_supported(p)) {
     const int ks = pair_split(p);

@@ -33,9 +33,14 @@ constexpr int LSP_THREADS = 192;
 constexpr int LSP_COLS = 128;  // columns of W per CTA
 constexpr int LSP_BK = 64;
 
-template <int TOK>
+// QX: X is quantised by the kernel itself, and its CTA's whole share of K lies in
+// shared memory, up to 16 K blocks of 2 KB.
+constexpr int LSP_QX_BLOCKS = 16;
+
+template <int TOK, bool QX = false>
 struct SplitSmem {
-  static constexpr int STAGES = TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : 6;
+  static_assert(!QX || TOK == 16, "rows that the kernel quantises");
+  static constexpr int STAGES = QX ? 4 : TOK <= 16 ? 5 : TOK <= 32 ? 4 : TOK <= 64 ? 3 : 6;
   static constexpr int CTAS = TOK <= 64 ? 2 : 1;  // resident per SM
   // With 128 rows the partial sums reuse the ring, once every CTA of the
   // cluster has finished its products; below, they have room of their own.
@@ -45,12 +50,14 @@ struct SplitSmem {
   static constexpr int X_STAGE = TOK * LSP_BK * 2;
   static constexpr int OFF_W = 0;
   static constexpr int OFF_X = OFF_W + STAGES * W_STAGE;
-  static constexpr int OFF_SUM = ALIAS ? 0 : OFF_X + STAGES * X_STAGE;  // [cs][TOK][128 / cs] fp32
-  static constexpr int OFF_BAR = OFF_X + STAGES * X_STAGE + (ALIAS ? 0 : TOK * LSP_COLS * 4);
+  static constexpr int X_BYTES = (QX ? LSP_QX_BLOCKS : STAGES) * X_STAGE;
+  static constexpr int OFF_SUM = ALIAS ? 0 : OFF_X + X_BYTES;  // [cs][TOK][128 / cs] fp32
+  static constexpr int OFF_BAR = OFF_X + X_BYTES + (ALIAS ? 0 : TOK * LSP_COLS * 4);
   static_assert(!ALIAS || TOK * LSP_COLS * 4 <= OFF_BAR, "the ring holds the partial sums");
   static constexpr int NUM_BARS = 2 * STAGES + 2;  // full, empty, acc_full, drain
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+  static constexpr int OFF_ROWS = OFF_MISC + 16;  // QX: the rows' maxima of 8 CTAs and this one, the rows' scales
+  static constexpr int ALLOC = OFF_ROWS + (QX ? 10 * TOK * 4 : 0) + 1024;
   static constexpr uint32_t TMEM_COLS = TOK < 32 ? 32 : TOK;
   static_assert((ALLOC + 1024) * CTAS <= 233472, "CTAS CTAs must fit one SM's shared memory");
 };
@@ -70,7 +77,86 @@ struct SplitParams {
   int64_t ldz;
   const float* xs;  // int8: factors of X's rows and of the product's columns
   const float* ws;
+  int early_w;  // W may be read before the kernel before this one on the stream has completed
+  // QX: X, of T
+  const void* x;
+  int64_t ldx;
+  int K;
+  int vec_x;  // its rows start on 16-byte boundaries
 };
+
+// X's rows [0, M) in columns [k0, k1) to int8 in `dst`, the shared-memory layout that
+// TMA gives the ring: K blocks of 16 rows of 128 bytes, 128-byte swizzle.  The
+// rows' maxima over all of K meet through the cluster.  A share that does not fit the
+// registers is read again (from L2).  All warps but the first.  `maxima`: [8][16]
+// received, then [16] of this CTA, then [16] scales.
+template <typename T>
+__device__ __forceinline__ void split_quantise_x(const SplitParams& p, int cs, int rank, int k0, int k1, unsigned char* dst,
+                                                 uint32_t* maxima, int warp, int lane) {
+  using Mag = Magnitude<T>;
+  constexpr int WARPS = LSP_THREADS / 32 - 1, ROWS = 16, PART = 256;  // a unit: 256 columns of a row to a warp
+  uint32_t* own = maxima + 8 * ROWS;
+  float* scales = reinterpret_cast<float*>(own + ROWS);
+  const int parts = (k1 - k0 + PART - 1) / PART, units = p.M * parts;
+  auto load = [&](int u) {
+    const int row = u / parts, k = k0 + (u - row * parts) * PART + 8 * lane;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx + k;
+    if (k + 8 <= p.K && p.vec_x) return k < k1 ? *reinterpret_cast<const uint4*>(x) : make_uint4(0, 0, 0, 0);
+    uint32_t w[4] = {};
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k < k1 && k + i < p.K) w[i / 2] |= static_cast<uint32_t>(h[i]) << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  constexpr int AHEAD = 8;
+  uint4 v[AHEAD];
+  for (int u = warp - 1; u < units; u += WARPS * AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) v[i] = u + i * WARPS < units ? load(u + i * WARPS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (u + i * WARPS >= units) break;
+      const uint32_t m =
+          __reduce_max_sync(0xffffffffu, Mag::fold(Mag::word(Mag::word(Mag::word(Mag::word(0u, v[i].x), v[i].y), v[i].z), v[i].w)));
+      if (lane == 0) atomicMax(&own[(u + i * WARPS) / parts], m);
+    }
+  }
+  named_bar_sync(1, 32 * WARPS);
+  const int t = static_cast<int>(threadIdx.x) - 32;
+  if (cs > 1) {
+    cluster_wait();  // every CTA of the cluster has started
+    for (int e = t; e < cs * ROWS; e += 32 * WARPS) {
+      const uint32_t to = map_to_rank(maxima + rank * ROWS + e % ROWS, static_cast<uint32_t>(e / ROWS));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(own[e % ROWS]) : "memory");
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+  for (int u = warp - 1; u < units; u += WARPS * AHEAD) {
+    if (units > WARPS * AHEAD) {  // else they are still in registers
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) v[i] = u + i * WARPS < units ? load(u + i * WARPS) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (u + i * WARPS >= units) break;
+      const int row = (u + i * WARPS) / parts, part = (u + i * WARPS) - row * parts, k = part * PART + 8 * lane;
+      uint32_t m = own[row];
+      for (int s = 0; s < cs && cs > 1; ++s) m = max(m, maxima[s * ROWS + row]);
+      const RowScale s = row_scale(Mag::value(m));
+      if (part == 0 && lane == 0) scales[row] = s.scale;
+      if (k < k1 - k0) {
+        const uint32_t lo = quantize4(pair_of<T>(v[i].x), pair_of<T>(v[i].y), s), hi = quantize4(pair_of<T>(v[i].z), pair_of<T>(v[i].w), s);
+        *reinterpret_cast<uint2*>(dst + (k >> 7) * (ROWS * 128) + row * 128 + ((((k & 127) >> 4) ^ (row & 7)) << 4) + (k & 8)) =
+            make_uint2(lo, hi);
+      }
+    }
+  }
+  fence_proxy_async_shared();
+  named_bar_sync(1, 32 * WARPS);
+}
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
@@ -86,14 +172,14 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
-// Op: T, or int8 (K-major; the partial sums are int32).
-template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T>
-__global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
+// Op: T, or int8 (K-major; the partial sums are int32), then with QX from an X of T.
+template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T, bool QX = false>
+__global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK, QX>::CTAS)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                         const SplitParams p) {
-  using L = SplitSmem<TOK>;
+  using L = SplitSmem<TOK, QX>;
   constexpr int STAGES = L::STAGES;
-  constexpr uint32_t STAGE_TX = static_cast<uint32_t>(L::W_STAGE + L::X_STAGE);
+  constexpr uint32_t STAGE_TX = static_cast<uint32_t>(L::W_STAGE + (QX ? 0 : L::X_STAGE));
   constexpr uint32_t FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr bool I8 = std::is_same<Op, int8_t>::value;
   static_assert(!I8 || !W_MN, "int8: K-major operands");
@@ -129,7 +215,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
     *abort_flag = 0;
     fence_mbarrier_init();
     prefetch_tmap(&tmW);
-    prefetch_tmap(&tmX);
+    if constexpr (!QX) prefetch_tmap(&tmX);
     // Warm L2 with the first stages of W while the previous kernel on the
     // stream drains; the loads themselves come after the dependent-launch wait.
     for (int kb = kb0; kb < min(kb1, kb0 + STAGES); ++kb) {
@@ -145,6 +231,8 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
     tmem_alloc(tmem_slot, L::TMEM_COLS);
     tmem_relinquish();
   }
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + L::OFF_ROWS);
+  if (QX && warp == 2 && lane < TOK) maxima[8 * TOK + lane] = 0u;
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -152,7 +240,34 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   // into a ring, has read it: the epilogue warps arrive after their accumulator).
   if (cs > 1 && !L::ALIAS) cluster_arrive_relaxed();
   const uint32_t tmem_base = *tmem_slot;
+  auto load_w = [&](int kb, int stage) {
+    mbar_arrive_expect_tx(&full[stage], STAGE_TX);
+    unsigned char* sw = smem + L::OFF_W + stage * L::W_STAGE;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // 64 columns of W each
+      const int c = n0 + (GATED ? j * p.w_up : 64 * j);
+      if constexpr (W_MN) tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], c, kb * BK, 0);
+      else tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], kb * BK, c, 0);
+    }
+  };
+  // The ring's first fill of W while the kernel before is at work on X.
+  int filled = 0;
+  if (I8 && p.early_w && warp == 0 && lane == 0)
+    for (; filled < min(STAGES, kb1 - kb0); ++filled) load_w(kb0 + filled, filled);
   grid_dependency_wait();
+  if constexpr (QX) {
+    if (warp == 0) {
+      if (lane == 0)
+        for (; filled < min(STAGES, kb1 - kb0); ++filled) load_w(kb0 + filled, filled);
+      __syncwarp();
+      if (cs > 1) {  // the two cluster barriers of split_quantise_x
+        cluster_wait();
+        cluster_arrive_relaxed();
+      }
+    } else {
+      split_quantise_x<T>(p, cs, rank, kb0 * BK, kb1 * BK, smem + L::OFF_X, maxima, warp, lane);
+    }
+  }
 
   if (warp == 0) {
     if (lane == 0) {
@@ -160,20 +275,14 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
       uint32_t phase = 0, issued_mask = 0, phase_mask = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
-          ok = false;
-          break;
+        if (kb - kb0 >= filled) {
+          if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
+            ok = false;
+            break;
+          }
+          load_w(kb, stage);
         }
-        mbar_arrive_expect_tx(&full[stage], STAGE_TX);
-        unsigned char* sw = smem + L::OFF_W + stage * L::W_STAGE;
-        const int k0 = kb * BK;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {  // 64 columns of W each
-          const int c = n0 + (GATED ? j * p.w_up : 64 * j);
-          if constexpr (W_MN) tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], c, k0, 0);
-          else tma_load_3d(sw + j * (64 * LSP_BK * 2), &tmW, &full[stage], k0, c, 0);
-        }
-        tma_load_3d(smem + L::OFF_X + stage * L::X_STAGE, &tmX, &full[stage], k0, 0, 0);
+        if constexpr (!QX) tma_load_3d(smem + L::OFF_X + stage * L::X_STAGE, &tmX, &full[stage], kb * BK, 0, 0);
         issued_mask |= 1u << stage;
         phase_mask = (phase_mask & ~(1u << stage)) | (phase << stage);
         if (++stage == STAGES) stage = 0, phase ^= 1u;
@@ -209,7 +318,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
         }
         tc_fence_after_sync();
         const uint32_t sw = smem_u32(smem + L::OFF_W + stage * L::W_STAGE);
-        const uint32_t sx = smem_u32(smem + L::OFF_X + stage * L::X_STAGE);
+        const uint32_t sx = smem_u32(smem + L::OFF_X + (QX ? kb - kb0 : stage) * L::X_STAGE);
 #pragma unroll
         for (int kk = 0; kk < LSP_BK / 16; ++kk) {
           const uint64_t wd = W_MN ? make_smem_desc_sw128(sw + kk * 2048, 64 * LSP_BK * 2, 1024)
@@ -238,13 +347,13 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
     }
     __syncwarp();
     if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
-    if (cs > 1) cluster_wait();
+    if (cs > 1 && !QX) cluster_wait();
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full, 0, kDevErrWaitTimeoutAccFull, abort_flag));
     tc_fence_after_sync();
     if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
-    if (cs > 1) cluster_wait();
+    if (cs > 1 && !QX) cluster_wait();
     // Owner of this lane's column of W, and the column's place among its own.
     const int l = 32 * q + lane;
     const int own = LSP_COLS / cs;
@@ -307,7 +416,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
             i0 += v.x;
             i1 += v.y;
           }
-          const float xs = p.xs[t];
+          const float xs = QX ? reinterpret_cast<const float*>(maxima + 9 * TOK)[t] : p.xs[t];
           const float* ws = p.ws + static_cast<int64_t>(h) * p.N + col;
           z[h][0] = __int2float_rn(i0) * xs * ws[0];
           if (two) z[h][1] = __int2float_rn(i1) * xs * ws[1];
@@ -348,9 +457,9 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK>::CTAS)
   });
 }
 
-template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T>
+template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T, bool QX = false>
 int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
-  using L = SplitSmem<TOK>;
+  using L = SplitSmem<TOK, QX>;
   constexpr bool I8 = std::is_same<Op, int8_t>::value;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -360,7 +469,8 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
                  : make_map(&mW, dt, p.W, p.K, p.w_cols(), 1, p.ldw, 0, LSP_BK, 64);
   // A single row has no stride: any multiple of 16 bytes serves.
   const int64_t ldx = p.M > 1 ? p.ldx : I8 ? (p.K + 15) / 16 * 16 : (p.K + 7) / 8 * 8;
-  ok &= I8 ? make_map_i8(&mX, p.X, p.K, p.M, ldx, TOK) : make_map(&mX, dt, p.X, p.K, p.M, 1, ldx, 0, LSP_BK, TOK);
+  if constexpr (QX) mX = CUtensorMap{};
+  else ok &= I8 ? make_map_i8(&mX, p.X, p.K, p.M, ldx, TOK) : make_map(&mX, dt, p.X, p.K, p.M, 1, ldx, 0, LSP_BK, TOK);
   if (!ok) return CUOPX_CUDA_ERROR;
   constexpr int TILE_N = GATED ? LSP_COLS / 2 : LSP_COLS;
   SplitParams prm;
@@ -379,8 +489,13 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   prm.ldz = p.ldz;
   prm.xs = p.xs;
   prm.ws = p.ws;
+  prm.early_w = p.early_w;
+  prm.x = p.X;
+  prm.ldx = p.ldx;
+  prm.K = static_cast<int>(p.K);
+  prm.vec_x = row_aligned16(p.X, p.M == 1 ? 0 : p.ldx);
   const int64_t tiles = (p.N + TILE_N - 1) / TILE_N;
-  auto kern = linear_split_kernel<T, W_MN, GATED, TOK, Op>;
+  auto kern = linear_split_kernel<T, W_MN, GATED, TOK, Op, QX>;
   static std::atomic<bool> attr_set[64] = {};
   static std::atomic<int> capacity[64][4] = {};  // clusters of 1, 2, 4, 8 CTAs that run at once, one CTA per SM
   int dev = 0;
@@ -404,6 +519,8 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
     const int64_t once = capacity[dev][i].load(std::memory_order_relaxed);
     if (tiles <= (L::CTAS == 2 ? once * 20 / 9 : once) && prm.k_blocks >= (2 << i)) cs = 1 << i;
   }
+  while (QX && cs < 8 && prm.k_blocks > cs * LSP_QX_BLOCKS) cs *= 2;
+  if (QX && prm.k_blocks > cs * LSP_QX_BLOCKS) return CUOPX_NOT_IMPLEMENTED;  // not reached: split_quantises
   prm.cs = cs;
   const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), L::ALLOC,
                                              stream, static_cast<unsigned>(cs), mW, mX, prm);
@@ -411,13 +528,19 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
     cudaGetLastError();
     return cuda_failure(err);
   }
-  if (I8) note_launch(GATED ? "int8_gated_linear_split" : "int8_linear_split");
+  if (QX) note_launch(GATED ? "int8_gated_linear_split_q" : "int8_linear_split_q");
+  else if (I8) note_launch(GATED ? "int8_gated_linear_split" : "int8_linear_split");
   else note_launch(GATED ? "gated_linear_split" : "linear_split");
   return check_launch();
 }
 
 template <typename T, int TOK>
 int linear_split_layout(const LinearProblem& p, cudaStream_t stream) {
+  if constexpr (TOK == 16) {
+    if (p.quant_x)
+      return p.gated ? launch_linear_split<T, false, true, TOK, int8_t, true>(p, stream)
+                     : launch_linear_split<T, false, false, TOK, int8_t, true>(p, stream);
+  }
   if (p.int8)
     return p.gated ? launch_linear_split<T, false, true, TOK, int8_t>(p, stream)
                    : launch_linear_split<T, false, false, TOK, int8_t>(p, stream);
@@ -436,12 +559,25 @@ int linear_split_rows(const LinearProblem& p, cudaStream_t stream) {
 
 }  // namespace
 
+// Whether the kernel quantises X itself, by sizes alone: few enough elements that
+// this, before the first MMA, takes no longer than another launch, and a share of K
+// that fits beside the ring, K being split over as many CTAs as the width of the
+// product leaves room for (launch_linear_split's rule on a whole part).  On the
+// device, us, by the kernel / by a launch before it whose work overlaps the first loads of
+// W: 1 x 1024 x 1024 5.1 / 5.1, 1 x 8192 x 8192 16.4 / 16.7, 16 x 1024 x 1024 6.9 / 5.6, 4 x
+// 4096 x (2 x 8192) 19.5 / 17.3; the host takes 3.5 us less for one launch.
+bool split_quantises(int64_t M, int64_t N, int64_t K, bool gated) {
+  const int64_t tiles = (N + (gated ? 63 : 127)) / (gated ? 64 : 128), blocks = (K + 127) / 128;
+  const int64_t cs = tiles <= 32 ? 8 : tiles <= 68 ? 4 : tiles <= 150 ? 2 : 1;
+  return M > 0 && M <= 16 && K > 0 && M * K <= 8192 && N > 0 && N <= INT32_MAX / 8 && blocks <= cs * LSP_QX_BLOCKS;
+}
+
 // Up to 128 rows.  TMA reads X and W; Y, Z, residual and bias may have any alignment.
 bool linear_split_supported(const LinearProblem& p) {
   if (p.M <= 0 || p.M > 128 || p.N <= 0 || p.K <= 0) return false;
   if (p.w_cols() > INT32_MAX / 4 || p.K > INT32_MAX / 2) return false;
   if (p.transX) return false;
-  if (!operand_aligned16(p, p.X, p.M == 1 ? 0 : p.ldx) || !operand_aligned16(p, p.W, p.ldw)) return false;
+  if ((!p.quant_x && !operand_aligned16(p, p.X, p.M == 1 ? 0 : p.ldx)) || !operand_aligned16(p, p.W, p.ldw)) return false;
   return !p.gated || p.transW || p.w_up % 8 == 0;  // the second projection's first column in W's rows
 }
 

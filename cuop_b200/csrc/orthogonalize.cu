@@ -18,13 +18,18 @@
 // is stored times a power of two that its bound allows (2^15 / bound): the
 // elements of A are far below fp16's normal range otherwise.
 //
-// One persistent launch does all products: 256 x PBN tiles on CTA pairs (tcgen05
-// cta_group::2), tile i of a phase on pair i mod the number of pairs, grid
-// barriers between phases.  A and the polynomial are symmetric: tiles on or below the
-// diagonal are computed, and those below it stored twice, once transposed.
-//   warp 0     TMA producer (both CTAs)
-//   warp 1     TMEM allocation; MMA issuer (even CTA)
-//   warps 2-9  epilogue: alpha * sums + beta * (what the phase adds), rounded, by TMA store
+// One persistent launch does all products: tiles of 256 x 256 or 256 x 128 on CTA
+// pairs (tcgen05 cta_group::2), tile i of a phase on pair i mod the number of pairs,
+// grid barriers between phases.  A and the polynomial are symmetric: tiles on or below
+// the diagonal are computed, and those below it stored twice, once transposed.
+//   warps 0, 10  TMA producers of the two operands (both CTAs)
+//   warp 1       TMEM allocation; MMA issuer (even CTA)
+//   warps 2-9    epilogue: alpha * sums + beta * (what the phase adds), rounded
+// Producers and issuer walk their loops as whole warps and let one elected lane
+// issue, with the next stage's barrier tested a stage ahead: what they compute then
+// stays in uniform registers, which TMA and MMA instructions take.  One producer
+// thread for both operands under `lane == 0` took 305 ns a stage, more than twice
+// what the tensor cores need for 256 x 128 x 64.
 #include <cmath>
 
 #include "common.cuh"
@@ -39,20 +44,21 @@ constexpr int ORT_MAX_STEPS = 32;
 constexpr int ORT_BM = 128;  // rows per CTA (pair: 256)
 constexpr int ORT_BK = 64;
 constexpr int ORT_EPI_WARPS = 8;
-constexpr int ORT_THREADS = 32 * (2 + ORT_EPI_WARPS);
+constexpr int ORT_THREADS = 32 * (3 + ORT_EPI_WARPS);
 constexpr uint32_t ORT_TMEM_COLS = 512;
+constexpr int ORT_SLOTS = 2;  // accumulators of up to 256 columns
 
-template <int PBN>
+// The ring of operand stages: A's 128 rows, then B's columns of this CTA, 64 of K
+// each.  Tiles of 512 columns (two MMAs of 256) have three stages of 48 KB, the
+// others five of 32 KB.  It is divided anew where a phase starts: nothing of
+// the phase before is on its way then.
 struct OrthoSmem {
-  static constexpr int SLOTS = static_cast<int>(ORT_TMEM_COLS) / PBN;
-  static constexpr int STAGES = PBN == 256 ? 5 : 6;
-  static constexpr int A_STAGE = ORT_BM * ORT_BK * 2;
-  static constexpr int B_STAGE = PBN / 2 * ORT_BK * 2;
-  static constexpr int OFF_A = 0;
-  static constexpr int OFF_B = STAGES * A_STAGE;
-  static constexpr int OFF_C = OFF_B + STAGES * B_STAGE;  // per warp: two staging buffers of 4 KB
+  static constexpr int STAGES = 5, WIDE_STAGES = 3;
+  static constexpr int OPERAND = ORT_BM * ORT_BK * 2;  // 16 KB: A, or B of one MMA
+  static constexpr int OFF_C = STAGES * 2 * OPERAND;   // per epilogue warp: two staging buffers of 4 KB
+  static_assert(WIDE_STAGES * 3 * OPERAND <= OFF_C, "the ring");
   static constexpr int OFF_BAR = OFF_C + ORT_EPI_WARPS * 2 * 4096;
-  static constexpr int NUM_BARS = 2 * STAGES + 2 * SLOTS + 3;  // full, empty, acc_full, acc_empty, drain, done, go
+  static constexpr int NUM_BARS = 2 * STAGES + 2 * ORT_SLOTS + 3;  // full, empty, acc_full, acc_empty, drain, done, go
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
   static_assert(ALLOC <= 232448, "shared memory budget exceeded");
@@ -64,20 +70,20 @@ enum OrthoPhase { kGram = 0, kPoly = 1, kUpdate = 2 };
 struct OrthoMaps {
   // Operands: [phase], for the two buffers that X alternates between.
   CUtensorMap a[3][2], b[3][2];
-  CUtensorMap gram, gram_t, poly, poly_t;  // stores, and transposed ones (boxes of 32 x 64)
-  CUtensorMap x[2], lo;
 };
 
 struct OrthoArgs {
   int batch, p, q, steps;
   bool tall;
+  int width[3];     // columns of a phase's tiles: 128, 256 or 512
   int tiles[3];     // of a phase, all batches
   int k_blocks[3];
   int tiles_m, tiles_n;  // of the update, one batch
   int sym_tiles;         // of the other two, one batch
-  const __half* x[2];
-  const __half* lo;
-  const __half* gram;
+  __half* x[2];
+  __half* lo;
+  __half* gram;
+  __half* poly;
   int64_t ldx, stride_x, ldp, stride_p;  // elements
   unsigned* barrier;
   float alpha[ORT_MAX_STEPS][3], beta[ORT_MAX_STEPS][3];
@@ -98,6 +104,7 @@ __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.pr
 __device__ __forceinline__ bool grid_wait(const unsigned* barrier, unsigned count, volatile int* abort) {
   const unsigned long long t0 = global_timer_ns();
   for (uint32_t it = 0; ld_acquire_gpu(barrier) < count; ++it) {
+    __nanosleep(40);
     if ((it & 63u) == 63u) {
       if (*abort) return false;
       if (global_timer_ns() - t0 > kWaitLimitNs) {
@@ -111,10 +118,15 @@ __device__ __forceinline__ bool grid_wait(const unsigned* barrier, unsigned coun
   return true;
 }
 
-// Tile t of a phase: batch, row tile (256 rows) and column tile (PBN columns).
-// Symmetric phases have the tiles whose first column is at most their last row.
-template <int PBN>
-__device__ __forceinline__ void ortho_tile(const OrthoArgs& g, int phase, int t, int& b, int& mt, int& nt) {
+// A whole warp's bounded wait, with one answer for all lanes; `ready`: a test has said so already.
+__device__ __forceinline__ bool warp_wait(bool ready, uint64_t* bar, uint32_t parity, int err, volatile int* abort) {
+  return __all_sync(0xffffffffu, ready || mbar_wait_bounded(bar, parity, err, abort));
+}
+
+// Tile t of a phase: batch, first row, first column.  Symmetric phases have the
+// tiles whose first column is at most their last row.
+__device__ __forceinline__ void ortho_tile(const OrthoArgs& g, int phase, int t, int& b, int& m, int& n) {
+  const int width = g.width[phase];
   if (phase == kUpdate) {
     const int per = g.tiles_m * g.tiles_n;
     b = t / per;
@@ -122,113 +134,136 @@ __device__ __forceinline__ void ortho_tile(const OrthoArgs& g, int phase, int t,
     constexpr int GROUP = 8;  // row tiles that share the columns' operand while it is in L2
     const int span = GROUP * g.tiles_n, grp = r / span, first = grp * GROUP;
     const int rows = min(GROUP, g.tiles_m - first), rr = r - grp * span;
-    mt = first + rr % rows;
-    nt = rr / rows;
+    m = (first + rr % rows) * 256;
+    n = rr / rows * width;
   } else {
-    constexpr int R = 256 / PBN;
+    // Row tile i has ceil((i + 1) 256 / width) tiles.
     b = t / g.sym_tiles;
-    const int r = t - b * g.sym_tiles;
-    int i = static_cast<int>((sqrtf(8.f * (r / R) + 1.f) - 1.f) * 0.5f);
-    while (R * i * (i + 1) / 2 > r) --i;
-    while (R * (i + 1) * (i + 2) / 2 <= r) ++i;
-    mt = i;
-    nt = r - R * i * (i + 1) / 2;
+    int r = t - b * g.sym_tiles;
+    auto before = [&](int i) {  // tiles in the row tiles before i
+      const int64_t h = i >> 1;
+      if (width == 512) return static_cast<int>(h * (h + 1) + (i & 1) * (h + 1));
+      return (256 / width) * (i * (i + 1) / 2);
+    };
+    int i = static_cast<int>(sqrtf(2.f * r * width / 256.f));
+    while (i > 0 && before(i) > r) --i;
+    while (before(i + 1) <= r) ++i;
+    m = i * 256;
+    n = (r - before(i)) * width;
   }
 }
 
-// 32 halves of a row, from L2 (other CTAs have written them in this launch).
-__device__ __forceinline__ void ortho_row32(const __half* row, int64_t col, int64_t cols, bool in, uint4 (&raw)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    raw[j] = make_uint4(0, 0, 0, 0);
-    if (in && col + 8 * j < cols) raw[j] = __ldcg(reinterpret_cast<const uint4*>(row + col + 8 * j));
-  }
-}
-
-// One warp's 32 rows of PART columns of a tile, in chunks of 64 columns.
-// UPDATE: hi and lo of X in, hi and lo out.  Else the sums, plus beta * r0
-// where beta is not 0, to `tm0`, and transposed to `tm1` if `mirror`.
-template <bool UPDATE, int PART, typename Wait, typename Release>
-__device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int n0, int m0, int b, int M, int N, float alpha, float beta,
-                                               const __half* r0, const __half* r1, int64_t ld, bool mirror,
-                                               const CUtensorMap* tm0, const CUtensorMap* tm1, unsigned char* stage, int lane,
-                                               Wait&& wait, Release&& release) {
+// One warp's 32 rows of `part` columns of a tile, in chunks of 64 columns.
+// UPDATE: hi and lo of X in (r0, r1), hi and lo out (o0, o1).  Else the sums, plus
+// beta * r0 where beta is not 0, to o0, and transposed below the diagonal block
+// of rows `diag`.. (what lies above it belongs to other tiles).
+//
+// Rows pass through shared memory (128-byte swizzle), so that global accesses are whole
+// 128-byte lines, eight lanes to a row; what the next chunk adds is on its way meanwhile.  Plain
+// stores: the fence before a TMA store waited for those loads (1.6 us a chunk).
+template <bool UPDATE, typename Wait, typename Release>
+__device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0, int m0, int M, int N, float alpha, float beta,
+                                               const __half* r0, const __half* r1, __half* o0, __half* o1, int64_t ld, int diag,
+                                               unsigned char* stage, int lane, Wait&& wait, Release&& release) {
   constexpr int BUF = 4096;
-  const bool in = m0 + lane < M && (UPDATE || beta != 0.f);
-  const __half* row0 = r0 + (m0 + lane) * ld;
-  const __half* row1 = r1 + (m0 + lane) * ld;
-  uint4 next0[4], next1[UPDATE ? 4 : 1];
-  auto fetch = [&](int64_t col) {
-    ortho_row32(row0, col, N, in, next0);
-    if constexpr (UPDATE) ortho_row32(row1, col, N, in, next1);
+  const int sub = lane & 7, line = lane >> 3;
+  const bool adds = UPDATE || beta != 0.f;
+  uint4 next0[8], next1[UPDATE ? 8 : 1];
+  auto fetch = [&](int col) {
+    col += 8 * sub;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = m0 + 4 * i + line;
+      const bool in = adds && row < M && col < N;
+      next0[i] = in ? __ldcg(reinterpret_cast<const uint4*>(r0 + row * ld + col)) : make_uint4(0, 0, 0, 0);
+      if constexpr (UPDATE) next1[i] = in ? __ldcg(reinterpret_cast<const uint4*>(r1 + row * ld + col)) : make_uint4(0, 0, 0, 0);
+    }
   };
   fetch(n0);
   if (!wait()) return false;
 #pragma unroll 1
-  for (int half = 0; half < PART / 32; ++half) {
-    const int h = half & 1;
-    uint32_t acc[32];
-    tmem_ld_32x32b_x32(t_row + 32 * half, acc);
-    tmem_wait_ld();
-    if (half == PART / 32 - 1) release();
-    float v[32];
+  for (int c = 0; c < part; c += 64) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w0[4] = {next0[j].x, next0[j].y, next0[j].z, next0[j].w};
+    for (int i = 0; i < 8; ++i) {
+      const int row = 4 * i + line, at = row * 128 + ((sub ^ (row & 7)) << 4);
+      *reinterpret_cast<uint4*>(stage + at) = next0[i];
+      if constexpr (UPDATE) *reinterpret_cast<uint4*>(stage + BUF + at) = next1[i];
+    }
+    __syncwarp();
+    if (c + 64 < part) fetch(n0 + c + 64);
+    const bool mirror = !UPDATE && n0 + c < diag;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 add = unpack2_layer<__half>(w0[i]);
-        if constexpr (UPDATE) {
-          const uint32_t w1[4] = {next1[j].x, next1[j].y, next1[j].z, next1[j].w};
-          add = add2(add, unpack2_layer<__half>(w1[i]));
+    for (int h = 0; h < 2; ++h) {
+      uint32_t acc[32];
+      tmem_ld_32x32b_x32(t_row + c + 32 * h, acc);
+      tmem_wait_ld();
+      if (h == 1 && c + 64 == part) release();
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unsigned char* at = stage + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4);
+        uint4 w0 = *reinterpret_cast<const uint4*>(at), w1 = make_uint4(0, 0, 0, 0);
+        if constexpr (UPDATE) w1 = *reinterpret_cast<const uint4*>(at + BUF);
+        uint32_t* a0 = &w0.x;
+        uint32_t* a1 = &w1.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float2 add = unpack2_layer<__half>(a0[i]);
+          if constexpr (UPDATE) add = add2(add, unpack2_layer<__half>(a1[i]));
+          const float2 s = make_float2(__uint_as_float(acc[8 * j + 2 * i]), __uint_as_float(acc[8 * j + 2 * i + 1]));
+          const float2 r = fma2(both(alpha), s, mul2(both(beta), add));
+          a0[i] = pack2_layer<__half>(r.x, r.y);
+          if constexpr (UPDATE) {
+            const float2 hi = unpack2_layer<__half>(a0[i]);
+            a1[i] = pack2_layer<__half>(r.x - hi.x, r.y - hi.y);
+          }
+          v[8 * j + 2 * i] = r.x, v[8 * j + 2 * i + 1] = r.y;
         }
-        const float2 s = make_float2(__uint_as_float(acc[8 * j + 2 * i]), __uint_as_float(acc[8 * j + 2 * i + 1]));
-        const float2 r = fma2(both(alpha), s, mul2(both(beta), add));
-        v[8 * j + 2 * i] = r.x, v[8 * j + 2 * i + 1] = r.y;
+        *reinterpret_cast<uint4*>(at) = w0;
+        if constexpr (UPDATE) *reinterpret_cast<uint4*>(at + BUF) = w1;
       }
-    }
-    if (half + 1 < PART / 32) fetch(n0 + 32 * (half + 1));
-    if (h == 0) {
-      if (lane == 0) bulk_wait_group_read<0>();
-      __syncwarp();
-    }
-    stage_row32<__half>(stage, lane, h, v);
-    if constexpr (UPDATE) {
+      if (mirror) {
+        // Row 32 h + i of the transposed chunk holds column i of this one, an
+        // element per lane; lanes trade elements so that each stores two at once.
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] -= __half2float(__float2half_rn(v[i]));
-      stage_row32<__half>(stage + BUF, lane, h, v);
-    } else if (mirror) {
-      // Row 32 h + i of the transposed chunk holds column i of this one, an
-      // element per lane; lanes trade elements so that each stores two at once.
+        for (int i = 0; i < 32; i += 2) {
+          const bool odd = lane & 1;
+          const float got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+          const uint32_t w = odd ? pack2_layer<__half>(got, v[i + 1]) : pack2_layer<__half>(v[i], got);
+          *reinterpret_cast<uint32_t*>(stage + BUF + (32 * h + i + (odd ? 1 : 0)) * 64 + (lane >> 1) * 4) = w;
+        }
+      }
+    }
+    __syncwarp();
+    if (UPDATE || n0 + c < diag + 256) {
+      const int col = n0 + c + 8 * sub;
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const bool odd = lane & 1;
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
-        const uint32_t w = odd ? pack2_layer<__half>(got, v[i + 1]) : pack2_layer<__half>(v[i], got);
-        *reinterpret_cast<uint32_t*>(stage + BUF + (32 * h + i + (odd ? 1 : 0)) * 64 + (lane >> 1) * 4) = w;
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + line, row = m0 + r, at = r * 128 + ((sub ^ (r & 7)) << 4);
+        if (row < M && col < N) {
+          *reinterpret_cast<uint4*>(o0 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + at);
+          if constexpr (UPDATE) *reinterpret_cast<uint4*>(o1 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + BUF + at);
+        }
       }
     }
-    if (h == 1) {
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) {
-        const int c = n0 + 32 * (half - 1);
-        tma_store_3d(tm0, stage, c, m0, b);
-        if constexpr (UPDATE) tma_store_3d(tm1, stage + BUF, c, m0, b);
-        else if (mirror) tma_store_3d(tm1, stage + BUF, m0, c, b);
-        bulk_commit_group();
+    if (mirror) {
+      const int col = m0 + 8 * (lane & 3);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 8 * i + (lane >> 2), row = n0 + c + r;
+        if (row < M && col < N)
+          *reinterpret_cast<uint4*>(o0 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + BUF + r * 64 + 16 * (lane & 3));
       }
     }
+    __syncwarp();
   }
   return true;
 }
 
-template <int PBN>
 __global__ void __launch_bounds__(ORT_THREADS, 1)
     ortho_pair_kernel(const __grid_constant__ OrthoMaps maps, const __grid_constant__ OrthoArgs g) {
-  using L = OrthoSmem<PBN>;
-  constexpr int STAGES = L::STAGES, SLOTS = L::SLOTS;
-  constexpr uint32_t PAIR_TX = 2u * static_cast<uint32_t>(L::A_STAGE + L::B_STAGE);
+  using L = OrthoSmem;
+  constexpr int STAGES = L::STAGES, SLOTS = ORT_SLOTS;
 
   extern __shared__ __align__(1024) unsigned char ortho_smem_raw[];
   unsigned char* smem = align_smem_1024(ortho_smem_raw);
@@ -238,20 +273,20 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
   uint64_t* acc_empty = acc_full + SLOTS;
   uint64_t* drain = acc_empty + SLOTS;
   uint64_t* done = drain + 1;  // the epilogue warps have stored a phase
-  uint64_t* go = drain + 2;    // every CTA has: the producer has seen the grid barrier
+  uint64_t* go = drain + 2;    // every CTA has: a producer has seen the grid barrier
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t rank = blockIdx.x & 1u;  // in the cluster of two
   const bool leader = rank == 0;
-  const int pair = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(gridDim.x) / 2;
+  const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x) / 2;
   const int phases = 3 * g.steps;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&full[s], 2);   // leader: its two producers; both CTAs' bytes
+      mbar_init(&empty[s], 1);  // one multicast commit per phase
     }
     for (int a = 0; a < SLOTS; ++a) {
       mbar_init(&acc_full[a], 1);
@@ -275,123 +310,161 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer (both CTAs)
-    if (lane == 0) {
+  if (warp == 0 || warp == 2 + ORT_EPI_WARPS) {
+    // ------------------------------------------------------------ producers (both CTAs)
+    const bool of_a = warp == 0;
+    uint32_t bits = 0, issued_mask = 0;  // bit s: parity of stage s's next phase; loaded at least once
+    bool ok = true, ready = false;
+    for (int ph = 0; ok && ph < phases; ++ph) {
+      const int kind = ph % 3, cur = (ph / 3) & 1;
+      const bool mn = kind == kGram ? g.tall : kind == kUpdate && !g.tall && !of_a;
+      const CUtensorMap* map = of_a ? &maps.a[kind][cur] : &maps.b[kind][cur];
+      const int width = g.width[kind], pieces = !of_a && width == 512 ? 2 : 1;
+      const int span = of_a ? ORT_BM : min(width, 256) / 2;  // rows or columns of the operand for one MMA
+      const int stages = width == 512 ? L::WIDE_STAGES : L::STAGES, stride = (width == 512 ? 3 : 2) * L::OPERAND;
+      const uint32_t bytes = static_cast<uint32_t>(pieces * span) * ORT_BK * 2;
+      unsigned char* const ring = smem + (of_a ? 0 : L::OPERAND);
       int stage = 0;
-      uint32_t phase_bit = 0, issued_mask = 0, phase_mask = 0;
-      bool ok = true;
-      for (int ph = 0; ok && ph < phases; ++ph) {
-        const int kind = ph % 3, cur = (ph / 3) & 1;
-        const bool a_mn = kind == kGram && g.tall, b_mn = kind == kGram ? g.tall : kind == kUpdate && !g.tall;
-        const CUtensorMap* ma = &maps.a[kind][cur];
-        const CUtensorMap* mb = &maps.b[kind][cur];
-        // The first phase reads what the kernel before has written.
-        if (ph > 0) {
-          if (!grid_wait(g.barrier, static_cast<unsigned>(ph) * gridDim.x, abort_flag)) {
+      ready = false;
+      if (elect_one_sync()) prefetch_tmap(map);
+      // The first phase reads what the kernel before has written.
+      if (ph > 0) {
+        if (!__all_sync(0xffffffffu, lane != 0 || grid_wait(g.barrier, static_cast<unsigned>(ph) * gridDim.x, abort_flag))) {
+          ok = false;
+          break;
+        }
+        if (of_a && elect_one_sync()) mbar_arrive(go);
+      }
+      for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
+        int b, m, n;
+        ortho_tile(g, kind, t, b, m, n);
+        const int first = (of_a ? m : n) + static_cast<int>(rank) * span;
+        for (int kb = 0; kb < g.k_blocks[kind]; ++kb) {
+          if (!warp_wait(ready, &empty[stage], ((bits >> stage) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
             ok = false;
             break;
           }
-          mbar_arrive(go);
-        }
-        for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
-          int b, mt, nt;
-          ortho_tile<PBN>(g, kind, t, b, mt, nt);
-          const int m0 = mt * 2 * ORT_BM + static_cast<int>(rank) * ORT_BM;
-          const int n0 = nt * PBN + static_cast<int>(rank) * (PBN / 2);
-          for (int kb = 0; kb < g.k_blocks[kind]; ++kb) {
-            if (!mbar_wait_bounded(&empty[stage], phase_bit ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
-              ok = false;
-              break;
-            }
-            if (leader) mbar_arrive_expect_tx(&full[stage], PAIR_TX);
+          if (elect_one_sync()) {
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * bytes);
             const uint32_t mbar = map_to_rank(&full[stage], 0);
-            unsigned char* sa = smem + L::OFF_A + stage * L::A_STAGE;
-            unsigned char* sb = smem + L::OFF_B + stage * L::B_STAGE;
+            unsigned char* dst = ring + stage * stride;
             const int k0 = kb * ORT_BK;
-            if (a_mn) {
-              for (int j = 0; j < ORT_BM / 64; ++j) tma_load_3d_pair(sa + j * 8192, ma, mbar, m0 + 64 * j, k0, b);
-            } else {
-              tma_load_3d_pair(sa, ma, mbar, k0, m0, b);
+            for (int h = 0; h < pieces; ++h) {
+              const int at = first + 256 * h;
+              if (mn) {
+                tma_load_3d_pair(dst + h * L::OPERAND, map, mbar, at, k0, b);
+                if (span > 64) tma_load_3d_pair(dst + h * L::OPERAND + 8192, map, mbar, at + 64, k0, b);
+              } else {
+                tma_load_3d_pair(dst + h * L::OPERAND, map, mbar, k0, at, b);
+              }
             }
-            if (b_mn) {
-              for (int j = 0; j < PBN / 128; ++j) tma_load_3d_pair(sb + j * 8192, mb, mbar, n0 + 64 * j, k0, b);
-            } else {
-              tma_load_3d_pair(sb, mb, mbar, k0, n0, b);
-            }
-            issued_mask |= 1u << stage;
-            phase_mask = (phase_mask & ~(1u << stage)) | (phase_bit << stage);
-            if (++stage == STAGES) stage = 0, phase_bit ^= 1u;
           }
+          __syncwarp();
+          issued_mask |= 1u << stage;
+          bits ^= 1u << stage;
+          stage = stage + 1 == stages ? 0 : stage + 1;
+          ready = mbar_test_wait(smem_u32(&empty[stage]), ((bits >> stage) & 1u) ^ 1u);
         }
       }
-      if (ok) {
-        // No commit may still be on its way to this CTA's barriers.
-        for (int i = 0; i < STAGES; ++i) {
-          if ((issued_mask >> stage) & 1u)
-            if (!mbar_wait_bounded(&empty[stage], phase_bit ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) break;
-          if (++stage == STAGES) stage = 0, phase_bit ^= 1u;
-        }
-      } else if (leader) {
-        // Abort: let every phase this pair issued land.
-        for (int s = 0; s < STAGES; ++s) {
-          if (!((issued_mask >> s) & 1u)) continue;
-          const uint32_t addr = smem_u32(&full[s]);
-          const unsigned long long t0 = global_timer_ns();
-          while (!mbar_try_wait(addr, (phase_mask >> s) & 1u)) {
-            if (global_timer_ns() - t0 > kWaitLimitNs) {
-              record_device_error(kDevErrAbortDrain);
-              break;
-            }
+    }
+    if (ok) {
+      // No commit may still be on its way to this CTA's barriers.
+      for (int s = 0; s < STAGES; ++s) {
+        if ((issued_mask >> s) & 1u)
+          if (!mbar_wait_bounded(&empty[s], ((bits >> s) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) break;
+      }
+    } else if (leader && lane == 0) {
+      // Abort: let every phase this pair issued land.
+      for (int s = 0; s < STAGES; ++s) {
+        if (!((issued_mask >> s) & 1u)) continue;
+        const uint32_t addr = smem_u32(&full[s]);
+        const unsigned long long t0 = global_timer_ns();
+        while (!mbar_try_wait(addr, ((bits >> s) & 1u) ^ 1u)) {
+          if (global_timer_ns() - t0 > kWaitLimitNs) {
+            record_device_error(kDevErrAbortDrain);
+            break;
           }
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
-    if (leader && lane == 0) {
-      int stage = 0, slot = 0;
-      uint32_t phase_bit = 0, empty_bits = 0;
-      bool ok = true, issued = false;
+    if (leader) {
+      uint32_t bits = 0, empty_bits = 0;  // parities of full[], and of acc_empty[]'s next phases
+      bool ok = true, issued = false, ready = false;
+      auto slot_free = [&](int slot) {
+        const bool free = warp_wait(false, &acc_empty[slot], ((empty_bits >> slot) & 1u) ^ 1u, kDevErrWaitTimeoutAccEmpty, abort_flag);
+        tc_fence_after_sync();
+        empty_bits ^= 1u << slot;
+        return free;
+      };
       for (int ph = 0; ok && ph < phases; ++ph) {
         const int kind = ph % 3;
         const bool a_mn = kind == kGram && g.tall, b_mn = kind == kGram ? g.tall : kind == kUpdate && !g.tall;
-        const uint32_t idesc = make_idesc(0u, a_mn, b_mn, 2 * ORT_BM, PBN);
-        const uint32_t a_step = a_mn ? 2048u : 32u, b_step = b_mn ? 2048u : 32u;
-        const uint32_t a_lbo = a_mn ? 8192u : 16u, b_lbo = b_mn ? 8192u : 16u;
+        const int width = g.width[kind];
+        const bool wide = width == 512;
+        const int stages = wide ? L::WIDE_STAGES : L::STAGES;
+        const uint32_t idesc = make_idesc(0u, a_mn, b_mn, 2 * ORT_BM, min(width, 256));
+        // Descriptors of the first stage's operands and what the next stage and K's
+        // next 16 add to them.
+        const uint32_t stride = (wide ? 3 : 2) * (L::OPERAND >> 4);
+        const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
+        const uint64_t a0 = make_smem_desc_sw128(smem_u32(smem), a_mn ? 8192u : 16u, 1024);
+        const uint64_t b0 = make_smem_desc_sw128(smem_u32(smem + L::OPERAND), b_mn ? 8192u : 16u, 1024);
+        int stage = 0, slot = 0;
+        ready = false;
         for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
-          if (!mbar_wait_bounded(&acc_empty[slot], ((empty_bits >> slot) & 1u) ^ 1u, kDevErrWaitTimeoutAccEmpty, abort_flag)) {
+          if (!slot_free(slot)) {
             ok = false;
             break;
           }
-          tc_fence_after_sync();
-          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(slot * PBN);
+          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(slot * 256);
           for (int kb = 0; kb < g.k_blocks[kind]; ++kb) {
             // A wait for the data may last as long as the phase before (another
             // pair's tiles), which the producer's own limit covers.
-            if (!mbar_wait_bounded(&full[stage], phase_bit, kDevErrWaitTimeoutFull, abort_flag)) {
+            if (!warp_wait(ready, &full[stage], (bits >> stage) & 1u, kDevErrWaitTimeoutFull, abort_flag)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
-            const uint32_t sa = smem_u32(smem + L::OFF_A + stage * L::A_STAGE);
-            const uint32_t sb = smem_u32(smem + L::OFF_B + stage * L::B_STAGE);
+            const uint64_t ad = a0 + static_cast<uint32_t>(stage) * stride;
+            const uint64_t bd = b0 + static_cast<uint32_t>(stage) * stride;
+            if (elect_one_sync()) {
 #pragma unroll
-            for (int kk = 0; kk < ORT_BK / 16; ++kk)
-              umma_f16_pair(d_tmem, make_smem_desc_sw128(sa + kk * a_step, a_lbo, 1024),
-                            make_smem_desc_sw128(sb + kk * b_step, b_lbo, 1024), idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              for (uint32_t kk = 0; kk < ORT_BK / 16; ++kk)
+                umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              if (!wide) umma_commit_pair(&empty[stage]);
+            }
+            __syncwarp();
             issued = true;
-            umma_commit_pair(&empty[stage]);
-            if (++stage == STAGES) stage = 0, phase_bit ^= 1u;
+            if (wide) {
+              // The second half of a wide tile may still be drained by the epilogue of the one before.
+              if (kb == 0 && !slot_free(1)) {
+                ok = false;
+                break;
+              }
+              if (elect_one_sync()) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < ORT_BK / 16; ++kk)
+                  umma_f16_pair(d_tmem + 256, ad + kk * a_step, bd + (L::OPERAND >> 4) + kk * b_step, idesc,
+                                (kb > 0 || kk > 0) ? 1u : 0u);
+                umma_commit_pair(&empty[stage]);
+              }
+              __syncwarp();
+            }
+            bits ^= 1u << stage;
+            stage = stage + 1 == stages ? 0 : stage + 1;
+            ready = mbar_test_wait(smem_u32(&full[stage]), (bits >> stage) & 1u);
           }
           if (!ok) break;
-          umma_commit_pair(&acc_full[slot]);
-          empty_bits ^= 1u << slot;
-          slot = slot + 1 == SLOTS ? 0 : slot + 1;
+          if (elect_one_sync()) umma_commit_pair(&acc_full[slot]);
+          __syncwarp();
+          if (!wide) slot ^= 1;
         }
       }
       if (!ok && issued) {
-        umma_commit_pair(drain);
+        if (elect_one_sync()) umma_commit_pair(drain);
+        __syncwarp();
         const uint32_t addr = smem_u32(drain);
         const unsigned long long t0 = global_timer_ns();
         while (!mbar_try_wait(addr, 0)) {
@@ -404,65 +477,70 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    constexpr int PART = PBN / 2;
-    const int quarter = warp & 3, c0 = (warp - 2) / 4 * PART;
+    const int quarter = warp & 3;
     unsigned char* stage = smem + L::OFF_C + (warp - 2) * 2 * 4096;
-    int slot = 0;
-    uint32_t full_bits = 0;
+    uint32_t full_bits = 0;  // parities of acc_full[]'s next phases
     bool ok = true;
     for (int ph = 0; ok && ph < phases; ++ph) {
       const int kind = ph % 3, step = ph / 3, cur = step & 1;
       const float alpha = g.alpha[step][kind], beta = g.beta[step][kind];
+      const int width = g.width[kind], part = min(width, 256) / 2, c0 = (warp - 2) / 4 * part;
+      int slot = 0;
       // What the epilogue adds was written in the phases before.
       if (ph > 0) {
         const bool there = mbar_wait_bounded(go, static_cast<uint32_t>(ph - 1) & 1u, kDevErrGridBarrier, abort_flag);
-        if (!__all_sync(0xffffffffu, there)) break;
+        if (!__all_sync(0xffffffffu, there)) {
+          ok = false;
+          break;
+        }
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
-        int b, mt, nt;
-        ortho_tile<PBN>(g, kind, t, b, mt, nt);
-        const int m0 = mt * 2 * ORT_BM + static_cast<int>(rank) * ORT_BM + 32 * quarter, n0 = nt * PBN + c0;
-        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>(slot * PBN + c0);
-        auto wait = [&] {
-          const bool done = mbar_wait_bounded(&acc_full[slot], (full_bits >> slot) & 1u, kDevErrWaitTimeoutAccFull, abort_flag);
-          tc_fence_after_sync();
-          return static_cast<bool>(__all_sync(0xffffffffu, done));
-        };
-        auto release = [&] {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(map_to_rank(&acc_empty[slot], 0));
-        };
-        if (kind == kUpdate) {
-          const int64_t off = b * g.stride_x;
-          ok = ortho_epilogue<true, PART>(t_row, n0, m0, b, g.tall ? g.q : g.p, g.tall ? g.p : g.q, alpha, beta, g.x[cur] + off,
-                                          g.lo + off, g.ldx, false, &maps.x[cur ^ 1], &maps.lo, stage, lane, wait, release);
-        } else {
-          const bool below = (nt + 1) * PBN <= mt * 2 * ORT_BM;
-          const __half* add = g.gram + b * g.stride_p;
-          ok = ortho_epilogue<false, PART>(t_row, n0, m0, b, g.p, g.p, alpha, kind == kPoly ? beta : 0.f, add, add, g.ldp, below,
-                                           kind == kPoly ? &maps.poly : &maps.gram, kind == kPoly ? &maps.poly_t : &maps.gram_t,
-                                           stage, lane, wait, release);
+        int b, m, n;
+        ortho_tile(g, kind, t, b, m, n);
+        const int m0 = m + static_cast<int>(rank) * ORT_BM + 32 * quarter;
+        for (int h = 0; ok && h < (width == 512 ? 2 : 1); ++h) {
+          const int n0 = n + 256 * h + c0;
+          const uint32_t t_row =
+              tmem_base + (static_cast<uint32_t>(32 * quarter) << 16) + static_cast<uint32_t>((slot + h) * 256 + c0);
+          auto wait = [&] {
+            bool got = true;
+            if (h == 0) {
+              got = mbar_wait_bounded(&acc_full[slot], (full_bits >> slot) & 1u, kDevErrWaitTimeoutAccFull, abort_flag);
+              tc_fence_after_sync();
+            }
+            return static_cast<bool>(__all_sync(0xffffffffu, got));
+          };
+          auto release = [&] {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(&acc_empty[slot + h], 0));
+          };
+          if (kind == kUpdate) {
+            const int64_t off = b * g.stride_x;
+            ok = ortho_epilogue<true>(t_row, part, n0, m0, g.tall ? g.q : g.p, g.tall ? g.p : g.q, alpha, beta, g.x[cur] + off,
+                                      g.lo + off, g.x[cur ^ 1] + off, g.lo + off, g.ldx, 0, stage, lane, wait, release);
+          } else {
+            __half* gram = g.gram + b * g.stride_p;
+            __half* out = kind == kPoly ? g.poly + b * g.stride_p : gram;
+            ok = ortho_epilogue<false>(t_row, part, n0, m0, g.p, g.p, alpha, kind == kPoly ? beta : 0.f, gram, gram, out, out,
+                                       g.ldp, m, stage, lane, wait, release);
+          }
         }
         if (!ok) break;
         full_bits ^= 1u << slot;
-        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+        if (width != 512) slot ^= 1;
       }
       if (!ok) break;
       // This CTA's share of the phase is in memory.
+      __syncwarp();
       if (lane == 0 && ph + 1 < phases) {
-        bulk_wait_group<0>();
-        fence_proxy_async_all();
         mbar_arrive(done);
         if (warp == 2 && mbar_wait_bounded(done, static_cast<uint32_t>(ph) & 1u, kDevErrGridBarrier, abort_flag)) {
-          __threadfence();
           red_release_gpu(g.barrier);
         }
       }
       __syncwarp();
     }
-    if (lane == 0) bulk_wait_group<0>();
-    __syncwarp();
   }
 
   tc_fence_before_sync();
@@ -548,8 +626,10 @@ __device__ __forceinline__ void ortho_store8(const OrthoTensor& t, int64_t b, in
 }
 
 struct OrthoIo {
-  int64_t rows, cols, groups;  // groups: of eight columns in a row
-  int blocks;                  // CTAs to a matrix
+  int64_t rows, cols;
+  int groups;  // of eight columns in a row
+  int across;  // log2 of the threads to a row; the others of a CTA have the next rows
+  int blocks;  // CTAs to a matrix
   OrthoTensor g, m, w;         // gradient; momentum; weight, or the result
   float mu;
   int nesterov;
@@ -572,29 +652,48 @@ __device__ __forceinline__ void ortho_update8(const OrthoIo& p, const float (&m)
   for (int i = 0; i < 8; ++i) g[i] = p.nesterov ? fmaf(p.mu, m[i], g[i]) : m[i];
 }
 
+// Calls f(row, first column, a second row or -1) for this thread's groups: two
+// rows at a time, so that their loads are on their way together.
+template <typename F>
+__device__ __forceinline__ void ortho_groups(const OrthoIo& p, F&& f) {
+  const int tpr = 1 << p.across;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (256 >> p.across);
+  for (int64_t row = blockIdx.x * static_cast<int64_t>(256 >> p.across) + (threadIdx.x >> p.across); row < p.rows; row += 2 * step)
+    for (int g = threadIdx.x & (tpr - 1); g < p.groups; g += tpr) f(row, 8 * g, row + step < p.rows ? row + step : -1);
+}
+
 // Momentum <- mu momentum + gradient, and the sum of the squares of what is
 // orthogonalised: in 64 bits, which neither large nor small numbers leave.
-__global__ void __launch_bounds__(256) ortho_sum_kernel(const OrthoIo p) {
+template <bool MOMENTUM>
+__global__ void __launch_bounds__(256, 4) ortho_sum_kernel(const OrthoIo p) {
   __shared__ double part[8];
-  const int64_t b = blockIdx.y, n = p.rows * p.groups;
+  const int64_t b = blockIdx.y;
   grid_dependency_wait();
   if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) *p.barrier = 0u;
   double s = 0.0;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = e / p.groups, c = (e - row * p.groups) * 8;
-    float g[8];
-    ortho_load8(p.g, b, row, c, p.cols, g);
-    if (p.m.dtype >= 0) {
-      float m[8];
-      ortho_load8(p.m, b, row, c, p.cols, m);
+  ortho_groups(p, [&](int64_t row, int64_t c, int64_t row2) {
+    float g[2][8], m[2][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m[i] = fmaf(p.mu, m[i], g[i]);
-      ortho_store8(p.m, b, row, c, p.cols, m);
-      ortho_update8(p, m, g);
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      ortho_load8(p.g, b, r, c, p.cols, g[k]);
+      if constexpr (MOMENTUM) ortho_load8(p.m, b, r, c, p.cols, m[k]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fma(static_cast<double>(g[i]), static_cast<double>(g[i]), s);
-  }
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      if constexpr (MOMENTUM) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[k][i] = fmaf(p.mu, m[k][i], g[k][i]);
+        ortho_store8(p.m, b, r, c, p.cols, m[k]);
+        ortho_update8(p, m[k], g[k]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fma(static_cast<double>(g[k][i]), static_cast<double>(g[k][i]), s);
+    }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
@@ -606,9 +705,10 @@ __global__ void __launch_bounds__(256) ortho_sum_kernel(const OrthoIo p) {
 }
 
 // X0 = G / (||G|| + eps), times its scale, as hi + lo.
-__global__ void __launch_bounds__(256) ortho_scale_kernel(const OrthoIo p) {
+template <bool MOMENTUM>
+__global__ void __launch_bounds__(256, 4) ortho_scale_kernel(const OrthoIo p) {
   __shared__ double part[256];
-  const int64_t b = blockIdx.y, n = p.rows * p.groups;
+  const int64_t b = blockIdx.y;
   grid_dependency_wait();
   double s = 0.0;
   for (int i = threadIdx.x; i < p.blocks; i += 256) s += p.partial[b * p.blocks + i];
@@ -622,60 +722,75 @@ __global__ void __launch_bounds__(256) ortho_scale_kernel(const OrthoIo p) {
   const double factor = p.x_scale / (sqrt(part[0]) + p.eps);
   const float pre = factor > 0x1p100 ? 0x1p100f : 1.f;
   const float f = static_cast<float>(factor > 0x1p100 ? factor * 0x1p-100 : factor);
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = e / p.groups, c = (e - row * p.groups) * 8;
-    float g[8];
-    ortho_load8(p.g, b, row, c, p.cols, g);
-    if (p.m.dtype >= 0) {
-      float m[8];
-      ortho_load8(p.m, b, row, c, p.cols, m);
-      ortho_update8(p, m, g);
-    }
-    uint32_t h[4], l[4];
+  ortho_groups(p, [&](int64_t row, int64_t c, int64_t row2) {
+    float g[2][8], m[2][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = make_float2(g[2 * i] * pre * f, g[2 * i + 1] * pre * f);
-      h[i] = pack2_layer<__half>(v.x, v.y);
-      const float2 r = unpack2_layer<__half>(h[i]);
-      l[i] = pack2_layer<__half>(v.x - r.x, v.y - r.y);
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      if (!MOMENTUM || p.nesterov) ortho_load8(p.g, b, r, c, p.cols, g[k]);
+      if constexpr (MOMENTUM) ortho_load8(p.m, b, r, c, p.cols, m[k]);
     }
-    const int64_t at = b * p.stride_x + row * p.ldx + c;
-    *reinterpret_cast<uint4*>(p.hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(p.lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-  }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      if constexpr (MOMENTUM) ortho_update8(p, m[k], g[k]);
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = make_float2(g[k][2 * i] * pre * f, g[k][2 * i + 1] * pre * f);
+        h[i] = pack2_layer<__half>(v.x, v.y);
+        const float2 hi = unpack2_layer<__half>(h[i]);
+        l[i] = pack2_layer<__half>(v.x - hi.x, v.y - hi.y);
+      }
+      const int64_t at = b * p.stride_x + r * p.ldx + c;
+      *reinterpret_cast<uint4*>(p.hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(p.lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+  });
 }
 
 // The result, or the weight's step.
-__global__ void __launch_bounds__(256) ortho_out_kernel(const OrthoIo p, int update) {
-  const int64_t b = blockIdx.y, n = p.rows * p.groups;
+template <bool UPDATE>
+__global__ void __launch_bounds__(256, 4) ortho_out_kernel(const OrthoIo p) {
+  const int64_t b = blockIdx.y;
   grid_dependency_wait();
   float keep = p.keep, step = p.step;
-  if (update && p.lr_dev) {
+  if (UPDATE && p.lr_dev) {
     const float lr = *p.lr_dev;
     keep = 1.f - lr * p.decay;
     step *= lr;
   }
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = e / p.groups, c = (e - row * p.groups) * 8;
-    const int64_t at = b * p.stride_x + row * p.ldx + c;
-    const uint4 h4 = *reinterpret_cast<const uint4*>(p.hi + at), l4 = *reinterpret_cast<const uint4*>(p.lo + at);
-    const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
-    float v[8], w[8];
+  ortho_groups(p, [&](int64_t row, int64_t c, int64_t row2) {
+    uint4 h4[2], l4[2];
+    float w[2][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = add2(unpack2_layer<__half>(h[i]), unpack2_layer<__half>(l[i]));
-      v[2 * i] = x.x, v[2 * i + 1] = x.y;
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      const int64_t at = b * p.stride_x + r * p.ldx + c;
+      h4[k] = *reinterpret_cast<const uint4*>(p.hi + at);
+      l4[k] = *reinterpret_cast<const uint4*>(p.lo + at);
+      if constexpr (UPDATE) ortho_load8(p.w, b, r, c, p.cols, w[k]);
     }
-    if (update) {
-      ortho_load8(p.w, b, row, c, p.cols, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(-step, v[i], keep * w[i]);
-    } else {
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = k ? row2 : row;
+      if (r < 0) break;
+      const uint32_t h[4] = {h4[k].x, h4[k].y, h4[k].z, h4[k].w}, l[4] = {l4[k].x, l4[k].y, l4[k].z, l4[k].w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= p.out;
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = add2(unpack2_layer<__half>(h[i]), unpack2_layer<__half>(l[i]));
+        if constexpr (UPDATE) {
+          w[k][2 * i] = fmaf(-step, x.x, keep * w[k][2 * i]), w[k][2 * i + 1] = fmaf(-step, x.y, keep * w[k][2 * i + 1]);
+        } else {
+          w[k][2 * i] = x.x * p.out, w[k][2 * i + 1] = x.y * p.out;
+        }
+      }
+      ortho_store8(p.w, b, r, c, p.cols, w[k]);
     }
-    ortho_store8(p.w, b, row, c, p.cols, v);
-  }
+  });
 }
 
 // ---------------------------------------------------------------- host
@@ -744,8 +859,7 @@ bool ortho_schedule(const double* coefficients, int steps, OrthoSchedule& o) {
 struct OrthoPlan {
   int64_t batch, p, q, ldx, stride_x, ldp, stride_p;
   bool tall;
-  int blocks;
-  int64_t groups;
+  int blocks, groups, across;
   size_t barrier_off, partial_off, hi_off[2], lo_off, gram_off, poly_off, bytes;
 };
 
@@ -757,10 +871,11 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   o.p = std::min(rows, cols), o.q = std::max(rows, cols);
   o.ldx = round8(cols), o.stride_x = rows * o.ldx;
   o.ldp = round8(o.p), o.stride_p = o.p * o.ldp;
-  o.groups = (cols + 7) / 8;
-  // About eight CTAs of 256 threads per SM over the whole stack, at least two groups a thread.
-  const int64_t most = std::max<int64_t>(1, device_sm_count() * 8 / batch);
-  o.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, rows * o.groups / 512)));
+  o.groups = static_cast<int>((cols + 7) / 8);
+  while (o.across < 8 && (1 << o.across) < o.groups) ++o.across;
+  // Four CTAs of 256 threads an SM, two waves over the whole stack, two rows a thread.
+  const int64_t most = std::max<int64_t>(1, device_sm_count() * 8 / batch), each = 2 * (256 >> o.across);
+  o.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, (rows + each - 1) / each)));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -777,10 +892,23 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   return o;
 }
 
-template <int PBN>
+// Tiles of a symmetric matrix of `rows` row tiles: those whose first column is at most their last row.
+int64_t ortho_sym_tiles(int64_t rows, int width) {
+  if (width == 512) return (rows / 2) * (rows / 2 + 1) + (rows & 1) * (rows / 2 + 1);
+  return 256 / width * (rows * (rows + 1) / 2);
+}
+
+// Width of a phase's tiles, by its waves.
+int ortho_width(int64_t tiles128, int64_t tiles256, int64_t tiles512, int64_t pairs) {
+  const int64_t t128 = (tiles128 + pairs - 1) / pairs * 13;
+  const int64_t t256 = (tiles256 + pairs - 1) / pairs * 20;
+  const int64_t t512 = (tiles512 + pairs - 1) / pairs * 38;
+  return t512 < std::min(t128, t256) ? 512 : t256 <= t128 ? 256 : 128;
+}
+
 int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps, char* ws, cudaStream_t stream) {
-  using L = OrthoSmem<PBN>;
-  auto kern = ortho_pair_kernel<PBN>;
+  using L = OrthoSmem;
+  auto kern = ortho_pair_kernel;
   static std::atomic<int> capacity[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -797,6 +925,15 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   __half* gram = reinterpret_cast<__half*>(ws + o.gram_off);
   __half* poly = reinterpret_cast<__half*>(ws + o.poly_off);
   const int64_t xr = o.tall ? o.q : o.p, xc = o.tall ? o.p : o.q;  // X as stored
+  const int64_t most = capacity[dev].load(std::memory_order_relaxed);  // pairs at once
+  const int64_t rows = (o.p + 255) / 256, tiles_m = (xr + 255) / 256;
+  auto sym = [&](int w) { return o.batch * ortho_sym_tiles(rows, w); };
+  auto upd = [&](int w) { return o.batch * tiles_m * ((xc + w - 1) / w); };
+  const int ws_sym = ortho_width(sym(128), sym(256), sym(512), most);
+  // X's tiles are read and written as hi and lo, in bursts of all pairs that take HBM's
+  // time: only tiles of 256 columns, with two accumulators, hide those (8192 x 28672: 3.46 ms with 512, 3.2 with 256).
+  const int ws_upd = ortho_width(upd(128), upd(256), INT32_MAX, most);
+  const int width[3] = {ws_sym, ws_sym, ws_upd};
   OrthoMaps m;
   bool ok = true;
   auto map_x = [&](CUtensorMap* t, const __half* x, int inner, int rows) {
@@ -808,45 +945,38 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   for (int i = 0; i < 2; ++i) {
     // K-major operands come in boxes of 64 x rows, MN-major ones in 64 x 64.
     map_x(&m.a[kGram][i], hi[i], 64, o.tall ? ORT_BK : ORT_BM);
-    map_x(&m.b[kGram][i], hi[i], 64, o.tall ? ORT_BK : PBN / 2);
+    map_x(&m.b[kGram][i], hi[i], 64, o.tall ? ORT_BK : std::min(width[kGram], 256) / 2);
     map_p(&m.a[kPoly][i], gram, 64, ORT_BM);
-    map_p(&m.b[kPoly][i], gram, 64, PBN / 2);
+    map_p(&m.b[kPoly][i], gram, 64, std::min(width[kPoly], 256) / 2);
     if (o.tall) {
       map_x(&m.a[kUpdate][i], hi[i], 64, ORT_BM);
-      map_p(&m.b[kUpdate][i], poly, 64, PBN / 2);
+      map_p(&m.b[kUpdate][i], poly, 64, std::min(width[kUpdate], 256) / 2);
     } else {
       map_p(&m.a[kUpdate][i], poly, 64, ORT_BM);
       map_x(&m.b[kUpdate][i], hi[i], 64, ORT_BK);
     }
-    map_x(&m.x[i], hi[i], 64, 32);
   }
-  map_x(&m.lo, lo, 64, 32);
-  map_p(&m.gram, gram, 64, 32);
-  map_p(&m.poly, poly, 64, 32);
-  ok &= make_map_es(&m.gram_t, dt, 2, gram, o.p, o.p, o.batch, o.ldp, o.stride_p, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
-  ok &= make_map_es(&m.poly_t, dt, 2, poly, o.p, o.p, o.batch, o.ldp, o.stride_p, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (!ok) return CUOPX_CUDA_ERROR;
   OrthoArgs a = {};
   a.batch = static_cast<int>(o.batch);
   a.p = static_cast<int>(o.p), a.q = static_cast<int>(o.q);
   a.steps = steps;
   a.tall = o.tall;
-  a.tiles_m = static_cast<int>((xr + 255) / 256), a.tiles_n = static_cast<int>((xc + PBN - 1) / PBN);
-  // Symmetric phases: row tile i has min(256 / PBN (i + 1), all) column tiles.
-  const int64_t rows = (o.p + 255) / 256;
-  a.sym_tiles = static_cast<int>(256 / PBN * (rows * (rows + 1) / 2));
+  for (int j = 0; j < 3; ++j) a.width[j] = width[j];
+  a.tiles_m = static_cast<int>(tiles_m), a.tiles_n = static_cast<int>((xc + ws_upd - 1) / ws_upd);
+  a.sym_tiles = static_cast<int>(ortho_sym_tiles(rows, ws_sym));
   a.tiles[kGram] = a.tiles[kPoly] = a.batch * a.sym_tiles;
   a.tiles[kUpdate] = a.batch * a.tiles_m * a.tiles_n;
   a.k_blocks[kGram] = static_cast<int>((o.q + ORT_BK - 1) / ORT_BK);
   a.k_blocks[kPoly] = a.k_blocks[kUpdate] = static_cast<int>((o.p + ORT_BK - 1) / ORT_BK);
-  a.x[0] = hi[0], a.x[1] = hi[1], a.lo = lo, a.gram = gram;
+  a.x[0] = hi[0], a.x[1] = hi[1], a.lo = lo, a.gram = gram, a.poly = poly;
   a.ldx = o.ldx, a.stride_x = o.stride_x, a.ldp = o.ldp, a.stride_p = o.stride_p;
   a.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
   for (int i = 0; i < steps; ++i)
     for (int j = 0; j < 3; ++j) a.alpha[i][j] = sched.alpha[i][j], a.beta[i][j] = sched.beta[i][j];
   // Cooperative: all CTAs run at once, whatever else the GPU does.
   cudaLaunchConfig_t cfg = {};
-  const int pairs = std::min(capacity[dev].load(std::memory_order_relaxed), std::max(a.tiles[kGram], a.tiles[kUpdate]));
+  const int pairs = std::min(static_cast<int>(most), std::max(a.tiles[kGram], a.tiles[kUpdate]));
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(ORT_THREADS);
   cfg.dynamicSmemBytes = L::ALLOC;
@@ -864,7 +994,7 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
     cudaGetLastError();
     return cuda_failure(err);
   }
-  note_launch(PBN == 256 ? "ortho_pair_256x256" : "ortho_pair_256x128");
+  note_launch("ortho_pair");
   return check_launch();
 }
 
@@ -881,8 +1011,7 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   OrthoSchedule sched;
   if (!ortho_schedule(coefficients, steps, sched)) return CUOPX_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
-  io.groups = o.groups;
-  io.blocks = o.blocks;
+  io.groups = o.groups, io.across = o.across, io.blocks = o.blocks;
   io.partial = reinterpret_cast<double*>(ws + o.partial_off);
   io.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
   io.x_scale = static_cast<float>(sched.first);
@@ -890,22 +1019,23 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   io.lo = reinterpret_cast<__half*>(ws + o.lo_off);
   io.hi = reinterpret_cast<__half*>(ws + o.hi_off[0]);
   const dim3 grid(static_cast<unsigned>(o.blocks), static_cast<unsigned>(o.batch));
-  cudaError_t err = launch_pdl(ortho_sum_kernel, grid, dim3(256), 0, stream, io);
+  const bool momentum = io.m.dtype >= 0;
+  cudaError_t err = launch_pdl(momentum ? ortho_sum_kernel<true> : ortho_sum_kernel<false>, grid, dim3(256), 0, stream, io);
   note_launch("ortho_sum");
-  if (err == cudaSuccess) err = launch_pdl(ortho_scale_kernel, grid, dim3(256), 0, stream, io);
+  if (err == cudaSuccess)
+    err = launch_pdl(momentum ? ortho_scale_kernel<true> : ortho_scale_kernel<false>, grid, dim3(256), 0, stream, io);
   note_launch("ortho_scale");
   if (err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
   if (steps > 0) {
-    const int rc = o.q >= 2048 ? launch_ortho_pairs<256>(o, sched, steps, ws, stream) : launch_ortho_pairs<128>(o, sched, steps, ws, stream);
-    if (rc != CUOPX_SUCCESS) return rc;
+    if (const int rc = launch_ortho_pairs(o, sched, steps, ws, stream); rc != CUOPX_SUCCESS) return rc;
   }
   io.hi = reinterpret_cast<__half*>(ws + o.hi_off[steps & 1]);
   io.out = static_cast<float>(out_factor / sched.last);
   io.step = static_cast<float>(out_factor / sched.last);
-  err = launch_pdl(ortho_out_kernel, grid, dim3(256), 0, stream, io, update ? 1 : 0);
+  err = launch_pdl(update ? ortho_out_kernel<true> : ortho_out_kernel<false>, grid, dim3(256), 0, stream, io);
   note_launch(update ? "ortho_step" : "ortho_out");
   if (err != cudaSuccess) {
     cudaGetLastError();

@@ -85,6 +85,7 @@ struct QuantParams {
 __device__ __forceinline__ uint32_t row_max(uint32_t m, int tpr, uint32_t* part) {
   m = __reduce_max_sync(0xffffffffu, m);
   if (tpr == 32) return m;
+  // Two of these arrays in turn: a barrier lies between a warp's last reads of one and the next writes.
   const int warp = threadIdx.x >> 5, first = warp - warp % (tpr >> 5);
   if ((threadIdx.x & 31) == 0) part[warp] = m;
   __syncthreads();
@@ -93,59 +94,75 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, int tpr, uint32_t* part)
 }
 
 // Rows on 16-byte boundaries (Q's on 8, or 4 for fp32): `tpr` threads hold a row in G
-// groups of 16 bytes each, so that X is read once.  HBM-bound (8192 x 8192 bf16).
+// groups of 16 bytes each, so that X is read once, and a CTA loads its next rows
+// before it works on the present ones.  HBM-bound.
 template <typename T, int G>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantParams p, int tpr) {
-  using Mag = Magnitude<T>;
-  constexpr int V = Mag::V;
-  __shared__ uint32_t part[32];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int t = threadIdx.x % tpr;
-  const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + threadIdx.x / tpr;
+__device__ __forceinline__ void load_row(const QuantParams& p, int64_t row, int t, int tpr, uint4 (&v)[G]) {
+  constexpr int V = Magnitude<T>::V;
   const T* x = static_cast<const T*>(p.X) + row * p.ldx;
-  uint4 v[G];
-  uint32_t m = 0;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int64_t c = (g * static_cast<int64_t>(tpr) + t) * V;
     v[g] = make_uint4(0, 0, 0, 0);
     if (row < p.rows && c < p.cols) {
       if (c + V <= p.cols) {
-        v[g] = *reinterpret_cast<const uint4*>(x + c);
+        v[g] = __ldcs(reinterpret_cast<const uint4*>(x + c));
       } else {
-        alignas(16) T part_v[V] = {};
+        alignas(16) T some[V] = {};
         for (int i = 0; i < V; ++i)
-          if (c + i < p.cols) part_v[i] = x[c + i];
-        v[g] = *reinterpret_cast<const uint4*>(part_v);
+          if (c + i < p.cols) some[i] = x[c + i];
+        v[g] = *reinterpret_cast<const uint4*>(some);
       }
     }
   }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantParams p, int tpr) {
+  using Mag = Magnitude<T>;
+  constexpr int V = Mag::V;
+  __shared__ uint32_t part[2][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int t = threadIdx.x % tpr, each = blockDim.x / tpr;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * each;
+  int64_t row = blockIdx.x * static_cast<int64_t>(each) + threadIdx.x / tpr;
+  const int64_t first = blockIdx.x * static_cast<int64_t>(each);
+  uint4 next[G];
+  load_row<T, G>(p, row, t, tpr, next);
+  int turn = 0;
+  for (int64_t at = first; at < p.rows; at += step, row += step, turn ^= 1) {
+    uint4 v[G];
+    uint32_t m = 0;
 #pragma unroll
-  for (int g = 0; g < G; ++g) m = Mag::word(Mag::word(Mag::word(Mag::word(m, v[g].x), v[g].y), v[g].z), v[g].w);
-  m = row_max(Mag::fold(m), tpr, part);
-  if (row >= p.rows) return;
-  const RowScale s = row_scale(Mag::value(m));
-  if (t == 0) p.scale[row] = s.scale;
-  int8_t* q = p.Q + row * p.ldq;
+    for (int g = 0; g < G; ++g) v[g] = next[g];
+    if (at + step < p.rows) load_row<T, G>(p, row + step, t, tpr, next);
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int64_t c = (g * static_cast<int64_t>(tpr) + t) * V;
-    if (c >= p.cols) break;
-    uint32_t w[V / 4];
-    if constexpr (V == 8) {
-      w[0] = quantize4(pair_of<T>(v[g].x), pair_of<T>(v[g].y), s);
-      w[V / 4 - 1] = quantize4(pair_of<T>(v[g].z), pair_of<T>(v[g].w), s);
-    } else {
-      w[0] = quantize4(make_float2(__uint_as_float(v[g].x), __uint_as_float(v[g].y)),
-                       make_float2(__uint_as_float(v[g].z), __uint_as_float(v[g].w)), s);
-    }
-    if (c + V <= p.cols) {
-      if constexpr (V == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[V / 4 - 1]);
-      else *reinterpret_cast<uint32_t*>(q + c) = w[0];
-    } else {
-      for (int i = 0; i < V; ++i)
-        if (c + i < p.cols) q[c + i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
+    for (int g = 0; g < G; ++g) m = Mag::word(Mag::word(Mag::word(Mag::word(m, v[g].x), v[g].y), v[g].z), v[g].w);
+    m = row_max(Mag::fold(m), tpr, part[turn]);
+    if (row >= p.rows) continue;
+    const RowScale s = row_scale(Mag::value(m));
+    if (t == 0) p.scale[row] = s.scale;
+    int8_t* q = p.Q + row * p.ldq;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int64_t c = (g * static_cast<int64_t>(tpr) + t) * V;
+      if (c >= p.cols) break;
+      uint32_t w[V / 4];
+      if constexpr (V == 8) {
+        w[0] = quantize4(pair_of<T>(v[g].x), pair_of<T>(v[g].y), s);
+        w[V / 4 - 1] = quantize4(pair_of<T>(v[g].z), pair_of<T>(v[g].w), s);
+      } else {
+        w[0] = quantize4(make_float2(__uint_as_float(v[g].x), __uint_as_float(v[g].y)),
+                         make_float2(__uint_as_float(v[g].z), __uint_as_float(v[g].w)), s);
+      }
+      if (c + V <= p.cols) {
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[V / 4 - 1]);
+        else *reinterpret_cast<uint32_t*>(q + c) = w[0];
+      } else {
+        for (int i = 0; i < V; ++i)
+          if (c + i < p.cols) q[c + i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
+      }
     }
   }
 }
@@ -172,6 +189,128 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
   }
 }
 
+// Columns, with Q transposed: a cluster holds a strip of X of 128 bytes' width in the shared
+// memory of its CTAs, a share of the rows each, so that X is read once.  The
+// strip's column maxima meet through distributed shared memory; every CTA then quantises its
+// rows in place, four of a column to a word, and writes them out along Q's rows.
+constexpr int QC_PITCH = 33;  // words of a row in shared memory
+constexpr int QC_MAX_SHARE = 1536;
+
+template <typename T>
+__global__ void __launch_bounds__(512) quantize_columns_kernel(const QuantParams p, int cs, int share, int words) {
+  using Mag = Magnitude<T>;
+  constexpr int PER = 4 / sizeof(T);  // columns to a word
+  extern __shared__ uint32_t qc_rows[];
+  __shared__ uint32_t part[32][32], top[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int rank = static_cast<int>(blockIdx.x) % cs;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x / cs) * (32 * PER), c = c0 + lane * PER, r0 = static_cast<int64_t>(rank) * share;
+  const int64_t left = p.rows - r0;
+  const int rows = left <= 0 ? 0 : left < share ? static_cast<int>(left) : share;
+  grid_dependency_wait();
+  uint32_t m = 0;
+  if (rows > 0) {
+    // Sixteen rows of a warp on their way at once; lanes beyond the last column read
+    // that one and are masked.
+    constexpr int AHEAD = 16;
+    const T* x = static_cast<const T*>(p.X) + r0 * p.ldx;
+    const int64_t last = p.cols - 1;
+    const uint32_t mask = c >= p.cols ? 0u : PER == 2 && c == last ? 0xffffu : ~0u;
+    uint32_t* dst = qc_rows + warp * QC_PITCH + lane;
+    // A row's word, or its two halves, `step` elements of E from row to row.
+    auto read = [&](auto word, const auto* at, int64_t step, int second) {
+      constexpr bool WORD = decltype(word)::value;
+      for (int r = warp; r < rows; r += warps * AHEAD) {
+        const int n = min(AHEAD, (rows - r + warps - 1) / warps);
+        uint32_t lo[AHEAD], hi[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const auto* row = at + min(i, n - 1) * step;
+          lo[i] = __ldcs(row);
+          if constexpr (!WORD) hi[i] = __ldcs(row + second);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const uint32_t w = (WORD ? lo[i] : lo[i] | hi[i] << 16) & mask;
+          m = Mag::word(m, w);
+          if (i < n) dst[i * warps * QC_PITCH] = w;
+        }
+        at += AHEAD * step;
+        dst += AHEAD * warps * QC_PITCH;
+      }
+    };
+    if (words)
+      read(std::true_type{}, reinterpret_cast<const uint32_t*>(x + warp * p.ldx + (c < p.cols ? c : 0)), warps * p.ldx / PER, 0);
+    else
+      read(std::false_type{}, reinterpret_cast<const unsigned short*>(x + warp * p.ldx) + min(c, last), warps * p.ldx, c < last ? 1 : 0);
+  }
+  part[warp][lane] = m;
+  __syncthreads();
+  if (warp == 0) {
+    for (int i = 1; i < warps; ++i) m = Mag::word(m, part[i][lane]);
+    top[lane] = m;
+  }
+  if (cs > 1) {
+    cluster_sync_all();  // every CTA's maxima are in place
+    m = 0;
+    for (int i = 0; i < cs; ++i) {
+      uint32_t w;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(map_to_rank(&top[lane], static_cast<uint32_t>(i))) : "memory");
+      m = Mag::word(m, w);
+    }
+    cluster_arrive_relaxed();  // has read the others'
+  } else {
+    __syncthreads();
+    m = top[lane];
+  }
+  RowScale s[PER];
+  if constexpr (PER == 2) {
+    s[0] = row_scale(Mag::value(m & 0xffffu));
+    s[PER - 1] = row_scale(Mag::value(m >> 16));
+  } else {
+    s[0] = row_scale(Mag::value(m));
+  }
+  if (rank == 0 && warp == 0) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (c + k < p.cols) p.scale[c + k] = s[k].scale;
+  }
+  // Four rows of a lane's columns to a word for each column, in the rows' own places.
+  for (int r = 4 * warp; r < rows; r += 4 * warps) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = qc_rows[(r + i) * QC_PITCH + lane];
+    if constexpr (PER == 2) {
+      float2 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = pair_of<T>(w[i]);
+      qc_rows[r * QC_PITCH + lane] = quantize4(make_float2(f[0].x, f[1].x), make_float2(f[2].x, f[3].x), s[0]);
+      qc_rows[(r + 1) * QC_PITCH + lane] = quantize4(make_float2(f[0].y, f[1].y), make_float2(f[2].y, f[3].y), s[PER - 1]);
+    } else {
+      qc_rows[r * QC_PITCH + lane] = quantize4(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                                               make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), s[0]);
+    }
+  }
+  __syncthreads();
+  const bool q_words = reinterpret_cast<uintptr_t>(p.Q) % 4 == 0 && p.ldq % 4 == 0;  // r0 is a multiple of 4
+  for (int k = warp; k < 32 * PER; k += warps) {
+    if (c0 + k >= p.cols) break;
+    int8_t* q = p.Q + (c0 + k) * p.ldq + r0;
+    const uint32_t* src = qc_rows + k % PER * QC_PITCH + k / PER;
+    for (int r = 4 * lane; r < rows; r += 128) {
+      const uint32_t w = src[r * QC_PITCH];
+      if (q_words && r + 4 <= rows) {
+        *reinterpret_cast<uint32_t*>(q + r) = w;
+      } else {
+        for (int i = 0; i < 4; ++i)
+          if (r + i < rows) q[r + i] = static_cast<int8_t>(w >> (8 * i));
+      }
+    }
+  }
+  if (cs > 1) cluster_wait();  // the others have read this CTA's maxima
+}
+
+// More rows than a cluster holds: maxima first, then a second pass.
 // Largest magnitudes of columns, as bits, in `top` (zeroed before): a thread
 // to a column, 8 row phases and a share of the rows to a CTA.
 template <typename T>
@@ -221,7 +360,8 @@ __global__ void __launch_bounds__(256) quantize_transpose_kernel(const QuantPara
 template <typename T, int G>
 cudaError_t launch_quantize_rows(const QuantParams& p, int tpr, cudaStream_t stream) {
   const int rows = std::max(1, 256 / tpr);
-  return launch_pdl(quantize_rows_kernel<T, G>, dim3(static_cast<unsigned>((p.rows + rows - 1) / rows)),
+  const int64_t resident = static_cast<int64_t>(device_sm_count()) * (1024 / std::max(256, tpr));
+  return launch_pdl(quantize_rows_kernel<T, G>, dim3(static_cast<unsigned>(std::min((p.rows + rows - 1) / rows, resident))),
                     dim3(static_cast<unsigned>(rows * tpr)), 0, stream, p, tpr);
 }
 
@@ -250,13 +390,47 @@ int quantize_rows_typed(const QuantParams& p, cudaStream_t stream) {
   return check_launch();
 }
 
+// CTAs of a cluster and their shares of the rows: 256 rows or more each, up to eight CTAs.
+int quantize_cluster(int64_t rows, int64_t& share) {
+  int cs = 1;
+  while (cs < 8 && rows > 256ll * cs) cs *= 2;
+  share = ((rows + cs - 1) / cs + 31) / 32 * 32;
+  return cs;
+}
+
 template <typename T>
 int quantize_columns_typed(const QuantParams& p, uint32_t* top, cudaStream_t stream) {
+  int64_t share = 0;
+  const int cs = quantize_cluster(p.rows, share);
+  if (share <= QC_MAX_SHARE) {
+    constexpr int PER = 4 / sizeof(T);
+    auto kern = quantize_columns_kernel<T>;
+    static std::atomic<bool> attr_set[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
+    if (!attr_set[dev].load(std::memory_order_relaxed)) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, QC_MAX_SHARE * QC_PITCH * 4) != cudaSuccess)
+        return CUOPX_CUDA_ERROR;
+      attr_set[dev].store(true, std::memory_order_relaxed);
+    }
+    const int words = reinterpret_cast<uintptr_t>(p.X) % 4 == 0 && (p.rows == 1 || p.ldx % PER == 0) && p.cols % PER == 0;  // fp32: always
+    const int64_t strips = (p.cols + 32 * PER - 1) / (32 * PER);
+    const unsigned threads = share <= 640 ? 256 : 512;
+    const cudaError_t err =
+        launch_pdl_cluster(kern, dim3(static_cast<unsigned>(strips * cs)), dim3(threads), static_cast<size_t>(share) * QC_PITCH * 4,
+                           stream, static_cast<unsigned>(cs), p, cs, static_cast<int>(share), words);
+    if (err != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_failure(err);
+    }
+    note_launch("quantize_columns");
+    return check_launch();
+  }
   if (const cudaError_t e = cudaMemsetAsync(top, 0, static_cast<size_t>(p.cols) * 4, stream); e != cudaSuccess)
     return cuda_failure(e);
   const int64_t strips = (p.cols + 31) / 32;
   const int64_t want = std::max<int64_t>(1, device_sm_count() * 16 / strips);
-  const int64_t share = std::max<int64_t>(64, (p.rows + want - 1) / want);
+  share = std::max<int64_t>(64, (p.rows + want - 1) / want);
   quantize_column_max_kernel<T><<<dim3(static_cast<unsigned>(strips), static_cast<unsigned>((p.rows + share - 1) / share)), 256, 0,
                                   stream>>>(p, top, share);
   note_launch("quantize_column_max");
@@ -275,7 +449,10 @@ int quantize_rows(int dtype, const QuantParams& p, cudaStream_t stream) {
 }
 
 size_t quantize_workspace(const cuopx_quantize_args& a) {
-  return a.trans && a.rows > 0 && a.cols > 0 ? static_cast<size_t>(a.cols) * 4 : 0;
+  int64_t share = 0;
+  if (!a.trans || a.rows <= 0 || a.cols <= 0) return 0;
+  quantize_cluster(a.rows, share);
+  return share > QC_MAX_SHARE ? static_cast<size_t>(a.cols) * 4 : 0;
 }
 
 int validate_quantize(const cuopx_quantize_args& a) {

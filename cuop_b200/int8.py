@@ -104,7 +104,7 @@ def _int8(fn, gated: bool, x, w, w_scale, bias, residual, x_scale, activation, d
     ldw = _matrix(w, wide, k, torch.int8, device, "w")
     wsp = _vector(w_scale, wide, torch.float32, device, "w_scale")
     if out is None:
-        out = _empty((m, n), dtype=dtype, device=x.device)
+        out = x.new_empty((m, n), dtype=dtype)
         ldy = n
     else:
         ldy = _matrix(out, m, n, dtype, device, "out")
@@ -113,13 +113,19 @@ def _int8(fn, gated: bool, x, w, w_scale, bias, residual, x_scale, activation, d
     if residual is not None:
         ldr = _matrix(residual, m, n, dtype, device, "residual")
         rp = residual.data_ptr()
-    head = (code, act, m, n, k, x.data_ptr(), ldx, xsp, w.data_ptr(), ldw, wsp, bp, rp, ldr, out.data_ptr(), ldy)
+    xp, wp = x.data_ptr(), w.data_ptr()
+    head = (code, act, m, n, k, xp, ldx, xsp, wp, ldw, wsp, bp, rp, ldr, out.data_ptr(), ldy)
     lib = N.lib()
-    ws = None
-    wsb = (lib.cuopx_int8_gated_linear_workspace_size if gated else lib.cuopx_int8_linear_workspace_size)(
-        _INT8.pack(*head, 0, 0))
-    if wsb:
-        ws = _empty(wsb, dtype=torch.uint8, device=x.device)
+    size = lib.cuopx_int8_gated_linear_workspace_size if gated else lib.cuopx_int8_linear_workspace_size
+    if (wp | ldw) & 15 or (xsp and (xp | ldx) & 15):
+        wsb = size(_INT8.pack(*head, 0, 0))
+    elif xsp or not (m and n and k):
+        wsb = 0
+    elif m * k <= 8192:  # the product's kernel may quantise x
+        wsb = size(_INT8.pack(*head, 0, 0))
+    else:  # as the size call says where nothing is copied: the quantised x and its scales
+        wsb = ((m * ((k + 15) & ~15) + 255) & ~255) + ((4 * m + 255) & ~255)
+    ws = x.new_empty(wsb, dtype=torch.uint8) if wsb else None
     call = lib.cuopx_int8_gated_linear if gated else lib.cuopx_int8_linear
     rc = call(_INT8.pack(*head, ws.data_ptr() if wsb else 0, wsb), _raw_stream(device))
     if rc:

@@ -57,6 +57,23 @@ def test_quantize(m, k, trans, dt):
     check_quantize(strided(x, 16, 8, float("nan"))[0], trans)
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("rows,cols", [(257, 200), (513, 64), (1100, 33), (2049, 70), (8200, 66), (12288, 40), (12289, 40), (40001, 7)])
+def test_quantize_columns_of_any_length(rows, cols, dt):
+    """One CTA, clusters of two to eight, and more rows than a cluster holds."""
+    x = values(gen(rows), rows, cols, dt)
+    check_quantize(x, True)
+    assert cx.last_kernel() == ("quantize_columns" if rows <= 12288 else "quantize_transpose")
+    check_quantize(strided(x, 1, 1, float("nan"))[0], True)
+
+
+@pytest.mark.parametrize("rows,cols", [(5000, 100), (3001, 1030), (2500, 4104), (700, 16384), (1300, 8200)])
+def test_quantize_more_rows_than_run_at_once(rows, cols):
+    x = values(gen(rows), rows, cols, BF)
+    check_quantize(x, False)
+    check_quantize(x.float(), False)
+
+
 @pytest.mark.parametrize("trans", [False, True])
 def test_quantize_large(trans):
     x = values(gen(1), 2051, 4099, BF)
@@ -141,12 +158,14 @@ def check(x, wq, ws, b, r, act, dt, gated, xs=None, **kw):
 
 
 # name, rows, outputs, depth: each reaches the kernel of that name.
-KERNELS = [("int8_linear_simt", 3, 8, 5), ("int8_linear_split", 1, 264, 1024), ("int8_linear_split", 16, 136, 2000),
+KERNELS = [("int8_linear_simt", 3, 8, 5), ("int8_linear_split_q", 1, 264, 1024), ("int8_linear_split_q", 8, 136, 1008),
+           ("int8_linear_split_q", 2, 1000, 4095), ("int8_linear_split_q", 16, 33, 500), ("int8_linear_split_q", 1, 8192, 8000), ("int8_linear_split", 16, 136, 2000),
            ("int8_linear_split", 30, 520, 640), ("int8_linear_split", 64, 1000, 1400), ("int8_linear_split", 100, 300, 528),
            ("int8_linear_split", 5, 7, 80000), ("int8_linear_pair_k2", 129, 257, 1601), ("int8_linear_pair_k2", 700, 264, 2000),
            ("int8_linear_pair_k4", 140, 264, 12416), ("int8_linear_pair_k4", 512, 257, 12801),
            ("int8_linear_tc2_256x256", 300, 520, 528), ("int8_linear_tc2_256x256", 2600, 2056, 272)]
-GATED_KERNELS = [("int8_gated_linear_simt", 3, 8, 5), ("int8_gated_linear_split", 2, 72, 1280),
+GATED_KERNELS = [("int8_gated_linear_simt", 3, 8, 5), ("int8_gated_linear_split_q", 2, 72, 1280),
+                 ("int8_gated_linear_split_q", 4, 300, 2000),
                  ("int8_gated_linear_split", 50, 200, 2064), ("int8_gated_linear_pair_k2", 129, 130, 1601),
                  ("int8_gated_linear_pair_k2", 600, 264, 2000), ("int8_gated_linear_tc2_256x128", 300, 264, 528),
                  ("int8_gated_linear_tc2_256x128", 1500, 1032, 400)]
@@ -159,17 +178,19 @@ def test_every_kernel(name, m, n, k):
     for dt, pad, shift in ((BF, 0, 0), (HF, 16, 16), (BF, 1, 1)):
         x, wq, ws, b, r = operands(g, m, n, k, dt, gated, True, not gated)
         small = m * n * (2 if gated else 1) * k < 1 << 20
-        aligned = shift != 1 and k % 16 == 0
+        plain = name.replace("_q", "")  # from an int8 x
         if pad:
             wq = strided(wq, pad, shift, 99)[0]
-        want = name if aligned or not small else "int8_gated_linear_simt" if gated else "int8_linear_simt"
+        odd = small and (wq.stride(0) % 16 or wq.data_ptr() % 16)
+        simt = "int8_gated_linear_simt" if gated else "int8_linear_simt"
         check(x, wq, ws, b, r, "gelu_tanh", dt, gated)
-        assert cx.last_kernel() == want
+        assert cx.last_kernel() == (simt if odd else name)
         xq, xs = Q.quantize(x)
         if pad:
             xq = strided(xq, pad, shift, 99)[0]
         check(xq, wq, ws, None, None, "silu", dt, gated, xs=xs)
-        assert cx.last_kernel() == want
+        odd = odd or small and (xq.data_ptr() % 16 or m > 1 and xq.stride(0) % 16)
+        assert cx.last_kernel() == (simt if odd else plain)
 
 
 SIZES = [(1, 1, 1), (1, 8, 16), (1, 64, 128), (1, 1000, 72), (2, 7, 31), (3, 40, 200), (5, 128, 64), (8, 264, 136),

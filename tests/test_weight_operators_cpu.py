@@ -51,8 +51,10 @@ def muon(**kw):
     (dict(dtype=N.F64), TYPE), (dict(dtype=9), TYPE), (dict(trans=2), BAD), (dict(rows=-1), BAD), (dict(cols=-1), BAD),
     (dict(X=0), BAD), (dict(Q=0), BAD), (dict(scale=0), BAD), (dict(ldx=7), BAD), (dict(ldq=7), BAD), (dict(X=A + 1), BAD),
     (dict(scale=3 * A + 2), BAD), (dict(Q=A), BAD), (dict(Q=A + 62), BAD), (dict(scale=A + 4), BAD), (dict(scale=2 * A + 4), BAD),
-    (dict(trans=1, ldq=4), ROOM), (dict(trans=1, ldq=4, ws=4 * A, wsb=31), ROOM), (dict(trans=1, ldq=3, ws=4 * A, wsb=32), BAD),
-    (dict(trans=1, ldq=4, ws=4 * A + 4, wsb=32), BAD), (dict(trans=1, ldq=4, ws=A, wsb=32), BAD), (dict(rows=1 << 31), BAD),
+    (dict(trans=1, rows=20000, ldq=20000), ROOM), (dict(trans=1, rows=20000, ldq=20000, ws=4 * A, wsb=31), ROOM),
+    (dict(trans=1, rows=20000, ldq=19999, ws=4 * A, wsb=32), BAD), (dict(trans=1, ldq=3), BAD),
+    (dict(trans=1, rows=20000, ldq=20000, ws=4 * A + 4, wsb=32), BAD), (dict(trans=1, ldq=4, ws=4 * A + 4, wsb=32), BAD),
+    (dict(trans=1, rows=20000, ldq=20000, ws=A, wsb=32), BAD), (dict(rows=1 << 31), BAD),
     (dict(rows=1 << 30, ldx=1 << 40), BAD), (dict(trans=1, rows=65535 * 128 + 1, ldq=1 << 24, ws=4 * A, wsb=1 << 20), BAD),
     (dict(rows=0), OK), (dict(trans=1, cols=0), OK)])
 def test_quantize_refusals(change, status):
@@ -66,8 +68,8 @@ def test_quantize_refusals(change, status):
     (dict(ws=0), BAD), (dict(ldx=15), BAD), (dict(ldw=15), BAD), (dict(ldy=7), BAD), (dict(R=6 * A, ldr=7), BAD),
     (dict(X=A + 1), BAD), (dict(xs=6 * A + 2), BAD), (dict(ws=3 * A + 1), BAD), (dict(bias=6 * A + 1), BAD), (dict(Y=4 * A + 1), BAD),
     (dict(Y=A), BAD), (dict(Y=2 * A + 64), BAD), (dict(Y=3 * A), BAD), (dict(xs=4 * A), BAD), (dict(bias=4 * A + 8), BAD),
-    (dict(R=4 * A, ldr=9), BAD), (dict(R=4 * A + 2, ldr=8), BAD), (dict(work=0), ROOM), (dict(wsb=64), ROOM),
-    (dict(work=5 * A + 8), BAD), (dict(work=A), BAD), (dict(work=4 * A), BAD), (dict(work=3 * A), BAD),
+    (dict(R=4 * A, ldr=9), BAD), (dict(R=4 * A + 2, ldr=8), BAD), (dict(M=40, work=0), ROOM), (dict(M=40, wsb=64), ROOM),
+    (dict(work=5 * A + 8), BAD), (dict(M=40, work=A), BAD), (dict(M=40, work=4 * A), BAD), (dict(M=40, work=3 * A), BAD),
     (dict(M=1 << 40, ldx=1 << 40), BAD), (dict(ldw=1 << 60), BAD), (dict(M=0), OK), (dict(N=0), OK)])
 def test_int8_linear_refusals(change, status):
     assert N.lib().cuopx_int8_linear(lin(**change), None) == status
@@ -84,7 +86,10 @@ def test_int8_gated_refusals():
 def test_int8_workspace():
     lib = N.lib()
     size = lambda **kw: lib.cuopx_int8_linear_workspace_size(lin(**kw))  # noqa: E731
-    assert size() == 256 + 256  # quantised X, scales
+    assert size() == 0  # few enough rows for the product's own kernel
+    assert size(M=17) == 512 + 256  # quantised X, scales
+    assert size(M=16, K=1024, ldx=1024, ldw=1024) == 16 * 1024 + 256 and size(M=8, K=1024, ldx=1024, ldw=1024) == 0
+    assert size(M=1, K=8192, ldx=8192, ldw=8192) == 0 and size(M=1, K=8192, ldx=8192, ldw=8192, N=9000) == 8192 + 256
     assert size(xs=6 * A) == 0
     assert size(M=100, K=100, ldx=100, N=200, ldw=112) == 100 * 112 + 64 + 512  # rounded up to 256 each
     assert size(xs=6 * A, M=100, K=100, ldx=100, N=200, ldw=112) == (100 * 112 + 255) // 256 * 256
@@ -92,7 +97,10 @@ def test_int8_workspace():
     assert lib.cuopx_int8_gated_linear_workspace_size(lin(xs=6 * A, M=100, K=100, ldx=112, N=200, ldw=100)) == 400 * 112
     assert size(xs=6 * A, M=1, K=31, ldx=31, N=8, ldw=31) == 0  # too small to copy for
     assert size(M=0) == 0 and size(K=0) == 0
-    assert lib.cuopx_quantize_workspace_size(quant(trans=1, cols=1000)) == 4000
+    # maxima of columns that no cluster holds
+    assert lib.cuopx_quantize_workspace_size(quant(trans=1, cols=1000)) == 0
+    assert lib.cuopx_quantize_workspace_size(quant(trans=1, rows=12289, cols=1000)) == 4000
+    assert lib.cuopx_quantize_workspace_size(quant(trans=0, rows=12289, cols=1000)) == 0
 
 
 @pytest.mark.parametrize("change,status", [
