@@ -170,8 +170,10 @@ Int8Plan int8_plan(const cuopx_int8_linear_args& a, bool gated) {
   const int64_t wide = gated ? 2 * a.N : a.N;
   const LinearProblem p = int8_problem(a, gated);
   q.quantise = a.x_scale == nullptr;
-  // Unaligned int8 operands are copied where the tensor cores pay for it (kRepackMinWork).
-  const bool tensor = static_cast<double>(a.M) * static_cast<double>(wide) * static_cast<double>(a.K) >= kRepackMinWork;
+  // Unaligned int8 operands are copied where the tensor cores pay for it: up to kRepackMinWork
+  // multiplications the kernel for any alignment is one launch instead of two or three, but takes 2 us
+  // for 32 of K (8 x 130 x 503: 36 us, 9 with copies).
+  const bool tensor = a.K > 64 || static_cast<double>(a.M) * static_cast<double>(wide) * static_cast<double>(a.K) >= kRepackMinWork;
   q.copy_x = a.x_scale && tensor && !operand_aligned16(p, a.X, a.M == 1 ? 0 : a.ldx);
   q.copy_w = tensor && !operand_aligned16(p, a.W, a.ldw);
   if (q.quantise && split_quantises(a.M, a.N, a.K, gated) && (q.copy_w || operand_aligned16(p, a.W, a.ldw))) {

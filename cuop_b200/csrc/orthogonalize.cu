@@ -22,6 +22,8 @@
 // pairs (tcgen05 cta_group::2), tile i of a phase on pair i mod the number of pairs,
 // grid barriers between phases.  A and the polynomial are symmetric: tiles on or below
 // the diagonal are computed, and those below it stored twice, once transposed.
+// Where A has few tiles and X is long, several pairs share a tile of X X^T, a part of the
+// depth each (ortho_split_epilogue).
 //   warps 0, 10  TMA producers of the two operands (both CTAs)
 //   warp 1       TMEM allocation; MMA issuer (even CTA)
 //   warps 2-9    epilogue: alpha * sums + beta * (what the phase adds), rounded
@@ -79,7 +81,10 @@ struct OrthoArgs {
   int tiles[3];     // of a phase, all batches
   int k_blocks[3];
   int tiles_m, tiles_n;  // of the update, one batch
-  int sym_tiles;         // of the other two, one batch
+  int sym_tiles[2];      // of the other two, one batch
+  int splits;            // pairs that share a tile of kGram: 1, or 2 to 8 with a tile for every pair at most
+  float* partial;        // their sums: [tile][pair of these][warp][column][32 rows]
+  unsigned* tickets;     // [tile][warp]: pairs that have stored theirs
   __half* x[2];
   __half* lo;
   __half* gram;
@@ -138,8 +143,8 @@ __device__ __forceinline__ void ortho_tile(const OrthoArgs& g, int phase, int t,
     n = rr / rows * width;
   } else {
     // Row tile i has ceil((i + 1) 256 / width) tiles.
-    b = t / g.sym_tiles;
-    int r = t - b * g.sym_tiles;
+    b = t / g.sym_tiles[phase];
+    const int r = t - b * g.sym_tiles[phase];
     auto before = [&](int i) {  // tiles in the row tiles before i
       const int64_t h = i >> 1;
       if (width == 512) return static_cast<int>(h * (h + 1) + (i & 1) * (h + 1));
@@ -260,6 +265,69 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
   return true;
 }
 
+// K blocks of unit t of a phase, and the tile that it works on.
+__device__ __forceinline__ int ortho_unit(const OrthoArgs& g, int kind, int t, int& kb0, int& kb1) {
+  kb0 = 0;
+  kb1 = g.k_blocks[kind];
+  if (kind != kGram || g.splits == 1) return t;
+  const int tile = t / g.splits, s = t - tile * g.splits, all = kb1;
+  kb0 = all * s / g.splits;
+  kb1 = all * (s + 1) / g.splits;
+  return tile;
+}
+
+// One warp's 32 rows of `part` columns of a tile of X X^T whose depth `splits` pairs
+// share (this one is number `split`): its sums go to memory, and when the same warps of the other
+// pairs have stored theirs, each adds up a share of the columns, in the
+// pairs' order, so that results do not depend on timing.  They run at once (there is a pair for every
+// unit), so the wait ends.
+template <typename Wait, typename Release>
+__device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_t t_row, int part, int n0, int m0, float alpha, int tile,
+                                                     int split, int step, int where, __half* out, int diag, int lane,
+                                                     volatile int* abort, Wait&& wait, Release&& release) {
+  const int64_t region = 32ll * part, stride = region * 16;  // of a warp, of a pair
+  float* base = g.partial + static_cast<int64_t>(tile) * g.splits * stride + where * region + lane;
+  if (!wait()) return false;
+#pragma unroll 1
+  for (int c = 0; c < part; c += 32) {
+    uint32_t acc[32];
+    tmem_ld_32x32b_x32(t_row + c, acc);
+    tmem_wait_ld();
+    if (c + 32 == part) release();
+    float* dst = base + split * stride + c * 32;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) __stcg(dst + 32 * i, __uint_as_float(acc[i]));
+  }
+  __syncwarp();
+  bool there = true;
+  if (lane == 0) {
+    unsigned* ticket = g.tickets + tile * 16 + where;
+    red_release_gpu(ticket);
+    there = grid_wait(ticket, static_cast<unsigned>((step + 1) * g.splits), abort);
+  }
+  if (!__all_sync(0xffffffffu, there)) return false;
+  const int share = part / g.splits, c0 = split * share, row = m0 + lane;  // 8 columns or more
+#pragma unroll 1
+  for (int c = c0; c < c0 + share; c += 8) {
+    float v[8] = {};
+    for (int s = 0; s < g.splits; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += __ldcg(base + s * stride + (c + i) * 32);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2_layer<__half>(alpha * v[2 * i], alpha * v[2 * i + 1]);
+    const int col = n0 + c;
+    if (col >= g.p || col >= diag + 256 || row >= g.p) continue;
+    *reinterpret_cast<uint4*>(out + row * g.ldp + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (col < diag) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < g.p) out[(col + i) * g.ldp + row] = __ushort_as_half(static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1))));
+    }
+  }
+  return true;
+}
+
 __global__ void __launch_bounds__(ORT_THREADS, 1)
     ortho_pair_kernel(const __grid_constant__ OrthoMaps maps, const __grid_constant__ OrthoArgs g) {
   using L = OrthoSmem;
@@ -336,10 +404,10 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
         if (of_a && elect_one_sync()) mbar_arrive(go);
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
-        int b, m, n;
-        ortho_tile(g, kind, t, b, m, n);
+        int b, m, n, kb0, kb1;
+        ortho_tile(g, kind, ortho_unit(g, kind, t, kb0, kb1), b, m, n);
         const int first = (of_a ? m : n) + static_cast<int>(rank) * span;
-        for (int kb = 0; kb < g.k_blocks[kind]; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!warp_wait(ready, &empty[stage], ((bits >> stage) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
             ok = false;
             break;
@@ -419,7 +487,9 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
             break;
           }
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(slot * 256);
-          for (int kb = 0; kb < g.k_blocks[kind]; ++kb) {
+          int kb0, kb1;
+          ortho_unit(g, kind, t, kb0, kb1);
+          for (int kb = kb0; kb < kb1; ++kb) {
             // A wait for the data may last as long as the phase before (another
             // pair's tiles), which the producer's own limit covers.
             if (!warp_wait(ready, &full[stage], (bits >> stage) & 1u, kDevErrWaitTimeoutFull, abort_flag)) {
@@ -432,14 +502,14 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
             if (elect_one_sync()) {
 #pragma unroll
               for (uint32_t kk = 0; kk < ORT_BK / 16; ++kk)
-                umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                umma_f16_pair(d_tmem, ad + kk * a_step, bd + kk * b_step, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
               if (!wide) umma_commit_pair(&empty[stage]);
             }
             __syncwarp();
             issued = true;
             if (wide) {
               // The second half of a wide tile may still be drained by the epilogue of the one before.
-              if (kb == 0 && !slot_free(1)) {
+              if (kb == kb0 && !slot_free(1)) {
                 ok = false;
                 break;
               }
@@ -447,7 +517,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
 #pragma unroll
                 for (uint32_t kk = 0; kk < ORT_BK / 16; ++kk)
                   umma_f16_pair(d_tmem + 256, ad + kk * a_step, bd + (L::OPERAND >> 4) + kk * b_step, idesc,
-                                (kb > 0 || kk > 0) ? 1u : 0u);
+                                (kb > kb0 || kk > 0) ? 1u : 0u);
                 umma_commit_pair(&empty[stage]);
               }
               __syncwarp();
@@ -495,8 +565,9 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
         }
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
-        int b, m, n;
-        ortho_tile(g, kind, t, b, m, n);
+        int b, m, n, kb0, kb1;
+        const int tile = ortho_unit(g, kind, t, kb0, kb1);
+        ortho_tile(g, kind, tile, b, m, n);
         const int m0 = m + static_cast<int>(rank) * ORT_BM + 32 * quarter;
         for (int h = 0; ok && h < (width == 512 ? 2 : 1); ++h) {
           const int n0 = n + 256 * h + c0;
@@ -519,6 +590,10 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
             const int64_t off = b * g.stride_x;
             ok = ortho_epilogue<true>(t_row, part, n0, m0, g.tall ? g.q : g.p, g.tall ? g.p : g.q, alpha, beta, g.x[cur] + off,
                                       g.lo + off, g.x[cur ^ 1] + off, g.lo + off, g.ldx, 0, stage, lane, wait, release);
+          } else if (kind == kGram && g.splits > 1) {
+            ok = ortho_split_epilogue(g, t_row, part, n0, m0, alpha, tile, t - tile * g.splits, step,
+                                      static_cast<int>(rank) * ORT_EPI_WARPS + warp - 2, g.gram + b * g.stride_p, m, lane, abort_flag,
+                                      wait, release);
           } else {
             __half* gram = g.gram + b * g.stride_p;
             __half* out = kind == kPoly ? g.poly + b * g.stride_p : gram;
@@ -634,7 +709,8 @@ struct OrthoIo {
   float mu;
   int nesterov;
   double* partial;    // [batch][blocks] sums of squares
-  unsigned* barrier;  // of ortho_pair_kernel
+  unsigned* barrier;  // of ortho_pair_kernel, and its tickets behind it
+  int words;          // of both
   float x_scale;      // of the stored X0
   double eps;
   __half* hi;
@@ -669,7 +745,8 @@ __global__ void __launch_bounds__(256, 4) ortho_sum_kernel(const OrthoIo p) {
   __shared__ double part[8];
   const int64_t b = blockIdx.y;
   grid_dependency_wait();
-  if (blockIdx.x == 0 && b == 0 && threadIdx.x == 0) *p.barrier = 0u;
+  if (blockIdx.x == 0 && b == 0)
+    for (int i = threadIdx.x; i < p.words; i += 256) p.barrier[i] = 0u;
   double s = 0.0;
   ortho_groups(p, [&](int64_t row, int64_t c, int64_t row2) {
     float g[2][8], m[2][8];
@@ -860,8 +937,24 @@ struct OrthoPlan {
   int64_t batch, p, q, ldx, stride_x, ldp, stride_p;
   bool tall;
   int blocks, groups, across;
-  size_t barrier_off, partial_off, hi_off[2], lo_off, gram_off, poly_off, bytes;
+  int gram_width, splits;  // of the first phase's tiles where pairs share them (splits > 1)
+  int words;
+  size_t sums_off, barrier_off, partial_off, hi_off[2], lo_off, gram_off, poly_off, bytes;
 };
+
+// Tiles of a symmetric matrix of `rows` row tiles: those whose first column is at most their last row.
+int64_t ortho_sym_tiles(int64_t rows, int width) {
+  if (width == 512) return (rows / 2) * (rows / 2 + 1) + (rows & 1) * (rows / 2 + 1);
+  return 256 / width * (rows * (rows + 1) / 2);
+}
+
+// Pairs that share a tile of X X^T, so that no more than `pairs` are at work: the
+// exchange takes about as long as 16 K blocks.
+int ortho_splits(int64_t tiles, int64_t k_blocks, int64_t pairs) {
+  int s = 1;
+  while (s < 8 && tiles * 2 * s <= pairs && k_blocks >= 8 * 2 * s) s *= 2;
+  return k_blocks - k_blocks / s >= 24 ? s : 1;
+}
 
 OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   OrthoPlan o = {};
@@ -882,7 +975,13 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
     off += round256(bytes);
     return at;
   };
-  o.barrier_off = take(4);
+  const int64_t tiles = (o.p + 255) / 256;
+  o.gram_width = o.p <= 128 ? 128 : 256;
+  const int64_t gram_tiles = o.p <= 128 ? batch : batch * ortho_sym_tiles(tiles, 256);
+  o.splits = ortho_splits(gram_tiles, (o.q + ORT_BK - 1) / ORT_BK, device_sm_count() / 2);
+  o.words = 1 + (o.splits > 1 ? static_cast<int>(gram_tiles) * 16 : 0);
+  o.sums_off = take(o.splits > 1 ? static_cast<size_t>(gram_tiles) * o.splits * 256 * o.gram_width * 4 : 0);
+  o.barrier_off = take(static_cast<size_t>(o.words) * 4);
   o.partial_off = take(static_cast<size_t>(batch) * o.blocks * 8);
   for (int i = 0; i < 2; ++i) o.hi_off[i] = take(static_cast<size_t>(batch) * o.stride_x * 2);
   o.lo_off = take(static_cast<size_t>(batch) * o.stride_x * 2);
@@ -890,12 +989,6 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   o.poly_off = take(static_cast<size_t>(batch) * o.stride_p * 2);
   o.bytes = off;
   return o;
-}
-
-// Tiles of a symmetric matrix of `rows` row tiles: those whose first column is at most their last row.
-int64_t ortho_sym_tiles(int64_t rows, int width) {
-  if (width == 512) return (rows / 2) * (rows / 2 + 1) + (rows & 1) * (rows / 2 + 1);
-  return 256 / width * (rows * (rows + 1) / 2);
 }
 
 // Width of a phase's tiles, by its waves.
@@ -933,7 +1026,10 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   // X's tiles are read and written as hi and lo, in bursts of all pairs that take HBM's
   // time: only tiles of 256 columns, with two accumulators, hide those (8192 x 28672: 3.46 ms with 512, 3.2 with 256).
   const int ws_upd = ortho_width(upd(128), upd(256), INT32_MAX, most);
-  const int width[3] = {ws_sym, ws_sym, ws_upd};
+  // On a part with fewer pairs at once the planned split does not fit.
+  const int64_t gram_tiles = o.words / 16;
+  const int splits = gram_tiles * o.splits <= most ? o.splits : 1;
+  const int width[3] = {splits > 1 ? o.gram_width : ws_sym, ws_sym, ws_upd};
   OrthoMaps m;
   bool ok = true;
   auto map_x = [&](CUtensorMap* t, const __half* x, int inner, int rows) {
@@ -964,8 +1060,14 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   a.tall = o.tall;
   for (int j = 0; j < 3; ++j) a.width[j] = width[j];
   a.tiles_m = static_cast<int>(tiles_m), a.tiles_n = static_cast<int>((xc + ws_upd - 1) / ws_upd);
-  a.sym_tiles = static_cast<int>(ortho_sym_tiles(rows, ws_sym));
-  a.tiles[kGram] = a.tiles[kPoly] = a.batch * a.sym_tiles;
+  for (int j = 0; j < 2; ++j) {
+    // p <= 128: the second tile of 128 columns holds nothing.
+    a.sym_tiles[j] = o.p <= 128 && width[j] == 128 ? 1 : static_cast<int>(ortho_sym_tiles(rows, width[j]));
+    a.tiles[j] = a.batch * a.sym_tiles[j] * (j == kGram ? splits : 1);
+  }
+  a.splits = splits;
+  a.partial = reinterpret_cast<float*>(ws + o.sums_off);
+  a.tickets = reinterpret_cast<unsigned*>(ws + o.barrier_off) + 1;
   a.tiles[kUpdate] = a.batch * a.tiles_m * a.tiles_n;
   a.k_blocks[kGram] = static_cast<int>((o.q + ORT_BK - 1) / ORT_BK);
   a.k_blocks[kPoly] = a.k_blocks[kUpdate] = static_cast<int>((o.p + ORT_BK - 1) / ORT_BK);
@@ -976,7 +1078,7 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
     for (int j = 0; j < 3; ++j) a.alpha[i][j] = sched.alpha[i][j], a.beta[i][j] = sched.beta[i][j];
   // Cooperative: all CTAs run at once, whatever else the GPU does.
   cudaLaunchConfig_t cfg = {};
-  const int pairs = std::min(static_cast<int>(most), std::max(a.tiles[kGram], a.tiles[kUpdate]));
+  const int pairs = std::min(static_cast<int>(most), std::max({a.tiles[kGram], a.tiles[kPoly], a.tiles[kUpdate]}));
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(ORT_THREADS);
   cfg.dynamicSmemBytes = L::ALLOC;
@@ -1011,7 +1113,7 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   OrthoSchedule sched;
   if (!ortho_schedule(coefficients, steps, sched)) return CUOPX_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
-  io.groups = o.groups, io.across = o.across, io.blocks = o.blocks;
+  io.groups = o.groups, io.across = o.across, io.blocks = o.blocks, io.words = o.words;
   io.partial = reinterpret_cast<double*>(ws + o.partial_off);
   io.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
   io.x_scale = static_cast<float>(sched.first);

@@ -66,7 +66,7 @@ def _stack(t: torch.Tensor, shape, device: int, what: str):
     batch = shape[0] if len(shape) == 3 else 1
     stride = t.stride(0) if batch > 1 else 0
     if rows <= 1:
-        ld = max(cols, stride * batch if 0 < stride * batch < 1 << 40 else 0)
+        ld = cols
     if cs != 1 and cols > 1:
         _error(N.INVALID_ARGUMENT, f"{what}: rows must be contiguous (strides {t.stride()})")
     return code, t.data_ptr(), ld, stride

@@ -70,6 +70,17 @@ def test_coefficients_of_each_step(m, n):
         check(gradient(gen(1), m, n, "noise"), coefficients)
 
 
+@pytest.mark.parametrize("shape", [(40, 2000), (64, 3001), (3000, 64), (128, 6136), (129, 2500), (300, 5000), (5001, 257), (700, 2600),
+                                   (3, 100, 4000), (2, 4000, 200), (20, 70, 1800), (256, 16384)])
+def test_long_and_narrow(shape):
+    """Several pairs share a tile of the Gram matrix."""
+    g = torch.randn(shape, generator=gen(sum(shape)), device="cuda")
+    check(g)
+    first = cx.orthogonalize(g)
+    for _ in range(5):
+        assert torch.equal(first, cx.orthogonalize(g))
+
+
 def test_larger():
     """Several tiles of each kernel, too large for singular values of every step: against the reference norm by norm."""
     for m, n in ((2100, 1030), (1000, 4100), (2560, 2570)):

@@ -96,6 +96,7 @@ def test_int8_workspace():
     assert size(xs=6 * A, M=100, K=100, ldx=112, N=200, ldw=100) == (200 * 112 + 255) // 256 * 256
     assert lib.cuopx_int8_gated_linear_workspace_size(lin(xs=6 * A, M=100, K=100, ldx=112, N=200, ldw=100)) == 400 * 112
     assert size(xs=6 * A, M=1, K=31, ldx=31, N=8, ldw=31) == 0  # too small to copy for
+    assert size(xs=6 * A, M=2, K=65, ldx=65, N=8, ldw=65) == 256 + 768
     assert size(M=0) == 0 and size(K=0) == 0
     # maxima of columns that no cluster holds
     assert lib.cuopx_quantize_workspace_size(quant(trans=1, cols=1000)) == 0
