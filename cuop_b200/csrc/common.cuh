@@ -316,10 +316,10 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar_addr, uint32_t parit
 }
 
 // Bounded wait for the phase with the given parity to complete.  Returns
-// false (and records `err`) after kWaitLimitNs, or immediately once another
+// false (and records `err`) after limit_ns, or immediately once another
 // role has raised *abort.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, int err,
-                                                  volatile int* abort) {
+                                                  volatile int* abort, unsigned long long limit_ns = kWaitLimitNs) {
   const uint32_t addr = smem_u32(bar);
   if (mbar_try_wait(addr, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
@@ -327,7 +327,7 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     if (mbar_try_wait(addr, parity)) return true;
     if ((it & 255u) == 0u) {
       if (*abort) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (global_timer_ns() - t0 > limit_ns) {
         record_device_error(err);
         *abort = 1;
         return false;

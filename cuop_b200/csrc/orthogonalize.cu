@@ -91,6 +91,9 @@ struct OrthoArgs {
   __half* poly;
   int64_t ldx, stride_x, ldp, stride_p;  // elements
   unsigned* barrier;
+  // Of any wait: a second, and ten times what the largest phase takes, since a pair
+  // waits for the others' tiles.
+  unsigned long long limit_ns;
   float alpha[ORT_MAX_STEPS][3], beta[ORT_MAX_STEPS][3];
 };
 
@@ -106,13 +109,13 @@ __device__ __forceinline__ void red_release_gpu(unsigned* p) {
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 // Waits until `count` CTAs have arrived (bounded).
-__device__ __forceinline__ bool grid_wait(const unsigned* barrier, unsigned count, volatile int* abort) {
+__device__ __forceinline__ bool grid_wait(const unsigned* barrier, unsigned count, volatile int* abort, unsigned long long limit_ns) {
   const unsigned long long t0 = global_timer_ns();
   for (uint32_t it = 0; ld_acquire_gpu(barrier) < count; ++it) {
     __nanosleep(40);
     if ((it & 63u) == 63u) {
       if (*abort) return false;
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
+      if (global_timer_ns() - t0 > limit_ns) {
         record_device_error(kDevErrGridBarrier);
         *abort = 1;
         return false;
@@ -124,8 +127,9 @@ __device__ __forceinline__ bool grid_wait(const unsigned* barrier, unsigned coun
 }
 
 // A whole warp's bounded wait, with one answer for all lanes; `ready`: a test has said so already.
-__device__ __forceinline__ bool warp_wait(bool ready, uint64_t* bar, uint32_t parity, int err, volatile int* abort) {
-  return __all_sync(0xffffffffu, ready || mbar_wait_bounded(bar, parity, err, abort));
+__device__ __forceinline__ bool warp_wait(bool ready, uint64_t* bar, uint32_t parity, int err, volatile int* abort,
+                                          unsigned long long limit_ns) {
+  return __all_sync(0xffffffffu, ready || mbar_wait_bounded(bar, parity, err, abort, limit_ns));
 }
 
 // Tile t of a phase: batch, first row, first column.  Symmetric phases have the
@@ -303,7 +307,7 @@ __device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_
   if (lane == 0) {
     unsigned* ticket = g.tickets + tile * 16 + where;
     red_release_gpu(ticket);
-    there = grid_wait(ticket, static_cast<unsigned>((step + 1) * g.splits), abort);
+    there = grid_wait(ticket, static_cast<unsigned>((step + 1) * g.splits), abort, g.limit_ns);
   }
   if (!__all_sync(0xffffffffu, there)) return false;
   const int share = part / g.splits, c0 = split * share, row = m0 + lane;  // 8 columns or more
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       if (elect_one_sync()) prefetch_tmap(map);
       // The first phase reads what the kernel before has written.
       if (ph > 0) {
-        if (!__all_sync(0xffffffffu, lane != 0 || grid_wait(g.barrier, static_cast<unsigned>(ph) * gridDim.x, abort_flag))) {
+        if (!__all_sync(0xffffffffu, lane != 0 || grid_wait(g.barrier, static_cast<unsigned>(ph) * gridDim.x, abort_flag, g.limit_ns))) {
           ok = false;
           break;
         }
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
         ortho_tile(g, kind, ortho_unit(g, kind, t, kb0, kb1), b, m, n);
         const int first = (of_a ? m : n) + static_cast<int>(rank) * span;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!warp_wait(ready, &empty[stage], ((bits >> stage) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag)) {
+          if (!warp_wait(ready, &empty[stage], ((bits >> stage) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag, g.limit_ns)) {
             ok = false;
             break;
           }
@@ -461,7 +465,8 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       uint32_t bits = 0, empty_bits = 0;  // parities of full[], and of acc_empty[]'s next phases
       bool ok = true, issued = false, ready = false;
       auto slot_free = [&](int slot) {
-        const bool free = warp_wait(false, &acc_empty[slot], ((empty_bits >> slot) & 1u) ^ 1u, kDevErrWaitTimeoutAccEmpty, abort_flag);
+        const bool free = warp_wait(false, &acc_empty[slot], ((empty_bits >> slot) & 1u) ^ 1u, kDevErrWaitTimeoutAccEmpty, abort_flag,
+                                    g.limit_ns);
         tc_fence_after_sync();
         empty_bits ^= 1u << slot;
         return free;
@@ -490,9 +495,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           int kb0, kb1;
           ortho_unit(g, kind, t, kb0, kb1);
           for (int kb = kb0; kb < kb1; ++kb) {
-            // A wait for the data may last as long as the phase before (another
-            // pair's tiles), which the producer's own limit covers.
-            if (!warp_wait(ready, &full[stage], (bits >> stage) & 1u, kDevErrWaitTimeoutFull, abort_flag)) {
+            if (!warp_wait(ready, &full[stage], (bits >> stage) & 1u, kDevErrWaitTimeoutFull, abort_flag, g.limit_ns)) {
               ok = false;
               break;
             }
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       int slot = 0;
       // What the epilogue adds was written in the phases before.
       if (ph > 0) {
-        const bool there = mbar_wait_bounded(go, static_cast<uint32_t>(ph - 1) & 1u, kDevErrGridBarrier, abort_flag);
+        const bool there = mbar_wait_bounded(go, static_cast<uint32_t>(ph - 1) & 1u, kDevErrGridBarrier, abort_flag, g.limit_ns);
         if (!__all_sync(0xffffffffu, there)) {
           ok = false;
           break;
@@ -576,7 +579,8 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           auto wait = [&] {
             bool got = true;
             if (h == 0) {
-              got = mbar_wait_bounded(&acc_full[slot], (full_bits >> slot) & 1u, kDevErrWaitTimeoutAccFull, abort_flag);
+              got = mbar_wait_bounded(&acc_full[slot], (full_bits >> slot) & 1u, kDevErrWaitTimeoutAccFull, abort_flag,
+                                      g.limit_ns);
               tc_fence_after_sync();
             }
             return static_cast<bool>(__all_sync(0xffffffffu, got));
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       __syncwarp();
       if (lane == 0 && ph + 1 < phases) {
         mbar_arrive(done);
-        if (warp == 2 && mbar_wait_bounded(done, static_cast<uint32_t>(ph) & 1u, kDevErrGridBarrier, abort_flag)) {
+        if (warp == 2 && mbar_wait_bounded(done, static_cast<uint32_t>(ph) & 1u, kDevErrGridBarrier, abort_flag, g.limit_ns)) {
           red_release_gpu(g.barrier);
         }
       }
@@ -1074,6 +1078,8 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   a.x[0] = hi[0], a.x[1] = hi[1], a.lo = lo, a.gram = gram, a.poly = poly;
   a.ldx = o.ldx, a.stride_x = o.stride_x, a.ldp = o.ldp, a.stride_p = o.stride_p;
   a.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
+  const double work = 2.0 * static_cast<double>(o.batch) * static_cast<double>(o.p) * static_cast<double>(o.p) * static_cast<double>(o.q);
+  a.limit_ns = kWaitLimitNs + static_cast<unsigned long long>(work / 1e5);  // at 100 TFLOP/s
   for (int i = 0; i < steps; ++i)
     for (int j = 0; j < 3; ++j) a.alpha[i][j] = sched.alpha[i][j], a.beta[i][j] = sched.beta[i][j];
   // Cooperative: all CTAs run at once, whatever else the GPU does.
