@@ -112,8 +112,10 @@ struct PairSmem {
   static constexpr int OFF_CLC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;
   static constexpr int OFF_CLC_BAR = OFF_CLC + P_CLC_SLOTS * 16;
   static constexpr int OFF_MISC = OFF_CLC_BAR + 2 * P_CLC_SLOTS * 8;
+  static constexpr int OFF_SCALES = OFF_MISC + 16;  // int8 layers: 128 bytes a projection for each epilogue warp
   static constexpr int ALLOC = OFF_MISC + 16 + 1024;
-  static_assert(ALLOC <= 232448, "shared memory budget exceeded");
+  static constexpr int ALLOC_I8 = ALLOC + PairWarps<MODE>::EPI * (MODE == kPairGated ? 256 : 128);
+  static_assert(ALLOC <= 232448 && (MODE == kPairGemm || ALLOC_I8 <= 232448), "shared memory budget exceeded");
 };
 
 constexpr int P_MAX_PEERS = 7;  // one node: up to 8 ranks
@@ -497,13 +499,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairWarps<MODE>::THR
         constexpr int COLS = MODE == kPairGated ? PBN / 2 : PBN;
         constexpr int PART = COLS * 4 / PairWarps<MODE>::EPI;  // this warp's columns of the tile
         const int c0 = (warp - 2) / 4 * PART;
+        Int8Scales<MODE == kPairGated> scales;
+        if constexpr (I8) {
+          scales = {layer.epi.ws, p.N,
+                    reinterpret_cast<float*>(smem + L::OFF_SCALES + (warp - 2) * (MODE == kPairGated ? 256 : 128)),
+                    m0 + row_in_tile < p.M ? __ldg(layer.epi.xs + m0 + row_in_tile) : 0.f, {}};
+          scales.fetch(nt * COLS + c0, lane);
+        }
         auto sums = [&](int half, float (&a)[32], float (&b)[MODE == kPairGated ? 32 : 1]) {
-          if constexpr (I8) {
-            const int64_t col = nt * COLS + c0 + 32 * half;
-            const float xs = m0 + row_in_tile < p.M ? __ldg(layer.epi.xs + m0 + row_in_tile) : 0.f;
-            scale_row32(a, xs, layer.epi.ws, col, p.N, layer.epi.vec_ws);
-            if constexpr (MODE == kPairGated) scale_row32(b, xs, layer.epi.ws + p.N, col, p.N, layer.epi.vec_ws);
-          }
+          if constexpr (I8) scales.apply(a, b, nt * COLS + c0 + 32 * (half + 1), lane);
         };
         const bool done = layer_epilogue_tile<T, MODE == kPairGated, COLS, PART>(
             t_row + static_cast<uint32_t>(c0), nt * COLS + c0, m0 + 32 * q, p.M, p.N, layer.epi, &tmC, &layer.tmZ,
@@ -728,17 +732,18 @@ int launch_tc2_layer(const LinearProblem& p, cudaStream_t stream, const char* na
   prm.tiles_n = static_cast<int>((p.N + COLS - 1) / COLS);
   prm.num_tiles = prm.tiles_m * prm.tiles_n;
   prm.k_blocks = static_cast<int>(p.k_blocks());
+  constexpr int SMEM = I8 ? L::ALLOC_I8 : L::ALLOC;
   auto kern = gemm_tc2_kernel<T, A_MN, B_MN, PBN, MODE, false, Op>;
   static std::atomic<bool> attr_set[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
   if (!attr_set[dev].load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
       return CUOPX_CUDA_ERROR;
     attr_set[dev].store(true, std::memory_order_relaxed);
   }
   const cudaError_t lerr = launch_pdl(kern, dim3(static_cast<unsigned>(prm.num_tiles * 2)),
-                                      dim3(PairWarps<MODE>::THREADS), L::ALLOC, stream, mA, mB, mC, prm, layer);
+                                      dim3(PairWarps<MODE>::THREADS), SMEM, stream, mA, mB, mC, prm, layer);
   if (lerr != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(lerr);

@@ -32,7 +32,6 @@ struct LayerEpi {
   // gate's N, then the other projection's N).
   const float* xs;
   const float* ws;
-  int vec_ws;  // ws can be read in 16-byte groups
 };
 
 inline LayerEpi layer_epi(const LinearProblem& p) {
@@ -53,7 +52,6 @@ inline LayerEpi layer_epi(const LinearProblem& p) {
   e.tma_z = p.Z && row_aligned16(p.Z, p.ldz) && (!p.gated || p.N % 8 == 0) ? inside : 0;  // gated: U starts at column N
   e.xs = p.xs;
   e.ws = p.ws;
-  e.vec_ws = p.N % 4 == 0 && row_aligned16(p.ws, 0);
   return e;
 }
 
@@ -125,29 +123,44 @@ __device__ __forceinline__ void stage_row32(unsigned char* buf, int lane, int h,
   }
 }
 
-// Integer sums (their bits in v) of columns `col`.. times the row's factor and
-// theirs: one rounding of the sum to 24 bits, one for each product.  The
-// factors are the same for all lanes.
-__device__ __forceinline__ void scale_row32(float (&v)[32], float xs, const float* ws, int64_t col, int64_t N, bool vec) {
+// int8 operands: integer sums (their bits in v) times the row's factor and the
+// columns': one rounding of the sum to 24 bits, one for each product.  The factors of
+// 32 columns, the same for all rows, are fetched one to a lane ahead of
+// time and pass through `room` in shared memory (128 bytes of a warp's own; GATED: twice).
+template <bool GATED>
+struct Int8Scales {
+  const float* ws;
+  int64_t N;
+  float* room;
+  float xs;
+  float next[GATED ? 2 : 1];
+
+  __device__ __forceinline__ void fetch(int64_t col, int lane) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int64_t c = col + 4 * j;
-    if (vec) {
-      if (c < N) f = __ldg(reinterpret_cast<const float4*>(ws + c));
-    } else {
-      if (c < N) f.x = __ldg(ws + c);
-      if (c + 1 < N) f.y = __ldg(ws + c + 1);
-      if (c + 2 < N) f.z = __ldg(ws + c + 2);
-      if (c + 3 < N) f.w = __ldg(ws + c + 3);
-    }
-    float2 lo = make_float2(__int2float_rn(__float_as_int(v[4 * j])), __int2float_rn(__float_as_int(v[4 * j + 1])));
-    float2 hi = make_float2(__int2float_rn(__float_as_int(v[4 * j + 2])), __int2float_rn(__float_as_int(v[4 * j + 3])));
-    lo = mul2(mul2(lo, both(xs)), make_float2(f.x, f.y));
-    hi = mul2(mul2(hi, both(xs)), make_float2(f.z, f.w));
-    v[4 * j] = lo.x, v[4 * j + 1] = lo.y, v[4 * j + 2] = hi.x, v[4 * j + 3] = hi.y;
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) next[h] = col + lane < N ? __ldg(ws + h * N + col + lane) : 0.f;
   }
-}
+  __device__ __forceinline__ void scale(float (&v)[32], const float* factors) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 f = *reinterpret_cast<const float4*>(factors + 4 * j);
+      float2 lo = make_float2(__int2float_rn(__float_as_int(v[4 * j])), __int2float_rn(__float_as_int(v[4 * j + 1])));
+      float2 hi = make_float2(__int2float_rn(__float_as_int(v[4 * j + 2])), __int2float_rn(__float_as_int(v[4 * j + 3])));
+      lo = mul2(mul2(lo, both(xs)), make_float2(f.x, f.y));
+      hi = mul2(mul2(hi, both(xs)), make_float2(f.z, f.w));
+      v[4 * j] = lo.x, v[4 * j + 1] = lo.y, v[4 * j + 2] = hi.x, v[4 * j + 3] = hi.y;
+    }
+  }
+  // The sums of the columns fetched last; then those from `col` on are fetched.
+  __device__ __forceinline__ void apply(float (&a)[32], float (&b)[GATED ? 32 : 1], int64_t col, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) room[32 * h + lane] = next[h];
+    __syncwarp();
+    fetch(col, lane);
+    scale(a, room);
+    if constexpr (GATED) scale(b, room + 32);
+  }
+};
 
 // One warp's rows of PART columns of one tile.  t_row: TMEM address of the
 // first of them in this warp's lane quarter; the second projection's (GATED)

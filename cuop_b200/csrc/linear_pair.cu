@@ -41,7 +41,8 @@ struct LpSmem {
   static constexpr int OFF_BAR = OFF_C + LP_EPI_WARPS * 2 * 4096;
   static constexpr int NUM_BARS = 2 * LP_STAGES + 2;  // full, empty, acc_full, drain
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+  static constexpr int OFF_SCALES = OFF_MISC + 16;  // int8: 128 bytes a projection for each finishing warp
+  static constexpr int ALLOC = OFF_SCALES + LP_EPI_WARPS * 128 + 1024;
   static_assert(ALLOC <= 232448, "shared memory budget exceeded");
   // Received sums: (KS - 1) x 128 rows x 256 / KS columns, 96 KB at most.
   static_assert(3 * LP_BM * (LP_BN / 4) * 4 <= OFF_C, "the ring holds the received sums");
@@ -257,6 +258,12 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       const int c0 = group * PART;  // among the pair's columns
       unsigned char* stage = smem + L::OFF_C + (warp - 2) * (GATED ? 3 : 2) * 4096;
       int ybuf = 0;
+      Int8Scales<GATED> scales;
+      if constexpr (I8) {
+        scales = {p.epi.ws, p.N, reinterpret_cast<float*>(smem + L::OFF_SCALES + (warp - 2) * (GATED ? 256 : 128)),
+                  m0 + row < p.M ? __ldg(p.epi.xs + m0 + row) : 0.f, {}};
+        scales.fetch(n0 + kp * OWN + c0, lane);
+      }
       layer_epilogue_tile<T, GATED, COLS, PART>(
           t_row + static_cast<uint32_t>(kp * OWN + c0), n0 + kp * OWN + c0, m0 + 32 * q, p.M, p.N, p.epi, &tmY, &tmZ, &tmZ2,
           stage, lane, ybuf, [] { return true; }, [] {},
@@ -277,10 +284,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
                 a[i] = __int_as_float(sa);
                 if constexpr (GATED) b[i] = __int_as_float(sb);
               }
-              const int64_t first = n0 + kp * OWN + c0 + 32 * half;
-              const float xs = m0 + row < p.M ? __ldg(p.epi.xs + m0 + row) : 0.f;
-              scale_row32(a, xs, p.epi.ws, first, p.N, p.epi.vec_ws);
-              if constexpr (GATED) scale_row32(b, xs, p.epi.ws + p.N, first, p.N, p.epi.vec_ws);
+              scales.apply(a, b, n0 + kp * OWN + c0 + 32 * (half + 1), lane);
               return;
             }
 #pragma unroll

@@ -57,9 +57,12 @@ struct SplitSmem {
   static constexpr int NUM_BARS = 2 * STAGES + 2;  // full, empty, acc_full, drain
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int OFF_ROWS = OFF_MISC + 16;  // QX: the rows' maxima of 8 CTAs and this one, the rows' scales
-  static constexpr int ALLOC = OFF_ROWS + (QX ? 10 * TOK * 4 : 0) + 1024;
+  // int8: w_scale and bias of this CTA's columns, x_scale of the rows
+  static constexpr int OFF_FACTORS = OFF_ROWS + (QX ? 10 * TOK * 4 : 0);
+  static constexpr int ALLOC = OFF_FACTORS + 1024;
+  static constexpr int ALLOC_I8 = ALLOC + (2 * LSP_COLS + TOK) * 4;
   static constexpr uint32_t TMEM_COLS = TOK < 32 ? 32 : TOK;
-  static_assert((ALLOC + 1024) * CTAS <= 233472, "CTAS CTAs must fit one SM's shared memory");
+  static_assert((ALLOC_I8 + 1024) * CTAS <= 233472, "CTAS CTAs must fit one SM's shared memory");
 };
 
 struct SplitParams {
@@ -350,6 +353,17 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK, QX>::CTAS)
     if (cs > 1 && !QX) cluster_wait();
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
+    if constexpr (I8) {
+      // What the outputs need is on its way while the products are made.
+      const int own = LSP_COLS / cs, outs = TILE_N / cs, e = threadIdx.x - 64;
+      float* factors = reinterpret_cast<float*>(smem + L::OFF_FACTORS);
+      const int h = e / outs, col = n0 + rank * outs + e - h * outs;
+      if (e < own && col < p.N) {
+        factors[e] = p.ws[static_cast<int64_t>(h) * p.N + col];
+        factors[LSP_COLS + e] = p.bias ? to_acc<T>(static_cast<const T*>(p.bias)[static_cast<int64_t>(h) * p.N + col]) : 0.f;
+      }
+      if (!QX && e < p.M) factors[2 * LSP_COLS + e] = p.xs[e];
+    }
     const bool got = __all_sync(0xffffffffu, mbar_wait_bounded(acc_full, 0, kDevErrWaitTimeoutAccFull, abort_flag));
     tc_fence_after_sync();
     if (cs > 1 && L::ALIAS) cluster_arrive_relaxed();
@@ -416,10 +430,11 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK, QX>::CTAS)
             i0 += v.x;
             i1 += v.y;
           }
-          const float xs = QX ? reinterpret_cast<const float*>(maxima + 9 * TOK)[t] : p.xs[t];
-          const float* ws = p.ws + static_cast<int64_t>(h) * p.N + col;
-          z[h][0] = __int2float_rn(i0) * xs * ws[0];
-          if (two) z[h][1] = __int2float_rn(i1) * xs * ws[1];
+          const float* factors = reinterpret_cast<const float*>(smem + L::OFF_FACTORS);
+          const float xs = QX ? reinterpret_cast<const float*>(maxima + 9 * TOK)[t] : factors[2 * LSP_COLS + t];
+          const float* ws = factors + h * outs + f;
+          z[h][0] = __int2float_rn(i0) * xs * ws[0] + ws[LSP_COLS];
+          if (two) z[h][1] = __int2float_rn(i1) * xs * ws[1] + ws[LSP_COLS + 1];
         } else {
           for (int s = 0; s < cs; ++s) {
             const float2 v = *reinterpret_cast<const float2*>(sums + (s * TOK + t) * own + h * outs + f);
@@ -427,7 +442,7 @@ __global__ void __launch_bounds__(LSP_THREADS, SplitSmem<TOK, QX>::CTAS)
             z[h][1] += v.y;
           }
         }
-        if (bias) {
+        if (!I8 && bias) {
           z[h][0] += to_acc<T>(bias[static_cast<int64_t>(h) * p.N + col]);
           if (two) z[h][1] += to_acc<T>(bias[static_cast<int64_t>(h) * p.N + col + 1]);
         }
@@ -461,6 +476,7 @@ template <typename T, bool W_MN, bool GATED, int TOK, typename Op = T, bool QX =
 int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   using L = SplitSmem<TOK, QX>;
   constexpr bool I8 = std::is_same<Op, int8_t>::value;
+  constexpr int SMEM = I8 ? L::ALLOC_I8 : L::ALLOC;
   const CUtensorMapDataType dt =
       std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap mW, mX;
@@ -501,10 +517,10 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
   if (!attr_set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
       return CUOPX_CUDA_ERROR;
     for (int i = 0; i < 4; ++i)
-      capacity[dev][i].store(cluster_capacity(kern, LSP_THREADS, L::ALLOC, 1u << i), std::memory_order_relaxed);
+      capacity[dev][i].store(cluster_capacity(kern, LSP_THREADS, SMEM, 1u << i), std::memory_order_relaxed);
     attr_set[dev].store(true, std::memory_order_release);
   }
   // Split K while the clusters still run in one wave and every CTA keeps two
@@ -522,7 +538,7 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
   while (QX && cs < 8 && prm.k_blocks > cs * LSP_QX_BLOCKS) cs *= 2;
   if (QX && prm.k_blocks > cs * LSP_QX_BLOCKS) return CUOPX_NOT_IMPLEMENTED;  // not reached: split_quantises
   prm.cs = cs;
-  const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), L::ALLOC,
+  const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), SMEM,
                                              stream, static_cast<unsigned>(cs), mW, mX, prm);
   if (err != cudaSuccess) {
     cudaGetLastError();

