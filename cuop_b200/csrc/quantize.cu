@@ -194,13 +194,15 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
 // memory of its CTAs, a share of the rows each, so that X is read once.  The
 // strip's column maxima meet through distributed shared memory; every CTA then quantises its
 // rows in place, four of a column to a word, and writes them out along Q's rows.
-// Issue-bound (21 instructions an element): 4096 x 10240 bf16 52 us, odd rows as in
-// 4095 x 10001 fp16, read in single elements, 75; two passes over X took 141.
+// A CTA's four phases, which other CTAs of the SM overlap only in part, bound it: 4096 x 10240 bf16
+// 46.8 us, rows off 4-byte boundaries as in 4095 x 10001 fp16 (WORD false: single elements) 55;
+// two passes over X took 141.  Half the threads: 52 and 73.  Loads by 4-byte cp.async, all of
+// a share at once: 76 and 89.
 constexpr int QC_PITCH = 33;  // words of a row in shared memory
 constexpr int QC_MAX_SHARE = 1536;
 
-template <typename T>
-__global__ void __launch_bounds__(512) quantize_columns_kernel(const QuantParams p, int cs, int share, int words) {
+template <typename T, bool WORD>
+__global__ void __maxnreg__(WORD ? 64 : 40) quantize_columns_kernel(const QuantParams p, int cs, int share) {
   using Mag = Magnitude<T>;
   constexpr int PER = 4 / sizeof(T);  // columns to a word
   extern __shared__ uint32_t qc_rows[];
@@ -213,39 +215,43 @@ __global__ void __launch_bounds__(512) quantize_columns_kernel(const QuantParams
   grid_dependency_wait();
   uint32_t m = 0;
   if (rows > 0) {
-    // Sixteen rows of a warp on their way at once; lanes beyond the last column read
-    // that one and are masked.
-    constexpr int AHEAD = 16;
+    // Sixteen loads of a warp on their way at once, from rows next to the other warps'.  Lanes
+    // beyond the last column read one that exists; it does not reach Q.
     const T* x = static_cast<const T*>(p.X) + r0 * p.ldx;
     const int64_t last = p.cols - 1;
-    const uint32_t mask = c >= p.cols ? 0u : PER == 2 && c == last ? 0xffffu : ~0u;
     uint32_t* dst = qc_rows + warp * QC_PITCH + lane;
-    // A row's word, or its two halves, `step` elements of E from row to row.
-    auto read = [&](auto word, const auto* at, int64_t step, int second) {
-      constexpr bool WORD = decltype(word)::value;
-      for (int r = warp; r < rows; r += warps * AHEAD) {
-        const int n = min(AHEAD, (rows - r + warps - 1) / warps);
+    // A row's word, or its two halves, `step` elements from one of the warp's rows to the next.
+    // Registers decide the order of the loads and how many CTAs share an SM: whole groups
+    // apart from the last one and 64 registers are best for words (40: 52 us instead of 47), one
+    // form and 40 for elements (with whole groups apart 79 instead of 55).
+    auto read = [&](const auto* at, int64_t step, int second) {
+      constexpr int AHEAD = WORD ? 16 : 8;
+      auto group = [&](auto whole, int n) {
         uint32_t lo[AHEAD], hi[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-          const auto* row = at + min(i, n - 1) * step;
+          const auto* row = at + (decltype(whole)::value ? i : min(i, n - 1)) * step;
           lo[i] = __ldcs(row);
           if constexpr (!WORD) hi[i] = __ldcs(row + second);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-          const uint32_t w = (WORD ? lo[i] : lo[i] | hi[i] << 16) & mask;
+          const uint32_t w = WORD ? lo[i] : __byte_perm(lo[i], hi[i], 0x5410);
           m = Mag::word(m, w);
-          if (i < n) dst[i * warps * QC_PITCH] = w;
+          if (decltype(whole)::value || i < n) dst[i * warps * QC_PITCH] = w;
         }
         at += AHEAD * step;
         dst += AHEAD * warps * QC_PITCH;
-      }
+      };
+      int n = (rows - warp + warps - 1) / warps;  // this warp's rows
+      if constexpr (WORD)
+        for (; n >= AHEAD; n -= AHEAD) group(std::true_type{}, n);
+      for (; n > 0; n -= AHEAD) group(std::false_type{}, n);
     };
-    if (words)
-      read(std::true_type{}, reinterpret_cast<const uint32_t*>(x + warp * p.ldx + (c < p.cols ? c : 0)), warps * p.ldx / PER, 0);
+    if constexpr (WORD)
+      read(reinterpret_cast<const uint32_t*>(x + warp * p.ldx + (c < p.cols ? c : 0)), warps * p.ldx / PER, 0);
     else
-      read(std::false_type{}, reinterpret_cast<const unsigned short*>(x + warp * p.ldx) + min(c, last), warps * p.ldx, c < last ? 1 : 0);
+      read(reinterpret_cast<const unsigned short*>(x + warp * p.ldx) + min(c, last), warps * p.ldx, c < last ? 1 : 0);
   }
   part[warp][lane] = m;
   __syncthreads();
@@ -278,36 +284,39 @@ __global__ void __launch_bounds__(512) quantize_columns_kernel(const QuantParams
     for (int k = 0; k < PER; ++k)
       if (c + k < p.cols) p.scale[c + k] = s[k].scale;
   }
-  // Four rows of a lane's columns to a word for each column, in the rows' own places.
+  // Four rows of a lane's columns to a word for each column, in the rows' own places: group g's
+  // words lie in its row (g / 8 + column) % 4, so that 32 groups of a column lie in 32 banks.
   for (int r = 4 * warp; r < rows; r += 4 * warps) {
     uint32_t w[4];
+    uint32_t* at = qc_rows + r * QC_PITCH + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = qc_rows[(r + i) * QC_PITCH + lane];
+    for (int i = 0; i < 4; ++i) w[i] = at[i * QC_PITCH];
     if constexpr (PER == 2) {
       float2 f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = pair_of<T>(w[i]);
-      qc_rows[r * QC_PITCH + lane] = quantize4(make_float2(f[0].x, f[1].x), make_float2(f[2].x, f[3].x), s[0]);
-      qc_rows[(r + 1) * QC_PITCH + lane] = quantize4(make_float2(f[0].y, f[1].y), make_float2(f[2].y, f[3].y), s[PER - 1]);
+      at[(r >> 5 & 3) * QC_PITCH] = quantize4(make_float2(f[0].x, f[1].x), make_float2(f[2].x, f[3].x), s[0]);
+      at[((r >> 5) + 1 & 3) * QC_PITCH] = quantize4(make_float2(f[0].y, f[1].y), make_float2(f[2].y, f[3].y), s[PER - 1]);
     } else {
-      qc_rows[r * QC_PITCH + lane] = quantize4(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])),
-                                               make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), s[0]);
+      at[(r >> 5 & 3) * QC_PITCH] = quantize4(make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                                              make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])), s[0]);
     }
   }
   __syncthreads();
-  const bool q_words = reinterpret_cast<uintptr_t>(p.Q) % 4 == 0 && p.ldq % 4 == 0;  // r0 is a multiple of 4
+  // Q's rows in whole words wherever they start; what lies before the first and behind the last in bytes.
   for (int k = warp; k < 32 * PER; k += warps) {
     if (c0 + k >= p.cols) break;
     int8_t* q = p.Q + (c0 + k) * p.ldq + r0;
-    const uint32_t* src = qc_rows + k % PER * QC_PITCH + k / PER;
-    for (int r = 4 * lane; r < rows; r += 128) {
-      const uint32_t w = src[r * QC_PITCH];
-      if (q_words && r + 4 <= rows) {
-        *reinterpret_cast<uint32_t*>(q + r) = w;
-      } else {
-        for (int i = 0; i < 4; ++i)
-          if (r + i < rows) q[r + i] = static_cast<int8_t>(w >> (8 * i));
-      }
+    auto group = [&](int g) { return qc_rows[(4 * g + ((g >> 3) + k % PER & 3)) * QC_PITCH + k / PER]; };
+    const int head = min(rows, static_cast<int>(-reinterpret_cast<uintptr_t>(q) & 3)), n = (rows - head) >> 2;
+    for (int g = lane; g < n; g += 32) {
+      uint32_t w = group(g);
+      if (head > 0) w = __funnelshift_r(w, group(g + 1), 8 * head);
+      *reinterpret_cast<uint32_t*>(q + head + 4 * g) = w;
+    }
+    if (lane < rows - 4 * n) {
+      const int e = lane < head ? lane : lane + 4 * n;
+      q[e] = static_cast<int8_t>(group(e >> 2) >> (8 * (e & 3)));
     }
   }
   if (cs > 1) cluster_wait();  // the others have read this CTA's maxima
@@ -407,21 +416,23 @@ int quantize_columns_typed(const QuantParams& p, uint32_t* top, cudaStream_t str
   const int cs = quantize_cluster(p.rows, share);
   if (share <= QC_MAX_SHARE) {
     constexpr int PER = 4 / sizeof(T);
-    auto kern = quantize_columns_kernel<T>;
-    static std::atomic<bool> attr_set[64] = {};
+    const bool words = sizeof(T) == 4 || (reinterpret_cast<uintptr_t>(p.X) % 4 == 0 && (p.rows == 1 || p.ldx % PER == 0) && p.cols % PER == 0);
+    auto kern = quantize_columns_kernel<T, true>;
+    if constexpr (PER == 2)
+      if (!words) kern = quantize_columns_kernel<T, false>;
+    static std::atomic<bool> attr_set[64][2] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
-    if (!attr_set[dev].load(std::memory_order_relaxed)) {
+    if (!attr_set[dev][words].load(std::memory_order_relaxed)) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, QC_MAX_SHARE * QC_PITCH * 4) != cudaSuccess)
         return CUOPX_CUDA_ERROR;
-      attr_set[dev].store(true, std::memory_order_relaxed);
+      attr_set[dev][words].store(true, std::memory_order_relaxed);
     }
-    const int words = reinterpret_cast<uintptr_t>(p.X) % 4 == 0 && (p.rows == 1 || p.ldx % PER == 0) && p.cols % PER == 0;  // fp32: always
     const int64_t strips = (p.cols + 32 * PER - 1) / (32 * PER);
-    const unsigned threads = share <= 640 ? 256 : 512;
+    const unsigned threads = share <= 640 ? 512 : 1024;
     const cudaError_t err =
         launch_pdl_cluster(kern, dim3(static_cast<unsigned>(strips * cs)), dim3(threads), static_cast<size_t>(share) * QC_PITCH * 4,
-                           stream, static_cast<unsigned>(cs), p, cs, static_cast<int>(share), words);
+                           stream, static_cast<unsigned>(cs), p, cs, static_cast<int>(share));
     if (err != cudaSuccess) {
       cudaGetLastError();
       return cuda_failure(err);
