@@ -95,6 +95,17 @@ def test_quantize_into_buffers(dt, trans):
         assert (buf[:, k:] == 77).all() and scale[0] == -1 and scale[-1] == -1
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("rows, cols", [(2, 3), (6, 65), (300, 130), (2050, 70), (4099, 33)])
+def test_quantize_columns_into_odd_rows(rows, cols, dt):
+    """Q's rows at all four offsets from a word, in each CTA's share; what lies around them stays."""
+    x = torch.randn(rows, cols, generator=gen(rows + cols), device="cuda").to(dt)
+    for first, pad in ((0, 1), (1, 3), (3, 2)):
+        buf = torch.full((cols, first + rows + pad), 77, dtype=torch.int8, device="cuda")
+        check_quantize(x, True, out=buf[:, first:first + rows])
+        assert bool((buf[:, :first] == 77).all()) and bool((buf[:, first + rows:] == 77).all())
+
+
 @pytest.mark.parametrize("trans", [False, True])
 @pytest.mark.parametrize("dt", [BF, HF, F32])
 @pytest.mark.parametrize("k", [5, 64, 4100])
