@@ -267,7 +267,9 @@ __global__ void __maxnreg__(WORD ? 64 : 40) quantize_columns_kernel(const QuantP
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(map_to_rank(&top[lane], static_cast<uint32_t>(i))) : "memory");
       m = Mag::word(m, w);
     }
-    cluster_arrive_relaxed();  // has read the others'
+    // Has read the others': the release keeps the reads before the arrival, after which another CTA
+    // may leave, one without rows at once.
+    cluster_arrive();
   } else {
     __syncthreads();
     m = top[lane];
