@@ -315,6 +315,7 @@ __device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_
     there = grid_wait(ticket, static_cast<unsigned>((step + 1) * g.splits), abort, g.limit_ns);
   }
   if (!__all_sync(0xffffffffu, there)) return false;
+  __syncwarp();  // what lane 0 has acquired is ordered before the other lanes' loads; the vote orders nothing
   const int share = part / g.splits, c0 = split * share, row = m0 + lane;  // 8 columns or more
 #pragma unroll 1
   for (int c = c0; c < c0 + share; c += 8) {
@@ -630,7 +631,9 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
 
   tc_fence_before_sync();
   __syncthreads();
-  cluster_sync_relaxed();  // the partner is done with this CTA's shared memory, barriers and TMEM
+  // The partner is done with this CTA's shared memory, barriers and TMEM: its last arrivals on the
+  // leader's acc_empty, for which nobody waits, are released before it.
+  cluster_sync_all();
   if (warp == 1) {
     tc_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(ORT_TMEM_COLS) : "memory");
