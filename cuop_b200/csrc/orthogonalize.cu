@@ -1014,7 +1014,15 @@ int ortho_width(int64_t tiles128, int64_t tiles256, int64_t tiles512, int64_t pa
   return t512 < std::min(t128, t256) ? 512 : t256 <= t128 ? 256 : 128;
 }
 
-int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps, char* ws, cudaStream_t stream) {
+// The products' launch.  Everything about it that can fail before it is queued is
+// found out by prepare_ortho_pairs, which a call makes before its first kernel changes the momentum.
+struct OrthoLaunch {
+  OrthoMaps maps;
+  OrthoArgs args;
+  int pairs;
+};
+
+int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps, char* ws, OrthoLaunch& launch) {
   using L = OrthoSmem;
   auto kern = ortho_pair_kernel;
   static std::atomic<int> capacity[64] = {};
@@ -1045,7 +1053,7 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   const int64_t gram_tiles = o.words / 16;
   const int splits = gram_tiles * o.splits <= most ? o.splits : 1;
   const int width[3] = {splits > 1 ? o.gram_width : ws_sym, ws_sym, ws_upd};
-  OrthoMaps m;
+  OrthoMaps& m = launch.maps;
   bool ok = true;
   auto map_x = [&](CUtensorMap* t, const __half* x, int inner, int rows) {
     ok &= make_map(t, dt, x, xc, xr, o.batch, o.ldx, o.stride_x, inner, rows);
@@ -1068,7 +1076,8 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
     }
   }
   if (!ok) return CUOPX_CUDA_ERROR;
-  OrthoArgs a = {};
+  OrthoArgs& a = launch.args;
+  a = {};
   a.batch = static_cast<int>(o.batch);
   a.p = static_cast<int>(o.p), a.q = static_cast<int>(o.q);
   a.steps = steps;
@@ -1093,12 +1102,16 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   a.limit_ns = kWaitLimitNs + static_cast<unsigned long long>(work / 1e5);  // at 100 TFLOP/s
   for (int i = 0; i < steps; ++i)
     for (int j = 0; j < 3; ++j) a.alpha[i][j] = sched.alpha[i][j], a.beta[i][j] = sched.beta[i][j];
+  launch.pairs = std::min(static_cast<int>(most), std::max({a.tiles[kGram], a.tiles[kPoly], a.tiles[kUpdate]}));
+  return CUOPX_SUCCESS;
+}
+
+int launch_ortho_pairs(const OrthoLaunch& launch, cudaStream_t stream) {
   // Cooperative: all CTAs run at once, whatever else the GPU does.
   cudaLaunchConfig_t cfg = {};
-  const int pairs = std::min(static_cast<int>(most), std::max({a.tiles[kGram], a.tiles[kPoly], a.tiles[kUpdate]}));
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * launch.pairs));
   cfg.blockDim = dim3(ORT_THREADS);
-  cfg.dynamicSmemBytes = L::ALLOC;
+  cfg.dynamicSmemBytes = OrthoSmem::ALLOC;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1109,7 +1122,7 @@ int launch_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps
   attr[1].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, m, a); err != cudaSuccess) {
+  if (const cudaError_t err = cudaLaunchKernelEx(&cfg, ortho_pair_kernel, launch.maps, launch.args); err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
@@ -1130,6 +1143,10 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   OrthoSchedule sched;
   if (!ortho_schedule(coefficients, steps, sched)) return CUOPX_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
+  OrthoLaunch products;
+  if (steps > 0) {
+    if (const int rc = prepare_ortho_pairs(o, sched, steps, ws, products); rc != CUOPX_SUCCESS) return rc;
+  }
   io.groups = o.groups, io.across = o.across, io.blocks = o.blocks, io.words = o.words;
   io.partial = reinterpret_cast<double*>(ws + o.partial_off);
   io.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
@@ -1140,26 +1157,27 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   const dim3 grid(static_cast<unsigned>(o.blocks), static_cast<unsigned>(o.batch));
   const bool momentum = io.m.dtype >= 0;
   cudaError_t err = launch_pdl(momentum ? ortho_sum_kernel<true> : ortho_sum_kernel<false>, grid, dim3(256), 0, stream, io);
-  note_launch("ortho_sum");
-  if (err == cudaSuccess)
+  if (err == cudaSuccess) {
+    note_launch("ortho_sum");
     err = launch_pdl(momentum ? ortho_scale_kernel<true> : ortho_scale_kernel<false>, grid, dim3(256), 0, stream, io);
-  note_launch("ortho_scale");
+  }
+  if (err == cudaSuccess) note_launch("ortho_scale");
   if (err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
   if (steps > 0) {
-    if (const int rc = launch_ortho_pairs(o, sched, steps, ws, stream); rc != CUOPX_SUCCESS) return rc;
+    if (const int rc = launch_ortho_pairs(products, stream); rc != CUOPX_SUCCESS) return rc;
   }
   io.hi = reinterpret_cast<__half*>(ws + o.hi_off[steps & 1]);
   io.out = static_cast<float>(out_factor / sched.last);
   io.step = static_cast<float>(out_factor / sched.last);
   err = launch_pdl(update ? ortho_out_kernel<true> : ortho_out_kernel<false>, grid, dim3(256), 0, stream, io);
-  note_launch(update ? "ortho_step" : "ortho_out");
   if (err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
+  note_launch(update ? "ortho_step" : "ortho_out");
   return check_launch();
 }
 

@@ -578,6 +578,9 @@ typedef struct cuopx_muon_args {
  * One step of Muon (K. Jordan, 2024): momentum = mu momentum + G,
  * U = G + mu momentum with nesterov, else momentum (as stored), O = U
  * orthogonalised, W = (1 - lr decay) W - lr scale O; each matrix rounded once.
+ * Momentum is written by the first of several launches: a call that is refused, or
+ * whose products cannot be set up on the device, launches nothing and leaves
+ * both as they were.
  */
 int cuopx_muon_step(const cuopx_muon_args* args, void* stream);
 
