@@ -32,25 +32,31 @@ _empty = torch.empty
 
 
 @lru_cache(maxsize=64)
-def _coefficients(triples, steps: int):
-    """(a, b, c) of each step as C doubles."""
-    flat = [float(v) for t in triples for v in t]
+def _coefficients(triples):
+    """(a, b, c) of each step as C doubles; triples holds plain floats, so that equal keys are equal numbers."""
+    flat = [v for t in triples for v in t]
     return (C.c_double * max(1, len(flat)))(*flat)
+
+
+def _triple(t):
+    a, b, c = t
+    return float(a), float(b), float(c)
 
 
 def _schedule(coefficients, steps: int, what: str):
     if steps < 0:
         _error(N.INVALID_ARGUMENT, f"{what}: {steps} steps")
+    triples = None
     try:
-        if len(coefficients) and isinstance(coefficients[0], (int, float)):
-            triples = (tuple(coefficients),) * steps
-        else:
-            triples = tuple(tuple(t) for t in coefficients)
-    except (TypeError, IndexError):
-        triples = None
-    if triples is None or len(triples) != steps or any(len(t) != 3 for t in triples):
+        try:
+            triples = (_triple(coefficients),) * steps  # one for all steps
+        except (TypeError, ValueError, RuntimeError):
+            triples = tuple(_triple(t) for t in coefficients)
+    except (TypeError, ValueError, RuntimeError):
+        pass
+    if triples is None or len(triples) != steps:
         _error(N.INVALID_ARGUMENT, f"{what}: coefficients must be (a, b, c), or {steps} of them for {steps} steps")
-    return _coefficients(triples, steps)
+    return _coefficients(triples)
 
 
 def _stack(t: torch.Tensor, shape, device: int, what: str):
