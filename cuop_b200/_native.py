@@ -105,6 +105,7 @@ SIGNATURES = [
     ("cuopx_int8_gated_linear_workspace_size", _sz, [_vp]),
     ("cuopx_int8_gated_linear", _int, [_vp, _vp]),
     ("cuopx_orthogonalize_workspace_size", _sz, [_i64, _i64, _i64]),
+    ("cuopx_orthogonalize_workspace_size_bits", _sz, [_i64, _i64, _i64, _int]),
     ("cuopx_orthogonalize", _int, [_vp, _vp]),
     ("cuopx_muon_step", _int, [_vp, _vp]),
 ]

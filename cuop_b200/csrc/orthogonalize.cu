@@ -17,6 +17,12 @@
 // both, and errors of 2e-4 (few large directions) to 1.6e-3 (equal ones) remain.  Every matrix
 // is stored times a power of two that its bound allows (2^15 / bound): the
 // elements of A are far below fp16's normal range otherwise.
+// That is with operands of 11 bits, for results of 16 bits and optimiser steps.  With 22 (FULL),
+// for fp32 results, A and P are kept as hi + lo too, and every product is hi lo + lo hi + hi hi, one
+// after the other along a depth three times as long; lo lo is 2^-24 of the sum.  What
+// remains is the tensor cores' fp32 sums, 5e-6 (64 x 3000) to 6e-5 (4096 x 10240) of the result, growing
+// with the depth.  Whole calls in fp32, us with 11 / 22 bits: 1024 x 1024 191 / 315, 5001 x 1777 504 / 1082,
+// 4096 x 10240 2558 / 7742.
 //
 // One persistent launch does all products: tiles of 256 x 256 or 256 x 128 on CTA
 // pairs (tcgen05 cta_group::2), tile i of a phase on pair i mod the number of pairs,
@@ -74,9 +80,10 @@ struct OrthoSmem {
 // The three phases of a step: A = X X^T, the polynomial P = bA + cAA, X <- aX + PX.
 enum OrthoPhase { kGram = 0, kPoly = 1, kUpdate = 2 };
 
+template <bool FULL>
 struct OrthoMaps {
-  // Operands: [phase], for the two buffers that X alternates between.
-  CUtensorMap a[3][2], b[3][2];
+  // Operands: hi, and with FULL lo; [phase], for the two buffers that X alternates between.
+  CUtensorMap a[FULL ? 2 : 1][3][2], b[FULL ? 2 : 1][3][2];
 };
 
 struct OrthoArgs {
@@ -84,16 +91,18 @@ struct OrthoArgs {
   bool tall;
   int width[3];     // columns of a phase's tiles: 128, 256 or 512
   int tiles[3];     // of a phase, all batches
-  int k_blocks[3];
+  int k_blocks[3];  // of one product
   int tiles_m, tiles_n;  // of the update, one batch
   int sym_tiles[2];      // of the other two, one batch
   int splits;            // pairs that share a tile of kGram: 1, or 2 to 8 with a tile for every pair at most
   float* partial;        // their sums: [tile][pair of these][warp][column][32 rows]
   unsigned* tickets;     // [tile][warp]: pairs that have stored theirs
   __half* x[2];
-  __half* lo;
+  __half* lo[2];  // the same buffer twice where no product reads it
   __half* gram;
   __half* poly;
+  __half* gram_lo;  // FULL
+  __half* poly_lo;
   int64_t ldx, stride_x, ldp, stride_p;  // elements
   unsigned* barrier;
   // Of any wait: a second, and ten times what the largest phase takes, since a pair
@@ -168,21 +177,21 @@ __device__ __forceinline__ void ortho_tile(const OrthoArgs& g, int phase, int t,
 }
 
 // One warp's 32 rows of `part` columns of a tile, in chunks of 64 columns.
-// UPDATE: hi and lo of X in (r0, r1), hi and lo out (o0, o1).  Else the sums, plus
-// beta * r0 where beta is not 0, to o0, and transposed below the diagonal block
-// of rows `diag`.. (what lies above it belongs to other tiles).
+// The sums, plus beta times (r0, r1) where beta is not 0, to (o0, o1): hi and lo with TWO, else
+// r0 and o0 alone.  SYM: also transposed below the diagonal block of rows `diag`.. (what
+// lies above it belongs to other tiles).
 //
 // Rows pass through shared memory (128-byte swizzle), so that global accesses are whole
 // 128-byte lines, eight lanes to a row; what the next chunk adds is on its way meanwhile.  Plain
 // stores: the fence before a TMA store waited for those loads (1.6 us a chunk).
-template <bool UPDATE, typename Wait, typename Release>
+template <bool TWO, bool SYM, typename Wait, typename Release>
 __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0, int m0, int M, int N, float alpha, float beta,
                                                const __half* r0, const __half* r1, __half* o0, __half* o1, int64_t ld, int diag,
                                                unsigned char* stage, int lane, Wait&& wait, Release&& release) {
   constexpr int BUF = 4096;
   const int sub = lane & 7, line = lane >> 3;
-  const bool adds = UPDATE || beta != 0.f;
-  uint4 next0[8], next1[UPDATE ? 8 : 1];
+  const bool adds = !SYM || beta != 0.f;
+  uint4 next0[8], next1[TWO ? 8 : 1];
   auto fetch = [&](int col) {
     col += 8 * sub;
 #pragma unroll
@@ -190,7 +199,7 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
       const int row = m0 + 4 * i + line;
       const bool in = adds && row < M && col < N;
       next0[i] = in ? __ldcg(reinterpret_cast<const uint4*>(r0 + row * ld + col)) : make_uint4(0, 0, 0, 0);
-      if constexpr (UPDATE) next1[i] = in ? __ldcg(reinterpret_cast<const uint4*>(r1 + row * ld + col)) : make_uint4(0, 0, 0, 0);
+      if constexpr (TWO) next1[i] = in ? __ldcg(reinterpret_cast<const uint4*>(r1 + row * ld + col)) : make_uint4(0, 0, 0, 0);
     }
   };
   fetch(n0);
@@ -201,11 +210,11 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
     for (int i = 0; i < 8; ++i) {
       const int row = 4 * i + line, at = row * 128 + ((sub ^ (row & 7)) << 4);
       *reinterpret_cast<uint4*>(stage + at) = next0[i];
-      if constexpr (UPDATE) *reinterpret_cast<uint4*>(stage + BUF + at) = next1[i];
+      if constexpr (TWO) *reinterpret_cast<uint4*>(stage + BUF + at) = next1[i];
     }
     __syncwarp();
     if (c + 64 < part) fetch(n0 + c + 64);
-    const bool mirror = !UPDATE && n0 + c < diag;
+    const bool mirror = SYM && n0 + c < diag;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t acc[32];
@@ -217,26 +226,26 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
       for (int j = 0; j < 4; ++j) {
         unsigned char* at = stage + lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4);
         uint4 w0 = *reinterpret_cast<const uint4*>(at), w1 = make_uint4(0, 0, 0, 0);
-        if constexpr (UPDATE) w1 = *reinterpret_cast<const uint4*>(at + BUF);
+        if constexpr (TWO) w1 = *reinterpret_cast<const uint4*>(at + BUF);
         uint32_t* a0 = &w0.x;
         uint32_t* a1 = &w1.x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float2 add = unpack2_layer<__half>(a0[i]);
-          if constexpr (UPDATE) add = add2(add, unpack2_layer<__half>(a1[i]));
+          if constexpr (TWO) add = add2(add, unpack2_layer<__half>(a1[i]));
           const float2 s = make_float2(__uint_as_float(acc[8 * j + 2 * i]), __uint_as_float(acc[8 * j + 2 * i + 1]));
           const float2 r = fma2(both(alpha), s, mul2(both(beta), add));
           a0[i] = pack2_layer<__half>(r.x, r.y);
-          if constexpr (UPDATE) {
+          if constexpr (TWO) {
             const float2 hi = unpack2_layer<__half>(a0[i]);
             a1[i] = pack2_layer<__half>(r.x - hi.x, r.y - hi.y);
           }
           v[8 * j + 2 * i] = r.x, v[8 * j + 2 * i + 1] = r.y;
         }
         *reinterpret_cast<uint4*>(at) = w0;
-        if constexpr (UPDATE) *reinterpret_cast<uint4*>(at + BUF) = w1;
+        if constexpr (TWO) *reinterpret_cast<uint4*>(at + BUF) = w1;
       }
-      if (mirror) {
+      if (!TWO && mirror) {
         // Row 32 h + i of the transposed chunk holds column i of this one, an
         // element per lane; lanes trade elements so that each stores two at once.
 #pragma unroll
@@ -249,14 +258,14 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
       }
     }
     __syncwarp();
-    if (UPDATE || n0 + c < diag + 256) {
+    if (!SYM || n0 + c < diag + 256) {
       const int col = n0 + c + 8 * sub;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + line, row = m0 + r, at = r * 128 + ((sub ^ (r & 7)) << 4);
         if (row < M && col < N) {
           *reinterpret_cast<uint4*>(o0 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + at);
-          if constexpr (UPDATE) *reinterpret_cast<uint4*>(o1 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + BUF + at);
+          if constexpr (TWO) *reinterpret_cast<uint4*>(o1 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + BUF + at);
         }
       }
     }
@@ -265,8 +274,26 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = 8 * i + (lane >> 2), row = n0 + c + r;
-        if (row < M && col < N)
+        if constexpr (TWO) {
+          // Both buffers hold rows: eight of them give an element each.
+          uint32_t w0[4], w1[4];
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            auto two = [&](const unsigned char* buf) {
+              const unsigned char* at = buf + (8 * (lane & 3) + j) * 128 + 2 * (r & 7);
+              return static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(at + (((r >> 3) ^ j) << 4))) |
+                     static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(at + 128 + (((r >> 3) ^ (j + 1)) << 4))) << 16;
+            };
+            w0[j / 2] = two(stage);
+            w1[j / 2] = two(stage + BUF);
+          }
+          if (row < M && col < N) {
+            *reinterpret_cast<uint4*>(o0 + row * ld + col) = make_uint4(w0[0], w0[1], w0[2], w0[3]);
+            *reinterpret_cast<uint4*>(o1 + row * ld + col) = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+          }
+        } else if (row < M && col < N) {
           *reinterpret_cast<uint4*>(o0 + row * ld + col) = *reinterpret_cast<const uint4*>(stage + BUF + r * 64 + 16 * (lane & 3));
+        }
       }
     }
     __syncwarp();
@@ -274,10 +301,12 @@ __device__ __forceinline__ bool ortho_epilogue(uint32_t t_row, int part, int n0,
   return true;
 }
 
-// K blocks of unit t of a phase, and the tile that it works on.
+// K blocks of unit t of a phase, and the tile that it works on.  FULL: those of the
+// three products, small ones first.
+template <bool FULL>
 __device__ __forceinline__ int ortho_unit(const OrthoArgs& g, int kind, int t, int& kb0, int& kb1) {
   kb0 = 0;
-  kb1 = g.k_blocks[kind];
+  kb1 = (FULL ? 3 : 1) * g.k_blocks[kind];
   if (kind != kGram || g.splits == 1) return t;
   const int tile = t / g.splits, s = t - tile * g.splits, all = kb1;
   kb0 = all * s / g.splits;
@@ -290,9 +319,9 @@ __device__ __forceinline__ int ortho_unit(const OrthoArgs& g, int kind, int t, i
 // pairs have stored theirs, each adds up a share of the columns, in the
 // pairs' order, so that results do not depend on timing.  They run at once (there is a pair for every
 // unit), so the wait ends.  A phase of 256 x 16384 65 -> 21 us.
-template <typename Wait, typename Release>
+template <bool FULL, typename Wait, typename Release>
 __device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_t t_row, int part, int n0, int m0, float alpha, int tile,
-                                                     int split, int step, int where, __half* out, int diag, int lane,
+                                                     int split, int step, int where, __half* out, __half* out_lo, int diag, int lane,
                                                      volatile int* abort, Wait&& wait, Release&& release) {
   const int64_t region = 32ll * part, stride = region * 16;  // of a warp, of a pair
   float* base = g.partial + static_cast<int64_t>(tile) * g.splits * stride + where * region + lane;
@@ -323,23 +352,33 @@ __device__ __forceinline__ bool ortho_split_epilogue(const OrthoArgs& g, uint32_
     for (int s = 0; s < g.splits; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += __ldcg(base + s * stride + (c + i) * 32);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack2_layer<__half>(alpha * v[2 * i], alpha * v[2 * i + 1]);
     const int col = n0 + c;
     if (col >= g.p || col >= diag + 256 || row >= g.p) continue;
-    *reinterpret_cast<uint4*>(out + row * g.ldp + col) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (col < diag) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < g.p) out[(col + i) * g.ldp + row] = __ushort_as_half(static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1))));
+    for (int part = 0; part < (FULL ? 2 : 1); ++part) {
+      __half* o = part ? out_lo : out;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (part == 0) v[2 * i] *= alpha, v[2 * i + 1] *= alpha;
+        w[i] = pack2_layer<__half>(v[2 * i], v[2 * i + 1]);
+        const float2 hi = unpack2_layer<__half>(w[i]);
+        v[2 * i] -= hi.x, v[2 * i + 1] -= hi.y;
+      }
+      *reinterpret_cast<uint4*>(o + row * g.ldp + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (col < diag) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < g.p) o[(col + i) * g.ldp + row] = __ushort_as_half(static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1))));
+      }
     }
   }
   return true;
 }
 
+template <bool FULL>
 __global__ void __launch_bounds__(ORT_THREADS, 1)
-    ortho_pair_kernel(const __grid_constant__ OrthoMaps maps, const __grid_constant__ OrthoArgs g) {
+    ortho_pair_kernel(const __grid_constant__ OrthoMaps<FULL> maps, const __grid_constant__ OrthoArgs g) {
   using L = OrthoSmem;
   constexpr int STAGES = L::STAGES, SLOTS = ORT_SLOTS;
 
@@ -396,7 +435,8 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
     for (int ph = 0; ok && ph < phases; ++ph) {
       const int kind = ph % 3, cur = (ph / 3) & 1;
       const bool mn = kind == kGram ? g.tall : kind == kUpdate && !g.tall && !of_a;
-      const CUtensorMap* map = of_a ? &maps.a[kind][cur] : &maps.b[kind][cur];
+      const CUtensorMap* const hi_map = of_a ? &maps.a[0][kind][cur] : &maps.b[0][kind][cur];
+      const CUtensorMap* const lo_map = of_a ? &maps.a[FULL][kind][cur] : &maps.b[FULL][kind][cur];
       const int width = g.width[kind], pieces = !of_a && width == 512 ? 2 : 1;
       const int span = of_a ? ORT_BM : min(width, 256) / 2;  // rows or columns of the operand for one MMA
       const int stages = width == 512 ? L::WIDE_STAGES : L::STAGES, stride = (width == 512 ? 3 : 2) * L::OPERAND;
@@ -404,7 +444,10 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       unsigned char* const ring = smem + (of_a ? 0 : L::OPERAND);
       int stage = 0;
       ready = false;
-      if (elect_one_sync()) prefetch_tmap(map);
+      if (elect_one_sync()) {
+        prefetch_tmap(hi_map);
+        if (FULL) prefetch_tmap(lo_map);
+      }
       // The first phase reads what the kernel before has written.
       if (ph > 0) {
         if (!__all_sync(0xffffffffu, lane != 0 || grid_wait(g.barrier, static_cast<unsigned>(ph) * gridDim.x, abort_flag, g.limit_ns))) {
@@ -416,7 +459,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
         int b, m, n, kb0, kb1;
-        ortho_tile(g, kind, ortho_unit(g, kind, t, kb0, kb1), b, m, n);
+        ortho_tile(g, kind, ortho_unit<FULL>(g, kind, t, kb0, kb1), b, m, n);
         const int first = (of_a ? m : n) + static_cast<int>(rank) * span;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!warp_wait(ready, &empty[stage], ((bits >> stage) & 1u) ^ 1u, kDevErrWaitTimeoutEmpty, abort_flag, g.limit_ns)) {
@@ -427,7 +470,9 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
             if (leader) mbar_arrive_expect_tx(&full[stage], 2 * bytes);
             const uint32_t mbar = map_to_rank(&full[stage], 0);
             unsigned char* dst = ring + stage * stride;
-            const int k0 = kb * ORT_BK;
+            const int each = g.k_blocks[kind], product = !FULL ? 2 : kb >= 2 * each ? 2 : kb >= each ? 1 : 0;
+            const CUtensorMap* const map = product == (of_a ? 1 : 0) ? lo_map : hi_map;  // hi lo, lo hi, hi hi
+            const int k0 = (FULL ? kb - product * each : kb) * ORT_BK;
             for (int h = 0; h < pieces; ++h) {
               const int at = first + 256 * h;
               if (mn) {
@@ -500,7 +545,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           }
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(slot * 256);
           int kb0, kb1;
-          ortho_unit(g, kind, t, kb0, kb1);
+          ortho_unit<FULL>(g, kind, t, kb0, kb1);
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!warp_wait(ready, &full[stage], (bits >> stage) & 1u, kDevErrWaitTimeoutFull, abort_flag, g.limit_ns)) {
               ok = false;
@@ -576,7 +621,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
       }
       for (int t = pair; ok && t < g.tiles[kind]; t += pairs) {
         int b, m, n, kb0, kb1;
-        const int tile = ortho_unit(g, kind, t, kb0, kb1);
+        const int tile = ortho_unit<FULL>(g, kind, t, kb0, kb1);
         ortho_tile(g, kind, tile, b, m, n);
         const int m0 = m + static_cast<int>(rank) * ORT_BM + 32 * quarter;
         for (int h = 0; ok && h < (width == 512 ? 2 : 1); ++h) {
@@ -599,17 +644,19 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           };
           if (kind == kUpdate) {
             const int64_t off = b * g.stride_x;
-            ok = ortho_epilogue<true>(t_row, part, n0, m0, g.tall ? g.q : g.p, g.tall ? g.p : g.q, alpha, beta, g.x[cur] + off,
-                                      g.lo + off, g.x[cur ^ 1] + off, g.lo + off, g.ldx, 0, stage, lane, wait, release);
+            ok = ortho_epilogue<true, false>(t_row, part, n0, m0, g.tall ? g.q : g.p, g.tall ? g.p : g.q, alpha, beta,
+                                             g.x[cur] + off, g.lo[FULL ? cur : 0] + off, g.x[cur ^ 1] + off,
+                                             g.lo[FULL ? cur ^ 1 : 0] + off, g.ldx, 0, stage, lane, wait, release);
           } else if (kind == kGram && g.splits > 1) {
-            ok = ortho_split_epilogue(g, t_row, part, n0, m0, alpha, tile, t - tile * g.splits, step,
-                                      static_cast<int>(rank) * ORT_EPI_WARPS + warp - 2, g.gram + b * g.stride_p, m, lane, abort_flag,
-                                      wait, release);
+            ok = ortho_split_epilogue<FULL>(g, t_row, part, n0, m0, alpha, tile, t - tile * g.splits, step,
+                                      static_cast<int>(rank) * ORT_EPI_WARPS + warp - 2, g.gram + b * g.stride_p,
+                                      g.gram_lo + b * g.stride_p, m, lane, abort_flag, wait, release);
           } else {
-            __half* gram = g.gram + b * g.stride_p;
-            __half* out = kind == kPoly ? g.poly + b * g.stride_p : gram;
-            ok = ortho_epilogue<false>(t_row, part, n0, m0, g.p, g.p, alpha, kind == kPoly ? beta : 0.f, gram, gram, out, out,
-                                       g.ldp, m, stage, lane, wait, release);
+            const int64_t off = b * g.stride_p;
+            __half* out = (kind == kPoly ? g.poly : g.gram) + off;
+            __half* out_lo = (kind == kPoly ? g.poly_lo : g.gram_lo) + off;
+            ok = ortho_epilogue<FULL, true>(t_row, part, n0, m0, g.p, g.p, alpha, kind == kPoly ? beta : 0.f, g.gram + off,
+                                            g.gram_lo + off, out, out_lo, g.ldp, m, stage, lane, wait, release);
           }
         }
         if (!ok) break;
@@ -952,7 +999,8 @@ struct OrthoPlan {
   int blocks, groups, across;
   int gram_width, splits;  // of the first phase's tiles where pairs share them (splits > 1)
   int words;
-  size_t sums_off, barrier_off, partial_off, hi_off[2], lo_off, gram_off, poly_off, bytes;
+  bool full;  // products of hi and lo
+  size_t sums_off, barrier_off, partial_off, hi_off[2], lo_off[2], gram_off[2], poly_off[2], bytes;
 };
 
 // Tiles of a symmetric matrix of `rows` row tiles: those whose first column is at most their last row.
@@ -969,8 +1017,9 @@ int ortho_splits(int64_t tiles, int64_t k_blocks, int64_t pairs) {
   return k_blocks - k_blocks / s >= 24 ? s : 1;
 }
 
-OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
+OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols, bool full) {
   OrthoPlan o = {};
+  o.full = full;
   if (batch <= 0 || rows <= 0 || cols <= 0) return o;
   o.batch = batch;
   o.tall = rows > cols;
@@ -991,15 +1040,18 @@ OrthoPlan ortho_plan(int64_t batch, int64_t rows, int64_t cols) {
   const int64_t tiles = (o.p + 255) / 256;
   o.gram_width = o.p <= 128 ? 128 : 256;
   const int64_t gram_tiles = o.p <= 128 ? batch : batch * ortho_sym_tiles(tiles, 256);
-  o.splits = ortho_splits(gram_tiles, (o.q + ORT_BK - 1) / ORT_BK, device_sm_count() / 2);
+  o.splits = ortho_splits(gram_tiles, (full ? 3 : 1) * ((o.q + ORT_BK - 1) / ORT_BK), device_sm_count() / 2);
   o.words = 1 + (o.splits > 1 ? static_cast<int>(gram_tiles) * 16 : 0);
   o.sums_off = take(o.splits > 1 ? static_cast<size_t>(gram_tiles) * o.splits * 256 * o.gram_width * 4 : 0);
   o.barrier_off = take(static_cast<size_t>(o.words) * 4);
   o.partial_off = take(static_cast<size_t>(batch) * o.blocks * 8);
   for (int i = 0; i < 2; ++i) o.hi_off[i] = take(static_cast<size_t>(batch) * o.stride_x * 2);
-  o.lo_off = take(static_cast<size_t>(batch) * o.stride_x * 2);
-  o.gram_off = take(static_cast<size_t>(batch) * o.stride_p * 2);
-  o.poly_off = take(static_cast<size_t>(batch) * o.stride_p * 2);
+  // Where products read lo it alternates as hi does; else a tile's owner alone reads and writes it.
+  for (int i = 0; i < 2; ++i) o.lo_off[i] = i == 0 || full ? take(static_cast<size_t>(batch) * o.stride_x * 2) : o.lo_off[0];
+  for (int i = 0; i < 2; ++i) {
+    o.gram_off[i] = i == 0 || full ? take(static_cast<size_t>(batch) * o.stride_p * 2) : o.gram_off[0];
+    o.poly_off[i] = i == 0 || full ? take(static_cast<size_t>(batch) * o.stride_p * 2) : o.poly_off[0];
+  }
   o.bytes = off;
   return o;
 }
@@ -1016,15 +1068,17 @@ int ortho_width(int64_t tiles128, int64_t tiles256, int64_t tiles512, int64_t pa
 
 // The products' launch.  Everything about it that can fail before it is queued is
 // found out by prepare_ortho_pairs, which a call makes before its first kernel changes the momentum.
+template <bool FULL>
 struct OrthoLaunch {
-  OrthoMaps maps;
+  OrthoMaps<FULL> maps;
   OrthoArgs args;
   int pairs;
 };
 
-int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps, char* ws, OrthoLaunch& launch) {
+template <bool FULL>
+int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int steps, char* ws, OrthoLaunch<FULL>& launch) {
   using L = OrthoSmem;
-  auto kern = ortho_pair_kernel;
+  auto kern = ortho_pair_kernel<FULL>;
   static std::atomic<int> capacity[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CUOPX_CUDA_ERROR;
@@ -1036,10 +1090,7 @@ int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int step
     capacity[dev].store(n, std::memory_order_release);
   }
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  __half* hi[2] = {reinterpret_cast<__half*>(ws + o.hi_off[0]), reinterpret_cast<__half*>(ws + o.hi_off[1])};
-  __half* lo = reinterpret_cast<__half*>(ws + o.lo_off);
-  __half* gram = reinterpret_cast<__half*>(ws + o.gram_off);
-  __half* poly = reinterpret_cast<__half*>(ws + o.poly_off);
+  auto half_at = [&](size_t off) { return reinterpret_cast<__half*>(ws + off); };
   const int64_t xr = o.tall ? o.q : o.p, xc = o.tall ? o.p : o.q;  // X as stored
   const int64_t most = capacity[dev].load(std::memory_order_relaxed);  // pairs at once
   const int64_t rows = (o.p + 255) / 256, tiles_m = (xr + 255) / 256;
@@ -1053,7 +1104,7 @@ int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int step
   const int64_t gram_tiles = o.words / 16;
   const int splits = gram_tiles * o.splits <= most ? o.splits : 1;
   const int width[3] = {splits > 1 ? o.gram_width : ws_sym, ws_sym, ws_upd};
-  OrthoMaps& m = launch.maps;
+  OrthoMaps<FULL>& m = launch.maps;
   bool ok = true;
   auto map_x = [&](CUtensorMap* t, const __half* x, int inner, int rows) {
     ok &= make_map(t, dt, x, xc, xr, o.batch, o.ldx, o.stride_x, inner, rows);
@@ -1061,18 +1112,23 @@ int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int step
   auto map_p = [&](CUtensorMap* t, const __half* x, int inner, int rows) {
     ok &= make_map(t, dt, x, o.p, o.p, o.batch, o.ldp, o.stride_p, inner, rows);
   };
-  for (int i = 0; i < 2; ++i) {
-    // K-major operands come in boxes of 64 x rows, MN-major ones in 64 x 64.
-    map_x(&m.a[kGram][i], hi[i], 64, o.tall ? ORT_BK : ORT_BM);
-    map_x(&m.b[kGram][i], hi[i], 64, o.tall ? ORT_BK : std::min(width[kGram], 256) / 2);
-    map_p(&m.a[kPoly][i], gram, 64, ORT_BM);
-    map_p(&m.b[kPoly][i], gram, 64, std::min(width[kPoly], 256) / 2);
-    if (o.tall) {
-      map_x(&m.a[kUpdate][i], hi[i], 64, ORT_BM);
-      map_p(&m.b[kUpdate][i], poly, 64, std::min(width[kUpdate], 256) / 2);
-    } else {
-      map_p(&m.a[kUpdate][i], poly, 64, ORT_BM);
-      map_x(&m.b[kUpdate][i], hi[i], 64, ORT_BK);
+  for (int l = 0; l < (FULL ? 2 : 1); ++l) {  // hi, lo
+    const __half* gram = half_at(o.gram_off[l]);
+    const __half* poly = half_at(o.poly_off[l]);
+    for (int i = 0; i < 2; ++i) {
+      const __half* x = half_at(l ? o.lo_off[i] : o.hi_off[i]);
+      // K-major operands come in boxes of 64 x rows, MN-major ones in 64 x 64.
+      map_x(&m.a[l][kGram][i], x, 64, o.tall ? ORT_BK : ORT_BM);
+      map_x(&m.b[l][kGram][i], x, 64, o.tall ? ORT_BK : std::min(width[kGram], 256) / 2);
+      map_p(&m.a[l][kPoly][i], gram, 64, ORT_BM);
+      map_p(&m.b[l][kPoly][i], gram, 64, std::min(width[kPoly], 256) / 2);
+      if (o.tall) {
+        map_x(&m.a[l][kUpdate][i], x, 64, ORT_BM);
+        map_p(&m.b[l][kUpdate][i], poly, 64, std::min(width[kUpdate], 256) / 2);
+      } else {
+        map_p(&m.a[l][kUpdate][i], poly, 64, ORT_BM);
+        map_x(&m.b[l][kUpdate][i], x, 64, ORT_BK);
+      }
     }
   }
   if (!ok) return CUOPX_CUDA_ERROR;
@@ -1095,10 +1151,12 @@ int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int step
   a.tiles[kUpdate] = a.batch * a.tiles_m * a.tiles_n;
   a.k_blocks[kGram] = static_cast<int>((o.q + ORT_BK - 1) / ORT_BK);
   a.k_blocks[kPoly] = a.k_blocks[kUpdate] = static_cast<int>((o.p + ORT_BK - 1) / ORT_BK);
-  a.x[0] = hi[0], a.x[1] = hi[1], a.lo = lo, a.gram = gram, a.poly = poly;
+  for (int i = 0; i < 2; ++i) a.x[i] = half_at(o.hi_off[i]), a.lo[i] = half_at(o.lo_off[i]);
+  a.gram = half_at(o.gram_off[0]), a.gram_lo = half_at(o.gram_off[1]);
+  a.poly = half_at(o.poly_off[0]), a.poly_lo = half_at(o.poly_off[1]);
   a.ldx = o.ldx, a.stride_x = o.stride_x, a.ldp = o.ldp, a.stride_p = o.stride_p;
   a.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
-  const double work = 2.0 * static_cast<double>(o.batch) * static_cast<double>(o.p) * static_cast<double>(o.p) * static_cast<double>(o.q);
+  const double work = (FULL ? 6.0 : 2.0) * static_cast<double>(o.batch) * static_cast<double>(o.p) * static_cast<double>(o.p) * static_cast<double>(o.q);
   a.limit_ns = kWaitLimitNs + static_cast<unsigned long long>(work / 1e5);  // at 100 TFLOP/s
   for (int i = 0; i < steps; ++i)
     for (int j = 0; j < 3; ++j) a.alpha[i][j] = sched.alpha[i][j], a.beta[i][j] = sched.beta[i][j];
@@ -1106,7 +1164,8 @@ int prepare_ortho_pairs(const OrthoPlan& o, const OrthoSchedule& sched, int step
   return CUOPX_SUCCESS;
 }
 
-int launch_ortho_pairs(const OrthoLaunch& launch, cudaStream_t stream) {
+template <bool FULL>
+int launch_ortho_pairs(const OrthoLaunch<FULL>& launch, cudaStream_t stream) {
   // Cooperative: all CTAs run at once, whatever else the GPU does.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * launch.pairs));
@@ -1122,11 +1181,11 @@ int launch_ortho_pairs(const OrthoLaunch& launch, cudaStream_t stream) {
   attr[1].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (const cudaError_t err = cudaLaunchKernelEx(&cfg, ortho_pair_kernel, launch.maps, launch.args); err != cudaSuccess) {
+  if (const cudaError_t err = cudaLaunchKernelEx(&cfg, ortho_pair_kernel<FULL>, launch.maps, launch.args); err != cudaSuccess) {
     cudaGetLastError();
     return cuda_failure(err);
   }
-  note_launch("ortho_pair");
+  note_launch(FULL ? "ortho_pair_full" : "ortho_pair");
   return check_launch();
 }
 
@@ -1138,12 +1197,13 @@ OrthoTensor ortho_tensor(const void* p, int dtype, int64_t ld, int64_t stride, i
 }
 
 // All launches of a call.  `io` has the tensors and what the last pass does.
-int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int steps, bool update, double out_factor, void* workspace,
+template <bool FULL>
+int ortho_run_as(OrthoIo io, const OrthoPlan& o, const double* coefficients, int steps, bool update, double out_factor, void* workspace,
               cudaStream_t stream) {
   OrthoSchedule sched;
   if (!ortho_schedule(coefficients, steps, sched)) return CUOPX_INVALID_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
-  OrthoLaunch products;
+  OrthoLaunch<FULL> products;
   if (steps > 0) {
     if (const int rc = prepare_ortho_pairs(o, sched, steps, ws, products); rc != CUOPX_SUCCESS) return rc;
   }
@@ -1152,7 +1212,7 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   io.barrier = reinterpret_cast<unsigned*>(ws + o.barrier_off);
   io.x_scale = static_cast<float>(sched.first);
   io.ldx = o.ldx, io.stride_x = o.stride_x;
-  io.lo = reinterpret_cast<__half*>(ws + o.lo_off);
+  io.lo = reinterpret_cast<__half*>(ws + o.lo_off[0]);
   io.hi = reinterpret_cast<__half*>(ws + o.hi_off[0]);
   const dim3 grid(static_cast<unsigned>(o.blocks), static_cast<unsigned>(o.batch));
   const bool momentum = io.m.dtype >= 0;
@@ -1170,6 +1230,7 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
     if (const int rc = launch_ortho_pairs(products, stream); rc != CUOPX_SUCCESS) return rc;
   }
   io.hi = reinterpret_cast<__half*>(ws + o.hi_off[steps & 1]);
+  io.lo = reinterpret_cast<__half*>(ws + o.lo_off[steps & 1]);
   io.out = static_cast<float>(out_factor / sched.last);
   io.step = static_cast<float>(out_factor / sched.last);
   err = launch_pdl(update ? ortho_out_kernel<true> : ortho_out_kernel<false>, grid, dim3(256), 0, stream, io);
@@ -1180,6 +1241,18 @@ int ortho_run(OrthoIo io, const OrthoPlan& o, const double* coefficients, int st
   note_launch(update ? "ortho_step" : "ortho_out");
   return check_launch();
 }
+
+int ortho_run(const OrthoIo& io, const OrthoPlan& o, const double* coefficients, int steps, bool update, double out_factor,
+              void* workspace, cudaStream_t stream) {
+  return o.full ? ortho_run_as<true>(io, o, coefficients, steps, update, out_factor, workspace, stream)
+                : ortho_run_as<false>(io, o, coefficients, steps, update, out_factor, workspace, stream);
+}
+
+// Bits that the products' operands keep: as asked for, or for orthogonalize by the result's type.  A
+// result of 16 bits is no finer than operands of 11 (fp16's own).  An optimiser step only takes a
+// direction from the result, and keeps 11 whatever W's type.
+bool ortho_bits_ok(int bits) { return bits == 0 || bits == 11 || bits == 22; }
+bool ortho_full(int bits, int result) { return bits == 0 ? result == CUOPX_F32 : bits == 22; }
 
 bool ortho_type_ok(int dtype) { return dtype == CUOPX_F32 || dtype == CUOPX_F16 || dtype == CUOPX_BF16; }
 
@@ -1209,7 +1282,7 @@ bool ortho_sizes_ok(int64_t batch, int64_t rows, int64_t cols) {
 int orthogonalize(const cuopx_orthogonalize_args* a, cudaStream_t stream) {
   if (a == nullptr) return CUOPX_INVALID_ARGUMENT;
   if (!ortho_type_ok(a->dtype) || !ortho_type_ok(a->out_dtype)) return CUOPX_UNSUPPORTED_TYPE;
-  if (a->steps < 0 || a->steps > ORT_MAX_STEPS || a->reserved != 0 || !(a->eps >= 0) || !std::isfinite(a->eps) ||
+  if (a->steps < 0 || a->steps > ORT_MAX_STEPS || !ortho_bits_ok(a->operand_bits) || !(a->eps >= 0) || !std::isfinite(a->eps) ||
       (a->steps > 0 && !a->coefficients) || !ortho_sizes_ok(a->batch, a->rows, a->cols))
     return CUOPX_INVALID_ARGUMENT;
   OrthoSchedule sched;
@@ -1218,7 +1291,7 @@ int orthogonalize(const cuopx_orthogonalize_args* a, cudaStream_t stream) {
   if (!ortho_layout_ok(a->G, a->dtype, a->ldg, a->strideG, a->batch, a->rows, a->cols) ||
       !ortho_layout_ok(a->out, a->out_dtype, a->ldo, a->strideO, a->batch, a->rows, a->cols) || !starts_on(256, a->workspace))
     return CUOPX_INVALID_ARGUMENT;
-  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols);
+  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols, ortho_full(a->operand_bits, a->out_dtype));
   if (!a->workspace || a->workspace_bytes < o.bytes) return CUOPX_RESOURCE_UNAVAILABLE;
   const size_t g_span = ortho_span(a->dtype, a->ldg, a->strideG, a->batch, a->rows, a->cols);
   const size_t o_span = ortho_span(a->out_dtype, a->ldo, a->strideO, a->batch, a->rows, a->cols);
@@ -1238,7 +1311,7 @@ int orthogonalize(const cuopx_orthogonalize_args* a, cudaStream_t stream) {
 int muon_step(const cuopx_muon_args* a, cudaStream_t stream) {
   if (a == nullptr) return CUOPX_INVALID_ARGUMENT;
   if (!ortho_type_ok(a->wdtype) || !ortho_type_ok(a->gdtype) || !ortho_type_ok(a->mdtype)) return CUOPX_UNSUPPORTED_TYPE;
-  if (a->steps < 0 || a->steps > ORT_MAX_STEPS || (a->nesterov != 0 && a->nesterov != 1) || a->reserved != 0 || !(a->eps >= 0) ||
+  if (a->steps < 0 || a->steps > ORT_MAX_STEPS || (a->nesterov != 0 && a->nesterov != 1) || !ortho_bits_ok(a->operand_bits) || !(a->eps >= 0) ||
       (a->steps > 0 && !a->coefficients) || !ortho_sizes_ok(a->batch, a->rows, a->cols))
     return CUOPX_INVALID_ARGUMENT;
   for (double v : {a->eps, a->lr, a->mu, a->decay, a->scale})
@@ -1254,7 +1327,7 @@ int muon_step(const cuopx_muon_args* a, cudaStream_t stream) {
   for (const auto& x : t)
     if (!ortho_layout_ok(x.p, x.dtype, x.ld, x.stride, a->batch, a->rows, a->cols)) return CUOPX_INVALID_ARGUMENT;
   if (!starts_on(256, a->workspace) || !starts_on(4, a->lr_dev)) return CUOPX_INVALID_ARGUMENT;
-  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols);
+  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols, a->operand_bits == 22);
   if (!a->workspace || a->workspace_bytes < o.bytes) return CUOPX_RESOURCE_UNAVAILABLE;
   size_t span[3];
   for (int i = 0; i < 3; ++i) {
@@ -1285,8 +1358,11 @@ int muon_step(const cuopx_muon_args* a, cudaStream_t stream) {
 
 extern "C" {
 
+size_t cuopx_orthogonalize_workspace_size_bits(int64_t batch, int64_t rows, int64_t cols, int operand_bits) {
+  return cuopx::ortho_sizes_ok(batch, rows, cols) ? cuopx::ortho_plan(batch, rows, cols, operand_bits != 11).bytes : 0;
+}
 size_t cuopx_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols) {
-  return cuopx::ortho_sizes_ok(batch, rows, cols) ? cuopx::ortho_plan(batch, rows, cols).bytes : 0;
+  return cuopx_orthogonalize_workspace_size_bits(batch, rows, cols, 22);
 }
 
 int cuopx_orthogonalize(const cuopx_orthogonalize_args* args, void* stream) {

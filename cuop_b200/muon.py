@@ -78,6 +78,12 @@ def _stack(t: torch.Tensor, shape, device: int, what: str):
     return code, t.data_ptr(), ld, stride
 
 
+def _bits(operand_bits: int, what: str) -> int:
+    if operand_bits not in (11, 22):
+        _error(N.INVALID_ARGUMENT, f"{what}: operand_bits must be 11 or 22, not {operand_bits!r}")
+    return int(operand_bits)
+
+
 def _sizes(t: torch.Tensor, what: str):
     if t.dim() not in (2, 3):
         _error(N.SHAPE_MISMATCH, f"{what} must be a matrix or a stack of matrices")
@@ -86,18 +92,21 @@ def _sizes(t: torch.Tensor, what: str):
 
 
 def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
-                  out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None, operand_bits: Optional[int] = None, stream=None) -> torch.Tensor:
     """X after `steps` times X = a X + (b A + c A A) X, A = X X^T, from g / (||g|| + eps) (cuopx_orthogonalize).
 
     g: [rows, cols] or [batch, rows, cols], float32, float16 or bfloat16; out:
     the same shape, any of these types (g's by default), or g itself.
     coefficients: (a, b, c), or one such triple for each step; a singular value
-    in [0, 1] may not grow beyond 1024 by them.  Products take fp16 operands,
-    scaled, and sum in fp32; X is kept in 22 bits: the result is off by 2e-4 to
-    2e-3 of its norm, whatever the types."""
+    in [0, 1] may not grow beyond 1024 by them.  operand_bits: what the products'
+    operands keep, 22 for a float32 result and 11 for others unless given.  With 11
+    the result is off by 2e-4 to 2e-3 of its norm; with 22, which takes up to three times
+    as long, by 5e-6 (64 x 3000) to 6e-5 (4096 x 10240): the tensor cores' fp32
+    sums, whose error grows with their depth.  X itself keeps 22 bits either way."""
     device = _device(g, "orthogonalize")
     if stream is not None or device != _current_device():
-        return _elsewhere(orthogonalize, device, stream, g, steps=steps, coefficients=coefficients, eps=eps, out=out)
+        return _elsewhere(orthogonalize, device, stream, g, steps=steps, coefficients=coefficients, eps=eps, out=out,
+                          operand_bits=operand_bits)
     batch, rows, cols = _sizes(g, "g")
     coeff = _schedule(coefficients, steps, "orthogonalize")
     gd, gp, ldg, sg = _stack(g, g.shape, device, "g")
@@ -105,10 +114,13 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
         out = _empty(g.shape, dtype=g.dtype, device=g.device)
     od, op, ldo, so = _stack(out, g.shape, device, "out")
     lib = N.lib()
-    wsb = lib.cuopx_orthogonalize_workspace_size(batch, rows, cols)
+    if operand_bits is None:
+        operand_bits = 22 if out.dtype == torch.float32 else 11
+    bits = _bits(operand_bits, "orthogonalize")
+    wsb = lib.cuopx_orthogonalize_workspace_size_bits(batch, rows, cols, bits)
     ws = _empty(wsb, dtype=torch.uint8, device=g.device) if wsb else None
     rc = lib.cuopx_orthogonalize(
-        _ORTHO.pack(gd, od, steps, 0, batch, rows, cols, eps, C.addressof(coeff), gp, ldg, sg, op, ldo, so,
+        _ORTHO.pack(gd, od, steps, bits, batch, rows, cols, eps, C.addressof(coeff), gp, ldg, sg, op, ldo, so,
                     ws.data_ptr() if wsb else 0, wsb), _raw_stream(device))
     if rc:
         N.check(rc, "cuopx_orthogonalize")
@@ -118,7 +130,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
 def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: float, mu: float = 0.95,
               weight_decay: float = 0.0, nesterov: bool = True, scale: Optional[float] = None, steps: int = 5,
               coefficients=COEFFICIENTS, eps: float = 1e-7, lr_tensor: Optional[torch.Tensor] = None,
-              stream=None) -> torch.Tensor:
+              operand_bits: int = 11, stream=None) -> torch.Tensor:
     """One step of Muon, in place on w and momentum; returns w (cuopx_muon_step).
 
       momentum = mu momentum + g;  u = g + mu momentum with nesterov, else momentum
@@ -128,12 +140,14 @@ def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: f
     float32, float16 or bfloat16.  scale: 0.2 sqrt(max(rows, cols)) by default,
     which gives the step a root mean square of about 0.2 lr whatever the shape,
     transposed weights too.  lr_tensor, one float32 on the device, multiplies lr when the
-    kernel runs, so that a captured graph can follow a schedule."""
+    kernel runs, so that a captured graph can follow a schedule.  operand_bits: as in
+    orthogonalize, but 11 for every type unless 22 is asked for: the step is then off by
+    2e-4 to 2e-3 of itself, less than training commonly allows it."""
     device = _device(w, "muon_step")
     if stream is not None or device != _current_device():
         return _elsewhere(muon_step, device, stream, w, g, momentum, lr=lr, mu=mu, weight_decay=weight_decay,
                           nesterov=nesterov, scale=scale, steps=steps, coefficients=coefficients, eps=eps,
-                          lr_tensor=lr_tensor)
+                          lr_tensor=lr_tensor, operand_bits=operand_bits)
     batch, rows, cols = _sizes(w, "w")
     coeff = _schedule(coefficients, steps, "muon_step")
     wd, wp, ldw, sw = _stack(w, w.shape, device, "w")
@@ -147,10 +161,11 @@ def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: f
     if scale is None:
         scale = 0.2 * math.sqrt(max(rows, cols, 1))
     lib = N.lib()
-    wsb = lib.cuopx_orthogonalize_workspace_size(batch, rows, cols)
+    bits = _bits(operand_bits, "muon_step")
+    wsb = lib.cuopx_orthogonalize_workspace_size_bits(batch, rows, cols, bits)
     ws = _empty(wsb, dtype=torch.uint8, device=w.device) if wsb else None
     rc = lib.cuopx_muon_step(
-        _MUON.pack(wd, gd, md, steps, 1 if nesterov else 0, 0, batch, rows, cols, eps, C.addressof(coeff), lr, mu,
+        _MUON.pack(wd, gd, md, steps, 1 if nesterov else 0, bits, batch, rows, cols, eps, C.addressof(coeff), lr, mu,
                    weight_decay, scale, lp, wp, ldw, sw, mp, ldm, sm, gp, ldg, sg, ws.data_ptr() if wsb else 0, wsb),
         _raw_stream(device))
     if rc:

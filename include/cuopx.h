@@ -530,7 +530,7 @@ typedef struct cuopx_orthogonalize_args {
   int32_t dtype;     /* of G: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
   int32_t out_dtype; /* of out, likewise */
   int32_t steps;     /* 0 to 32 */
-  int32_t reserved;  /* 0 */
+  int32_t operand_bits; /* of the products: 11, 22, or 0: 22 where out is CUOPX_F32, else 11 */
   int64_t batch, rows, cols;
   double eps;                 /* finite, >= 0 */
   const double* coefficients; /* host, steps x (a, b, c) */
@@ -543,22 +543,29 @@ typedef struct cuopx_orthogonalize_args {
 } cuopx_orthogonalize_args;
 
 /*
- * out = the iteration's X.  The norm is summed in 64 bits; products take fp16
- * operands (scaled by powers of two to fit) and sum in fp32; X is kept in 22
- * bits between them.  Against the iteration in 64 bits the result is off by 2e-4 to 2e-3 of its
- * norm, whatever the types.  Coefficients that let a singular value in [0, 1]
- * grow beyond 1024 are refused.  CUOPX_RESOURCE_UNAVAILABLE when the workspace
- * is smaller than the size call says (about 6 bytes an element of G and 4 an
- * element of A).
+ * out = the iteration's X.  The norm is summed in 64 bits; X is kept in 22
+ * bits between products, which sum in fp32.  operand_bits says what the products
+ * read of their operands (scaled by powers of two to fit), and so how far the result is off
+ * the iteration in 64 bits: 11 (one fp16 number) 2e-4 to 2e-3 of its norm; 22 (two,
+ * three products in place of one) 5e-6 to 6e-5, by the fp32 sums' depth.  0: 22 for a CUOPX_F32 out, else 11.
+ *
+ * Coefficients that let a singular value in [0, 1] grow beyond 1024 are
+ * refused, as are batch > 65535 and rows or cols > 2^24.  G and out either are
+ * one (same address, type and strides) or lie in address ranges that do not
+ * overlap: column slices of one buffer are refused.
+ * CUOPX_RESOURCE_UNAVAILABLE when the workspace is smaller than the size call
+ * says for the bits that are used: with 11 about 6 bytes an element of G and 4 an element of
+ * A, with 22 about 8 of each.  cuopx_orthogonalize_workspace_size is enough for any.
  */
 size_t cuopx_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols);
+size_t cuopx_orthogonalize_workspace_size_bits(int64_t batch, int64_t rows, int64_t cols, int operand_bits);
 int cuopx_orthogonalize(const cuopx_orthogonalize_args* args, void* stream);
 
 typedef struct cuopx_muon_args {
   int32_t wdtype, gdtype, mdtype; /* of W, G and momentum: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
   int32_t steps;                  /* as above */
   int32_t nesterov;               /* 0 or 1 */
-  int32_t reserved;               /* 0 */
+  int32_t operand_bits;           /* as above; 0: 11 */
   int64_t batch, rows, cols;
   double eps;
   const double* coefficients;
@@ -570,7 +577,7 @@ typedef struct cuopx_muon_args {
   int64_t ldm, strideM;
   const void* G;
   int64_t ldg, strideG;
-  void* workspace; /* cuopx_orthogonalize_workspace_size */
+  void* workspace; /* cuopx_orthogonalize_workspace_size, or ..._bits */
   size_t workspace_bytes;
 } cuopx_muon_args;
 
@@ -580,7 +587,7 @@ typedef struct cuopx_muon_args {
  * orthogonalised, W = (1 - lr decay) W - lr scale O; each matrix rounded once.
  * Momentum is written by the first of several launches: a call that is refused, or
  * whose products cannot be set up on the device, launches nothing and leaves
- * both as they were.
+ * both as they were.  W, momentum and G lie in address ranges that do not overlap.
  */
 int cuopx_muon_step(const cuopx_muon_args* args, void* stream);
 
