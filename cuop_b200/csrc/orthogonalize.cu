@@ -1238,7 +1238,9 @@ int ortho_run_as(OrthoIo io, const OrthoPlan& o, const double* coefficients, int
     cudaGetLastError();
     return cuda_failure(err);
   }
-  note_launch(update ? "ortho_step" : "ortho_out");
+  // Named after the products' widest tiles, which have a ring and an accumulator of their own.
+  if (steps > 0 && products.args.width[kPoly] == 512) note_launch(update ? "ortho_step_w512" : "ortho_out_w512");
+  else note_launch(update ? "ortho_step" : "ortho_out");
   return check_launch();
 }
 
