@@ -535,8 +535,9 @@ int launch_linear_split(const LinearProblem& p, cudaStream_t stream) {
     const int64_t once = capacity[dev][i].load(std::memory_order_relaxed);
     if (tiles <= (L::CTAS == 2 ? once * 20 / 9 : once) && prm.k_blocks >= (2 << i)) cs = 1 << i;
   }
-  while (QX && cs < 8 && prm.k_blocks > cs * LSP_QX_BLOCKS) cs *= 2;
-  if (QX && prm.k_blocks > cs * LSP_QX_BLOCKS) return CUOPX_NOT_IMPLEMENTED;  // not reached: split_quantises
+  // A part that holds fewer clusters than split_quantises reckons with splits K further all the same: its
+  // 8192 elements are 64 K blocks at most, which four CTAs hold.
+  while (QX && prm.k_blocks > cs * LSP_QX_BLOCKS) cs *= 2;
   prm.cs = cs;
   const cudaError_t err = launch_pdl_cluster(kern, dim3(static_cast<unsigned>(tiles * cs)), dim3(LSP_THREADS), SMEM,
                                              stream, static_cast<unsigned>(cs), mW, mX, prm);

@@ -68,6 +68,19 @@ def quantize_int8(x: torch.Tensor, *, trans: bool = False, out: Optional[torch.T
     return out, scale
 
 
+def _scratch(size, head) -> int:
+    """What the size call says for these arguments, without the call (0.6 us of a 17 us step) where nothing is copied
+    and the product's kernel does not quantise x: nothing for an int8 x, else the quantised x and its scales."""
+    _, _, m, n, k, xp, ldx, xsp, wp, ldw = head[:10]
+    if (wp | ldw) & 15 or (xsp and (xp | ldx) & 15):
+        return size(_INT8.pack(*head, 0, 0))
+    if xsp or not (m and n and k):
+        return 0
+    if m * k <= 8192:  # the product's kernel may quantise x
+        return size(_INT8.pack(*head, 0, 0))
+    return ((m * ((k + 15) & ~15) + 255) & ~255) + ((4 * m + 255) & ~255)
+
+
 def _int8(fn, gated: bool, x, w, w_scale, bias, residual, x_scale, activation, dtype, out, stream):
     what = "int8_gated_linear" if gated else "int8_linear"
     device = _device(x, what)
@@ -117,14 +130,7 @@ def _int8(fn, gated: bool, x, w, w_scale, bias, residual, x_scale, activation, d
     head = (code, act, m, n, k, xp, ldx, xsp, wp, ldw, wsp, bp, rp, ldr, out.data_ptr(), ldy)
     lib = N.lib()
     size = lib.cuopx_int8_gated_linear_workspace_size if gated else lib.cuopx_int8_linear_workspace_size
-    if (wp | ldw) & 15 or (xsp and (xp | ldx) & 15):
-        wsb = size(_INT8.pack(*head, 0, 0))
-    elif xsp or not (m and n and k):
-        wsb = 0
-    elif m * k <= 8192:  # the product's kernel may quantise x
-        wsb = size(_INT8.pack(*head, 0, 0))
-    else:  # as the size call says where nothing is copied: the quantised x and its scales
-        wsb = ((m * ((k + 15) & ~15) + 255) & ~255) + ((4 * m + 255) & ~255)
+    wsb = _scratch(size, head)
     ws = x.new_empty(wsb, dtype=torch.uint8) if wsb else None
     call = lib.cuopx_int8_gated_linear if gated else lib.cuopx_int8_linear
     rc = call(_INT8.pack(*head, ws.data_ptr() if wsb else 0, wsb), _raw_stream(device))
