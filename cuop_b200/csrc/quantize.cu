@@ -261,15 +261,22 @@ __global__ void __maxnreg__(WORD ? 64 : 40) quantize_columns_kernel(const QuantP
   }
   if (cs > 1) {
     cluster_sync_all();  // every CTA's maxima are in place
-    m = 0;
-    for (int i = 0; i < cs; ++i) {
-      uint32_t w;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(map_to_rank(&top[lane], static_cast<uint32_t>(i))) : "memory");
-      m = Mag::word(m, w);
+    if (warp == 0) {
+      m = 0;
+      for (int i = 0; i < cs; ++i) {
+        uint32_t w;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(map_to_rank(&top[lane], static_cast<uint32_t>(i))) : "memory");
+        m = Mag::word(m, w);
+      }
+      part[0][lane] = m;
     }
-    // Has read the others': the release keeps the reads before the arrival, after which another CTA
-    // may leave, one without rows at once.
-    cluster_arrive();
+    __syncthreads();
+    m = part[0][lane];
+    // Has read the others': the release of the warp that did keeps its reads before the arrival, after which
+    // another CTA may leave, one without rows at once.  (Every warp reading, and releasing here: 4096 x
+    // 10240 12 us more; releasing behind the next phase: 7.)
+    if (warp == 0) cluster_arrive();
+    else cluster_arrive_relaxed();
   } else {
     __syncthreads();
     m = top[lane];
