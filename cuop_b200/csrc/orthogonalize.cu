@@ -640,7 +640,10 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
           auto release = [&] {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(map_to_rank(&acc_empty[slot + h], 0));
+            // The last tile's accumulator is not handed back: nobody waits for it, and an arrival on its way to the
+            // leader's barrier could outlive the leader.
+            if (lane == 0 && (ph + 1 < phases || t + pairs < g.tiles[kind]))
+              mbar_arrive_remote(map_to_rank(&acc_empty[slot + h], 0));
           };
           if (kind == kUpdate) {
             const int64_t off = b * g.stride_x;
@@ -678,9 +681,7 @@ __global__ void __launch_bounds__(ORT_THREADS, 1)
 
   tc_fence_before_sync();
   __syncthreads();
-  // The partner is done with this CTA's shared memory, barriers and TMEM: its last arrivals on the
-  // leader's acc_empty, for which nobody waits, are released before it.
-  cluster_sync_all();
+  cluster_sync_relaxed();  // the partner is done with this CTA's shared memory, barriers and TMEM
   if (warp == 1) {
     tc_fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(ORT_TMEM_COLS) : "memory");
