@@ -17,12 +17,12 @@
 // both, and errors of 2e-4 (few large directions) to 1.6e-3 (equal ones) remain.  Every matrix
 // is stored times a power of two that its bound allows (2^15 / bound): the
 // elements of A are far below fp16's normal range otherwise.
-// That is with operands of 11 bits, for results of 16 bits and optimiser steps.  With 22 (FULL),
-// for fp32 results, A and P are kept as hi + lo too, and every product is hi lo + lo hi + hi hi, one
+// That is with operands of 11 bits, for results in bf16, whose rounding is above it.  With 22 (FULL),
+// for fp16 and fp32, A and P are kept as hi + lo too, and every product is hi lo + lo hi + hi hi, one
 // after the other along a depth three times as long; lo lo is 2^-24 of the sum.  What
-// remains is the tensor cores' fp32 sums, 5e-6 (64 x 3000) to 6e-5 (4096 x 10240) of the result, growing
-// with the depth.  Whole calls in fp32, us with 11 / 22 bits: 1024 x 1024 191 / 315, 5001 x 1777 504 / 1082,
-// 4096 x 10240 2558 / 7742.
+// remains is the tensor cores' fp32 sums, 5e-6 (64 x 3000) to 2e-4 (8192 x 28672) of the result, growing
+// with the depth.  Whole calls in fp32, us with 11 / 22 bits: 1024 x 1024 162 / 310, 5001 x 1777 494 / 1051,
+// 4096 x 10240 2527 / 7187.
 //
 // One persistent launch does all products: tiles of 256 x 256 or 256 x 128 on CTA
 // pairs (tcgen05 cta_group::2), tile i of a phase on pair i mod the number of pairs,
@@ -39,7 +39,7 @@
 // thread for both operands under `lane == 0` took 305 ns a stage, more than twice
 // what the tensor cores need for 256 x 128 x 64 (now 250; 256 x 256 x 64 300).
 //
-// Measured, whole calls, bf16, work with symmetric products counted by halves: 1024 x 1024 162
+// Measured, whole calls, bf16 (11 bits), work with symmetric products counted by halves: 1024 x 1024 162
 // us, of which 15 phases of about 10 us (4.4 with nothing to compute); 5001 x 1777 490 us
 // (540 TFLOP/s); eight 2048 x 2048 1.39 ms (990); 8192 x 28672 28 ms (1.1 PFLOP/s, at the
 // power cap).  Middle sizes are bound by L2: 256-wide tiles pull 10 TB/s from it.
@@ -1251,11 +1251,10 @@ int ortho_run(const OrthoIo& io, const OrthoPlan& o, const double* coefficients,
                 : ortho_run_as<false>(io, o, coefficients, steps, update, out_factor, workspace, stream);
 }
 
-// Bits that the products' operands keep: as asked for, or for orthogonalize by the result's type.  A
-// result of 16 bits is no finer than operands of 11 (fp16's own).  An optimiser step only takes a
-// direction from the result, and keeps 11 whatever W's type.
+// Bits that the products' operands keep: as asked for, or by the result's type.  Operands of 11
+// leave 1.2e-3 of the result, less than bf16's own rounding (1.7e-3) but six times fp16's.
 bool ortho_bits_ok(int bits) { return bits == 0 || bits == 11 || bits == 22; }
-bool ortho_full(int bits, int result) { return bits == 0 ? result == CUOPX_F32 : bits == 22; }
+bool ortho_full(int bits, int result) { return bits == 0 ? result != CUOPX_BF16 : bits == 22; }
 
 bool ortho_type_ok(int dtype) { return dtype == CUOPX_F32 || dtype == CUOPX_F16 || dtype == CUOPX_BF16; }
 
@@ -1330,7 +1329,7 @@ int muon_step(const cuopx_muon_args* a, cudaStream_t stream) {
   for (const auto& x : t)
     if (!ortho_layout_ok(x.p, x.dtype, x.ld, x.stride, a->batch, a->rows, a->cols)) return CUOPX_INVALID_ARGUMENT;
   if (!starts_on(256, a->workspace) || !starts_on(4, a->lr_dev)) return CUOPX_INVALID_ARGUMENT;
-  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols, a->operand_bits == 22);
+  const OrthoPlan o = ortho_plan(a->batch, a->rows, a->cols, ortho_full(a->operand_bits, a->wdtype));
   if (!a->workspace || a->workspace_bytes < o.bytes) return CUOPX_RESOURCE_UNAVAILABLE;
   size_t span[3];
   for (int i = 0; i < 3; ++i) {

@@ -78,9 +78,12 @@ def _stack(t: torch.Tensor, shape, device: int, what: str):
     return code, t.data_ptr(), ld, stride
 
 
-def _bits(operand_bits: int, what: str) -> int:
+def _bits(operand_bits: Optional[int], result: torch.dtype, what: str) -> int:
+    """Bits that the products' operands keep: those asked for, else by the result's type (as in the C call)."""
+    if operand_bits is None:
+        return 11 if result == torch.bfloat16 else 22
     if operand_bits not in (11, 22):
-        _error(N.INVALID_ARGUMENT, f"{what}: operand_bits must be 11 or 22, not {operand_bits!r}")
+        _error(N.INVALID_ARGUMENT, f"{what}: operand_bits must be 11, 22 or None, not {operand_bits!r}")
     return int(operand_bits)
 
 
@@ -99,9 +102,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     the same shape, any of these types (g's by default), or g itself.
     coefficients: (a, b, c), or one such triple for each step; a singular value
     in [0, 1] may not grow beyond 1024 by them.  operand_bits: what the products'
-    operands keep, 22 for a float32 result and 11 for others unless given.  With 11
-    the result is off by 2e-4 to 2e-3 of its norm; with 22, which takes up to three times
-    as long, by 5e-6 (64 x 3000) to 6e-5 (4096 x 10240): the tensor cores' fp32
+    operands keep, 11 for a bfloat16 result and 22 for others unless given.  With 11
+    the result is off by 2e-4 to 2e-3 of its norm, bfloat16's own rounding by 1.7e-3; with 22, which takes up to three times
+    as long, by 5e-6 (64 x 3000) to 2e-4 (8192 x 28672): the tensor cores' fp32
     sums, whose error grows with their depth.  X itself keeps 22 bits either way."""
     device = _device(g, "orthogonalize")
     if stream is not None or device != _current_device():
@@ -114,9 +117,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
         out = _empty(g.shape, dtype=g.dtype, device=g.device)
     od, op, ldo, so = _stack(out, g.shape, device, "out")
     lib = N.lib()
-    if operand_bits is None:
-        operand_bits = 22 if out.dtype == torch.float32 else 11
-    bits = _bits(operand_bits, "orthogonalize")
+    bits = _bits(operand_bits, out.dtype, "orthogonalize")
     wsb = lib.cuopx_orthogonalize_workspace_size_bits(batch, rows, cols, bits)
     ws = _empty(wsb, dtype=torch.uint8, device=g.device) if wsb else None
     rc = lib.cuopx_orthogonalize(
@@ -130,7 +131,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
 def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: float, mu: float = 0.95,
               weight_decay: float = 0.0, nesterov: bool = True, scale: Optional[float] = None, steps: int = 5,
               coefficients=COEFFICIENTS, eps: float = 1e-7, lr_tensor: Optional[torch.Tensor] = None,
-              operand_bits: int = 11, stream=None) -> torch.Tensor:
+              operand_bits: Optional[int] = None, stream=None) -> torch.Tensor:
     """One step of Muon, in place on w and momentum; returns w (cuopx_muon_step).
 
       momentum = mu momentum + g;  u = g + mu momentum with nesterov, else momentum
@@ -141,8 +142,8 @@ def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: f
     which gives the step a root mean square of about 0.2 lr whatever the shape,
     transposed weights too.  lr_tensor, one float32 on the device, multiplies lr when the
     kernel runs, so that a captured graph can follow a schedule.  operand_bits: as in
-    orthogonalize, but 11 for every type unless 22 is asked for: the step is then off by
-    2e-4 to 2e-3 of itself, less than training commonly allows it."""
+    orthogonalize, w being the result; 11 makes the steps of float16 and float32 weights as
+    fast as bfloat16 weights', each off by 2e-4 to 2e-3 of itself."""
     device = _device(w, "muon_step")
     if stream is not None or device != _current_device():
         return _elsewhere(muon_step, device, stream, w, g, momentum, lr=lr, mu=mu, weight_decay=weight_decay,
@@ -161,7 +162,7 @@ def muon_step(w: torch.Tensor, g: torch.Tensor, momentum: torch.Tensor, *, lr: f
     if scale is None:
         scale = 0.2 * math.sqrt(max(rows, cols, 1))
     lib = N.lib()
-    bits = _bits(operand_bits, "muon_step")
+    bits = _bits(operand_bits, w.dtype, "muon_step")
     wsb = lib.cuopx_orthogonalize_workspace_size_bits(batch, rows, cols, bits)
     ws = _empty(wsb, dtype=torch.uint8, device=w.device) if wsb else None
     rc = lib.cuopx_muon_step(

@@ -530,7 +530,7 @@ typedef struct cuopx_orthogonalize_args {
   int32_t dtype;     /* of G: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
   int32_t out_dtype; /* of out, likewise */
   int32_t steps;     /* 0 to 32 */
-  int32_t operand_bits; /* of the products: 11, 22, or 0: 22 where out is CUOPX_F32, else 11 */
+  int32_t operand_bits; /* of the products: 11, 22, or 0: 11 where out is CUOPX_BF16, else 22 */
   int64_t batch, rows, cols;
   double eps;                 /* finite, >= 0 */
   const double* coefficients; /* host, steps x (a, b, c) */
@@ -547,7 +547,7 @@ typedef struct cuopx_orthogonalize_args {
  * bits between products, which sum in fp32.  operand_bits says what the products
  * read of their operands (scaled by powers of two to fit), and so how far the result is off
  * the iteration in 64 bits: 11 (one fp16 number) 2e-4 to 2e-3 of its norm; 22 (two,
- * three products in place of one) 5e-6 to 6e-5, by the fp32 sums' depth.  0: 22 for a CUOPX_F32 out, else 11.
+ * three products in place of one) 5e-6 to 2e-4, by the fp32 sums' depth.  0: 11 for a CUOPX_BF16 out, else 22.
  *
  * Coefficients that let a singular value in [0, 1] grow beyond 1024 are
  * refused, as are batch > 65535 and rows or cols > 2^24.  G and out either are
@@ -565,7 +565,7 @@ typedef struct cuopx_muon_args {
   int32_t wdtype, gdtype, mdtype; /* of W, G and momentum: CUOPX_F32, CUOPX_F16 or CUOPX_BF16 */
   int32_t steps;                  /* as above */
   int32_t nesterov;               /* 0 or 1 */
-  int32_t operand_bits;           /* as above; 0: 11 */
+  int32_t operand_bits;           /* as above, 0: by W's type */
   int64_t batch, rows, cols;
   double eps;
   const double* coefficients;

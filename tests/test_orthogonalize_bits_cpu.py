@@ -23,10 +23,10 @@ def test_workspace():
         assert few < full == lib.cuopx_orthogonalize_workspace_size(*size) == lib.cuopx_orthogonalize_workspace_size_bits(*size, 0)
         batch, rows, cols = size
         for kw, need in ((dict(reserved=11), few), (dict(reserved=22), full), (dict(reserved=11, out_dtype=N.F32), few),
-                         (dict(out_dtype=N.F32), full), (dict(), few)):
+                         (dict(out_dtype=N.F32), full), (dict(out_dtype=N.F16), full), (dict(), few)):
             kw.update(batch=batch, rows=rows, cols=cols, ldg=cols, ldo=cols, sg=rows * cols, so=rows * cols)
             assert lib.cuopx_orthogonalize(ortho(wsb=need - 1, **kw), None) == ROOM
-        for kw, need in ((dict(reserved=11), few), (dict(reserved=22), full), (dict(reserved=22, wd=N.F32), full), (dict(wd=N.F32), few),
+        for kw, need in ((dict(reserved=11), few), (dict(reserved=22), full), (dict(reserved=11, wd=N.F32), few), (dict(wd=N.F32), full), (dict(wd=N.F16), full),
                          (dict(), few)):
             kw.update(batch=batch, rows=rows, cols=cols, ldw=cols, ldm=cols, ldg=cols, sw=rows * cols, sm=rows * cols, sg=rows * cols)
             assert lib.cuopx_muon_step(muon(wsb=need - 1, **kw), None) == ROOM
