@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantParams p
   }
 }
 
-// Any alignment and any length: a CTA to a row, elements, the row read twice.
+// Any alignment and any length: a CTA to a row, elements, the row read twice (the second time from
+// L2).  8192 x 8192 bf16 off 16-byte boundaries 65 us (aligned 37), 1024 x 40000 100 us.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParams p) {
   using Mag = Magnitude<T>;
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const QuantParam
 // strip's column maxima meet through distributed shared memory; every CTA then quantises its
 // rows in place, four of a column to a word, and writes them out along Q's rows.
 // A CTA's four phases, which other CTAs of the SM overlap only in part, bound it: 4096 x 10240 bf16
-// 46.8 us, rows off 4-byte boundaries as in 4095 x 10001 fp16 (WORD false: single elements) 55;
+// 47 us, rows off 4-byte boundaries as in 4095 x 10001 fp16 (WORD false: single elements) 57;
 // two passes over X took 141.  Half the threads: 52 and 73.  Loads by 4-byte cp.async, all of
 // a share at once: 76 and 89.
 constexpr int QC_PITCH = 33;  // words of a row in shared memory
@@ -331,7 +332,8 @@ __global__ void __maxnreg__(WORD ? 64 : 40) quantize_columns_kernel(const QuantP
   if (cs > 1) cluster_wait();  // the others have read this CTA's maxima
 }
 
-// More rows than a cluster holds: maxima first, then a second pass.
+// More rows than a cluster holds: maxima first, then a second pass, single elements in both: 28672 x 8192
+// bf16 650 us, 109 being its floor.
 // Largest magnitudes of columns, as bits, in `top` (zeroed before): a thread
 // to a column, 8 row phases and a share of the rows to a CTA.
 template <typename T>

@@ -480,7 +480,7 @@ typedef struct cuopx_quantize_args {
  * infinity or a NaN gets that as its scale, and zeros.  The layout with trans is the one in
  * which cuopx_int8_linear takes weights stored [K][columns].
  * CUOPX_RESOURCE_UNAVAILABLE when the workspace is smaller than the size call
- * says (0 without trans).
+ * says (0 without trans).  With trans up to 65535 * 128 rows are taken.
  */
 size_t cuopx_quantize_workspace_size(const cuopx_quantize_args* args);
 int cuopx_quantize(const cuopx_quantize_args* args, void* stream);
